@@ -345,6 +345,76 @@ int dk_argmax_advance(const void* logits, int V, int64_t* tok, int32_t* pos, voi
 int dk_argmax_advance_split(const void* logits, int V, int64_t* tok, int32_t* pos, uint64_t* work, void* stream);
 
 /*
+ * Per-head RMSNorm of q and k, RoPE and KV append of M rows in one pass: rows of a prompt or of a drafted token tree.
+ * Row m of qkv [M, (n_q + 2 n_kv) head_dim] is cache token T = *pos + m and rotates at position R = *pos + depth[m]
+ * (depth NULL: R = T). With weights q_w, k_w (fp16 [head_dim]; both or neither) a q or k head x first becomes
+ * x * w / sqrt(mean(x^2) + eps); then pairs (i, i + D/2) rotate by row R of the fp32 tables [max_pos, D/2]; all of it in
+ * fp32 with one rounding to fp16 at the end (without weights: bit for bit dk_rope_append_rows). The rotated q goes to
+ * q_out (row stride q_stride values; q_out = qkv with q_stride = (n_q + 2 n_kv) head_dim is in place, else disjoint from
+ * qkv), rotated k and v to the cache slot of T; k and v in qkv stay as they were. A row whose R is outside [0, max_pos)
+ * or whose T is negative touches nothing; a T without a mapped page is rotated but not appended. qkv, q_out, q_w, k_w,
+ * kc, vc and the tables 16-byte aligned, q_stride % 8 == 0, M 1..2^20. No counterpart in the reference (its models have
+ * no per-head norms; rope_append, kernels/bindings.cpp:81-88, is one token at *pos).
+ */
+int dk_qk_norm_rope_append_rows(const void* qkv, const void* q_w, const void* k_w, float eps, const float* cos_t,
+                                const float* sin_t, const int32_t* pos, const int32_t* depth, const int32_t* bt,
+                                void* kc, void* vc, void* q_out, long long q_stride, int M, int n_q, int n_kv,
+                                int head_dim, int page, int max_pos, int n_pages, int n_bt, void* stream);
+
+/*
+ * Attention of the M nodes of a drafted token tree over the paged cache, which already holds them: node j is cache token
+ * *pos + j (dk_qk_norm_rope_append_rows). Node i attends the committed tokens [0, *pos) and the nodes j whose bit j % 64
+ * of word j / 64 is set in row i of mask (int64 [M, ceil(M / 64)]; NULL: a chain, j <= i); bits at and past M are not
+ * read as nodes. A node that attends nothing gets zeros. Tokens at positions >= max_ctx (pass *pos + M or more), past the
+ * block table or without a mapped page are neither read nor attended, and neither values nor NaN of a token reach a node
+ * that does not attend it; *pos < 0: no token is attended. q: row m's heads at q + m q_stride (q_stride % 8 == 0), already
+ * rotated; out [M, n_q * head_dim] fp16, not overlapping q. fp32 scores and softmax, scale 1/sqrt(head_dim). n_q / n_kv
+ * in {1, 2, 4, 8}, M 1..1024. q, kc, vc and out 16-byte aligned.
+ * The context is split over workgroups whose fp32 partials meet in `workspace` (16-byte aligned, overlapping nothing
+ * else) and are joined in split order by a second launch; dk_attention_tree_workspace_bytes gives what the sizes can use
+ * (0: they do not split). A smaller workspace runs the most splits it holds, NULL runs unsplit. No counterpart in the
+ * reference.
+ */
+size_t dk_attention_tree_workspace_bytes(int M, int n_q, int n_kv, int head_dim, int max_ctx);
+int dk_attention_tree(const void* q, long long q_stride, const int64_t* mask, const int32_t* pos, const int32_t* bt,
+                      int n_bt, const void* kc, const void* vc, int n_pages, int page, int n_q, int n_kv, int head_dim,
+                      int M, int max_ctx, void* out, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Log probabilities of given tokens, entropy and top alternatives of M rows of logits [M, V] (row stride ld values;
+ * dtype 0 fp16, 1 bf16, 2 fp32), in fp32 from one read of the logits: with lse = log sum_v exp(x_v),
+ *   logprobs[m] = x[tokens[m]] - lse  (NaN for an id outside [0, V), which is not read),
+ *   entropy[m]  = lse - sum_v p_v x_v, p = exp(x - lse)  (-inf logits have p = 0 and add nothing),
+ *   top_ids[m, 0..k), top_logprobs[m, 0..k): the k largest logits, descending, lowest index first among equals (NaN
+ *   ranks highest, as dk_argmax_advance), and x - lse.
+ * A row with a NaN, with +inf or of nothing but -inf has no distribution: its three kinds of values are NaN, its ids stand.
+ * tokens and logprobs may both be NULL, so may entropy; top_ids and top_logprobs are NULL where k is 0. k 0..32, k <= V;
+ * M 1..2^20, V 1..2^24; logits aligned to their type. Outputs overlap nothing. `workspace` (16-byte aligned) lets a row be
+ * split over workgroups; dk_token_logprobs_workspace_bytes gives what the sizes can use (0: no split); NULL or a smaller
+ * one runs unsplit. No counterpart in the reference (its only reader of the logits is torch.argmax,
+ * runtime/model.py:232).
+ */
+size_t dk_token_logprobs_workspace_bytes(int M, int V, int k, int dtype);
+int dk_token_logprobs(const void* logits, int dtype, long long ld, const int64_t* tokens, float* logprobs,
+                      float* entropy, int64_t* top_ids, float* top_logprobs, int M, int V, int k, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
+/*
+ * Greedy acceptance of a verified token tree, and the move of its cache rows. Node 0 is the token that was pending;
+ * from node i the walk goes to the lowest-numbered child c (parents[c] == i < c) with tokens[c] == picks[i * picks_stride]
+ * (the model's pick after node i), and ends where there is none. path[0..M) receives the nodes walked, then -1; *count
+ * their number (>= 1); *tok the pick after the last of them, the next pending token. Then, for every t < *count, the K / V
+ * row of token *pos + path[t] is copied to token *pos + t in each of the n_caches caches (kv: n_caches consecutive
+ * [n_pages, n_kv, page, head_dim] arrays, e.g. K and V of every layer), so that the accepted tokens are contiguous; a row
+ * whose source or target has no mapped page stays. *pos is not advanced (the caller adds *count). kv may be NULL with
+ * n_caches 0. path, count and tok overlap neither each other nor the inputs. M 1..1024; kv 16-byte aligned. No counterpart
+ * in the reference.
+ */
+int dk_tree_accept(const int64_t* tokens, const int32_t* parents, const int64_t* picks, long long picks_stride, int M,
+                   const int32_t* pos, const int32_t* bt, int n_bt, void* kv, int n_caches, int n_pages, int n_kv,
+                   int page, int head_dim, int32_t* path, int32_t* count, int64_t* tok, void* stream);
+
+/*
  * INT4 format producer on the GPU: round-to-nearest asymmetric group quantization of fp16 W [N, K] and packing,
  * bit-identical to runtime/quant.py quantize (:42-48, RTN branch of group_params :20-28) + pack (:100-109) +
  * pack_scale_zero (:122-124). Writes packed int32 [N, K/8] and sz fp16 [N, K/G, 2].

@@ -700,6 +700,200 @@ int dk_argmax_advance_split(const void* logits, int V, int64_t* tok, int32_t* po
   return launched("argmax_advance_split");
 }
 
+// ---- one verification step of speculative decoding --------------------------------------------------------------
+
+int dk_qk_norm_rope_append_rows(const void* qkv, const void* q_w, const void* k_w, float eps, const float* cos_t,
+                                const float* sin_t, const int32_t* pos, const int32_t* depth, const int32_t* bt,
+                                void* kc, void* vc, void* q_out, long long q_stride, int M, int n_q, int n_kv,
+                                int head_dim, int page, int max_pos, int n_pages, int n_bt, void* stream) {
+  if (!qkv || !cos_t || !sin_t || !pos || !bt || !kc || !vc || !q_out)
+    return fail(DK_ERR_NULL, "qk_norm_rope_append_rows: null pointer argument");
+  if ((q_w == nullptr) != (k_w == nullptr))
+    return fail(DK_ERR_NULL, "qk_norm_rope_append_rows: q_w and k_w come together or not at all");
+  if (head_dim != 64 && head_dim != 128)
+    return fail(DK_ERR_SHAPE, "qk_norm_rope_append_rows: head_dim must be 64 or 128, got %d", head_dim);
+  if (n_q <= 0 || n_kv <= 0 || n_q > 65535 || n_kv > 65535)
+    return fail(DK_ERR_SHAPE, "qk_norm_rope_append_rows: bad head counts (n_q=%d n_kv=%d)", n_q, n_kv);
+  if (M < 1 || M > (1 << 20)) return fail(DK_ERR_SHAPE, "qk_norm_rope_append_rows: M must be 1..2^20, got %d", M);
+  if (!pow2(page)) return fail(DK_ERR_DOMAIN, "page size must be a power of two, got %d", page);
+  if (max_pos < 1 || n_pages < 1 || n_bt < 1)
+    return fail(DK_ERR_SHAPE, "qk_norm_rope_append_rows: empty rope table, cache or block table");
+  if (!aligned16(qkv) || !aligned16(q_out) || !aligned16(kc) || !aligned16(vc) || !aligned16(cos_t) ||
+      !aligned16(sin_t) || (q_w && (!aligned16(q_w) || !aligned16(k_w))))
+    return fail(DK_ERR_ALIGN, "qk_norm_rope_append_rows: qkv, q_out, q_w, k_w, kc, vc and the tables must be 16B aligned");
+  if (!aligned4(pos) || !aligned4(bt) || (depth && !aligned4(depth)))
+    return fail(DK_ERR_ALIGN, "qk_norm_rope_append_rows: pos, depth and bt must be 4B aligned");
+  const long long qkv_stride = ((long long)n_q + 2LL * n_kv) * head_dim, q_row = (long long)n_q * head_dim;
+  if (q_stride % 8 != 0 || q_stride < q_row || q_stride > (1LL << 40))
+    return fail(DK_ERR_SHAPE, "qk_norm_rope_append_rows: q_stride must be a multiple of 8 and >= n_q * head_dim, got %lld",
+                q_stride);
+  const bool in_place = q_out == qkv && q_stride == qkv_stride;
+  if (!in_place && ranges_overlap(qkv, (size_t)(M * qkv_stride) * 2, q_out, (size_t)((M - 1) * q_stride + q_row) * 2))
+    return fail(DK_ERR_DOMAIN, "qk_norm_rope_append_rows: q_out must be qkv itself (with its row stride) or disjoint "
+                "from it");
+  clear_error();
+  dk::launch_qk_norm_rope({qkv, q_w, k_w, eps, cos_t, sin_t, pos, depth, bt, kc, vc, q_out, q_stride, M, n_q, n_kv,
+                           head_dim, ilog2(page), max_pos, n_pages, n_bt}, (hipStream_t)stream);
+  return launched("qk_norm_rope_append_rows");
+}
+
+static bool tree_attn_sizes(int M, int n_q, int n_kv, int head_dim, int max_ctx) {
+  if (M < 1 || M > dk::kTreeMaxNodes || n_kv < 1 || n_kv > 65535 || n_q < 1 || n_q % n_kv != 0) return false;
+  const int hpg = n_q / n_kv;
+  return (hpg == 1 || hpg == 2 || hpg == 4 || hpg == 8) && (head_dim == 64 || head_dim == 128) && max_ctx >= 1;
+}
+
+size_t dk_attention_tree_workspace_bytes(int M, int n_q, int n_kv, int head_dim, int max_ctx) {
+  if (!tree_attn_sizes(M, n_q, n_kv, head_dim, max_ctx)) return 0;
+  const int s = dk::attention_tree_splits(M, n_q, n_kv, head_dim, max_ctx);
+  return s > 1 ? (size_t)s * dk::attention_tree_part_bytes(M, n_q, n_kv, head_dim) : 0;
+}
+
+int dk_attention_tree(const void* q, long long q_stride, const int64_t* mask, const int32_t* pos, const int32_t* bt,
+                      int n_bt, const void* kc, const void* vc, int n_pages, int page, int n_q, int n_kv, int head_dim,
+                      int M, int max_ctx, void* out, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!q || !pos || !bt || !kc || !vc || !out) return fail(DK_ERR_NULL, "attention_tree: null pointer argument");
+  if (head_dim != 64 && head_dim != 128)
+    return fail(DK_ERR_SHAPE, "attention_tree: head_dim must be 64 or 128, got %d", head_dim);
+  if (M < 1 || M > dk::kTreeMaxNodes)
+    return fail(DK_ERR_SHAPE, "attention_tree: M must be 1..%d, got %d", dk::kTreeMaxNodes, M);
+  if (max_ctx < 1) return fail(DK_ERR_DOMAIN, "attention_tree: max_ctx must be >= 1, got %d", max_ctx);
+  if (n_kv > 65535) return fail(DK_ERR_SHAPE, "attention_tree: too many kv heads");
+  if (!tree_attn_sizes(M, n_q, n_kv, head_dim, max_ctx))
+    return fail(DK_ERR_SHAPE, "heads-per-group must be 1/2/4/8 (n_q=%d n_kv=%d)", n_q, n_kv);
+  if (!pow2(page)) return fail(DK_ERR_DOMAIN, "page size must be a power of two, got %d", page);
+  if (n_pages < 1 || n_bt < 1) return fail(DK_ERR_SHAPE, "attention_tree: empty cache or block table");
+  const long long row = (long long)n_q * head_dim;
+  if (q_stride % 8 != 0 || q_stride < row || q_stride > (1LL << 40))
+    return fail(DK_ERR_SHAPE, "attention_tree: q_stride must be a multiple of 8 and >= n_q * head_dim, got %lld", q_stride);
+  if (!aligned16(q) || !aligned16(kc) || !aligned16(vc) || !aligned16(out))
+    return fail(DK_ERR_ALIGN, "attention_tree: q, kc, vc and out must be 16B aligned");
+  if (!aligned4(pos) || !aligned4(bt) || (reinterpret_cast<uintptr_t>(mask) & 7u))
+    return fail(DK_ERR_ALIGN, "attention_tree: pos and bt must be 4B and mask 8B aligned");
+  const size_t q_bytes = (size_t)((M - 1) * q_stride + row) * 2, out_bytes = (size_t)(M * row) * 2;
+  if (ranges_overlap(q, q_bytes, out, out_bytes))
+    return fail(DK_ERR_DOMAIN, "attention_tree: out must not overlap q");
+  int splits = 1;
+  if (workspace != nullptr) {
+    if (!aligned16(workspace)) return fail(DK_ERR_ALIGN, "attention_tree: workspace must be 16B aligned");
+    const size_t part = dk::attention_tree_part_bytes(M, n_q, n_kv, head_dim);
+    splits = dk::attention_tree_splits(M, n_q, n_kv, head_dim, max_ctx);
+    if (workspace_bytes / part < (size_t)splits) splits = workspace_bytes / part < 2 ? 1 : (int)(workspace_bytes / part);
+    const size_t used = splits > 1 ? (size_t)splits * part : 0;
+    const size_t mask_bytes = mask ? (size_t)M * ((M + 63) / 64) * 8 : 0;
+    if (used > 0 && (ranges_overlap(workspace, used, q, q_bytes) || ranges_overlap(workspace, used, out, out_bytes) ||
+                     ranges_overlap(workspace, used, mask, mask_bytes)))
+      return fail(DK_ERR_DOMAIN, "attention_tree: workspace must not overlap q, out or mask");
+  }
+  clear_error();
+  dk::launch_attention_tree({q, q_stride, mask, pos, bt, n_bt, kc, vc, n_pages, ilog2(page), n_q, n_kv, head_dim, M,
+                             max_ctx, out, splits, workspace}, (hipStream_t)stream);
+  return launched("attention_tree");
+}
+
+static int logprobs_sizes(int M, int V, int k, int dtype) {
+  if (dtype < 0 || dtype > 2) return fail(DK_ERR_DOMAIN, "token_logprobs: dtype must be 0, 1 or 2, got %d", dtype);
+  if (M < 1 || M > (1 << 20)) return fail(DK_ERR_SHAPE, "token_logprobs: M must be 1..2^20, got %d", M);
+  if (V < 1 || V > (1 << 24)) return fail(DK_ERR_SHAPE, "token_logprobs: V must be 1..2^24, got %d", V);
+  if (k < 0 || k > dk::kLogprobsMaxK || k > V)
+    return fail(DK_ERR_SHAPE, "token_logprobs: k must be 0..%d and at most V, got %d", dk::kLogprobsMaxK, k);
+  return DK_OK;
+}
+
+size_t dk_token_logprobs_workspace_bytes(int M, int V, int k, int dtype) {
+  if (logprobs_sizes(M, V, k, dtype) != DK_OK) return 0;
+  const int s = dk::token_logprobs_splits(M, V, k, dtype);
+  return s > 1 ? dk::token_logprobs_ws_bytes(M, k, s) : 0;
+}
+
+int dk_token_logprobs(const void* logits, int dtype, long long ld, const int64_t* tokens, float* logprobs,
+                      float* entropy, int64_t* top_ids, float* top_logprobs, int M, int V, int k, void* workspace,
+                      size_t workspace_bytes, void* stream) {
+  if (!logits) return fail(DK_ERR_NULL, "token_logprobs: null pointer argument");
+  const int rc = logprobs_sizes(M, V, k, dtype);
+  if (rc != DK_OK) return rc;
+  if ((tokens == nullptr) != (logprobs == nullptr))
+    return fail(DK_ERR_NULL, "token_logprobs: tokens and logprobs come together or not at all");
+  if ((k > 0) != (top_ids != nullptr) || (k > 0) != (top_logprobs != nullptr))
+    return fail(DK_ERR_NULL, "token_logprobs: top_ids and top_logprobs belong to k > 0 (k = %d)", k);
+  if (!logprobs && !entropy && k == 0) return fail(DK_ERR_NULL, "token_logprobs: no output asked for");
+  if (ld < V || ld > (1LL << 40)) return fail(DK_ERR_SHAPE, "token_logprobs: the row stride must be >= V, got %lld", ld);
+  const size_t es = dtype == 2 ? 4 : 2;
+  if (reinterpret_cast<uintptr_t>(logits) & (es - 1))
+    return fail(DK_ERR_ALIGN, "token_logprobs: logits must be aligned to their type");
+  if ((reinterpret_cast<uintptr_t>(tokens) & 7u) || (reinterpret_cast<uintptr_t>(top_ids) & 7u) || !aligned4(logprobs) ||
+      !aligned4(entropy) || !aligned4(top_logprobs))
+    return fail(DK_ERR_ALIGN, "token_logprobs: ids must be 8B and fp32 outputs 4B aligned");
+  const size_t m = (size_t)M, in_bytes = ((m - 1) * (size_t)ld + V) * es;
+  const void* outs[4] = {logprobs, entropy, top_ids, top_logprobs};
+  const size_t sizes[4] = {m * 4, m * 4, m * k * 8, m * k * 4};
+  for (int i = 0; i < 4; ++i) {
+    if (!outs[i]) continue;
+    bool bad = ranges_overlap(outs[i], sizes[i], logits, in_bytes) || (tokens && ranges_overlap(outs[i], sizes[i], tokens, m * 8));
+    for (int j = 0; j < i; ++j) bad = bad || (outs[j] && ranges_overlap(outs[i], sizes[i], outs[j], sizes[j]));
+    if (bad) return fail(DK_ERR_DOMAIN, "token_logprobs: outputs must overlap neither the inputs nor each other");
+  }
+  int splits = 1;
+  if (workspace != nullptr) {
+    if (!aligned16(workspace)) return fail(DK_ERR_ALIGN, "token_logprobs: workspace must be 16B aligned");
+    splits = dk::token_logprobs_splits(M, V, k, dtype);
+    const size_t need = splits > 1 ? dk::token_logprobs_ws_bytes(M, k, splits) : 0;
+    if (workspace_bytes < need) splits = 1;
+    if (splits > 1) {
+      bool bad = ranges_overlap(workspace, need, logits, in_bytes) || (tokens && ranges_overlap(workspace, need, tokens, m * 8));
+      for (int i = 0; i < 4; ++i) bad = bad || (outs[i] && ranges_overlap(workspace, need, outs[i], sizes[i]));
+      if (bad) return fail(DK_ERR_DOMAIN, "token_logprobs: workspace must overlap neither inputs nor outputs");
+    }
+  }
+  clear_error();
+  dk::launch_token_logprobs({logits, dtype, ld, tokens, logprobs, entropy, top_ids, top_logprobs, M, V, k, splits,
+                             workspace}, (hipStream_t)stream);
+  return launched("token_logprobs");
+}
+
+int dk_tree_accept(const int64_t* tokens, const int32_t* parents, const int64_t* picks, long long picks_stride, int M,
+                   const int32_t* pos, const int32_t* bt, int n_bt, void* kv, int n_caches, int n_pages, int n_kv,
+                   int page, int head_dim, int32_t* path, int32_t* count, int64_t* tok, void* stream) {
+  if (!tokens || !parents || !picks || !path || !count || !tok)
+    return fail(DK_ERR_NULL, "tree_accept: null pointer argument");
+  if (M < 1 || M > dk::kTreeMaxNodes)
+    return fail(DK_ERR_SHAPE, "tree_accept: M must be 1..%d, got %d", dk::kTreeMaxNodes, M);
+  if (picks_stride < 1 || picks_stride > (1LL << 40))
+    return fail(DK_ERR_SHAPE, "tree_accept: picks_stride must be >= 1, got %lld", picks_stride);
+  if ((kv == nullptr) != (n_caches == 0) || n_caches < 0)
+    return fail(DK_ERR_SHAPE, "tree_accept: kv and n_caches must both be given or neither (n_caches=%d)", n_caches);
+  if (kv) {
+    if (!pos || !bt) return fail(DK_ERR_NULL, "tree_accept: null pointer argument");
+    if (head_dim != 64 && head_dim != 128)
+      return fail(DK_ERR_SHAPE, "tree_accept: head_dim must be 64 or 128, got %d", head_dim);
+    if (n_kv < 1 || n_kv > 65535) return fail(DK_ERR_SHAPE, "tree_accept: bad head count (n_kv=%d)", n_kv);
+    if (!pow2(page)) return fail(DK_ERR_DOMAIN, "page size must be a power of two, got %d", page);
+    if (n_pages < 1 || n_bt < 1) return fail(DK_ERR_SHAPE, "tree_accept: empty cache or block table");
+    if (n_caches > (1 << 20) || (long long)n_caches * n_kv * head_dim > (1LL << 34))
+      return fail(DK_ERR_SHAPE, "tree_accept: too many caches (%d)", n_caches);
+    if (!aligned16(kv)) return fail(DK_ERR_ALIGN, "tree_accept: kv must be 16B aligned");
+    if (!aligned4(pos) || !aligned4(bt)) return fail(DK_ERR_ALIGN, "tree_accept: pos and bt must be 4B aligned");
+  }
+  if ((reinterpret_cast<uintptr_t>(tokens) & 7u) || (reinterpret_cast<uintptr_t>(picks) & 7u) ||
+      (reinterpret_cast<uintptr_t>(tok) & 7u) || !aligned4(parents) || !aligned4(path) || !aligned4(count))
+    return fail(DK_ERR_ALIGN, "tree_accept: ids must be 8B, parents, path and count 4B aligned");
+  const size_t m = (size_t)M;
+  const void* outs[3] = {path, count, tok};
+  const size_t osz[3] = {m * 4, 4, 8};
+  const void* ins[5] = {tokens, parents, picks, pos, bt};
+  const size_t isz[5] = {m * 8, m * 4, ((m - 1) * (size_t)picks_stride + 1) * 8, 4, (size_t)(n_bt > 0 ? n_bt : 1) * 4};
+  for (int i = 0; i < 3; ++i) {
+    bool bad = false;
+    for (int j = 0; j < 5; ++j) bad = bad || (ins[j] && ranges_overlap(outs[i], osz[i], ins[j], isz[j]));
+    for (int j = 0; j < i; ++j) bad = bad || ranges_overlap(outs[i], osz[i], outs[j], osz[j]);
+    if (bad) return fail(DK_ERR_DOMAIN, "tree_accept: path, count and tok must overlap neither the inputs nor each other");
+  }
+  clear_error();
+  dk::launch_tree_accept({tokens, parents, picks, picks_stride, M, pos, bt, n_bt, kv, n_caches, n_pages, n_kv,
+                          kv ? ilog2(page) : 0, head_dim, path, count, tok}, (hipStream_t)stream);
+  return launched("tree_accept");
+}
+
 int dk_quantize_w4(const void* w, void* packed, void* sz, int N, int K, int group, int clip, void* stream) {
   if (!w || !packed || !sz) return fail(DK_ERR_NULL, "quantize_w4: null pointer argument");
   if (N <= 0 || K <= 0) return fail(DK_ERR_SHAPE, "quantize_w4: N and K must be positive");

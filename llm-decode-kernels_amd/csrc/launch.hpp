@@ -155,6 +155,85 @@ void launch_argmax_advance(const void* logits, int V, int64_t* tok, int32_t* pos
 void launch_argmax_split(const void* logits, int V, int64_t* tok, int32_t* pos, unsigned long long* work,
                          hipStream_t st);
 
+// Rows of a prompt or of a drafted tree: per-head RMSNorm of q and k (qw null: none), RoPE at *pos + depth[m] (depth
+// null: *pos + m), append at token *pos + m; q to q_out (row stride q_stride).
+struct QkNormRope {
+  const void* qkv;
+  const void* q_w;
+  const void* k_w;
+  float eps;
+  const float* cos_t;
+  const float* sin_t;
+  const int32_t* pos;
+  const int32_t* depth;
+  const int32_t* bt;
+  void* kc;
+  void* vc;
+  void* q_out;
+  long long q_stride;
+  int M, n_q, n_kv, head_dim, log2P, max_pos, n_pages, n_bt;
+};
+void launch_qk_norm_rope(const QkNormRope& a, hipStream_t st);
+
+// Attention of the M nodes of a drafted tree over the paged cache, the context in `splits` parts (1: no workspace).
+constexpr int kTreeMaxNodes = 1024;
+struct TreeAttn {
+  const void* q;
+  long long q_stride;
+  const int64_t* mask;  // [M, ceil(M / 64)] or null (a chain)
+  const int32_t* pos;
+  const int32_t* bt;
+  int n_bt;
+  const void* kc;
+  const void* vc;
+  int n_pages, log2P, n_q, n_kv, head_dim, M, max_ctx;
+  void* out;
+  int splits;
+  void* ws;
+};
+// the parts that these sizes run in when the workspace holds them all, and the workspace bytes of one of them
+int attention_tree_splits(int M, int n_q, int n_kv, int head_dim, int max_ctx);
+size_t attention_tree_part_bytes(int M, int n_q, int n_kv, int head_dim);
+void launch_attention_tree(const TreeAttn& a, hipStream_t st);
+
+// Log probabilities, entropy and the k largest of M rows of logits (dtype 0 fp16, 1 bf16, 2 fp32), each row in `splits`
+// slices (1: no workspace).
+constexpr int kLogprobsMaxK = 32;
+struct Logprobs {
+  const void* logits;
+  int dtype;
+  long long ld;
+  const int64_t* tokens;
+  float* logprobs;
+  float* entropy;
+  int64_t* top_ids;
+  float* top_logprobs;
+  int M, V, k;
+  int splits;
+  void* ws;
+};
+int token_logprobs_splits(int M, int V, int k, int dtype);
+size_t token_logprobs_ws_bytes(int M, int k, int splits);
+void launch_token_logprobs(const Logprobs& a, hipStream_t st);
+
+// Greedy walk down a verified tree and the move of its rows in n_caches consecutive paged caches.
+struct TreeAccept {
+  const int64_t* tokens;
+  const int32_t* parents;
+  const int64_t* picks;
+  long long picks_stride;
+  int M;
+  const int32_t* pos;
+  const int32_t* bt;
+  int n_bt;
+  void* kv;
+  int n_caches, n_pages, n_kv, log2P, head_dim;
+  int32_t* path;
+  int32_t* count;
+  int64_t* tok;
+};
+void launch_tree_accept(const TreeAccept& a, hipStream_t st);
+
 void launch_quantize_w4(const void* w, void* packed, void* sz, int N, int K, int log2G, int clip, hipStream_t st);
 
 
