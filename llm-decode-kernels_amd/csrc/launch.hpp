@@ -199,6 +199,7 @@ void launch_attention_tree(const TreeAttn& a, hipStream_t st);
 // Log probabilities, entropy and the k largest of M rows of logits (dtype 0 fp16, 1 bf16, 2 fp32), each row in `splits`
 // slices (1: no workspace).
 constexpr int kLogprobsMaxK = 32;
+constexpr int kLogprobsMaxSplits = 64;  // one per lane of the join
 struct Logprobs {
   const void* logits;
   int dtype;
@@ -213,6 +214,7 @@ struct Logprobs {
   void* ws;
 };
 int token_logprobs_splits(int M, int V, int k, int dtype);
+size_t logprobs_sums_bytes(int M, int splits);  // the workspace's first part; the slices' keys follow
 size_t token_logprobs_ws_bytes(int M, int k, int splits);
 void launch_token_logprobs(const Logprobs& a, hipStream_t st);
 
