@@ -369,7 +369,7 @@ int dk_qk_norm_rope_append_rows(const void* qkv, const void* q_w, const void* k_
  * block table or without a mapped page are neither read nor attended, and neither values nor NaN of a token reach a node
  * that does not attend it; *pos < 0: no token is attended. q: row m's heads at q + m q_stride (q_stride % 8 == 0), already
  * rotated; out [M, n_q * head_dim] fp16, not overlapping q. fp32 scores and softmax, scale 1/sqrt(head_dim). n_q / n_kv
- * in {1, 2, 4, 8}, M 1..1024. q, kc, vc and out 16-byte aligned.
+ * in {1, 2, 4, 8}, M 1..1024, max_ctx 1..2^30. q, kc, vc and out 16-byte aligned.
  * The context is split over workgroups whose fp32 partials meet in `workspace` (16-byte aligned, overlapping nothing
  * else) and are joined in split order by a second launch; dk_attention_tree_workspace_bytes gives what the sizes can use
  * (0: they do not split). A smaller workspace runs the most splits it holds, NULL runs unsplit. No counterpart in the

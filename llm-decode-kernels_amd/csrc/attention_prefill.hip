@@ -49,25 +49,6 @@ constexpr float kLazy = 8.0f;  // log2 units
 constexpr float kLift = 7.0f;  // p's exponent at the reference maximum
 static_assert(kLazy + kLift <= 15.0f, "p fits fp16");
 
-typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-typedef float f2 __attribute__((ext_vector_type(2)));
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-
-__device__ __forceinline__ f32x16 mfma32x32(h8 a, h8 b, f32x16 c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
-}
-
-// Keeps loads where they are written (no sinking to their first use).
-__device__ __forceinline__ void pf_fence() { asm volatile("" ::: "memory"); }
-
-// Transposing LDS read of 4 x 16-bit per lane.
-__device__ __forceinline__ u32x2 read_tr(const uint8_t* p) {
-  typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
-  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(p)));
-}
-
 // p - (float)(low / high half of an fp16 pair), one instruction each (the compiler converts and subtracts)
 __device__ __forceinline__ float minus_lo(float p, uint32_t pair) {
   float r;

@@ -1,5 +1,48 @@
-// Attention of the nodes of a drafted token tree over the paged cache: node i (row i of q) attends the committed tokens
-// [0, *pos) and the nodes (tokens *pos + j) whose bit is set in its mask row.
+// Attention of the nodes of a drafted token tree over the paged cache on gfx950: node i (row i of q) attends the committed
+// tokens [0, *pos) and the nodes (tokens *pos + j) whose bit is set in its mask row.
+//
+// A column is a (node, query head) pair of one kv head; a wave has 32 columns, so every column does work at any GQA ratio.
+// A workgroup has CW waves of columns, KVS times: group g of KVS takes the token blocks b (of BT tokens) with b % KVS == g,
+// so K / V in LDS once serve CW waves, and few columns still fill a workgroup. The context is further split over `splits`
+// workgroups in whole rounds of KVS blocks; the ends follow *pos, so one captured launch serves every position. The kv head
+// is the fastest grid index: with 8 of them each XCD's L2 holds one head's K / V for all its workgroups, and its partials
+// for the join.
+// K / V go from the cache straight into LDS (16-byte global-to-LDS loads), double-buffered: a round's loads go out between
+// the products of the round before it, spread, since a wave that issues them in a row waits for the other waves' to be taken
+// in (250 nodes at 32768 tokens: 155.9 -> 154.5 us).
+//
+// Per block, on v_mfma_f32_32x32x16_f16:
+//   * S^T = K . Q^T: A = 32 token rows of K from LDS, B = the wave's Q columns (registers). Lane (h, r) receives column r,
+//     tokens 8 q + 4 h + v: a column's scores, maximum, sum and output live in the lane pair (r, r + 32).
+//   * online softmax in the log2 domain, scale and log2 e in one multiplier; the reference maximum moves only when a block's
+//     maximum passes it by kTreeLazy (2^8). p = 2^(s - ref + kTreeLift) <= 2^15, so that what fp16 cannot hold of a small p
+//     is 2^-32 of the largest.
+//   * O^T += V^T . P^T: the score accumulator, rounded to fp16 to nearest, is the B operand as it is; V^T comes out of the
+//     row-major V tile through the transposing LDS read. One fp16 part of p instead of two: its 2^-11, unbiased and beside
+//     an output that is rounded to fp16 itself, against a half more of the products. The sum of the weights keeps fp32.
+//
+// Masks cost nothing where every column of the wave sees the whole block (all mapped, all before *pos). In the others a
+// lane holds its column's 64 token bits: mapped tokens inside the context, and for tokens from *pos on the node bits of the
+// mask row, shifted to the block. Scores of tokens that are not seen become -inf whatever K holds; their p is an exact 0.
+// Since 0 times NaN or infinity is NaN, check_v zeroes in LDS the V chunks of tokens that do not exist, and those with such
+// values in blocks that reach *pos; the latter are added at the end, value by value, for the columns that see their token.
+//
+// What bounds it (250 nodes at 32768 tokens, 8 x 4 heads of 128: 154 us against 114 at the rate of a large matrix product,
+// 0.87 PFLOP/s): a wave's products, softmax and load issue follow one another, at two waves per SIMD. Without the softmax
+// it takes 134, without the loads 122, without either 106, the products' own time. 64 nodes at 16001 take 36 (floor 14), of
+// which about 19 are products and the rest launch, first loads and 17 MB of partials. Small ones are launch, a chain of
+// dependent loads (position, page, K / V) and the join: 26 nodes at 4096 17, 5 at 300 9.5.
+// No gain: two halves of the workgroup half a block apart, so that one's softmax meets the other's products; deeper LDS
+// read-ahead; wave priorities; registers cut for three waves per SIMD.
+//
+// LDS: rows of 2 D bytes without padding. K chunk q (16 bytes) of row t at q ^ (t & 15) (D 128) or q ^ ((t >> 1) & 7) (D 64),
+// V in 64-byte units, unit u of row t at u ^ (t & 3) (D 128) or u ^ ((t >> 1) & 1) (D 64): reads fall in distinct banks
+// (the lane that loads a chunk picks the one that belongs at its place). The groups of a workgroup meet in LDS, the splits
+// in the workspace and a second launch, both in order.
+#include <limits.h>
+
+#include <type_traits>
+
 #include "common.hpp"
 #include "launch.hpp"
 #include "attn_common.hpp"
@@ -7,89 +50,607 @@
 namespace dk {
 namespace {
 
-constexpr int kTreeThreads = 256;
+// Reference maximum of a column that has seen no token: a finite stand-in for -infinity (no -inf - (-inf)).
+constexpr float kTreeNoMax = -1e30f;
+constexpr float kTreeLazy = 8.0f;  // log2 units
+constexpr float kTreeLift = 7.0f;  // p's exponent at the reference maximum
+static_assert(kTreeLazy + kTreeLift <= 15.0f, "p fits fp16");
 
-// One workgroup per (node, query head): scores of 256 tokens at a time into LDS, online softmax over the blocks, then
-// thread (g, d) adds the tokens t % G == g of dim d.
+constexpr int kTreeMaxSplits = 64;
+
+struct TreeArgs {
+  const f16* q;
+  long long q_stride;
+  const int64_t* mask;
+  const int32_t* pos;
+  const int32_t* bt;
+  const f16* kc;
+  const f16* vc;
+  int n_pages, log2P, n_kv, lhpg, M, cap;  // cap: tokens at and past it do not exist
+  int splits;
+  float c2;  // log2(e) / sqrt(D)
+  f16* out;  // [M, n_q D]
+  float4* part_o;   // [splits][n_kv][column waves][D / 8][64 lanes]: the accumulators as the lanes hold them
+  float2* part_ml;  // [splits][n_kv][column waves][32]: reference maximum, sum
+};
+
+// Tokens that exist: [0, ctx).
+__device__ __forceinline__ int tree_context(long long pos, int M, int cap) {
+  return pos < 0 ? 0 : (int)min(pos + M, (long long)cap);
+}
+
+// 16 bytes with a half that is no finite number.
+__device__ __forceinline__ bool has_nonfinite(u32x4 v) {
+  bool bad = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    bad = bad || (v[i] & 0x7C00u) == 0x7C00u || (v[i] & 0x7C000000u) == 0x7C000000u;
+  return bad;
+}
+
+template <int D, int CW, int KVS, int BT, bool UP>
+__global__ void __launch_bounds__(CW * KVS * kWave, 2)
+attn_tree_kernel(const TreeArgs a) {
+  constexpr int NTH = CW * KVS * kWave;      // threads
+  constexpr int CH = D / 8;                  // 16-byte chunks per K / V row
+  constexpr int RB = 2 * D;                  // bytes per row
+  constexpr int SB = BT * KVS;               // tokens per round (one block per group)
+  constexpr int LPT = SB * CH / NTH;         // 16-byte K (and V) loads per thread per round
+  constexpr int RPI = NTH / CH;              // token rows covered per load index
+  constexpr int NT = BT / 32, DT = D / 32;   // 32-token score tiles per block, 32-dim output tiles
+  constexpr int KS = D / 16;                 // k steps of the scores
+  static_assert(LPT * RPI == SB && RPI % 16 == 0, "staging covers a round");
+  constexpr int kTile = SB * RB;             // bytes of one K (or V) buffer
+  // K and V buffers as arrays of their own: the compiler then knows that the loads which fill one in flight touch no other.
+  // In the end the groups' accumulators, DT of their 4 DT rows in each.
+  static_assert((KVS - 1) * CW * kWave * 16 * DT <= kTile, "a merge row set fits a buffer");
+  __shared__ __align__(16) uint8_t s_k0[kTile], s_k1[kTile], s_v0[kTile], s_v1[kTile];
+  __shared__ float s_m[KVS > 1 ? KVS * CW * 32 : 1], s_l[KVS > 1 ? KVS * CW * 32 : 1];
+  // by block from the one of *pos on: the tokens that have V chunks which check_v took out
+  __shared__ unsigned long long s_bad[kTreeMaxNodes / BT + 1];
+
+  const int kvh = blockIdx.x, cb = blockIdx.y, split = blockIdx.z;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int grp = wave / CW, gw = wave % CW;  // group, and the wave's columns within it
+  const int r = lane & 31, h = lane >> 5;
+  const int P = 1 << a.log2P;
+  const long long pos = *a.pos;
+  const int ctx = tree_context(pos, a.M, a.cap);
+  const int tail_block = pos < ctx ? (int)(pos / BT) : INT_MAX / 2;  // the first block with tokens that not every column sees
+  // this split's rounds [r0, r1): the first nr % splits splits have one more
+  const unsigned nr = (ctx + SB - 1u) / SB, per = nr / (unsigned)a.splits, more = nr - per * (unsigned)a.splits;
+  const int r0 = (int)(split * per + min((unsigned)split, more)), r1 = r0 + (int)per + ((unsigned)split < more);
+  const int n_q = a.n_kv << a.lhpg, cols = a.M << a.lhpg;
+  // this lane's column: node m, head hd; columns past the last repeat it
+  const int col = (cb * CW + gw) * 32 + r;
+  const int cc = min(col, cols - 1);
+  const int m = cc >> a.lhpg, hd = (kvh << a.lhpg) + (cc & ((1 << a.lhpg) - 1));
+  h8 q[KS];
+  auto load_q = [&]() __attribute__((always_inline)) {
+    const f16* qh = a.q + (size_t)m * a.q_stride + (size_t)hd * D + 8 * h;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) q[s] = __builtin_bit_cast(h8, *reinterpret_cast<const u32x4*>(qh + 16 * s));
+  };
+
+  // Thread's share of a round: chunk tid % CH of token rows tid / CH + RPI i. Pages are looked up a round ahead of the K / V
+  // loads; tokens without a page, or past ctx, read a row that exists and are zeroed on the way to LDS. UP: a load
+  // instruction's rows lie in one page, lane i looks up the page of load i, and the base is a scalar.
+  const int sch = tid % CH, sr = tid / CH;
+  constexpr int RPW = kWave / CH;            // rows per load instruction of a wave
+  constexpr int NP = UP ? 1 : LPT;
+  const uint64_t page_bytes = (uint64_t)a.n_kv << a.log2P << (D == 128 ? 8 : 7);
+  const uint64_t head_bytes = (uint64_t)kvh << a.log2P << (D == 128 ? 8 : 7);
+  const uint8_t *kp = reinterpret_cast<const uint8_t*>(a.kc) + head_bytes, *vp = reinterpret_cast<const uint8_t*>(a.vc) + head_bytes;
+  // lane j of a load fills bytes [16 j, 16 j + 16) of the load's rows in LDS: with the chunk that belongs there
+  const uint32_t row_off = UP ? (lane / CH) * RB : 0;
+  const uint32_t k_place = row_off + 16 * (D == 128 ? sch ^ (sr & 15) : sch ^ ((sr >> 1) & 7));
+  const uint32_t v_place = row_off + 64 * ((sch >> 2) ^ (D == 128 ? sr & 3 : (sr >> 1) & 1)) + 16 * (sch & 3);
+  int pg[NP], vpg;        // pages of the loads; of token `lane` of the group's block
+  struct Rows {           // where a round's rows lie (UP: lane i's those of load i)
+    uint64_t base[NP];
+    uint32_t ok;          // bit i: this thread's row of load i exists
+  };
+  auto lookup = [&](int rnd) __attribute__((always_inline)) {
+    const int last = ctx - 1;
+    if constexpr (UP) {
+      pg[0] = a.bt[min(rnd * SB + RPW * wave + RPI * (lane % LPT), last) >> a.log2P];
+    } else {
+#pragma unroll
+      for (int i = 0; i < LPT; ++i) pg[i] = a.bt[min(rnd * SB + sr + RPI * i, last) >> a.log2P];
+    }
+  };
+  auto locate = [&](int rnd) __attribute__((always_inline)) {  // from the looked-up pages
+    Rows w;
+    w.ok = 0;
+    uint64_t maps = 0;
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int t = UP ? rnd * SB + RPW * wave + RPI * (lane % LPT) : rnd * SB + sr + RPI * i;
+      const bool mapped = (unsigned)pg[i] < (unsigned)a.n_pages;
+      w.base[i] = (uint64_t)(uint32_t)(mapped ? pg[i] : 0) * page_bytes + (uint32_t)((t & (P - 1)) * RB);
+      if constexpr (UP)
+        maps = __ballot(mapped);
+      else
+        w.ok |= t < ctx && mapped ? 1u << i : 0u;
+    }
+    if constexpr (UP) {
+#pragma unroll
+      for (int i = 0; i < LPT; ++i) w.ok |= rnd * SB + sr + RPI * i < ctx && (maps >> i & 1) ? 1u << i : 0u;
+    }
+    return w;
+  };
+  auto rows_of = [&](const Rows& w, int i) __attribute__((always_inline)) -> uint64_t {  // bytes ahead of the rows of load i
+    return UP ? (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(w.base[0] >> 32), i) << 32 |
+                    (uint32_t)__builtin_amdgcn_readlane((int)w.base[0], i)
+              : w.base[UP ? 0 : i];
+  };
+  auto fetch = [&](const uint8_t* cache, const Rows& w, int i, uint32_t place, uint8_t* buf) __attribute__((always_inline)) {  // load i of a round
+    typedef __attribute__((address_space(1))) const void* gptr;
+    typedef __attribute__((address_space(3))) void* lptr;
+    __builtin_amdgcn_global_load_lds((gptr)(cache + rows_of(w, i) + place), (lptr)(buf + (RPI * i + RPW * wave) * RB), 16, 0,
+                                     0);
+  };
+  // V chunks that must not meet a p of 0, looked over in LDS by the lane that loaded them: those of tokens that do not exist,
+  // and those with NaN or infinity of tokens that not every column sees
+  auto check_v = [&](int rnd, const Rows& w, uint8_t* buf) __attribute__((always_inline)) {
+    const bool tail = (rnd + 1) * (long long)SB > pos;  // uniform
+    if (!tail && __all(w.ok == (1u << LPT) - 1)) return;
+    asm volatile("");  // stays a branch
+#pragma unroll
+    for (int i = 0; i < LPT; ++i) {
+      const int row = sr + RPI * i;
+      u32x4* x = reinterpret_cast<u32x4*>(buf + row * RB + 16 * sch);
+      const bool ok = w.ok >> i & 1;
+      const int blk = rnd * KVS + row / BT - tail_block;
+      const bool bad = ok && tail && blk >= 0 && has_nonfinite(*x);
+      if (bad) atomicOr(&s_bad[blk], 1ull << (row % BT));
+      if (!ok || bad) *x = u32x4{0u, 0u, 0u, 0u};
+    }
+  };
+
+  float mref = kTreeNoMax, l = 0.f;  // the column's reference maximum (log2 units); this lane's half of its sum
+  f32x16 acc[DT];
+#pragma unroll
+  for (int t = 0; t < DT; ++t) acc[t] = f32x16{};
+
+  // LDS addresses: K row r of the group's block (chunk bits apart), and the lane's row of a transposing V read
+  const int krow = (grp * BT + r) * RB, ksw = D == 128 ? r & 15 : (r >> 1) & 7;
+  const int vt = 4 * h + ((lane & 15) >> 2);               // token (of 8) that the lane addresses
+  const int vd = 32 * ((lane >> 4) & 1) + 8 * (lane & 3);  // byte of its 4 dims within the 64-byte unit
+  const int vrow = (grp * BT + vt) * RB + vd, vsw = D == 128 ? vt & 3 : (vt >> 1) & 1;
+
+  // bits of tokens [t0, t0 + 64) that column node m sees by position and mask
+  auto seen_bits = [&](int t0) __attribute__((always_inline)) -> uint64_t {
+    const long long d = (long long)t0 - pos;  // node index of token t0
+    int m = cc;
+    asm volatile("" : "+v"(m));  // nothing of this is kept in registers around the loop
+    m >>= a.lhpg;
+    auto low = [](long long n) -> uint64_t { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1; };
+    if (a.mask == nullptr) return low(m + 1 - d);
+    const int W = (a.M + 63) >> 6;
+    const int64_t* row = a.mask + (size_t)m * W;
+    if (d <= 0) return d <= -64 ? ~0ull : low(-d) | (uint64_t)row[0] << (int)-d;
+    const int w = (int)(d >> 6), sh = (int)(d & 63);
+    uint64_t bits = w < W ? (uint64_t)row[w] >> sh : 0ull;
+    if (sh != 0 && w + 1 < W) bits |= (uint64_t)row[w + 1] << (64 - sh);
+    return bits;
+  };
+  auto block_start = [&](int rnd) __attribute__((always_inline)) { return (rnd * KVS + grp) * BT; };
+  auto lookup_block = [&](int rnd) __attribute__((always_inline)) { vpg = a.bt[min(block_start(rnd) + lane % BT, ctx - 1) >> a.log2P]; };
+
+  // ---- the three steps of a block
+  f32x16 sc[NT];  // scores
+  h8 ph[2 * NT];  // p in fp16: the B operand of the output's products
+  auto scores = [&](int rnd, const uint8_t* buf, auto after) __attribute__((always_inline)) {
+    const int t0 = block_start(rnd);
+    const uint64_t valid = __ballot(t0 + lane % BT < ctx && (unsigned)vpg < (unsigned)a.n_pages && lane < BT);
+    constexpr uint64_t kAll = BT == 64 ? ~0ull : (1ull << BT) - 1;
+    const bool masked = valid != kAll || t0 + BT > pos;  // uniform per wave
+    uint64_t vis = 0;
+    if (masked) vis = seen_bits(t0) & valid;
+#pragma unroll
+    for (int tt = 0; tt < NT; ++tt) sc[tt] = f32x16{};
+    // K fragments (k step f / NT, token tile f % NT), each read from LDS RA fragments ahead of its MFMA
+    constexpr int NF = KS * NT, RA = 2;
+    u32x4 ka[RA + 1];
+    int kat = krow + ((h ^ ksw) << 4);
+    asm volatile("" : "+v"(kat));  // (the chunks' places are worked out per block: eight of them held would not fit)
+    auto read_k = [&](int f) __attribute__((always_inline)) {
+      return *reinterpret_cast<const u32x4*>(buf + (f % NT) * 32 * RB + (kat ^ (f / NT << 5)));
+    };
+#pragma unroll
+    for (int f = 0; f < RA; ++f) ka[f] = read_k(f);
+#pragma unroll
+    for (int f = 0; f < NF; ++f) {
+      if (f + RA < NF) ka[(f + RA) % (RA + 1)] = read_k(f + RA);
+      sc[f % NT] = mfma32x32(__builtin_bit_cast(h8, ka[f % (RA + 1)]), q[f / NT], sc[f % NT]);
+      after(f);
+      __builtin_amdgcn_sched_barrier(0x7);
+    }
+    if (masked) {
+      asm volatile("");  // stays a branch
+#pragma unroll
+      for (int tt = 0; tt < NT; ++tt) {
+        const uint32_t bits = (uint32_t)(vis >> (32 * tt)) >> (4 * h);
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (!(bits & (1u << (8 * (i >> 2) + (i & 3))))) sc[tt][i] = -INFINITY;
+      }
+    }
+  };
+  auto softmax = [&]() __attribute__((always_inline)) {
+    float mx = sc[0][0];
+#pragma unroll
+    for (int tt = 0; tt < NT; ++tt) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[tt][i]);
+    }
+    mx = fmaxf(mx, __shfl_xor(mx, 32, kWave)) * a.c2;
+    const bool move = mx > mref + kTreeLazy;
+    if (__any(move)) {
+      const float mn = move ? mx : mref;
+      const float alpha = __builtin_amdgcn_exp2f(mref - mn);  // 1 for a column that stays
+      mref = mn;
+      l *= alpha;
+#pragma unroll
+      for (int t = 0; t < DT; ++t) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[t][i] *= alpha;
+      }
+    }
+    const float lift = kTreeLift - mref;
+    float ps[2] = {0.f, 0.f};
+#pragma unroll
+    for (int ks = 0; ks < 2 * NT; ++ks) {
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[ks >> 1][8 * (ks & 1) + e], a.c2, lift));
+        const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[ks >> 1][8 * (ks & 1) + e + 1], a.c2, lift));
+        ps[0] += p0;
+        ps[1] += p1;
+        const h2 hi = __builtin_convertvector(f2{p0, p1}, h2);
+        ph[ks][e] = hi[0];
+        ph[ks][e + 1] = hi[1];
+      }
+    }
+    l += ps[0] + ps[1];
+  };
+  auto output = [&](const uint8_t* buf) __attribute__((always_inline)) {
+    int vat = vrow + (vsw << 6);
+    asm volatile("" : "+v"(vat));
+#pragma unroll
+    for (int ks = 0; ks < 2 * NT; ++ks) {
+      h8 v[DT];
+#pragma unroll
+      for (int t = 0; t < DT; ++t) {
+        const uint8_t* src = buf + ks * 16 * RB + (vat ^ (t << 6));
+        const u32x2 x = read_tr(src), y = read_tr(src + 8 * RB);
+        v[t] = __builtin_bit_cast(h8, u32x4{x[0], x[1], y[0], y[1]});
+      }
+#pragma unroll
+      for (int t = 0; t < DT; ++t) acc[t] = mfma32x32(v[t], ph[ks], acc[t]);
+    }
+  };
+
+  // Round rnd, in buffer B: the loads of round rnd + 1 go out, straight into the other buffer (every wave finished reading
+  // it before the last barrier).
+  Rows rows;
+  auto start = [&](int j, uint8_t* k, uint8_t* v) __attribute__((always_inline)) {  // load j of K's and V's 2 LPT
+    if (j < LPT)
+      fetch(kp, rows, j, k_place, k);
+    else
+      fetch(vp, rows, j - LPT, v_place, v);
+  };
+  auto finish = [&](int rnd, uint8_t* v) __attribute__((always_inline)) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    check_v(rnd, rows, v);
+    __syncthreads();
+  };
+  auto round = [&](int rnd, auto B) __attribute__((always_inline)) {
+    constexpr bool odd = decltype(B)::value;
+    uint8_t *kb = odd ? s_k1 : s_k0, *vb = odd ? s_v1 : s_v0, *kn = odd ? s_k0 : s_k1, *vn = odd ? s_v0 : s_v1;
+    rows = locate(rnd + 1);  // past the end: rows that are never computed on
+    // spread over the products: issued in a row they hold a wave up while the other waves' are taken in
+    constexpr int NF = KS * NT, NL = 2 * LPT;
+    scores(rnd, kb, [&](int f) __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < NL; ++j)
+        if (f == j * NF / NL) start(j, kn, vn);
+    });
+    pf_fence();
+    lookup(rnd + 2);
+    lookup_block(rnd + 1);
+    pf_fence();
+    softmax();
+    output(vb);
+    pf_fence();
+    finish(rnd + 1, vn);
+  };
+  if (r0 < r1) {  // uniform
+    lookup(r0);
+    if (tid < kTreeMaxNodes / BT + 1) s_bad[tid] = 0ull;
+    rows = locate(r0);
+#pragma unroll
+    for (int j = 0; j < 2 * LPT; ++j) start(j, s_k0, s_v0);
+    pf_fence();  // (loads return in order: what is wanted later goes out later)
+    lookup_block(r0);
+    lookup(r0 + 1);
+    load_q();
+    pf_fence();
+    __syncthreads();  // (s_bad)
+    finish(r0, s_v0);
+    for (int rnd = r0; rnd < r1; rnd += 2) {
+      round(rnd, std::false_type{});
+      if (rnd + 1 < r1) round(rnd + 1, std::true_type{});
+    }
+    // ---- add_bad_rows: the chunks that check_v took out, from the cache, for the columns that see their token; its weight
+    // once more from q and k
+    for (int blk = max(tail_block, r0 * KVS); blk < min(r1 * KVS, (ctx + BT - 1) / BT); ++blk) {
+      if (blk % KVS != grp) continue;
+      unsigned long long bad = s_bad[blk - tail_block];
+      bad = __builtin_amdgcn_readfirstlane((uint32_t)bad) |
+            (unsigned long long)__builtin_amdgcn_readfirstlane((uint32_t)(bad >> 32)) << 32;
+      if (bad == 0) continue;
+      const uint64_t vis = seen_bits(blk * BT);
+      for (; bad != 0; bad &= bad - 1) {
+        const int i = __builtin_ctzll(bad), t = blk * BT + i;
+        const int page = a.bt[t >> a.log2P];  // a token in this set is mapped and inside the context
+        const size_t at = ((((size_t)page * a.n_kv + kvh) << a.log2P) + (t & (P - 1))) * D;
+        float dot = 0.f;  // this lane's half of the dims
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          const u32x4 k = *reinterpret_cast<const u32x4*>(a.kc + at + 16 * s + 8 * h);
+          const u32x4 qs = __builtin_bit_cast(u32x4, q[s]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) dot = dot2(as_f16x2(k[j]), as_f16x2(qs[j]), dot);
+        }
+        dot += __shfl_xor(dot, 32, kWave);
+        const float p = __builtin_amdgcn_exp2f(fmaf(dot, a.c2, kTreeLift - mref));
+        const bool see = (vis >> i) & 1;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+          const u32x4 x = *reinterpret_cast<const u32x4*>(a.vc + at + 8 * c);
+          if (!has_nonfinite(x) || !see) continue;
+          const f16x2 lo = as_f16x2(h ? x[2] : x[0]), hi = as_f16x2(h ? x[3] : x[1]);
+          const float f[4] = {(float)lo[0], (float)lo[1], (float)hi[0], (float)hi[1]};
+#pragma unroll
+          for (int v = 0; v < 4; ++v) acc[c / 4][4 * (c % 4) + v] = fmaf(p, f[v], acc[c / 4][4 * (c % 4) + v]);
+        }
+      }
+    }
+  }
+  l += __shfl_xor(l, 32, kWave);
+  // ---- merge: groups 1 .. KVS - 1 leave maximum and sum per column and the accumulator per lane in LDS (over the K / V
+  // buffers, which every wave has finished reading at the last barrier); group 0 merges them in group order
+  if constexpr (KVS > 1) {
+    auto merge_row = [&](int row, int g) -> float4* {  // row (of 4 DT) of group g's accumulators, this wave's columns
+      uint8_t* buf = row / DT == 0 ? s_k0 : row / DT == 1 ? s_k1 : row / DT == 2 ? s_v0 : s_v1;
+      return reinterpret_cast<float4*>(buf) + ((row % DT * (KVS - 1) + g - 1) * CW + gw) * kWave + lane;
+    };
+    if (h == 0) {
+      s_m[(grp * CW + gw) * 32 + r] = mref;
+      s_l[(grp * CW + gw) * 32 + r] = l;
+    }
+    if (grp > 0) {
+#pragma unroll
+      for (int i = 0; i < 4 * DT; ++i)
+        *merge_row(i, grp) = float4{acc[i / 4][4 * (i % 4)], acc[i / 4][4 * (i % 4) + 1], acc[i / 4][4 * (i % 4) + 2],
+                                    acc[i / 4][4 * (i % 4) + 3]};
+    }
+    __syncthreads();
+    if (grp > 0) return;  // uniform per wave; no barrier follows
+    float mx = mref;
+#pragma unroll
+    for (int k = 1; k < KVS; ++k) mx = fmaxf(mx, s_m[(k * CW + gw) * 32 + r]);
+    const float w0 = __builtin_amdgcn_exp2f(mref - mx);  // a group that saw no token weighs 0 beside one that did
+    l *= w0;
+#pragma unroll
+    for (int t = 0; t < DT; ++t) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[t][i] *= w0;
+    }
+#pragma unroll
+    for (int k = 1; k < KVS; ++k) {
+      const float wk = __builtin_amdgcn_exp2f(s_m[(k * CW + gw) * 32 + r] - mx);
+      l = fmaf(wk, s_l[(k * CW + gw) * 32 + r], l);
+#pragma unroll
+      for (int i = 0; i < 4 * DT; ++i) {
+        const float4 o = *merge_row(i, k);
+        f32x16& d = acc[i / 4];
+        d[4 * (i % 4)] = fmaf(wk, o.x, d[4 * (i % 4)]);
+        d[4 * (i % 4) + 1] = fmaf(wk, o.y, d[4 * (i % 4) + 1]);
+        d[4 * (i % 4) + 2] = fmaf(wk, o.z, d[4 * (i % 4) + 2]);
+        d[4 * (i % 4) + 3] = fmaf(wk, o.w, d[4 * (i % 4) + 3]);
+      }
+    }
+    mref = mx;
+  }
+  // ---- output: acc[t][4 q + v] = O[column r][dim 32 t + 8 q + 4 h + v]
+  if (col >= cols) return;
+  const size_t at = (size_t)m * n_q + hd;
+  if (a.splits == 1) {
+    const float inv = l == 0.f ? 0.f : 1.0f / l;  // a NaN stays
+    f16* dst = a.out + at * D + 4 * h;
+#pragma unroll
+    for (int t = 0; t < DT; ++t) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f16 o0 = (f16)(acc[t][4 * i] * inv), o1 = (f16)(acc[t][4 * i + 1] * inv);
+        const f16 o2 = (f16)(acc[t][4 * i + 2] * inv), o3 = (f16)(acc[t][4 * i + 3] * inv);
+        *reinterpret_cast<u32x2*>(dst + 32 * t + 8 * i) = u32x2{as_u32(f16x2{o0, o1}), as_u32(f16x2{o2, o3})};
+      }
+    }
+    return;
+  }
+  const int waves = (cols + 31) >> 5;
+  const size_t part = ((size_t)split * a.n_kv + kvh) * waves + (cb * CW + gw);
+  if (h == 0) a.part_ml[part * 32 + r] = float2{mref, l};
+  if (r0 >= r1) return;  // a split without tokens: the join reads no accumulator of it
+  float4* dst = a.part_o + part * (DT * 4 * kWave);  // uniform per wave
+#pragma unroll
+  for (int t = 0; t < DT; ++t) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      store_through16(dst, (uint32_t)(((4 * t + i) * kWave + lane) * 16),
+                      __builtin_bit_cast(u32x4, f4{acc[t][4 * i], acc[t][4 * i + 1], acc[t][4 * i + 2], acc[t][4 * i + 3]}));
+  }
+}
+
+// Joins the splits of a column in split order. A workgroup takes kRows of the D / 8 accumulator rows of one wave's 32
+// columns, a thread one float4 of it (4 dims of a column). The first kBatch partials are loaded ahead of the maxima and
+// sums, so that one memory round trip covers both; the accumulator of a split that saw no token was not written and is
+// dropped.
+constexpr int kTreeJoinRows = 4;
 template <int D>
-__global__ void __launch_bounds__(kTreeThreads)
-tree_attn_simple_kernel(const f16* __restrict__ q, long long q_stride, const int64_t* __restrict__ mask,
-                        const int32_t* __restrict__ pos_ptr, const int32_t* __restrict__ bt, int n_bt,
-                        const f16* __restrict__ kc, const f16* __restrict__ vc, int n_pages, int log2P, int hpg,
-                        int n_kv, int M, int max_ctx, float scale, f16* __restrict__ out) {
-  constexpr int G = kTreeThreads / D;
-  __shared__ float s_p[kTreeThreads], s_red[kTreeThreads / kWave], s_acc[G][D];
-  __shared__ int s_pg[kTreeThreads];
-  const int head = blockIdx.x, i = blockIdx.y, kvh = head / hpg, tid = threadIdx.x, W = (M + 63) >> 6;
-  const long long pos = *pos_ptr, cap = min((long long)max_ctx, (long long)n_bt << log2P);
-  const int ctx = pos < 0 ? 0 : (int)min(pos + M, cap);
-  const f16* qh = q + (size_t)i * q_stride + (size_t)head * D;
-  const int g = tid / D, d = tid % D;
-  float m = -INFINITY, l = 0.f, acc = 0.f;
-  for (int t0 = 0; t0 < ctx; t0 += kTreeThreads) {
-    const int t = t0 + tid;
-    bool see = t < ctx;
-    if (see && t >= pos) {
-      const int j = (int)(t - pos);
-      see = mask ? (mask[(size_t)i * W + (j >> 6)] >> (j & 63)) & 1 : j <= i;
+__global__ void __launch_bounds__(kTreeJoinRows * kWave)
+attn_tree_join_kernel(const float4* __restrict__ part_o, const float2* __restrict__ part_ml, int cols, int lhpg, int n_kv,
+                      int splits, f16* __restrict__ out) {
+  constexpr int kRows = kTreeJoinRows, kBatch = 8, kGroups = 2 * kRows;  // kGroups threads share a column's maxima and sums
+  __shared__ float s_w[kTreeMaxSplits][32];          // a split's weight in a column, -1 where it saw no token
+  __shared__ float s_l[32];
+  const int tid = threadIdx.x, lane = tid & 63, r = lane & 31, h = lane >> 5;
+  const int kvh = blockIdx.x, row = (blockIdx.y % (D / 8 / kRows)) * kRows + (tid >> 6);
+  const int waves = gridDim.y / (D / 8 / kRows), cw = blockIdx.y / (D / 8 / kRows), col = cw * 32 + r;
+  const bool live = col < cols;
+  const size_t wave = (size_t)kvh * waves + cw, wstep = (size_t)n_kv * waves;  // per split
+  const float4* src = part_o + (wave * (D / 8) + row) * kWave + lane;
+  const size_t step = wstep * (D / 8) * kWave;
+  float4 p[kBatch];
+  auto load = [&](int s0) {
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) p[k] = src[(size_t)min(s0 + k, splits - 1) * step];
+  };
+  if (live) load(0);
+  // weights: thread (column c, g) takes splits g, g + 8, ...
+  {
+    const int c = tid / kGroups, g = tid % kGroups;
+    constexpr int kMl = kTreeMaxSplits / kGroups;
+    float2 ml[kMl];
+    float mx = kTreeNoMax;
+#pragma unroll
+    for (int j = 0; j < kMl; ++j) {
+      const int s = g + kGroups * j;
+      ml[j] = s < splits ? part_ml[((size_t)s * wstep + wave) * 32 + c] : float2{kTreeNoMax, 0.f};
+      mx = fmaxf(mx, ml[j].x);
     }
-    const int page = see ? bt[t >> log2P] : -1;
-    see = see && (unsigned)page < (unsigned)n_pages;
-    float sc = -INFINITY;
-    if (see) {
-      const f16* kr = kc + ((((size_t)page * n_kv + kvh) << log2P) + (t & ((1 << log2P) - 1))) * D;
-      float a = 0.f;
-      for (int e = 0; e < D; ++e) a = fmaf((float)qh[e], (float)kr[e], a);
-      sc = a * scale;
+    mx = group_max<kGroups>(mx);
+    float L = 0.f;
+#pragma unroll
+    for (int j = 0; j < kMl; ++j) {
+      const int s = g + kGroups * j;
+      const bool saw = ml[j].x != kTreeNoMax || ml[j].y != 0.f;  // (a NaN sum counts)
+      const float w = __builtin_amdgcn_exp2f(ml[j].x - mx);
+      L = saw ? fmaf(w, ml[j].y, L) : L;
+      if (s < splits) s_w[s][c] = saw ? w : -1.f;
     }
-    s_pg[tid] = see ? page : -1;
-    const float wm = group_max<64>(sc);
-    if ((tid & 63) == 0) s_red[tid >> 6] = wm;
-    __syncthreads();
-    float mn = m;
-    for (int w = 0; w < kTreeThreads / kWave; ++w) mn = fmaxf(mn, s_red[w]);
-    const float alpha = mn == -INFINITY ? 0.f : expf(m - mn);
-    const float p = see ? expf(sc - mn) : 0.f;
-    s_p[tid] = p;
-    m = mn;
-    const float ws = group_sum<64>(p);
-    __syncthreads();
-    if ((tid & 63) == 0) s_red[tid >> 6] = ws;
-    __syncthreads();
-    l *= alpha;
-    for (int w = 0; w < kTreeThreads / kWave; ++w) l += s_red[w];
-    acc *= alpha;
-    for (int k = g; k < kTreeThreads; k += G) {
-      if (s_pg[k] < 0) continue;
-      const f16* vr = vc + ((((size_t)s_pg[k] * n_kv + kvh) << log2P) + ((t0 + k) & ((1 << log2P) - 1))) * D;
-      acc = fmaf(s_p[k], (float)vr[d], acc);
-    }
-    __syncthreads();
+    L = group_sum<kGroups>(L);
+    if (g == 0) s_l[c] = L;
   }
-  s_acc[g][d] = acc;
   __syncthreads();
-  if (g == 0) {
-    for (int k = 1; k < G; ++k) acc += s_acc[k][d];
-    out[((size_t)i * n_kv * hpg + head) * D + d] = (f16)(l == 0.f ? 0.f : acc / l);
+  if (!live) return;
+  float4 o = {0.f, 0.f, 0.f, 0.f};
+  for (int s0 = 0; s0 < splits; s0 += kBatch) {
+    if (s0 > 0) load(s0);
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const float w = s0 + k < splits ? s_w[s0 + k][r] : -1.f;
+      if (w < 0.f) continue;
+      o.x = fmaf(w, p[k].x, o.x);
+      o.y = fmaf(w, p[k].y, o.y);
+      o.z = fmaf(w, p[k].z, o.z);
+      o.w = fmaf(w, p[k].w, o.w);
+    }
   }
+  const float L = s_l[r], inv = L == 0.f ? 0.f : 1.0f / L;  // a NaN stays
+  const int m = col >> lhpg, hd = (kvh << lhpg) + (col & ((1 << lhpg) - 1));
+  f16* dst = out + ((size_t)m * (n_kv << lhpg) + hd) * D + 32 * (row >> 2) + 8 * (row & 3) + 4 * h;
+  *reinterpret_cast<u32x2*>(dst) =
+      u32x2{as_u32(f16x2{(f16)(o.x * inv), (f16)(o.y * inv)}), as_u32(f16x2{(f16)(o.z * inv), (f16)(o.w * inv)})};
+}
+
+// Workgroup shape (CW, KVS, BT) by the column waves of a kv head and the longest context. Each shape's time against the best
+// of six, geometric mean and worst over 210 cases (1-250 nodes, six head layouts, contexts of 200 to 32000):
+//   D 128   (4,2,32)  1.02 / 1.20 to eight waves, 1.00 beyond at 4000 tokens, 1.08 / 1.13 beyond at 16000 and 32000
+//           (8,1,64)  1.01 / 1.14 to 1000 tokens, 1.06 - 1.15 / 1.38 in the rest, but 1.00 / 1.03 beyond eight waves at 16000
+//           (4,2,64)  1.06 - 1.23 / 1.61, but ahead of (4,2,32) at seven and eight waves: 25.1 against 26.1 us at 8000
+//                     tokens, 36.3 : 38.1 at 16001, 56.5 : 61.0 at 32000 (8 kv heads; (8,1,64) 28.5, 38.3, 57.7)
+//   D  64   (4,1,64)  1.01 / 1.14 to 1000 tokens, 1.08 - 1.17 / 1.31 at more
+//           (2,4,32)  1.06 / 1.15 to 1000 tokens, 1.02 / 1.17 at more and to eight waves, 1.04 - 1.19 / 1.35 beyond
+//           (4,2,64)  1.06 / 1.15, 1.06 / 1.20, 1.02 - 1.05 / 1.22
+struct TreeShape {
+  int cw, kvs, bt;
+};
+TreeShape tree_shape(int M, int n_q, int n_kv, int D, int max_ctx) {
+  const int waves = (M * (n_q / n_kv) + 31) / 32;
+  if (D == 128) {
+    if (max_ctx < 8000 || waves <= 4) return TreeShape{4, 2, 32};
+    return waves > 8 ? TreeShape{8, 1, 64} : TreeShape{4, 2, 64};
+  }
+  return max_ctx <= 2048 ? TreeShape{4, 1, 64} : waves > 8 ? TreeShape{4, 2, 64} : TreeShape{2, 4, 32};
 }
 
 }  // namespace
 
-int attention_tree_splits(int, int, int, int, int) { return 1; }
-size_t attention_tree_part_bytes(int M, int n_q, int, int head_dim) { return (size_t)M * n_q * (head_dim + 2) * 4; }
+// One workgroup per CU, in splits of equal length.
+int attention_tree_splits(int M, int n_q, int n_kv, int D, int max_ctx) {
+  const TreeShape s = tree_shape(M, n_q, n_kv, D, max_ctx);
+  const int blocks = (M * (n_q / n_kv) + 32 * s.cw - 1) / (32 * s.cw), round = s.bt * s.kvs;
+  const int rounds = max_ctx / round + (max_ctx % round != 0);
+  int want = 256 / (blocks * n_kv);
+  want = want < 1 ? 1 : want > kTreeMaxSplits ? kTreeMaxSplits : want;
+  const int per = rounds / want + (rounds % want != 0);
+  return (rounds + per - 1) / per;
+}
+size_t attention_tree_part_bytes(int M, int n_q, int n_kv, int head_dim) {
+  return (size_t)n_kv * ((M * (n_q / n_kv) + 31) / 32) * 32 * (head_dim + 2) * sizeof(float);
+}
+
+template <int D, int CW, int KVS, int BT>
+static void launch_tree_shape(const TreeArgs& a, int cols, hipStream_t st) {
+  const dim3 grid(a.n_kv, (cols + 32 * CW - 1) / (32 * CW), a.splits), block(CW * KVS * kWave);
+  if ((1 << a.log2P) >= 512 / D)
+    hipLaunchKernelGGL((attn_tree_kernel<D, CW, KVS, BT, true>), grid, block, 0, st, a);
+  else
+    hipLaunchKernelGGL((attn_tree_kernel<D, CW, KVS, BT, false>), grid, block, 0, st, a);
+}
+
+template <int D>
+static void launch_tree(const TreeAttn& t, hipStream_t st) {
+  int lhpg = 0;
+  while ((t.n_kv << lhpg) < t.n_q) ++lhpg;
+  const int cols = t.M << lhpg, waves = (cols + 31) / 32;
+  float4* part_o = (float4*)t.ws;
+  TreeArgs a{(const f16*)t.q, t.q_stride, t.mask, t.pos, t.bt, (const f16*)t.kc, (const f16*)t.vc, t.n_pages, t.log2P,
+             t.n_kv, lhpg, t.M, (int)min((long long)t.max_ctx, (long long)t.n_bt << t.log2P), t.splits,
+             (float)(1.4426950408889634 / sqrt((double)D)), (f16*)t.out, part_o,
+             (float2*)(part_o + (size_t)t.splits * t.n_kv * waves * 8 * D)};
+  const TreeShape s = tree_shape(t.M, t.n_q, t.n_kv, D, t.max_ctx);
+  if constexpr (D == 128) {
+    if (s.cw == 8)
+      launch_tree_shape<D, 8, 1, 64>(a, cols, st);
+    else if (s.bt == 64)
+      launch_tree_shape<D, 4, 2, 64>(a, cols, st);
+    else
+      launch_tree_shape<D, 4, 2, 32>(a, cols, st);
+  } else {
+    if (s.kvs == 1)
+      launch_tree_shape<D, 4, 1, 64>(a, cols, st);
+    else if (s.cw == 4)
+      launch_tree_shape<D, 4, 2, 64>(a, cols, st);
+    else
+      launch_tree_shape<D, 2, 4, 32>(a, cols, st);
+  }
+  if (t.splits > 1)
+    hipLaunchKernelGGL(attn_tree_join_kernel<D>, dim3(t.n_kv, waves * (D / 8 / kTreeJoinRows)), dim3(kTreeJoinRows * kWave), 0, st, part_o, a.part_ml,
+                       cols, lhpg, t.n_kv, t.splits, (f16*)t.out);
+}
 
 void launch_attention_tree(const TreeAttn& a, hipStream_t st) {
-  const float scale = 1.0f / sqrtf((float)a.head_dim);
-  auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(a.n_q, a.M), dim3(kTreeThreads), 0, st, (const f16*)a.q, a.q_stride, a.mask, a.pos,
-                       a.bt, a.n_bt, (const f16*)a.kc, (const f16*)a.vc, a.n_pages, a.log2P, a.n_q / a.n_kv, a.n_kv, a.M,
-                       a.max_ctx, scale, (f16*)a.out);
-  };
   if (a.head_dim == 64)
-    go(tree_attn_simple_kernel<64>);
+    launch_tree<64>(a, st);
   else
-    go(tree_attn_simple_kernel<128>);
+    launch_tree<128>(a, st);
 }
 
 }  // namespace dk

@@ -1,5 +1,5 @@
 // Decode-attention helpers shared by the split kernels, the prefill kernel and the o projection's combine prologue:
-// split count, RoPE of a 16-byte slice, and the 16 x 16 f16 MFMA tile helpers.
+// split count, RoPE of a 16-byte slice, and the 16 x 16 and 32 x 32 f16 MFMA tile helpers.
 #pragma once
 #include "common.hpp"
 
@@ -53,6 +53,25 @@ __device__ __forceinline__ float rows_max(float v) {
 __device__ __forceinline__ float rows_sum(float v) {
   v += __shfl_xor(v, 16, kWave);
   return v + __shfl_xor(v, 32, kWave);
+}
+
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef float f2 __attribute__((ext_vector_type(2)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ f32x16 mfma32x32(h8 a, h8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
+// Keeps loads where they are written (no sinking to their first use).
+__device__ __forceinline__ void pf_fence() { asm volatile("" ::: "memory"); }
+
+// Transposing LDS read of 4 x 16-bit per lane.
+__device__ __forceinline__ u32x2 read_tr(const uint8_t* p) {
+  typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(p)));
 }
 
 template <int VD>

@@ -740,7 +740,8 @@ int dk_qk_norm_rope_append_rows(const void* qkv, const void* q_w, const void* k_
 static bool tree_attn_sizes(int M, int n_q, int n_kv, int head_dim, int max_ctx) {
   if (M < 1 || M > dk::kTreeMaxNodes || n_kv < 1 || n_kv > 65535 || n_q < 1 || n_q % n_kv != 0) return false;
   const int hpg = n_q / n_kv;
-  return (hpg == 1 || hpg == 2 || hpg == 4 || hpg == 8) && (head_dim == 64 || head_dim == 128) && max_ctx >= 1;
+  return (hpg == 1 || hpg == 2 || hpg == 4 || hpg == 8) && (head_dim == 64 || head_dim == 128) && max_ctx >= 1 &&
+         max_ctx <= dk::kTreeMaxCtx;
 }
 
 size_t dk_attention_tree_workspace_bytes(int M, int n_q, int n_kv, int head_dim, int max_ctx) {
@@ -757,7 +758,8 @@ int dk_attention_tree(const void* q, long long q_stride, const int64_t* mask, co
     return fail(DK_ERR_SHAPE, "attention_tree: head_dim must be 64 or 128, got %d", head_dim);
   if (M < 1 || M > dk::kTreeMaxNodes)
     return fail(DK_ERR_SHAPE, "attention_tree: M must be 1..%d, got %d", dk::kTreeMaxNodes, M);
-  if (max_ctx < 1) return fail(DK_ERR_DOMAIN, "attention_tree: max_ctx must be >= 1, got %d", max_ctx);
+  if (max_ctx < 1 || max_ctx > dk::kTreeMaxCtx)
+    return fail(DK_ERR_DOMAIN, "attention_tree: max_ctx must be 1..%d, got %d", dk::kTreeMaxCtx, max_ctx);
   if (n_kv > 65535) return fail(DK_ERR_SHAPE, "attention_tree: too many kv heads");
   if (!tree_attn_sizes(M, n_q, n_kv, head_dim, max_ctx))
     return fail(DK_ERR_SHAPE, "heads-per-group must be 1/2/4/8 (n_q=%d n_kv=%d)", n_q, n_kv);

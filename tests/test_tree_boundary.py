@@ -49,6 +49,7 @@ TREE = dict(q=AT[0], q_stride=1024, mask=AT[1], pos=AT[2], bt=AT[3], n_bt=8, kc=
 @pytest.mark.parametrize("kw,code,msg", [
     (dict(q=None), 1, "null"), (dict(out=None), 1, "null"), (dict(pos=None), 1, "null"), (dict(head_dim=32), 3, "head_dim"),
     (dict(M=0), 3, "M must be 1..1024"), (dict(M=1025), 3, "M must be 1..1024"), (dict(max_ctx=0), 4, "max_ctx"),
+    (dict(max_ctx=(1 << 30) + 1), 4, "max_ctx must be 1..1073741824"),
     (dict(n_q=6), 3, "heads-per-group"), (dict(n_q=32), 3, "heads-per-group"), (dict(n_kv=0), 3, "heads-per-group"),
     (dict(n_kv=65536, n_q=65536), 3, "too many"), (dict(page=24), 4, "power of two"), (dict(n_bt=0), 3, "empty"),
     (dict(n_pages=0), 3, "empty"), (dict(q_stride=1020), 3, "q_stride"), (dict(q_stride=512), 3, "q_stride"),
