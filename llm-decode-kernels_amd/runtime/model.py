@@ -34,6 +34,7 @@ import torch
 
 from . import ext
 from .quant import QuantLinear
+from .tree import tree_layout
 
 PKG = Path(__file__).resolve().parents[1]
 
@@ -700,6 +701,26 @@ class Model:
             lin._il = (interleave_halves(lin.packed), interleave_halves(lin.sz))
         return lin._il
 
+    def _layers_rows(self, B, attend):
+        """All layers over the rows of B["tok"]; attend(li, kc, vc) rotates and appends B["qkv"] and leaves B["attn"].
+        Returns (x, xn, delta): the residual rows, a buffer for the normed ones and the last projection's delta."""
+        x, xn, delta = B["x"], B["xn"], None
+        for li, lw in enumerate(self.layers):
+            if li == 0:
+                self.K.rmsnorm_rows(self.emb, B["tok"], None, lw["ln1"], x, xn, self.eps)
+            else:
+                self._add_norm_rows(x, delta, lw["ln1"], xn)
+            self.gemm(lw["qkv"], xn, B["qkv"])
+            attend(li, self.kv[li, 0], self.kv[li, 1])
+            self._add_norm_rows(x, self._proj_delta(lw["o"], B["attn"], B["o"]), lw["ln2"], xn)
+            if lw["gu"].quant:
+                self.gemm(lw["gu"], xn, B["act"], epilogue=1)
+            else:
+                gu = torch.mm(xn, lw["gu"].w.t())
+                B["act"].copy_(torch.nn.functional.silu(gu[:, : self.I].float()).half() * gu[:, self.I:])
+            delta = self._proj_delta(lw["down"], B["act"], B["down"])
+        return x, xn, delta
+
     def prefill(self, tokens):
         """Process a prompt in one pass: every projection of the M tokens is one W4A16 GEMM, rope/append and the
         residual + RMSNorm run over all rows, attention is causal over the paged cache (row m at position pos + m).
@@ -718,24 +739,12 @@ class Model:
             raise RuntimeError(f"prefill: context {start + M} exceeds max_ctx {self.cfg.max_ctx}")
         B = self._prefill_buffers(M)
         B["tok"].copy_(toks)
-        x, xn, delta = B["x"], B["xn"], None
-        eps = self.eps
-        for li, lw in enumerate(self.layers):
-            if li == 0:
-                self.K.rmsnorm_rows(self.emb, B["tok"], None, lw["ln1"], x, xn, eps)
-            else:
-                self._add_norm_rows(x, delta, lw["ln1"], xn)
-            self.gemm(lw["qkv"], xn, B["qkv"])
-            kc, vc = self.kv[li, 0], self.kv[li, 1]
+
+        def attend(li, kc, vc):
             self.K.rope_append_rows(B["qkv"], self.cos, self.sin, self.pos, self.bt, kc, vc, self.n_q, self.n_kv)
             self.K.attention_prefill(B["qkv"], self.pos, self.bt, kc, vc, self.n_q, self.n_kv, start + M, B["attn"])
-            self._add_norm_rows(x, self._proj_delta(lw["o"], B["attn"], B["o"]), lw["ln2"], xn)
-            if lw["gu"].quant:
-                self.gemm(lw["gu"], xn, B["act"], epilogue=1)
-            else:
-                gu = torch.mm(xn, lw["gu"].w.t())
-                B["act"].copy_(torch.nn.functional.silu(gu[:, : self.I].float()).half() * gu[:, self.I:])
-            delta = self._proj_delta(lw["down"], B["act"], B["down"])
+
+        x, xn, delta = self._layers_rows(B, attend)
         last = slice(M - 1, M)
         self._add_norm_rows(x[last], delta[:, last] if delta.dtype == torch.float32 else delta[last], self.norm_f,
                             xn[last])
@@ -744,6 +753,70 @@ class Model:
             self.pos.add_(M - 1)
         self.pick_next()
         self.host_pos = start + M
+
+    def _tree_buffers(self, M, max_ctx):
+        """Logits of M rows, the results that verify reads back (one int32 buffer) and the split workspace of its kernels."""
+        need = max(self.K.attention_tree_workspace_bytes(M, self.n_q, self.n_kv, self.D, max_ctx),
+                   self.K.token_logprobs_workspace_bytes(M, self.V, 1))
+        if getattr(self, "_tree_rows", 0) < M:
+            self._tree_rows = M
+            self._tree_logits = torch.empty(M, self.V, dtype=torch.half, device=self.cfg.device)
+            self._tree_results = torch.empty(4 * M + 1, dtype=torch.int32, device=self.cfg.device)
+        if need and (getattr(self, "_tree_ws", None) is None or self._tree_ws.numel() < need):
+            self._tree_ws = torch.empty(need, dtype=torch.uint8, device=self.cfg.device)
+        return self._tree_logits[:M], self._tree_results[: 4 * M + 1], getattr(self, "_tree_ws", None)
+
+    def verify(self, draft, parents=None):
+        """One step of speculative decoding: the pending token and n drafted ones run through the model in one pass, as
+        the nodes of a tree, and the path that greedy decoding takes is kept. draft: n token ids (0 .. 1023 of them),
+        nodes 1 .. n behind node 0, the pending token; parents[i] in 0 .. i: the node that draft[i] follows (None: each
+        follows the one before it). Returns (tokens, logprobs): the tokens that greedy decoding emits from here, the
+        accepted drafts and the pick after the last of them (at least one token), with their log probabilities.
+        Leaves the state of as many steps: their cache rows, the logits of the last one, tok = tokens[-1] and
+        pos += len(tokens), up to the summation order of the projections, as prefill does. The cache needs room for all
+        n + 1 nodes."""
+        ids = torch.as_tensor(draft, dtype=torch.long).reshape(-1).cpu()
+        M = ids.numel() + 1
+        if M > 1 and (int(ids.min()) < 0 or int(ids.max()) >= self.V):
+            raise ValueError(f"verify: token ids must lie in [0, {self.V})")
+        chain = parents is None
+        parents = list(range(M - 1)) if chain else torch.as_tensor(parents).reshape(-1).tolist()
+        if len(parents) != M - 1:
+            raise ValueError(f"verify: {M - 1} drafted tokens with {len(parents)} parents")
+        up, depth, mask = tree_layout(parents)
+        start = self.host_pos
+        if start + M > self.cfg.max_ctx:
+            raise RuntimeError(f"verify: context {start + M} exceeds max_ctx {self.cfg.max_ctx}")
+        # one upload: the ids, parents and depths, mask words
+        sent = torch.cat([torch.zeros(1, dtype=torch.long), ids, torch.cat([up, depth]).view(torch.long),
+                          mask.reshape(-1)]).to(self.cfg.device)
+        up, depth = sent[M:2 * M].view(torch.int32).view(2, M)
+        mask = sent[2 * M:].view(M, -1)
+        B = self._prefill_buffers(M)
+        B["tok"].copy_(sent[:M])
+        B["tok"][:1].copy_(self.tok)
+        logits, res, ws = self._tree_buffers(M, start + M)
+        q = B["qkv"][:, : self.n_q * self.D]
+
+        def attend(li, kc, vc):
+            self.K.qk_norm_rope_append_rows(B["qkv"], None, None, self.eps, self.cos, self.sin, self.pos,
+                                            None if chain else depth, self.bt, kc, vc, self.n_q, self.n_kv)
+            self.K.attention_tree(q, None if chain else mask, self.pos, self.bt, kc, vc, start + M, B["attn"], ws)
+
+        x, xn, delta = self._layers_rows(B, attend)
+        self._add_norm_rows(x, delta, self.norm_f, xn)
+        self.gemm(self.lm_head, xn, logits)
+        picks, path, count = res[: 2 * M].view(torch.long), res[2 * M:3 * M], res[3 * M:3 * M + 1]
+        logp = res[3 * M + 1:].view(torch.float32)
+        self.K.token_logprobs(logits, None, None, None, picks.view(M, 1), logp.view(M, 1), ws)
+        self.K.tree_accept(B["tok"], up, picks, self.pos, self.bt, self.kv, path, count, self.tok)
+        self.pos.add_(count)
+        res = res.cpu()  # one read back, after which the host knows the position
+        n = int(res[3 * M])
+        path = res[2 * M:2 * M + n].long()
+        self.logits.copy_(logits[int(path[-1])])
+        self.host_pos = start + n
+        return res[: 2 * M].view(torch.long)[path].tolist(), res[3 * M + 1:].view(torch.float32)[path].tolist()
 
     def generate(self, prompt, n_new, use_graph=True, prefill=False):
         """Greedy decoding from position 0 (runtime/model.py:278-286): the prompt teacher-forced (or prefilled in one
