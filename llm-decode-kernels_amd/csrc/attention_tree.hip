@@ -389,8 +389,8 @@ attn_tree_kernel(const TreeArgs a) {
     for (int blk = max(tail_block, r0 * KVS); blk < min(r1 * KVS, (ctx + BT - 1) / BT); ++blk) {
       if (blk % KVS != grp) continue;
       unsigned long long bad = s_bad[blk - tail_block];
-      bad = __builtin_amdgcn_readfirstlane((uint32_t)bad) |
-            (unsigned long long)__builtin_amdgcn_readfirstlane((uint32_t)(bad >> 32)) << 32;
+      bad = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)bad) |  // (the builtin is signed)
+            (unsigned long long)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(bad >> 32)) << 32;
       if (bad == 0) continue;
       const uint64_t vis = seen_bits(blk * BT);
       for (; bad != 0; bad &= bad - 1) {

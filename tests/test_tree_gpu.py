@@ -198,6 +198,34 @@ def test_attention_tree_keeps_unattended_values_out(K, D, ctx, bad):
 
 
 @pytest.mark.parametrize("page", [16, 2])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("M", [20, 60, 80])
+@pytest.mark.parametrize("ctx,cap", [(90, 256), (290, 384), (700, 1500), (700, 5000), (700, 20000)])
+def test_attention_tree_every_workgroup_shape(K, page, D, M, ctx, cap):
+    """The sizes and the cap choose the shape; each against values that must not spread (NaN in K and V of one node, an
+    infinity in V of another, a page that is not mapped) and splits without a token."""
+    n_q, n_kv = 8, 2
+    ctx = min(ctx, cap - M)
+    q, rows, kc, vc, bt = tree_inputs(M, n_q, n_kv, D, page, ctx, 3, seed=7)
+    for node, bad in ((5, float("nan")), (11, float("inf"))):
+        c = T.token_row(bt.tolist(), ctx + node, page, kc.size(0))
+        if bad != bad:
+            kc[c[0], 0, c[1], 3] = bad
+        vc[c[0], :, c[1], 9] = bad
+    bt[40 // page] = -1
+    kept = [i for i in range(M) if not rows[i, 5] and not rows[i, 11]]
+    assert 4 < len(kept) < M - 1
+    want, bound = T.attention_tree(q, rows, ctx, bt, kc, vc)
+    qd, words, btd, kd, vd = dev(q, T.mask_words(rows), bt, kc, vc)
+    for ws in ("full", "none"):
+        out = run_tree(K, qd, words, i32(ctx), btd, kd, vd, cap, ws)
+        T.within(out[kept], want[kept], bound[kept])
+        seen = [i for i in range(M) if rows[i, 5] or rows[i, 11]]
+        hit = out.view(M, n_q, D)[seen][:, n_q // n_kv:]         # the kv head whose K is finite
+        assert not bool(torch.isfinite(hit[..., 9]).any()) and bool(torch.isfinite(hit[..., :8]).all())
+
+
+@pytest.mark.parametrize("page", [16, 2])
 def test_attention_tree_unmapped_pages_and_cap(K, page):
     """Tokens without a mapped page, past the block table or past max_ctx are not attended, nodes among them too; with
     *pos < 0 nothing is."""
