@@ -578,15 +578,22 @@ attn_tree_join_kernel(const float4* __restrict__ part_o, const float2* __restric
 //   D  64   (4,1,64)  1.01 / 1.14 to 1000 tokens, 1.08 - 1.17 / 1.31 at more
 //           (2,4,32)  1.06 / 1.15 to 1000 tokens, 1.02 / 1.17 at more and to eight waves, 1.04 - 1.19 / 1.35 beyond
 //           (4,2,64)  1.06 / 1.15, 1.06 / 1.20, 1.02 - 1.05 / 1.22
+// A context that four groups of 32 tokens get through in three rounds (D 64) or two (D 128) is not split: one launch instead
+// of two. 26 nodes, 4 x 8 heads of 64: at 100 tokens 6.9 us against 9.4 split, at 300 8.8 : 9.7, at 500 10.7 : 10.6 (250
+// nodes 11.3 : 13.0, 13.0 : 14.6, 13.8 : 15.1); 8 x 4 heads of 128: at 100 10.7 : 11.7, at 200 12.0 : 11.9, at 300 13.4 : 11.9.
+// Called eagerly the second launch costs another 3 us of host time.
 struct TreeShape {
   int cw, kvs, bt;
+  bool split = true;
 };
 TreeShape tree_shape(int M, int n_q, int n_kv, int D, int max_ctx) {
   const int waves = (M * (n_q / n_kv) + 31) / 32;
   if (D == 128) {
-    if (max_ctx < 8000 || waves <= 4) return TreeShape{4, 2, 32};
+    if (max_ctx <= 2 * 128) return {2, 4, 32, false};
+    if (max_ctx < 8000 || waves <= 4) return {4, 2, 32};
     return waves > 8 ? TreeShape{8, 1, 64} : TreeShape{4, 2, 64};
   }
+  if (max_ctx <= 3 * 128) return {1, 4, 32, false};
   return max_ctx <= 2048 ? TreeShape{4, 1, 64} : waves > 8 ? TreeShape{4, 2, 64} : TreeShape{2, 4, 32};
 }
 
@@ -595,6 +602,7 @@ TreeShape tree_shape(int M, int n_q, int n_kv, int D, int max_ctx) {
 // One workgroup per CU, in splits of equal length.
 int attention_tree_splits(int M, int n_q, int n_kv, int D, int max_ctx) {
   const TreeShape s = tree_shape(M, n_q, n_kv, D, max_ctx);
+  if (!s.split) return 1;
   const int blocks = (M * (n_q / n_kv) + 32 * s.cw - 1) / (32 * s.cw), round = s.bt * s.kvs;
   const int rounds = max_ctx / round + (max_ctx % round != 0);
   int want = 256 / (blocks * n_kv);
@@ -627,19 +635,23 @@ static void launch_tree(const TreeAttn& t, hipStream_t st) {
              (float2*)(part_o + (size_t)t.splits * t.n_kv * waves * 8 * D)};
   const TreeShape s = tree_shape(t.M, t.n_q, t.n_kv, D, t.max_ctx);
   if constexpr (D == 128) {
-    if (s.cw == 8)
+    if (s.cw == 2)
+      launch_tree_shape<D, 2, 4, 32>(a, cols, st);
+    else if (s.cw == 8)
       launch_tree_shape<D, 8, 1, 64>(a, cols, st);
     else if (s.bt == 64)
       launch_tree_shape<D, 4, 2, 64>(a, cols, st);
     else
       launch_tree_shape<D, 4, 2, 32>(a, cols, st);
   } else {
-    if (s.kvs == 1)
-      launch_tree_shape<D, 4, 1, 64>(a, cols, st);
-    else if (s.cw == 4)
-      launch_tree_shape<D, 4, 2, 64>(a, cols, st);
-    else
+    if (s.cw == 1)
+      launch_tree_shape<D, 1, 4, 32>(a, cols, st);
+    else if (s.cw == 2)
       launch_tree_shape<D, 2, 4, 32>(a, cols, st);
+    else if (s.kvs == 1)
+      launch_tree_shape<D, 4, 1, 64>(a, cols, st);
+    else
+      launch_tree_shape<D, 4, 2, 64>(a, cols, st);
   }
   if (t.splits > 1)
     hipLaunchKernelGGL(attn_tree_join_kernel<D>, dim3(t.n_kv, waves * (D / 8 / kTreeJoinRows)), dim3(kTreeJoinRows * kWave), 0, st, part_o, a.part_ml,
