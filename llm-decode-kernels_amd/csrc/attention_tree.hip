@@ -31,7 +31,7 @@
 // 0.87 PFLOP/s): a wave's products, softmax and load issue follow one another, at two waves per SIMD. Without the softmax
 // it takes 134, without the loads 122, without either 106, the products' own time. 64 nodes at 16001 take 36 (floor 14), of
 // which about 19 are products and the rest launch, first loads and 17 MB of partials. Small ones are launch, a chain of
-// dependent loads (position, page, K / V) and the join: 26 nodes at 4096 17, 5 at 300 9.5.
+// dependent loads (position, page, K / V) and the join: 26 nodes at 4096 16, 5 at 300, unsplit, 8.6 (7.5 in a row).
 // No gain: two halves of the workgroup half a block apart, so that one's softmax meets the other's products; deeper LDS
 // read-ahead; wave priorities; registers cut for three waves per SIMD.
 //

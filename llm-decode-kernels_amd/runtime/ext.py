@@ -98,18 +98,31 @@ def _stream(t):
 
 
 def _check_all(what, device, *tensors):
-    """(tensor or None, name, dtype) triples: contiguous CUDA tensors of their type, all on `device` (an index)."""
+    """(tensor or None, name, dtype) triples: contiguous CUDA tensors of their type, all on `device` (an index, -1 for none).
+    Returns their addresses. One pass with three questions per tensor: asked one by one, with an address each later, they were
+    2.5 us of an op's 9 us of host time."""
+    ptrs = []
     for t, name, dtype in tensors:
-        if t is not None:
+        if t is None:
+            ptrs.append(None)
+            continue
+        if t.dtype is not dtype or t.get_device() != device or not t.is_contiguous() or device < 0:
             _check_cuda(t, name)
             if t.dtype != dtype:
                 raise RuntimeError(f"{what}: {name} must be {dtype}, got {t.dtype}")
-            if t.get_device() != device:
-                raise RuntimeError(f"{what}: {name} is on another device than the other tensors")
+            raise RuntimeError(f"{what}: {name} is on another device than the other tensors")
+        ptrs.append(t.data_ptr())
+    return ptrs
 
 
-def _ptr(t):
-    return None if t is None else t.data_ptr()
+def _workspace(what, device, t):
+    """(address, bytes) of a workspace on `device`, of nothing for None."""
+    if t is None:
+        return None, 0
+    if t.get_device() != device or not t.is_contiguous():
+        _check_cuda(t, "workspace")
+        raise RuntimeError(f"{what}: workspace is on another device than the other tensors")
+    return t.data_ptr(), t.nbytes
 
 
 LOGITS_DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
@@ -614,11 +627,14 @@ class DecodeKernels:
     def _call_on(self, device, fn, *args):
         """_call with the stream of `device` as the last argument and that device current (the default stream's handle
         names the current device's)."""
-        args += (torch._C._cuda_getCurrentRawStream(device),)
-        if device == torch.cuda.current_device():
-            return self._call(fn, *args)
+        stream = torch._C._cuda_getCurrentRawStream(device)
+        if device == torch._C._cuda_getDevice():
+            rc = fn(*args, stream)
+            if rc != 0:
+                raise RuntimeError(self.lib.dk_last_error().decode() or f"decode kernel error {rc}")
+            return
         with torch.cuda.device(device):
-            self._call(fn, *args)
+            self._call(fn, *args, stream)
 
     # rows of a prompt or of a drafted tree: per-head RMSNorm of q and k (models with q_norm / k_norm), RoPE, KV append
     def qk_norm_rope_append_rows(self, qkv, q_w, k_w, eps, cos_t, sin_t, pos, depth, bt, kc, vc, n_q, n_kv, q_out=None):
@@ -626,33 +642,33 @@ class DecodeKernels:
         prompt, *pos + m). q_w, k_w [D] (None: no norm) weight the RMSNorm of each q and k head. The rotated q goes to
         q_out [M, n_q * D] (rows may be strided; None: in place in qkv), rotated k and v to the cache."""
         what, dev = "qk_norm_rope_append_rows", qkv.get_device()
-        _check_all(what, dev, (qkv, "qkv", torch.float16), (q_w, "q_w", torch.float16), (k_w, "k_w", torch.float16),
-                   (cos_t, "cos_t", torch.float32), (sin_t, "sin_t", torch.float32), (pos, "pos", torch.int32),
-                   (depth, "depth", torch.int32), (bt, "bt", torch.int32), (kc, "kc", torch.float16),
-                   (vc, "vc", torch.float16))
-        if kc.dim() != 4 or kc.size(3) not in (64, 128) or vc.shape != kc.shape or kc.size(1) != n_kv:
+        p_qkv, p_qw, p_kw, p_cos, p_sin, p_pos, p_depth, p_bt, p_kc, p_vc = _check_all(
+            what, dev, (qkv, "qkv", torch.float16), (q_w, "q_w", torch.float16), (k_w, "k_w", torch.float16),
+            (cos_t, "cos_t", torch.float32), (sin_t, "sin_t", torch.float32), (pos, "pos", torch.int32),
+            (depth, "depth", torch.int32), (bt, "bt", torch.int32), (kc, "kc", torch.float16), (vc, "vc", torch.float16))
+        cache, table, rows = kc.shape, cos_t.shape, qkv.shape
+        if len(cache) != 4 or cache[3] not in (64, 128) or vc.shape != cache or cache[1] != n_kv:
             raise RuntimeError("cache must be [pages, n_kv, P, 64|128]")
-        D = kc.size(3)
+        D = cache[3]
         row = (n_q + 2 * n_kv) * D
-        if qkv.dim() != 2 or qkv.size(1) != row or cos_t.dim() != 2 or cos_t.size(1) * 2 != D \
-                or sin_t.shape != cos_t.shape or pos.numel() < 1:
+        if len(rows) != 2 or rows[1] != row or len(table) != 2 or table[1] * 2 != D or sin_t.shape != table \
+                or pos.numel() < 1:
             raise RuntimeError(f"{what}: qkv must be [M, (n_q + 2 n_kv) * D], cos and sin [max_pos, D/2], pos [1]")
-        M = qkv.size(0)
+        M = rows[0]
         if depth is not None and depth.numel() != M:
             raise RuntimeError(f"{what}: depth must be int32 [M]")
         if (q_w is None) != (k_w is None) or (q_w is not None and (q_w.numel() != D or k_w.numel() != D)):
             raise RuntimeError(f"{what}: q_w and k_w must both be [D] or both None")
         if q_out is None:
-            q_out, q_stride = qkv, row
+            p_out, q_stride = p_qkv, row
         else:
-            if not q_out.is_cuda or q_out.dtype != torch.float16 or q_out.get_device() != dev \
-                    or q_out.shape != (M, n_q * D) or q_out.stride(1) != 1:
+            if q_out.dtype is not torch.float16 or q_out.get_device() != dev or q_out.shape != (M, n_q * D) \
+                    or q_out.stride(1) != 1:
                 raise RuntimeError(f"{what}: q_out must be a CUDA fp16 [M, n_q * D] with contiguous rows")
-            q_stride = q_out.stride(0) if M > 1 else row if q_out.data_ptr() == qkv.data_ptr() else n_q * D
-        self._call_on(dev, self.lib.dk_qk_norm_rope_append_rows, qkv.data_ptr(), _ptr(q_w), _ptr(k_w), float(eps),
-                      cos_t.data_ptr(), sin_t.data_ptr(), pos.data_ptr(), _ptr(depth), bt.data_ptr(), kc.data_ptr(),
-                      vc.data_ptr(), q_out.data_ptr(), q_stride, M, int(n_q), int(n_kv), D, kc.size(2), cos_t.size(0),
-                      kc.size(0), bt.numel())
+            p_out = q_out.data_ptr()
+            q_stride = q_out.stride(0) if M > 1 else row if p_out == p_qkv else n_q * D
+        self._call_on(dev, self.lib.dk_qk_norm_rope_append_rows, p_qkv, p_qw, p_kw, float(eps), p_cos, p_sin, p_pos, p_depth,
+                      p_bt, p_kc, p_vc, p_out, q_stride, M, int(n_q), int(n_kv), D, cache[2], table[0], cache[0], bt.numel())
 
     # attention of the nodes of a drafted token tree (speculative decoding) over the paged cache
     def attention_tree_workspace_bytes(self, M, n_q, n_kv, head_dim, max_ctx):
@@ -664,28 +680,26 @@ class DecodeKernels:
         tokens [0, *pos) and the nodes j (tokens *pos + j, in the cache already) whose bit j % 64 of mask[i, j // 64] is
         set (mask int64 [M, ceil(M / 64)]; None: a chain, j <= i). max_ctx: *pos + M or more. out [M, n_q * D]."""
         what, dev = "attention_tree", q.get_device()
-        _check_all(what, dev, (mask, "mask", torch.int64), (pos, "pos", torch.int32), (bt, "bt", torch.int32),
-                   (kc, "kc", torch.float16), (vc, "vc", torch.float16), (out, "out", torch.float16))
-        if kc.dim() != 4 or kc.size(3) not in (64, 128) or vc.shape != kc.shape:
+        p_mask, p_pos, p_bt, p_kc, p_vc, p_out = _check_all(
+            what, dev, (mask, "mask", torch.int64), (pos, "pos", torch.int32), (bt, "bt", torch.int32),
+            (kc, "kc", torch.float16), (vc, "vc", torch.float16), (out, "out", torch.float16))
+        cache, rows = kc.shape, q.shape
+        if len(cache) != 4 or cache[3] not in (64, 128) or vc.shape != cache:
             raise RuntimeError("cache must be [pages, n_kv, P, 64|128]")
-        n_kv, D = kc.size(1), kc.size(3)
-        if not q.is_cuda or q.dtype != torch.float16 or q.dim() not in (2, 3) or q.stride(-1) != 1 \
-                or (q.dim() == 3 and (q.size(2) != D or (q.size(1) > 1 and q.stride(1) != D))):
+        D, strides = cache[3], q.stride()
+        if q.dtype is not torch.float16 or len(rows) not in (2, 3) or strides[-1] != 1 \
+                or (len(rows) == 3 and (rows[2] != D or (rows[1] > 1 and strides[1] != D))):
             raise RuntimeError(f"{what}: q must be a CUDA fp16 [M, n_q, D] or [M, n_q * D] with contiguous rows")
-        M = q.size(0)
-        width = q.size(1) if q.dim() == 2 else q.size(1) * D
+        M = rows[0]
+        width = rows[1] if len(rows) == 2 else rows[1] * D
         if width % D != 0 or out.shape != (M, width) or pos.numel() < 1:
             raise RuntimeError(f"{what}: q rows must hold n_q * D values, out be [M, n_q * D] and pos [1]")
         if mask is not None and mask.shape != (M, (M + 63) // 64):
             raise RuntimeError(f"{what}: mask must be int64 [M, ceil(M / 64)]")
-        if workspace is not None:
-            _check_cuda(workspace, "workspace")
-            if workspace.get_device() != dev:
-                raise RuntimeError(f"{what}: workspace is on another device than the other tensors")
-        self._call_on(dev, self.lib.dk_attention_tree, q.data_ptr(), q.stride(0) if M > 1 else width, _ptr(mask),
-                      pos.data_ptr(), bt.data_ptr(), bt.numel(), kc.data_ptr(), vc.data_ptr(), kc.size(0), kc.size(2),
-                      width // D, n_kv, D, M, int(max_ctx), out.data_ptr(), _ptr(workspace),
-                      0 if workspace is None else workspace.numel() * workspace.element_size())
+        p_ws, ws_bytes = _workspace(what, dev, workspace)
+        self._call_on(dev, self.lib.dk_attention_tree, q.data_ptr(), strides[0] if M > 1 else width, p_mask, p_pos, p_bt,
+                      bt.numel(), p_kc, p_vc, cache[0], cache[2], width // D, cache[1], D, M, int(max_ctx), p_out, p_ws,
+                      ws_bytes)
 
     # log probabilities of given tokens with entropy and top alternatives (the picks of a verified tree, prompt scoring)
     def token_logprobs_workspace_bytes(self, M, V, k, dtype=torch.float16):
@@ -699,28 +713,24 @@ class DecodeKernels:
         largest logits' ids and log probabilities (top_ids int64, top_logprobs [M, k], k <= 32; descending, the lowest
         index first among equals). Outputs fp32; any of them may be None (tokens and logprobs together)."""
         what, dev = "token_logprobs", logits.get_device()
-        _check_all(what, dev, (tokens, "tokens", torch.int64), (logprobs, "logprobs", torch.float32),
-                   (entropy, "entropy", torch.float32), (top_ids, "top_ids", torch.int64),
-                   (top_logprobs, "top_logprobs", torch.float32))
-        if not logits.is_cuda or logits.dtype not in LOGITS_DTYPES or logits.dim() != 2 \
-                or (logits.stride(1) != 1 and logits.size(1) > 1):
+        p_tokens, p_logprobs, p_entropy, p_ids, p_top = _check_all(
+            what, dev, (tokens, "tokens", torch.int64), (logprobs, "logprobs", torch.float32),
+            (entropy, "entropy", torch.float32), (top_ids, "top_ids", torch.int64),
+            (top_logprobs, "top_logprobs", torch.float32))
+        dtype, rows = LOGITS_DTYPES.get(logits.dtype), logits.shape
+        if dev < 0 or dtype is None or len(rows) != 2 or (logits.stride(1) != 1 and rows[1] > 1):
             raise RuntimeError(f"{what}: logits must be a CUDA fp16, bf16 or fp32 [M, V] with contiguous rows")
-        M, V = logits.shape
+        M, V = rows
         for t, name in ((tokens, "tokens"), (logprobs, "logprobs"), (entropy, "entropy")):
             if t is not None and t.numel() != M:
                 raise RuntimeError(f"{what}: {name} must hold M values")
         k = 0 if top_ids is None else top_ids.size(-1)
-        for t, name in ((top_ids, "top_ids"), (top_logprobs, "top_logprobs")):
-            if (t is None) != (k == 0) or (t is not None and t.shape != (M, k)):
-                raise RuntimeError(f"{what}: top_ids and top_logprobs must both be [M, k] or both None")
-        if workspace is not None:
-            _check_cuda(workspace, "workspace")
-            if workspace.get_device() != dev:
-                raise RuntimeError(f"{what}: workspace is on another device than the other tensors")
-        self._call_on(dev, self.lib.dk_token_logprobs, logits.data_ptr(), LOGITS_DTYPES[logits.dtype],
-                      logits.stride(0) if M > 1 else V, _ptr(tokens), _ptr(logprobs), _ptr(entropy), _ptr(top_ids),
-                      _ptr(top_logprobs), M, V, k, _ptr(workspace),
-                      0 if workspace is None else workspace.numel() * workspace.element_size())
+        if (top_ids is None) != (top_logprobs is None) \
+                or (top_ids is not None and (k == 0 or not top_ids.shape == top_logprobs.shape == (M, k))):
+            raise RuntimeError(f"{what}: top_ids and top_logprobs must both be [M, k] or both None")
+        p_ws, ws_bytes = _workspace(what, dev, workspace)
+        self._call_on(dev, self.lib.dk_token_logprobs, logits.data_ptr(), dtype, logits.stride(0) if M > 1 else V, p_tokens,
+                      p_logprobs, p_entropy, p_ids, p_top, M, V, k, p_ws, ws_bytes)
 
     # the greedy walk down a verified tree, and its cache rows made contiguous
     def tree_accept(self, tokens, parents, picks, pos, bt, kv, path, count, tok):
@@ -729,25 +739,25 @@ class DecodeKernels:
         tok int64 [1] (the next pending token); kv [..., pages, n_kv, P, D] (any leading sizes, e.g. layers and K / V; None:
         no move): the rows of tokens *pos + path[t] move to *pos + t in every cache. pos stays: the caller adds count."""
         what, dev = "tree_accept", tokens.get_device()
-        _check_all(what, dev, (tokens, "tokens", torch.int64), (parents, "parents", torch.int32),
-                   (pos, "pos", torch.int32), (bt, "bt", torch.int32), (kv, "kv", torch.float16),
-                   (path, "path", torch.int32), (count, "count", torch.int32), (tok, "tok", torch.int64))
+        p_tokens, p_parents, p_pos, p_bt, p_kv, p_path, p_count, p_tok = _check_all(
+            what, dev, (tokens, "tokens", torch.int64), (parents, "parents", torch.int32), (pos, "pos", torch.int32),
+            (bt, "bt", torch.int32), (kv, "kv", torch.float16), (path, "path", torch.int32), (count, "count", torch.int32),
+            (tok, "tok", torch.int64))
         M = tokens.numel()
-        if not picks.is_cuda or picks.dtype != torch.int64 or picks.get_device() != dev or picks.shape != (M,):
+        if picks.dtype is not torch.int64 or picks.get_device() != dev or picks.shape != (M,):
             raise RuntimeError(f"{what}: picks must be a CUDA int64 [M]")
         if parents.numel() != M or path.numel() != M or count.numel() != 1 or tok.numel() != 1:
             raise RuntimeError(f"{what}: parents and path must hold M values, count and tok one")
         if kv is None:
             n_caches, cache = 0, (0, 0, 0, 0)
         else:
-            if kv.dim() < 4 or kv.size(-1) not in (64, 128):
+            cache = kv.shape[-4:]
+            if len(cache) < 4 or cache[3] not in (64, 128):
                 raise RuntimeError("cache must be [pages, n_kv, P, 64|128]")
-            cache = tuple(kv.shape[-4:])
             n_caches = kv.numel() // max(1, cache[0] * cache[1] * cache[2] * cache[3])
-        self._call_on(dev, self.lib.dk_tree_accept, tokens.data_ptr(), parents.data_ptr(), picks.data_ptr(),
-                      picks.stride(0) if M > 1 else 1, M, _ptr(pos), _ptr(bt), 0 if bt is None else bt.numel(), _ptr(kv),
-                      n_caches, cache[0], cache[1], cache[2], cache[3], path.data_ptr(), count.data_ptr(),
-                      tok.data_ptr())
+        self._call_on(dev, self.lib.dk_tree_accept, p_tokens, p_parents, picks.data_ptr(), picks.stride(0) if M > 1 else 1, M,
+                      p_pos, p_bt, 0 if bt is None else bt.numel(), p_kv, n_caches, cache[0], cache[1], cache[2], cache[3],
+                      p_path, p_count, p_tok)
 
     # runtime/quant.py:42-48,100-124 on the GPU
     def quantize_w4(self, w, packed, sz, group, clip=False):
