@@ -169,6 +169,43 @@ def test_verify_generates_as_greedy_decoding(K):
     assert m.host_pos == int(m.pos) == len(seq) - 1
 
 
+def test_captured_verify_replays(K):
+    """Two recorded sizes in turn, with eager work (a larger tree, whose buffers grow; decoding; prefill) between the
+    replays; capturing leaves the state, and each replay is checked against decoding."""
+    m = model(64)
+    m.reset(0)
+    m.prefill(prompt(20, seed=2))
+    before = (m.kv.clone(), int(m.tok), int(m.pos))
+    for n in (4, 25):
+        m.capture_verify(n)
+    assert torch.equal(m.kv, before[0]) and (int(m.tok), int(m.pos)) == before[1:] and m.host_pos == 20
+    for turn in range(3):
+        path, margin = greedy(m, 4)
+        sure = next((i for i, x in enumerate(margin) if x <= 2 * REL), 4)
+        toks, _ = checked_verify(m, path)                                         # 4: a recorded chain
+        assert toks[:sure] == path[:sure]
+        checked_verify(m, *branching(greedy(m, 2)[0], 24 - turn, seed=turn))      # not a recorded size
+        path, margin = greedy(m, 5)
+        sure = next((i for i, x in enumerate(margin) if x <= 2 * REL), 5)
+        draft, parents = branching(path, 20, seed=turn + 9)
+        assert len(draft) == 25
+        toks, _ = checked_verify(m, draft, parents)                               # 25: a recorded tree
+        assert toks[:sure] == path[:sure]
+        m.run_step()
+        m.prefill([7, 8, 9])
+    assert m.host_pos == int(m.pos)
+
+
+def test_capture_verify_refusals(K):
+    with pytest.raises(NotImplementedError, match="INT4"):
+        model(64, weights="fp16").capture_verify(4)
+    with pytest.raises(NotImplementedError, match="INT4"):
+        model(64, lm_head="fp16").capture_verify(4)
+    for n in (-1, 1024):
+        with pytest.raises(ValueError, match="drafted tokens"):
+            model(64).capture_verify(n)
+
+
 def test_verify_on_a_side_stream(K):
     m = model(64)
     out = []
