@@ -7,16 +7,18 @@
 // workgroups in whole rounds of KVS blocks; the ends follow *pos, so one captured launch serves every position. The kv head
 // is the fastest grid index: with 8 of them each XCD's L2 holds one head's K / V for all its workgroups, and its partials
 // for the join.
-// K / V go from the cache straight into LDS (16-byte global-to-LDS loads), double-buffered: a round's loads go out between
-// the products of the round before it, spread, since a wave that issues them in a row waits for the other waves' to be taken
-// in (250 nodes at 32768 tokens: 155.9 -> 154.5 us).
+// K / V go from the cache straight into LDS (16-byte loads), double-buffered: a round's loads go out between the products of
+// the round before it, spread, since a wave that issues them in a row waits for the other waves' to be taken in (250 nodes at
+// 32768 tokens: 155.9 -> 154.5 us). As buffer loads, whose base is a scalar where a load's rows lie in one page: behind
+// global loads to LDS the compiler waits for every LDS read in flight instead of the one it needs (159.6 -> 156.7).
 //
-// Per block, on v_mfma_f32_32x32x16_f16:
-//   * S^T = K . Q^T: A = 32 token rows of K from LDS, B = the wave's Q columns (registers). Lane (h, r) receives column r,
-//     tokens 8 q + 4 h + v: a column's scores, maximum, sum and output live in the lane pair (r, r + 32).
-//   * online softmax in the log2 domain, scale and log2 e in one multiplier; the reference maximum moves only when a block's
-//     maximum passes it by kTreeLazy (2^8). p = 2^(s - ref + kTreeLift) <= 2^15, so that what fp16 cannot hold of a small p
-//     is 2^-32 of the largest.
+// Per tile of 32 tokens, on v_mfma_f32_32x32x16_f16:
+//   * S^T = K . Q^T: A = the tile's rows of K from LDS, B = the wave's Q columns (registers). Lane (h, r) receives column r,
+//     tokens 8 q + 4 h + v: a column's scores, sum and output live in the lane pair (r, r + 32).
+//   * p = 2^(s - ref + kTreeLift), scale and log2 e in one multiplier, while the next tile's products run. The reference is
+//     a maximum of scores seen so far, not the running one: it moves to the tile's maximum where a lane's sum of p passes
+//     kTreeMost, so that p fits fp16 and no maximum is taken otherwise; what fp16 cannot hold of a small p is 2^-32 of p at
+//     the reference. (With a maximum per block of 64 tokens ahead of its weights 156.7 -> 153.3 us.)
 //   * O^T += V^T . P^T: the score accumulator, rounded to fp16 to nearest, is the B operand as it is; V^T comes out of the
 //     row-major V tile through the transposing LDS read. One fp16 part of p instead of two: its 2^-11, unbiased and beside
 //     an output that is rounded to fp16 itself, against a half more of the products. The sum of the weights keeps fp32.
@@ -27,13 +29,17 @@
 // Since 0 times NaN or infinity is NaN, check_v zeroes in LDS the V chunks of tokens that do not exist, and those with such
 // values in blocks that reach *pos; the latter are added at the end, value by value, for the columns that see their token.
 //
-// What bounds it (250 nodes at 32768 tokens, 8 x 4 heads of 128: 154 us against 114 at the rate of a large matrix product,
-// 0.87 PFLOP/s): a wave's products, softmax and load issue follow one another, at two waves per SIMD. Without the softmax
-// it takes 134, without the loads 122, without either 106, the products' own time. 64 nodes at 16001 take 36 (floor 14), of
-// which about 19 are products and the rest launch, first loads and 17 MB of partials. Small ones are launch, a chain of
-// dependent loads (position, page, K / V) and the join: 26 nodes at 4096 16, 5 at 300, unsplit, 8.6 (7.5 in a row).
-// No gain: two halves of the workgroup half a block apart, so that one's softmax meets the other's products; deeper LDS
-// read-ahead; wave priorities; registers cut for three waves per SIMD.
+// What bounds it (250 nodes at 32768 tokens, 8 x 4 heads of 128: 148 us against 114 at the rate of a large matrix product,
+// 0.91 PFLOP/s): instructions, at two waves per SIMD and a clock that these products lower to 2.0 GHz. Per product a wave
+// issues 4 others of its softmax, 1.5 LDS reads and its share of the addresses; a loop of nothing but that runs a product
+// and those in 45 cycles, the product alone in 33. With blocks of 64 tokens, 156 us: without the exponentials it takes
+// 139, without reading V 142, without both 119 and without loads too 100; the products' own time is 62. 64 columns per wave would halve the reads, but then
+// scores lie in accumulation registers, which the softmax cannot use. 64 nodes at 16001 take 31 (floor 14), of which about
+// 18 are this and the rest launch, first loads and 17 MB of partials. Small ones are launch, a chain of dependent loads
+// (position, page, K / V) and the join: 26 nodes at 4096 16, 5 at 300, unsplit, 7.3.
+// No gain: two halves of the workgroup half a block apart, so that one's softmax meets the other's products; a block's
+// weights behind the next one's scores; wave priorities; 168 registers for three waves per SIMD; sums of p by dot products;
+// the first pages looked up ahead of the position.
 //
 // LDS: rows of 2 D bytes without padding. K chunk q (16 bytes) of row t at q ^ (t & 15) (D 128) or q ^ ((t >> 1) & 7) (D 64),
 // V in 64-byte units, unit u of row t at u ^ (t & 3) (D 128) or u ^ ((t >> 1) & 1) (D 64): reads fall in distinct banks
@@ -52,9 +58,8 @@ namespace {
 
 // Reference maximum of a column that has seen no token: a finite stand-in for -infinity (no -inf - (-inf)).
 constexpr float kTreeNoMax = -1e30f;
-constexpr float kTreeLazy = 8.0f;  // log2 units
-constexpr float kTreeLift = 7.0f;  // p's exponent at the reference maximum
-static_assert(kTreeLazy + kTreeLift <= 15.0f, "p fits fp16");
+constexpr float kTreeLift = 7.0f;     // p's exponent at the reference maximum
+constexpr float kTreeMost = 32768.f;  // the reference moves where a lane's sum of p over a tile passes this: p fits fp16
 
 constexpr int kTreeMaxSplits = 64;
 
@@ -106,8 +111,9 @@ attn_tree_kernel(const TreeArgs a) {
   static_assert((KVS - 1) * CW * kWave * 16 * DT <= kTile, "a merge row set fits a buffer");
   __shared__ __align__(16) uint8_t s_k0[kTile], s_k1[kTile], s_v0[kTile], s_v1[kTile];
   __shared__ float s_m[KVS > 1 ? KVS * CW * 32 : 1], s_l[KVS > 1 ? KVS * CW * 32 : 1];
-  // by block from the one of *pos on: the tokens that have V chunks which check_v took out
-  __shared__ unsigned long long s_bad[kTreeMaxNodes / BT + 1];
+  // by 32 tokens from those of *pos on: the tokens that have V chunks which check_v took out
+  constexpr int kBadWords = kTreeMaxNodes / 32 + 1;
+  __shared__ uint32_t s_bad[kBadWords];
 
   const int kvh = blockIdx.x, cb = blockIdx.y, split = blockIdx.z;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -117,7 +123,7 @@ attn_tree_kernel(const TreeArgs a) {
   const int P = 1 << a.log2P;
   const long long pos = *a.pos;
   const int ctx = tree_context(pos, a.M, a.cap);
-  const int tail_block = pos < ctx ? (int)(pos / BT) : INT_MAX / 2;  // the first block with tokens that not every column sees
+  const int tail = pos < ctx ? (int)(pos / 32) : INT_MAX / 2;  // the first 32 tokens with some that not every column sees
   // this split's rounds [r0, r1): the first nr % splits splits have one more
   const unsigned nr = (ctx + SB - 1u) / SB, per = nr / (unsigned)a.splits, more = nr - per * (unsigned)a.splits;
   const int r0 = (int)(split * per + min((unsigned)split, more)), r1 = r0 + (int)per + ((unsigned)split < more);
@@ -146,7 +152,8 @@ attn_tree_kernel(const TreeArgs a) {
   const uint32_t row_off = UP ? (lane / CH) * RB : 0;
   const uint32_t k_place = row_off + 16 * (D == 128 ? sch ^ (sr & 15) : sch ^ ((sr >> 1) & 7));
   const uint32_t v_place = row_off + 64 * ((sch >> 2) ^ (D == 128 ? sr & 3 : (sr >> 1) & 1)) + 16 * (sch & 3);
-  int pg[NP], vpg;        // pages of the loads; of token `lane` of the group's block
+  constexpr int NB = (BT + 63) / 64;
+  int pg[NP], vpg[NB];    // pages of the loads; of token `lane` of the group's block, by 64
   struct Rows {           // where a round's rows lie (UP: lane i's those of load i)
     uint64_t base[NP];
     uint32_t ok;          // bit i: this thread's row of load i exists
@@ -188,23 +195,29 @@ attn_tree_kernel(const TreeArgs a) {
   auto fetch = [&](const uint8_t* cache, const Rows& w, int i, uint32_t place, uint8_t* buf) __attribute__((always_inline)) {  // load i of a round
     typedef __attribute__((address_space(1))) const void* gptr;
     typedef __attribute__((address_space(3))) void* lptr;
-    __builtin_amdgcn_global_load_lds((gptr)(cache + rows_of(w, i) + place), (lptr)(buf + (RPI * i + RPW * wave) * RB), 16, 0,
-                                     0);
+    lptr at = (lptr)(buf + (RPI * i + RPW * wave) * RB);
+    if constexpr (UP) {
+      const __amdgpu_buffer_rsrc_t res =
+          __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(cache) + rows_of(w, i), 0, RPW * RB, 0x00020000);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(res, at, 16, (int)place, 0, 0, 0);
+    } else {
+      __builtin_amdgcn_global_load_lds((gptr)(cache + rows_of(w, i) + place), at, 16, 0, 0);
+    }
   };
   // V chunks that must not meet a p of 0, looked over in LDS by the lane that loaded them: those of tokens that do not exist,
   // and those with NaN or infinity of tokens that not every column sees
   auto check_v = [&](int rnd, const Rows& w, uint8_t* buf) __attribute__((always_inline)) {
-    const bool tail = (rnd + 1) * (long long)SB > pos;  // uniform
-    if (!tail && __all(w.ok == (1u << LPT) - 1)) return;
+    const bool reaches = (rnd + 1) * (long long)SB > pos;  // uniform
+    if (!reaches && __all(w.ok == (1u << LPT) - 1)) return;
     asm volatile("");  // stays a branch
 #pragma unroll
     for (int i = 0; i < LPT; ++i) {
       const int row = sr + RPI * i;
       u32x4* x = reinterpret_cast<u32x4*>(buf + row * RB + 16 * sch);
       const bool ok = w.ok >> i & 1;
-      const int blk = rnd * KVS + row / BT - tail_block;
-      const bool bad = ok && tail && blk >= 0 && has_nonfinite(*x);
-      if (bad) atomicOr(&s_bad[blk], 1ull << (row % BT));
+      const int word = rnd * (SB / 32) + row / 32 - tail;
+      const bool bad = ok && reaches && word >= 0 && has_nonfinite(*x);
+      if (bad) atomicOr(&s_bad[word], 1u << (row % 32));
       if (!ok || bad) *x = u32x4{0u, 0u, 0u, 0u};
     }
   };
@@ -237,99 +250,124 @@ attn_tree_kernel(const TreeArgs a) {
     return bits;
   };
   auto block_start = [&](int rnd) __attribute__((always_inline)) { return (rnd * KVS + grp) * BT; };
-  auto lookup_block = [&](int rnd) __attribute__((always_inline)) { vpg = a.bt[min(block_start(rnd) + lane % BT, ctx - 1) >> a.log2P]; };
+  auto lookup_block = [&](int rnd) __attribute__((always_inline)) {
+#pragma unroll
+    for (int c = 0; c < NB; ++c) vpg[c] = a.bt[min(block_start(rnd) + 64 * c + lane % BT, ctx - 1) >> a.log2P];
+  };
 
-  // ---- the three steps of a block
-  f32x16 sc[NT];  // scores
-  h8 ph[2 * NT];  // p in fp16: the B operand of the output's products
-  auto scores = [&](int rnd, const uint8_t* buf, auto after) __attribute__((always_inline)) {
+  // ---- a block, by tiles of 32 tokens
+  f32x16 sc[2];        // scores of a tile and the next
+  h8 ph[2];            // p in fp16: the B operand of the output's products
+  constexpr int RA = 4;  // K fragments in flight from LDS
+  u32x4 ka[RA + 1];
+  h8 va[2][DT];        // V fragments: 16 tokens, in two sets
+  float psum[2];       // sums of p over the tile
+  auto weigh = [&](const f32x16& s, int e, float lift) __attribute__((always_inline)) {  // p of scores e, e + 1
+    const float p0 = __builtin_amdgcn_exp2f(fmaf(s[e], a.c2, lift)), p1 = __builtin_amdgcn_exp2f(fmaf(s[e + 1], a.c2, lift));
+    psum[0] = e == 0 ? p0 : psum[0] + p0;
+    psum[1] = e == 0 ? p1 : psum[1] + p1;
+    const h2 p = __builtin_convertvector(f2{p0, p1}, h2);
+    ph[e >> 3][e & 7] = p[0];
+    ph[e >> 3][(e & 7) + 1] = p[1];
+  };
+  auto block = [&](int rnd, const uint8_t* kb, const uint8_t* vb, auto send) __attribute__((always_inline)) {
     const int t0 = block_start(rnd);
-    const uint64_t valid = __ballot(t0 + lane % BT < ctx && (unsigned)vpg < (unsigned)a.n_pages && lane < BT);
-    constexpr uint64_t kAll = BT == 64 ? ~0ull : (1ull << BT) - 1;
-    const bool masked = valid != kAll || t0 + BT > pos;  // uniform per wave
-    uint64_t vis = 0;
-    if (masked) vis = seen_bits(t0) & valid;
+    bool plain = t0 + BT <= pos;  // every token is seen; uniform per wave
+    uint64_t vis[NB];
 #pragma unroll
-    for (int tt = 0; tt < NT; ++tt) sc[tt] = f32x16{};
-    // K fragments (k step f / NT, token tile f % NT), each read from LDS RA fragments ahead of its MFMA
-    constexpr int NF = KS * NT, RA = 2;
-    u32x4 ka[RA + 1];
-    int kat = krow + ((h ^ ksw) << 4);
-    asm volatile("" : "+v"(kat));  // (the chunks' places are worked out per block: eight of them held would not fit)
-    auto read_k = [&](int f) __attribute__((always_inline)) {
-      return *reinterpret_cast<const u32x4*>(buf + (f % NT) * 32 * RB + (kat ^ (f / NT << 5)));
-    };
-#pragma unroll
-    for (int f = 0; f < RA; ++f) ka[f] = read_k(f);
-#pragma unroll
-    for (int f = 0; f < NF; ++f) {
-      if (f + RA < NF) ka[(f + RA) % (RA + 1)] = read_k(f + RA);
-      sc[f % NT] = mfma32x32(__builtin_bit_cast(h8, ka[f % (RA + 1)]), q[f / NT], sc[f % NT]);
-      after(f);
-      __builtin_amdgcn_sched_barrier(0x7);
+    for (int c = 0; c < NB; ++c) {
+      vis[c] = __ballot(t0 + 64 * c + lane % BT < ctx && (unsigned)vpg[c] < (unsigned)a.n_pages && lane < BT);
+      plain = plain && vis[c] == (BT == 32 ? 0xffffffffull : ~0ull);
     }
-    if (masked) {
+    if (!plain) {
       asm volatile("");  // stays a branch
 #pragma unroll
-      for (int tt = 0; tt < NT; ++tt) {
-        const uint32_t bits = (uint32_t)(vis >> (32 * tt)) >> (4 * h);
+      for (int c = 0; c < NB; ++c) vis[c] &= seen_bits(t0 + 64 * c);
+    }
+    int kat = krow + ((h ^ ksw) << 4), vat = vrow + (vsw << 6);
+    asm volatile("" : "+v"(kat), "+v"(vat));  // (the chunks' places are worked out per block: all of them held would not fit)
+    auto read_k = [&](int f) __attribute__((always_inline)) {  // k step f % KS of tile f / KS
+      ka[f % (RA + 1)] = *reinterpret_cast<const u32x4*>(kb + f / KS * 32 * RB + (kat ^ (f % KS << 5)));
+    };
+    auto read_v = [&](int ks) __attribute__((always_inline)) {  // 16 tokens
+#pragma unroll
+      for (int t = 0; t < DT; ++t) {
+        const uint8_t* src = vb + ks * 16 * RB + (vat ^ (t << 6));
+        const u32x2 x = read_tr(src), y = read_tr(src + 8 * RB);
+        va[ks & 1][t] = __builtin_bit_cast(h8, u32x4{x[0], x[1], y[0], y[1]});
+      }
+    };
+    // scores of tile tt, with after(k) behind product k
+    auto scores = [&](int tt, auto after) __attribute__((always_inline)) {
+      sc[tt & 1] = f32x16{};
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        const int f = tt * KS + k;
+        if (k + RA < KS) read_k(f + RA);
+        sc[tt & 1] = mfma32x32(__builtin_bit_cast(h8, ka[f % (RA + 1)]), q[k], sc[tt & 1]);
+        send(f);
+        after(k);
+        __builtin_amdgcn_sched_barrier(0x7f7);  // products stay in order
+      }
+      if (!plain) {
+        asm volatile("");
+        const uint32_t bits = (uint32_t)(vis[tt / 2] >> (32 * (tt & 1))) >> (4 * h);
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-          if (!(bits & (1u << (8 * (i >> 2) + (i & 3))))) sc[tt][i] = -INFINITY;
+          if (!(bits & (1u << (8 * (i >> 2) + (i & 3))))) sc[tt & 1][i] = -INFINITY;
       }
-    }
-  };
-  auto softmax = [&]() __attribute__((always_inline)) {
-    float mx = sc[0][0];
+    };
+    auto ahead_k = [&](int tt) __attribute__((always_inline)) {
+#pragma unroll
+      for (int k = 0; k < (RA < KS ? RA : KS); ++k) read_k(tt * KS + k);
+    };
+    ahead_k(0);
+    scores(0, [](int) {});
+    if (NT > 1) ahead_k(1);
 #pragma unroll
     for (int tt = 0; tt < NT; ++tt) {
+      const f32x16& s = sc[tt & 1];
+      float lift = kTreeLift - mref;
+      read_v(2 * tt);
+      if (tt + 1 < NT) {
+        scores(tt + 1, [&](int k) __attribute__((always_inline)) {
+          constexpr int NE = 16 / KS;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sc[tt][i]);
-    }
-    mx = fmaxf(mx, __shfl_xor(mx, 32, kWave)) * a.c2;
-    const bool move = mx > mref + kTreeLazy;
-    if (__any(move)) {
-      const float mn = move ? mx : mref;
-      const float alpha = __builtin_amdgcn_exp2f(mref - mn);  // 1 for a column that stays
-      mref = mn;
-      l *= alpha;
+          for (int e = 0; e < NE; e += 2) weigh(s, NE * k + e, lift);
+        });
+      } else {
 #pragma unroll
-      for (int t = 0; t < DT; ++t) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[t][i] *= alpha;
+        for (int e = 0; e < 16; e += 2) weigh(s, e, lift);
       }
-    }
-    const float lift = kTreeLift - mref;
-    float ps[2] = {0.f, 0.f};
+      float sum = psum[0] + psum[1];
+      if (__any(!(sum <= kTreeMost))) {  // the reference moves to this tile's maximum where that is higher
+        asm volatile("");
+        float mx = s[0];
 #pragma unroll
-    for (int ks = 0; ks < 2 * NT; ++ks) {
+        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
+        mx = fmaxf(mx, __shfl_xor(mx, 32, kWave)) * a.c2;
+        const float mn = fmaxf(mref, mx);
+        const float alpha = __builtin_amdgcn_exp2f(mref - mn);  // 1 for a column that stays
+        mref = mn;
+        l *= alpha;
 #pragma unroll
-      for (int e = 0; e < 8; e += 2) {
-        const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[ks >> 1][8 * (ks & 1) + e], a.c2, lift));
-        const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[ks >> 1][8 * (ks & 1) + e + 1], a.c2, lift));
-        ps[0] += p0;
-        ps[1] += p1;
-        const h2 hi = __builtin_convertvector(f2{p0, p1}, h2);
-        ph[ks][e] = hi[0];
-        ph[ks][e + 1] = hi[1];
+        for (int t = 0; t < DT; ++t) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[t][i] *= alpha;
+        }
+        lift = kTreeLift - mref;
+  #pragma unroll
+        for (int e = 0; e < 16; e += 2) weigh(s, e, lift);
+        sum = psum[0] + psum[1];
       }
-    }
-    l += ps[0] + ps[1];
-  };
-  auto output = [&](const uint8_t* buf) __attribute__((always_inline)) {
-    int vat = vrow + (vsw << 6);
-    asm volatile("" : "+v"(vat));
+      l += sum;
+      if (tt + 2 < NT) ahead_k(tt + 2);
+      read_v(2 * tt + 1);
 #pragma unroll
-    for (int ks = 0; ks < 2 * NT; ++ks) {
-      h8 v[DT];
+      for (int ks = 0; ks < 2; ++ks) {
 #pragma unroll
-      for (int t = 0; t < DT; ++t) {
-        const uint8_t* src = buf + ks * 16 * RB + (vat ^ (t << 6));
-        const u32x2 x = read_tr(src), y = read_tr(src + 8 * RB);
-        v[t] = __builtin_bit_cast(h8, u32x4{x[0], x[1], y[0], y[1]});
+        for (int t = 0; t < DT; ++t) acc[t] = mfma32x32(va[ks][t], ph[ks], acc[t]);
       }
-#pragma unroll
-      for (int t = 0; t < DT; ++t) acc[t] = mfma32x32(v[t], ph[ks], acc[t]);
     }
   };
 
@@ -353,23 +391,21 @@ attn_tree_kernel(const TreeArgs a) {
     rows = locate(rnd + 1);  // past the end: rows that are never computed on
     // spread over the products: issued in a row they hold a wave up while the other waves' are taken in
     constexpr int NF = KS * NT, NL = 2 * LPT;
-    scores(rnd, kb, [&](int f) __attribute__((always_inline)) {
+    block(rnd, kb, vb, [&](int f) __attribute__((always_inline)) {
 #pragma unroll
       for (int j = 0; j < NL; ++j)
         if (f == j * NF / NL) start(j, kn, vn);
+      if (f == NF - 1) {
+        lookup(rnd + 2);
+        lookup_block(rnd + 1);
+      }
     });
-    pf_fence();
-    lookup(rnd + 2);
-    lookup_block(rnd + 1);
-    pf_fence();
-    softmax();
-    output(vb);
     pf_fence();
     finish(rnd + 1, vn);
   };
   if (r0 < r1) {  // uniform
     lookup(r0);
-    if (tid < kTreeMaxNodes / BT + 1) s_bad[tid] = 0ull;
+    if (tid < kBadWords) s_bad[tid] = 0u;
     rows = locate(r0);
 #pragma unroll
     for (int j = 0; j < 2 * LPT; ++j) start(j, s_k0, s_v0);
@@ -386,15 +422,13 @@ attn_tree_kernel(const TreeArgs a) {
     }
     // ---- add_bad_rows: the chunks that check_v took out, from the cache, for the columns that see their token; its weight
     // once more from q and k
-    for (int blk = max(tail_block, r0 * KVS); blk < min(r1 * KVS, (ctx + BT - 1) / BT); ++blk) {
-      if (blk % KVS != grp) continue;
-      unsigned long long bad = s_bad[blk - tail_block];
-      bad = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)bad) |  // (the builtin is signed)
-            (unsigned long long)(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(bad >> 32)) << 32;
+    for (int word = max(tail, r0 * (SB / 32)); word < min(r1 * (SB / 32), (ctx + 31) / 32); ++word) {
+      if (word * 32 / BT % KVS != grp) continue;
+      uint32_t bad = __builtin_amdgcn_readfirstlane(s_bad[word - tail]);
       if (bad == 0) continue;
-      const uint64_t vis = seen_bits(blk * BT);
+      const uint64_t vis = seen_bits(word * 32);
       for (; bad != 0; bad &= bad - 1) {
-        const int i = __builtin_ctzll(bad), t = blk * BT + i;
+        const int i = __builtin_ctz(bad), t = word * 32 + i;
         const int page = a.bt[t >> a.log2P];  // a token in this set is mapped and inside the context
         const size_t at = ((((size_t)page * a.n_kv + kvh) << a.log2P) + (t & (P - 1))) * D;
         float dot = 0.f;  // this lane's half of the dims
@@ -570,14 +604,17 @@ attn_tree_join_kernel(const float4* __restrict__ part_o, const float2* __restric
 }
 
 // Workgroup shape (CW, KVS, BT) by the column waves of a kv head and the longest context. Each shape's time against the best
-// of six, geometric mean and worst over 210 cases (1-250 nodes, six head layouts, contexts of 200 to 32000):
-//   D 128   (4,2,32)  1.02 / 1.20 to eight waves, 1.00 beyond at 4000 tokens, 1.08 / 1.13 beyond at 16000 and 32000
-//           (8,1,64)  1.01 / 1.14 to 1000 tokens, 1.06 - 1.15 / 1.38 in the rest, but 1.00 / 1.03 beyond eight waves at 16000
-//           (4,2,64)  1.06 - 1.23 / 1.61, but ahead of (4,2,32) at seven and eight waves: 25.1 against 26.1 us at 8000
-//                     tokens, 36.3 : 38.1 at 16001, 56.5 : 61.0 at 32000 (8 kv heads; (8,1,64) 28.5, 38.3, 57.7)
-//   D  64   (4,1,64)  1.01 / 1.14 to 1000 tokens, 1.08 - 1.17 / 1.31 at more
-//           (2,4,32)  1.06 / 1.15 to 1000 tokens, 1.02 / 1.17 at more and to eight waves, 1.04 - 1.19 / 1.35 beyond
-//           (4,2,64)  1.06 / 1.15, 1.06 / 1.20, 1.02 - 1.05 / 1.22
+// of seven, geometric mean / worst over 288 cases (1-250 nodes, six head layouts, contexts of 500 to 32000):
+//             to 4 waves: 1000, 4000, 8000, from 16000   5 to 8: the same                        9 and more: the same
+//   D 128
+//   (4,1,64)  1.00/1.00 1.06/1.21 1.03/1.18 1.03/1.09   1.00/1.00 1.05/1.12 1.02/1.06 1.08/1.16   1.04/1.17 1.11 1.09 1.19
+//   (2,4,32)  1.11/1.21 1.05/1.12 1.03/1.11 1.02/1.10   1.05/1.08 1.03/1.07 1.02/1.04 1.08/1.16   1.06/1.11 1.06 1.09 1.18
+//   (4,2,64)  1.10/1.18 1.05/1.11 1.07/1.27 1.02/1.11   1.07/1.09 1.05/1.08 1.03/1.08 1.00/1.02   1.02/1.05 1.01 1.02 1.02
+//   (8,1,128) 1.16/1.30 1.13/1.22 1.16/1.28 1.23/1.44   1.15/1.19 1.28/1.39 1.19/1.31 1.08/1.21   1.13/1.18 1.14 1.03 1.02
+//             (250 nodes, 8 x 4 heads: (4,2,64) 80.7 us at 16000, 150.6 at 32000, (8,1,128) 80.4, 140.1)
+//   D 64
+//   (2,4,32)  1.05/1.12 1.02/1.09 1.01/1.03 1.00/1.06   1.00/1.00 1.00/1.00 1.00/1.01 1.04/1.13   1.02/1.09 1.03 1.05 1.13
+//   (4,2,64)  1.06/1.13 1.05/1.11 1.05/1.26 1.05/1.19   1.05/1.07 1.08/1.19 1.12/1.30 1.04/1.22   1.04/1.10 1.07 1.04 1.02
 // A context that four groups of 32 tokens get through in three rounds (D 64) or two (D 128) is not split: one launch instead
 // of two. 26 nodes, 4 x 8 heads of 64: at 100 tokens 6.9 us against 9.4 split, at 300 8.8 : 9.7, at 500 10.7 : 10.6 (250
 // nodes 11.3 : 13.0, 13.0 : 14.6, 13.8 : 15.1); 8 x 4 heads of 128: at 100 10.7 : 11.7, at 200 12.0 : 11.9, at 300 13.4 : 11.9.
@@ -590,11 +627,12 @@ TreeShape tree_shape(int M, int n_q, int n_kv, int D, int max_ctx) {
   const int waves = (M * (n_q / n_kv) + 31) / 32;
   if (D == 128) {
     if (max_ctx <= 2 * 128) return {2, 4, 32, false};
-    if (max_ctx < 8000 || waves <= 4) return {4, 2, 32};
-    return waves > 8 ? TreeShape{8, 1, 64} : TreeShape{4, 2, 64};
+    if (waves <= 8 && max_ctx <= 2048) return {4, 1, 64};
+    if (waves <= 4) return {2, 4, 32};
+    return waves > 8 && max_ctx >= 20000 ? TreeShape{8, 1, 128} : TreeShape{4, 2, 64};
   }
   if (max_ctx <= 3 * 128) return {1, 4, 32, false};
-  return max_ctx <= 2048 ? TreeShape{4, 1, 64} : waves > 8 ? TreeShape{4, 2, 64} : TreeShape{2, 4, 32};
+  return waves > 8 && max_ctx >= 8000 ? TreeShape{4, 2, 64} : TreeShape{2, 4, 32};
 }
 
 }  // namespace
@@ -638,18 +676,16 @@ static void launch_tree(const TreeAttn& t, hipStream_t st) {
     if (s.cw == 2)
       launch_tree_shape<D, 2, 4, 32>(a, cols, st);
     else if (s.cw == 8)
-      launch_tree_shape<D, 8, 1, 64>(a, cols, st);
-    else if (s.bt == 64)
-      launch_tree_shape<D, 4, 2, 64>(a, cols, st);
+      launch_tree_shape<D, 8, 1, 128>(a, cols, st);
+    else if (s.kvs == 1)
+      launch_tree_shape<D, 4, 1, 64>(a, cols, st);
     else
-      launch_tree_shape<D, 4, 2, 32>(a, cols, st);
+      launch_tree_shape<D, 4, 2, 64>(a, cols, st);
   } else {
     if (s.cw == 1)
       launch_tree_shape<D, 1, 4, 32>(a, cols, st);
     else if (s.cw == 2)
       launch_tree_shape<D, 2, 4, 32>(a, cols, st);
-    else if (s.kvs == 1)
-      launch_tree_shape<D, 4, 1, 64>(a, cols, st);
     else
       launch_tree_shape<D, 4, 2, 64>(a, cols, st);
   }

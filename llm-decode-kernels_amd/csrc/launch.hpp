@@ -177,7 +177,7 @@ void launch_qk_norm_rope(const QkNormRope& a, hipStream_t st);
 
 // Attention of the M nodes of a drafted tree over the paged cache, the context in `splits` parts (1: no workspace).
 constexpr int kTreeMaxNodes = 1024;
-constexpr int kTreeMaxCtx = 1 << 30;  // so that token indexes two rounds past the last stay in 32 bits
+constexpr int kTreeMaxCtx = 1 << 30;  // so that token indexes past the last round stay in 32 bits
 struct TreeAttn {
   const void* q;
   long long q_stride;
