@@ -368,12 +368,12 @@ int dk_qk_norm_rope_append_rows(const void* qkv, const void* q_w, const void* k_
  * read as nodes. A node that attends nothing gets zeros. Tokens at positions >= max_ctx (pass *pos + M or more), past the
  * block table or without a mapped page are neither read nor attended, and neither values nor NaN of a token reach a node
  * that does not attend it; *pos < 0: no token is attended. q: row m's heads at q + m q_stride (q_stride % 8 == 0), already
- * rotated; out [M, n_q * head_dim] fp16, not overlapping q. fp32 scores and softmax, scale 1/sqrt(head_dim). n_q / n_kv
- * in {1, 2, 4, 8}, M 1..1024, max_ctx 1..2^30. q, kc, vc and out 16-byte aligned.
+ * rotated; out [M, n_q * head_dim] fp16, not overlapping q or mask. fp32 scores and softmax, scale 1/sqrt(head_dim).
+ * n_q / n_kv in {1, 2, 4, 8}, M 1..1024, max_ctx 1..2^30. q, kc, vc and out 16-byte aligned.
  * The context is split over workgroups whose fp32 partials meet in `workspace` (16-byte aligned, overlapping nothing
  * else) and are joined in split order by a second launch; dk_attention_tree_workspace_bytes gives what the sizes can use
- * (0: they do not split). A smaller workspace runs the most splits it holds, NULL runs unsplit. No counterpart in the
- * reference.
+ * (0: they do not split). A smaller workspace runs the most splits it holds, NULL runs unsplit. Calls that may overlap (on
+ * two streams) need a workspace each; captured ones that run in turn can share one. No counterpart in the reference.
  */
 size_t dk_attention_tree_workspace_bytes(int M, int n_q, int n_kv, int head_dim, int max_ctx);
 int dk_attention_tree(const void* q, long long q_stride, const int64_t* mask, const int32_t* pos, const int32_t* bt,
@@ -391,8 +391,8 @@ int dk_attention_tree(const void* q, long long q_stride, const int64_t* mask, co
  * tokens and logprobs may both be NULL, so may entropy; top_ids and top_logprobs are NULL where k is 0. k 0..32, k <= V;
  * M 1..2^20, V 1..2^24; logits aligned to their type. Outputs overlap nothing. `workspace` (16-byte aligned) lets a row be
  * split over workgroups; dk_token_logprobs_workspace_bytes gives what the sizes can use (0: no split); NULL or a smaller
- * one runs unsplit. No counterpart in the reference (its only reader of the logits is torch.argmax,
- * runtime/model.py:232).
+ * one runs unsplit; calls that may overlap need one each. No counterpart in the reference (its only reader of the logits
+ * is torch.argmax, runtime/model.py:232).
  */
 size_t dk_token_logprobs_workspace_bytes(int M, int V, int k, int dtype);
 int dk_token_logprobs(const void* logits, int dtype, long long ld, const int64_t* tokens, float* logprobs,

@@ -33,13 +33,14 @@
 // 0.91 PFLOP/s): instructions, at two waves per SIMD and a clock that these products lower to 2.0 GHz. Per product a wave
 // issues 4 others of its softmax, 1.5 LDS reads and its share of the addresses; a loop of nothing but that runs a product
 // and those in 45 cycles, the product alone in 33. With blocks of 64 tokens, 156 us: without the exponentials it takes
-// 139, without reading V 142, without both 119 and without loads too 100; the products' own time is 62. 64 columns per wave would halve the reads, but then
-// scores lie in accumulation registers, which the softmax cannot use. 64 nodes at 16001 take 31 (floor 14), of which about
-// 18 are this and the rest launch, first loads and 17 MB of partials. Small ones are launch, a chain of dependent loads
-// (position, page, K / V) and the join: 26 nodes at 4096 16, 5 at 300, unsplit, 7.3.
+// 139, without reading V 142, without both 119 and without loads too 100; the products' own time is 62. 64 columns per
+// wave would halve the reads, but then scores lie in accumulation registers, which the softmax cannot use.
+// 64 nodes at 16001 take 31 (floor 14), of which about 18 are this and the rest launch, first loads and 17 MB of partials.
+// Small ones are launch, a chain of dependent loads (position, page, K / V: 3 us to the first product), partials and the
+// join: 26 nodes at 4096 16, 5 at 300, unsplit, 7.3.
 // No gain: two halves of the workgroup half a block apart, so that one's softmax meets the other's products; a block's
 // weights behind the next one's scores; wave priorities; 168 registers for three waves per SIMD; sums of p by dot products;
-// the first pages looked up ahead of the position.
+// the first pages looked up ahead of the position; the first two rounds' loads sent together.
 //
 // LDS: rows of 2 D bytes without padding. K chunk q (16 bytes) of row t at q ^ (t & 15) (D 128) or q ^ ((t >> 1) & 7) (D 64),
 // V in 64-byte units, unit u of row t at u ^ (t & 3) (D 128) or u ^ ((t >> 1) & 1) (D 64): reads fall in distinct banks

@@ -773,8 +773,9 @@ int dk_attention_tree(const void* q, long long q_stride, const int64_t* mask, co
   if (!aligned4(pos) || !aligned4(bt) || (reinterpret_cast<uintptr_t>(mask) & 7u))
     return fail(DK_ERR_ALIGN, "attention_tree: pos and bt must be 4B and mask 8B aligned");
   const size_t q_bytes = (size_t)((M - 1) * q_stride + row) * 2, out_bytes = (size_t)(M * row) * 2;
-  if (ranges_overlap(q, q_bytes, out, out_bytes))
-    return fail(DK_ERR_DOMAIN, "attention_tree: out must not overlap q");
+  const size_t mask_bytes = mask ? (size_t)M * ((M + 63) / 64) * 8 : 0;
+  if (ranges_overlap(q, q_bytes, out, out_bytes) || (mask && ranges_overlap(mask, mask_bytes, out, out_bytes)))
+    return fail(DK_ERR_DOMAIN, "attention_tree: out must not overlap q or mask");
   int splits = 1;
   if (workspace != nullptr) {
     if (!aligned16(workspace)) return fail(DK_ERR_ALIGN, "attention_tree: workspace must be 16B aligned");
@@ -782,7 +783,6 @@ int dk_attention_tree(const void* q, long long q_stride, const int64_t* mask, co
     splits = dk::attention_tree_splits(M, n_q, n_kv, head_dim, max_ctx);
     if (workspace_bytes / part < (size_t)splits) splits = workspace_bytes / part < 2 ? 1 : (int)(workspace_bytes / part);
     const size_t used = splits > 1 ? (size_t)splits * part : 0;
-    const size_t mask_bytes = mask ? (size_t)M * ((M + 63) / 64) * 8 : 0;
     if (used > 0 && (ranges_overlap(workspace, used, q, q_bytes) || ranges_overlap(workspace, used, out, out_bytes) ||
                      ranges_overlap(workspace, used, mask, mask_bytes)))
       return fail(DK_ERR_DOMAIN, "attention_tree: workspace must not overlap q, out or mask");

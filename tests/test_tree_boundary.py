@@ -54,7 +54,7 @@ TREE = dict(q=AT[0], q_stride=1024, mask=AT[1], pos=AT[2], bt=AT[3], n_bt=8, kc=
     (dict(n_kv=65536, n_q=65536), 3, "too many"), (dict(page=24), 4, "power of two"), (dict(n_bt=0), 3, "empty"),
     (dict(n_pages=0), 3, "empty"), (dict(q_stride=1020), 3, "q_stride"), (dict(q_stride=512), 3, "q_stride"),
     (dict(q=AT[0] + 8), 2, "16B"), (dict(out=AT[6] + 2), 2, "16B"), (dict(mask=AT[1] + 4), 2, "8B"),
-    (dict(bt=AT[3] + 2), 2, "4B"), (dict(out=AT[0] + 64), 4, "overlap q"), (dict(ws=AT[7] + 8), 2, "workspace must be 16B")])
+    (dict(bt=AT[3] + 2), 2, "4B"), (dict(out=AT[0] + 64), 4, "overlap q"), (dict(out=AT[1] - 16), 4, "overlap q or mask"), (dict(ws=AT[7] + 8), 2, "workspace must be 16B")])
 def test_attention_tree_refusals(lib, kw, code, msg):
     refused(lib, call(lib, "dk_attention_tree", TREE, kw), code, msg)
 

@@ -505,3 +505,93 @@ def test_caches_past_32_bit_offsets(K):
     path, count, tok = torch.empty(M, dtype=torch.int32, device=DEV), i32(0), torch.tensor([0], device=DEV)
     K.tree_accept(*dev(tokens, parents, picks), i32(ctx), btd, kv, path, count, tok)
     assert path.tolist() == want[0] and int(count) > 1 and torch.equal(kv[:, lo:].cpu(), want[3])
+
+
+# ------------------------------------------------------------------------------------------------ the op module, streams
+def test_op_module_refusals(K):
+    """Wrong types, shapes and layouts raise before anything is launched."""
+    z = lambda *s, t=torch.half: torch.zeros(*s, dtype=t, device=DEV)
+    i64 = torch.int64
+    kc, bt, pos, cos = z(4, 2, 16, 64), z(4, t=torch.int32), z(1, t=torch.int32), z(64, 32, t=torch.float32)
+    qkv, dep = z(3, 6 * 64), z(3, t=torch.int32)
+    qk = dict(qkv=qkv, q_w=None, k_w=None, eps=0.0, cos_t=cos, sin_t=cos, pos=pos, depth=dep, bt=bt, kc=kc, vc=kc.clone(),
+              n_q=2, n_kv=2)
+    for kw, msg in ((dict(qkv=qkv.float()), "qkv must be"), (dict(qkv=z(6 * 64, 3).t()), "contiguous CUDA"),
+                    (dict(qkv=z(3, 320)), "qkv must be"), (dict(q_w=z(64)), "both be"), (dict(depth=dep.long()), "depth must"),
+                    (dict(depth=dep[:2].contiguous()), "depth must"), (dict(kc=z(4, 2, 16, 96)), "cache must be"),
+                    (dict(vc=z(4, 2, 16, 64).cpu()), "vc must be"), (dict(pos=pos.long()), "pos must be"),
+                    (dict(sin_t=z(64, 16, t=torch.float32)), "cos and sin"), (dict(q_out=z(3, 120)), "q_out must"),
+                    (dict(q_out=z(128, 3).t()), "q_out must"), (dict(n_kv=1), "cache must be")):
+        with pytest.raises(RuntimeError, match=msg):
+            K.qk_norm_rope_append_rows(**dict(qk, **kw))
+    at = dict(q=z(3, 4, 64), mask=z(3, 1, t=i64), pos=pos, bt=bt, kc=kc, vc=kc, max_ctx=30, out=z(3, 256))
+    for kw, msg in ((dict(q=z(3, 4, 128)), "q must be"), (dict(q=z(3, 4, 64).bfloat16()), "q must be"),
+                    (dict(q=z(3, 64, 4).transpose(1, 2)), "q must be"), (dict(q=z(3, 250)), "must hold"),
+                    (dict(out=z(3, 128)), "must hold"), (dict(mask=z(3, 2, t=i64)), "mask must"),
+                    (dict(mask=z(3, 1, t=torch.int32)), "mask must be"), (dict(max_ctx=0), "max_ctx"),
+                    (dict(workspace=z(64, 2).t()), "contiguous CUDA"), (dict(q=z(3, 6, 64), out=z(3, 384)), "heads-per-group"),
+                    (dict(q=z(1, 256).expand(3, 256)), "q_stride")):
+        with pytest.raises(RuntimeError, match=msg):
+            K.attention_tree(**dict(at, **kw))
+    f = lambda *s: z(*s, t=torch.float32)
+    lp = dict(logits=z(3, 100), tokens=z(3, t=i64), logprobs=f(3), entropy=f(3), top_ids=z(3, 4, t=i64), top_logprobs=f(3, 4))
+    for kw, msg in ((dict(logits=z(3, 100).double()), "fp16, bf16 or fp32"), (dict(logits=z(100, 3).t()), "contiguous rows"),
+                    (dict(tokens=z(3, t=torch.int32)), "tokens must be"), (dict(logprobs=f(2)), "M values"),
+                    (dict(top_logprobs=None), "both be"), (dict(top_ids=z(3, 0, t=i64), top_logprobs=f(3, 0)), "both be"),
+                    (dict(top_ids=z(3, 40, t=i64), top_logprobs=f(3, 40)), "k must"), (dict(tokens=None), "tokens and logprobs")):
+        with pytest.raises(RuntimeError, match=msg):
+            K.token_logprobs(**dict(lp, **kw))
+    ac = dict(tokens=z(3, t=i64), parents=z(3, t=torch.int32), picks=z(3, t=i64), pos=pos, bt=bt, kv=kc,
+              path=z(3, t=torch.int32), count=z(1, t=torch.int32), tok=z(1, t=i64))
+    for kw, msg in ((dict(picks=z(3, t=torch.int32)), "picks must"), (dict(picks=z(2, t=i64)), "picks must"),
+                    (dict(parents=z(3, t=i64)), "parents must be"), (dict(path=z(2, t=torch.int32)), "M values"),
+                    (dict(count=z(2, t=torch.int32)), "count and tok"), (dict(kv=z(4, 2, 16, 96)), "cache must be"),
+                    (dict(kv=z(2, 16, 64)), "cache must be"), (dict(bt=None), "null pointer")):
+        with pytest.raises(RuntimeError, match=msg):
+            K.tree_accept(**dict(ac, **kw))
+    torch.cuda.synchronize()
+
+
+def test_graphs_share_a_workspace_and_streams(K):
+    """Two captured calls of different sizes with one workspace, replayed in turn with eager work (torch's and the ops' own,
+    on another stream with a workspace of its own) between; every replay against the eager result."""
+    cases = []
+    for M, ctx, V in ((30, 900, 40000), (7, 2500, 128256)):
+        q, rows, kc, vc, bt = tree_inputs(M, 16, 4, 128, 16, ctx, 3)
+        x = torch.randn(M, V, generator=gen(V)).half()
+        qd, words, btd, kd, vd, xd = dev(q, T.mask_words(rows), bt, kc, vc, x)
+        cases.append(dict(a=(qd, words, i32(ctx), btd, kd, vd, ctx + M), x=xd, tok=torch.arange(M, device=DEV),
+                          out=torch.empty(M, 16 * 128, dtype=torch.half, device=DEV), lp=torch.empty(M, device=DEV),
+                          ent=torch.empty(M, device=DEV), ids=torch.empty(M, 3, dtype=torch.int64, device=DEV),
+                          top=torch.empty(M, 3, device=DEV)))
+    need = max([K.attention_tree_workspace_bytes(c["x"].size(0), 16, 4, 128, c["a"][6]) for c in cases] +
+               [K.token_logprobs_workspace_bytes(*c["x"].shape, 3) for c in cases])
+    assert need > 0
+    ws = [torch.full((need,), 255, dtype=torch.uint8, device=DEV) for _ in range(2)]
+
+    def go(c, w):
+        K.attention_tree(*c["a"], c["out"], w)
+        K.token_logprobs(c["x"], c["tok"], c["lp"], c["ent"], c["ids"], c["top"], w)
+
+    results = lambda c: [c[k].clone() for k in ("out", "lp", "ent", "ids", "top")]
+    side = torch.cuda.Stream()
+    graphs, want = [], []
+    for c in cases:
+        go(c, ws[0])
+        want.append(results(c))
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            go(c, ws[0])
+        graphs.append(g)
+    for turn in range(3):
+        for i, (c, g) in enumerate(zip(cases, graphs)):
+            for k in ("out", "lp", "ent", "ids", "top"):
+                c[k].zero_()
+            g.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(results(c), want[i])), (turn, i)
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                go(cases[1 - i], ws[1])
+            torch.cuda.current_stream().wait_stream(side)
+            assert all(torch.equal(a, b) for a, b in zip(results(cases[1 - i]), want[1 - i])), (turn, i)
