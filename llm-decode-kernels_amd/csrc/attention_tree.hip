@@ -23,21 +23,23 @@
 //     row-major V tile through the transposing LDS read. One fp16 part of p instead of two: its 2^-11, unbiased and beside
 //     an output that is rounded to fp16 itself, against a half more of the products. The sum of the weights keeps fp32.
 //
-// Masks cost nothing where every column of the wave sees the whole block (all mapped, all before *pos). In the others a
-// lane holds its column's 64 token bits: mapped tokens inside the context, and for tokens from *pos on the node bits of the
-// mask row, shifted to the block. Scores of tokens that are not seen become -inf whatever K holds; their p is an exact 0.
+// Masks cost nothing where every column of the wave sees the whole block: all before *pos, all mapped, which a workgroup asks
+// once for its split (per block 151.8 us instead of 148.0). In the others a lane holds its column's 64 token bits: mapped
+// tokens inside the context, and for tokens from *pos on the node bits of the mask row, shifted to the block. Scores of
+// tokens that are not seen become -inf whatever K holds; their p is an exact 0.
 // Since 0 times NaN or infinity is NaN, check_v zeroes in LDS the V chunks of tokens that do not exist, and those with such
 // values in blocks that reach *pos; the latter are added at the end, value by value, for the columns that see their token.
 //
-// What bounds it (250 nodes at 32768 tokens, 8 x 4 heads of 128: 148 us against 114 at the rate of a large matrix product,
-// 0.91 PFLOP/s): instructions, at two waves per SIMD and a clock that these products lower to 2.0 GHz. Per product a wave
-// issues 4 others of its softmax, 1.5 LDS reads and its share of the addresses; a loop of nothing but that runs a product
-// and those in 45 cycles, the product alone in 33. With blocks of 64 tokens, 156 us: without the exponentials it takes
-// 139, without reading V 142, without both 119 and without loads too 100; the products' own time is 62. 64 columns per
-// wave would halve the reads, but then scores lie in accumulation registers, which the softmax cannot use.
-// 64 nodes at 16001 take 31 (floor 14), of which about 18 are this and the rest launch, first loads and 17 MB of partials.
+// What bounds it (250 nodes at 32768 tokens, 8 x 4 heads of 128: 146 us against 114 at the rate of a large matrix product,
+// 0.93 PFLOP/s): the work beside the products, at the 2.0 GHz that the card keeps up under them. Per product a wave issues 4
+// instructions of its softmax, 1.5 LDS reads and its share of the addresses; a loop of nothing but that, two waves per SIMD,
+// runs a product and those in 45 cycles, the product alone in 33. With blocks of 64 tokens, 156 us: without the exponentials
+// it takes 139, without reading V 142, without both 119 and without loads too 100; the products' own time is 62. Barriers
+// and waits taken out changed nothing. 64 columns per wave would halve the reads, but then scores lie in accumulation
+// registers, which the softmax cannot use.
+// 64 nodes at 16001 take 30 (floor 14), of which about 18 are this and the rest launch, first loads and 17 MB of partials.
 // Small ones are launch, a chain of dependent loads (position, page, K / V: 3 us to the first product), partials and the
-// join: 26 nodes at 4096 16, 5 at 300, unsplit, 7.3.
+// join: 26 nodes at 4096 16, 5 at 300, unsplit, 7.0.
 // No gain: two halves of the workgroup half a block apart, so that one's softmax meets the other's products; a block's
 // weights behind the next one's scores; wave priorities; 168 registers for three waves per SIMD; sums of p by dot products;
 // the first pages looked up ahead of the position; the first two rounds' loads sent together.
@@ -115,6 +117,7 @@ attn_tree_kernel(const TreeArgs a) {
   // by 32 tokens from those of *pos on: the tokens that have V chunks which check_v took out
   constexpr int kBadWords = kTreeMaxNodes / 32 + 1;
   __shared__ uint32_t s_bad[kBadWords];
+  __shared__ int s_holes;  // a page of this split's tokens is not mapped
 
   const int kvh = blockIdx.x, cb = blockIdx.y, split = blockIdx.z;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -141,7 +144,7 @@ attn_tree_kernel(const TreeArgs a) {
   };
 
   // Thread's share of a round: chunk tid % CH of token rows tid / CH + RPI i. Pages are looked up a round ahead of the K / V
-  // loads; tokens without a page, or past ctx, read a row that exists and are zeroed on the way to LDS. UP: a load
+  // loads; tokens without a page, or past ctx, read a row that exists; check_v zeroes it. UP: a load
   // instruction's rows lie in one page, lane i looks up the page of load i, and the base is a scalar.
   const int sch = tid % CH, sr = tid / CH;
   constexpr int RPW = kWave / CH;            // rows per load instruction of a wave
@@ -153,12 +156,12 @@ attn_tree_kernel(const TreeArgs a) {
   const uint32_t row_off = UP ? (lane / CH) * RB : 0;
   const uint32_t k_place = row_off + 16 * (D == 128 ? sch ^ (sr & 15) : sch ^ ((sr >> 1) & 7));
   const uint32_t v_place = row_off + 64 * ((sch >> 2) ^ (D == 128 ? sr & 3 : (sr >> 1) & 1)) + 16 * (sch & 3);
-  constexpr int NB = (BT + 63) / 64;
-  int pg[NP], vpg[NB];    // pages of the loads; of token `lane` of the group's block, by 64
+  int pg[NP];             // pages of the loads
   struct Rows {           // where a round's rows lie (UP: lane i's those of load i)
     uint64_t base[NP];
-    uint32_t ok;          // bit i: this thread's row of load i exists
   };
+  bool whole = true;      // every page of this split's tokens is mapped; uniform
+  auto mapped = [&](int t) __attribute__((always_inline)) { return (unsigned)a.bt[t >> a.log2P] < (unsigned)a.n_pages; };
   auto lookup = [&](int rnd) __attribute__((always_inline)) {
     const int last = ctx - 1;
     if constexpr (UP) {
@@ -170,21 +173,11 @@ attn_tree_kernel(const TreeArgs a) {
   };
   auto locate = [&](int rnd) __attribute__((always_inline)) {  // from the looked-up pages
     Rows w;
-    w.ok = 0;
-    uint64_t maps = 0;
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
       const int t = UP ? rnd * SB + RPW * wave + RPI * (lane % LPT) : rnd * SB + sr + RPI * i;
-      const bool mapped = (unsigned)pg[i] < (unsigned)a.n_pages;
-      w.base[i] = (uint64_t)(uint32_t)(mapped ? pg[i] : 0) * page_bytes + (uint32_t)((t & (P - 1)) * RB);
-      if constexpr (UP)
-        maps = __ballot(mapped);
-      else
-        w.ok |= t < ctx && mapped ? 1u << i : 0u;
-    }
-    if constexpr (UP) {
-#pragma unroll
-      for (int i = 0; i < LPT; ++i) w.ok |= rnd * SB + sr + RPI * i < ctx && (maps >> i & 1) ? 1u << i : 0u;
+      w.base[i] = (uint64_t)(uint32_t)((unsigned)pg[i] < (unsigned)a.n_pages ? pg[i] : 0) * page_bytes +
+                  (uint32_t)((t & (P - 1)) * RB);
     }
     return w;
   };
@@ -207,18 +200,17 @@ attn_tree_kernel(const TreeArgs a) {
   };
   // V chunks that must not meet a p of 0, looked over in LDS by the lane that loaded them: those of tokens that do not exist,
   // and those with NaN or infinity of tokens that not every column sees
-  auto check_v = [&](int rnd, const Rows& w, uint8_t* buf) __attribute__((always_inline)) {
-    const bool reaches = (rnd + 1) * (long long)SB > pos;  // uniform
-    if (!reaches && __all(w.ok == (1u << LPT) - 1)) return;
+  auto check_v = [&](int rnd, uint8_t* buf) __attribute__((always_inline)) {
+    const bool reaches = (rnd + 1) * (long long)SB > min(pos, (long long)ctx);  // uniform
+    if (!reaches && whole) return;
     asm volatile("");  // stays a branch
 #pragma unroll
     for (int i = 0; i < LPT; ++i) {
-      const int row = sr + RPI * i;
+      const int row = sr + RPI * i, t = rnd * SB + row, word = t / 32 - tail;
       u32x4* x = reinterpret_cast<u32x4*>(buf + row * RB + 16 * sch);
-      const bool ok = w.ok >> i & 1;
-      const int word = rnd * (SB / 32) + row / 32 - tail;
-      const bool bad = ok && reaches && word >= 0 && has_nonfinite(*x);
-      if (bad) atomicOr(&s_bad[word], 1u << (row % 32));
+      const bool ok = t < ctx && (whole || mapped(t));
+      const bool bad = ok && word >= 0 && has_nonfinite(*x);
+      if (bad) atomicOr(&s_bad[word], 1u << (t % 32));
       if (!ok || bad) *x = u32x4{0u, 0u, 0u, 0u};
     }
   };
@@ -251,11 +243,6 @@ attn_tree_kernel(const TreeArgs a) {
     return bits;
   };
   auto block_start = [&](int rnd) __attribute__((always_inline)) { return (rnd * KVS + grp) * BT; };
-  auto lookup_block = [&](int rnd) __attribute__((always_inline)) {
-#pragma unroll
-    for (int c = 0; c < NB; ++c) vpg[c] = a.bt[min(block_start(rnd) + 64 * c + lane % BT, ctx - 1) >> a.log2P];
-  };
-
   // ---- a block, by tiles of 32 tokens
   f32x16 sc[2];        // scores of a tile and the next
   h8 ph[2];            // p in fp16: the B operand of the output's products
@@ -273,17 +260,17 @@ attn_tree_kernel(const TreeArgs a) {
   };
   auto block = [&](int rnd, const uint8_t* kb, const uint8_t* vb, auto send) __attribute__((always_inline)) {
     const int t0 = block_start(rnd);
-    bool plain = t0 + BT <= pos;  // every token is seen; uniform per wave
+    // every token is seen; uniform per wave
+    const bool plain = whole && t0 + (long long)BT <= min(pos, (long long)ctx);
+    constexpr int NB = (BT + 63) / 64;
     uint64_t vis[NB];
-#pragma unroll
-    for (int c = 0; c < NB; ++c) {
-      vis[c] = __ballot(t0 + 64 * c + lane % BT < ctx && (unsigned)vpg[c] < (unsigned)a.n_pages && lane < BT);
-      plain = plain && vis[c] == (BT == 32 ? 0xffffffffull : ~0ull);
-    }
     if (!plain) {
       asm volatile("");  // stays a branch
 #pragma unroll
-      for (int c = 0; c < NB; ++c) vis[c] &= seen_bits(t0 + 64 * c);
+      for (int c = 0; c < NB; ++c) {
+        const int t = t0 + 64 * c + lane % BT;
+        vis[c] = __ballot(t < ctx && lane < BT && (whole || mapped(t))) & seen_bits(t0 + 64 * c);
+      }
     }
     int kat = krow + ((h ^ ksw) << 4), vat = vrow + (vsw << 6);
     asm volatile("" : "+v"(kat), "+v"(vat));  // (the chunks' places are worked out per block: all of them held would not fit)
@@ -383,7 +370,7 @@ attn_tree_kernel(const TreeArgs a) {
   };
   auto finish = [&](int rnd, uint8_t* v) __attribute__((always_inline)) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    check_v(rnd, rows, v);
+    if (rnd < r1) check_v(rnd, v);
     __syncthreads();
   };
   auto round = [&](int rnd, auto B) __attribute__((always_inline)) {
@@ -396,10 +383,7 @@ attn_tree_kernel(const TreeArgs a) {
 #pragma unroll
       for (int j = 0; j < NL; ++j)
         if (f == j * NF / NL) start(j, kn, vn);
-      if (f == NF - 1) {
-        lookup(rnd + 2);
-        lookup_block(rnd + 1);
-      }
+      if (f == NF - 1) lookup(rnd + 2);
     });
     pf_fence();
     finish(rnd + 1, vn);
@@ -407,15 +391,20 @@ attn_tree_kernel(const TreeArgs a) {
   if (r0 < r1) {  // uniform
     lookup(r0);
     if (tid < kBadWords) s_bad[tid] = 0u;
+    if (tid == 0) s_holes = 0;
     rows = locate(r0);
 #pragma unroll
     for (int j = 0; j < 2 * LPT; ++j) start(j, s_k0, s_v0);
     pf_fence();  // (loads return in order: what is wanted later goes out later)
-    lookup_block(r0);
     lookup(r0 + 1);
     load_q();
     pf_fence();
-    __syncthreads();  // (s_bad)
+    const int last_page = (min(r1 * SB, ctx) - 1) >> a.log2P;
+    for (int p = (r0 * SB >> a.log2P) + tid; p <= last_page; p += NTH) whole = whole && (unsigned)a.bt[p] < (unsigned)a.n_pages;
+    __syncthreads();  // (s_bad, s_holes)
+    if (!whole) s_holes = 1;
+    __syncthreads();
+    whole = __builtin_amdgcn_readfirstlane(s_holes) == 0;
     finish(r0, s_v0);
     for (int rnd = r0; rnd < r1; rnd += 2) {
       round(rnd, std::false_type{});
