@@ -10,8 +10,8 @@
 // counting, and cut to its k largest, at the end and whenever it is half full; T is then what follows the k-th. With more
 // than one slice the (m, l, s) and k keys of each go to the workspace and a second launch joins them in slice order.
 // Measured (captured, us): 512 x 128256 fp32 45 with one alternative (5.8 TB/s), 63 with 20, 66 with 32; fp16 35, 55, 57;
-// 61 x 128256 fp16 13 with one, 17 with 5, 19 with 20; 1 x 128256 9, 11, 13; 1 x 32000 9, 11, 13 (two launches of a memory
-// round trip each). What the alternatives cost at 512 rows is the barrier per block that the list needs; one slice per
+// 61 x 128256 fp16 13 with one, 17 with 5, 19 with 20; 1 x 128256 9, 10, 13; 1 x 32000 8 (one launch), 10, 13 (two, of a
+// memory round trip each). What the alternatives cost at 512 rows is the barrier per block that the list needs; one slice per
 // row is the fastest there (two 65-79, four 68-83, sixteen 96-114 with 2 to 20), eight of two blocks at 61 rows. Two
 // passes (maximum and sums, then one pass per alternative) took 5175 at 512 x 128256 fp32 with 20.
 // Rows at odd addresses: 16-byte chunks lie on 16-byte boundaries, the first and last one are read value by value.
@@ -456,19 +456,27 @@ logprobs_join_kernel(const void* __restrict__ logits, long long ld, const int64_
                logprobs, entropy, top_ids, top_logprobs, V, k, s_top);
 }
 
-// Blocks of a row: small ones (256 threads, a chunk each) while a launch of full ones would leave CUs idle.
+// Blocks of a row: one workgroup and launch takes up to four full ones (512 threads, 8192 values), two where k asks for a
+// list: 32000 fp16 values with k 1 in 7.9 us for one row and 8.2 for 61, split 8.2 and 10.0 (called eagerly 7.4 and 7.9 : 9.9
+// and 10.2); 16000 with k 5 8.7 and 9.5 : 10.3 and 11.5; past that 64000 with k 1 11.6 : 8.5, 32000 with k 5 11.5 : 10.1.
+// Longer rows are split, in small blocks (256 threads, a chunk each) while a launch of full ones would leave CUs idle; a row
+// that has to run unsplit takes full ones (128256 fp16 values, k 5: 33 us, small ones 74).
 constexpr int kLpFullThreads = 512, kLpSmallThreads = 256;
 constexpr int lp_full_chunks(int dtype) { return dtype == 2 ? 4 : 2; }
 struct LpPlan {
   bool small;
   int blocks, splits;
 };
-LpPlan lp_plan(int M, int V, int dtype) {
+int lp_blocks(int V, int dtype, int size) {  // of `size` 16-byte chunks
   const int epc = dtype == 2 ? 4 : 8;
   const long long chunks = ((long long)V + epc - 1) / epc + 1;  // one more where the row starts inside a chunk
-  auto blocks_of = [&](long long size) { return (int)((chunks + size - 1) / size); };
-  LpPlan p = {false, blocks_of(kLpFullThreads * lp_full_chunks(dtype)), 0};
-  if ((long long)M * p.blocks < 256) p = {true, blocks_of(kLpSmallThreads), 0};
+  return (int)((chunks + size - 1) / size);
+}
+LpPlan lp_unsplit(int V, int dtype) { return {false, lp_blocks(V, dtype, kLpFullThreads * lp_full_chunks(dtype)), 1}; }
+LpPlan lp_plan(int M, int V, int k, int dtype) {
+  LpPlan p = lp_unsplit(V, dtype);
+  if (p.blocks <= (k >= 2 ? 2 : 4)) return p;
+  if ((long long)M * p.blocks < 256) p = {true, lp_blocks(V, dtype, kLpSmallThreads), 0};
   // slices for as many workgroups as are resident at once (two of 512 threads or four of 256 per CU), of equal length
   int want = (p.small ? 1024 : 512) / M;
   want = want < 1 ? 1 : want > kLogprobsMaxSplits ? kLogprobsMaxSplits : want;
@@ -479,8 +487,9 @@ LpPlan lp_plan(int M, int V, int dtype) {
 
 template <class T, int DTYPE>
 void launch_lp(const Logprobs& a, hipStream_t st) {
-  LpPlan p = lp_plan(a.M, a.V, a.dtype);
+  LpPlan p = lp_plan(a.M, a.V, a.k, a.dtype);
   const int S = a.splits;
+  if (S == 1) p = lp_unsplit(a.V, a.dtype);
   Sums* sums = reinterpret_cast<Sums*>(a.ws);
   uint64_t* keys = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(a.ws) + logprobs_sums_bytes(a.M, S));
   auto go = [&](auto kernel, int threads) {
@@ -501,7 +510,7 @@ void launch_lp(const Logprobs& a, hipStream_t st) {
 
 }  // namespace
 
-int token_logprobs_splits(int M, int V, int, int dtype) { return lp_plan(M, V, dtype).splits; }
+int token_logprobs_splits(int M, int V, int k, int dtype) { return lp_plan(M, V, k, dtype).splits; }
 size_t logprobs_sums_bytes(int M, int splits) {
   return ((size_t)M * splits * sizeof(Sums) + 15) & ~(size_t)15;
 }

@@ -311,6 +311,18 @@ def test_token_logprobs(K, dtype, M, V, k):
     check_logprobs(K, x, tokens, k)
 
 
+@pytest.mark.parametrize("M,V,k", [(3, 16376, 4), (3, 16384, 4), (2, 32760, 1), (2, 32768, 1), (2, 32768, 0), (300, 20000, 1),
+                                   (300, 20000, 3)])
+def test_token_logprobs_last_unsplit_sizes(K, M, V, k):
+    """Both sides of the row lengths that one launch takes, with a workspace for as many slices as there are and without."""
+    g = gen(M + V + k)
+    x = (torch.randn(M, V, generator=g) * 2).half()
+    x[0] = 1.0                                            # a row of equal values
+    tokens = torch.randint(0, V, (M,), generator=g).to(DEV)
+    check_logprobs(K, x.to(DEV), tokens, k)
+    assert (K.token_logprobs_workspace_bytes(M, V, k) > 0) == (V in (16384, 32768))
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("offset", [0, 1, 3])
 def test_token_logprobs_strided_rows(K, dtype, offset):
