@@ -30,8 +30,8 @@
 // Since 0 times NaN or infinity is NaN, check_v zeroes in LDS the V chunks of tokens that do not exist, and those with such
 // values in blocks that reach *pos; the latter are added at the end, value by value, for the columns that see their token.
 //
-// What bounds it (250 nodes at 32768 tokens, 8 x 4 heads of 128: 146 us against 114 at the rate of a large matrix product,
-// 0.93 PFLOP/s): the work beside the products, at the 2.0 GHz that the card keeps up under them. Per product a wave issues 4
+// What bounds it (250 nodes at 32768 tokens, 8 x 4 heads of 128: 140-146 us against 114 at the rate of a large matrix product,
+// 0.93-0.97 PFLOP/s): the work beside the products, at the 2.0 GHz that the card keeps up under them. Per product a wave issues 4
 // instructions of its softmax, 1.5 LDS reads and its share of the addresses; a loop of nothing but that, two waves per SIMD,
 // runs a product and those in 45 cycles, the product alone in 33. With blocks of 64 tokens, 156 us: without the exponentials
 // it takes 139, without reading V 142, without both 119 and without loads too 100; the products' own time is 62. Barriers
@@ -39,7 +39,7 @@
 // registers, which the softmax cannot use.
 // 64 nodes at 16001 take 30 (floor 14), of which about 18 are this and the rest launch, first loads and 17 MB of partials.
 // Small ones are launch, a chain of dependent loads (position, page, K / V: 3 us to the first product), partials and the
-// join: 26 nodes at 4096 16, 5 at 300, unsplit, 7.0.
+// join: 26 nodes at 4096 16, 5 at 300, unsplit, 6.7.
 // No gain: two halves of the workgroup half a block apart, so that one's softmax meets the other's products; a block's
 // weights behind the next one's scores; wave priorities; 168 registers for three waves per SIMD; sums of p by dot products;
 // the first pages looked up ahead of the position; the first two rounds' loads sent together.
@@ -111,7 +111,7 @@ attn_tree_kernel(const TreeArgs a) {
   constexpr int kTile = SB * RB;             // bytes of one K (or V) buffer
   // K and V buffers as arrays of their own: the compiler then knows that the loads which fill one in flight touch no other.
   // In the end the groups' accumulators, DT of their 4 DT rows in each.
-  static_assert((KVS - 1) * CW * kWave * 16 * DT <= kTile, "a merge row set fits a buffer");
+  static_assert(KVS * CW * kWave * 16 * DT <= kTile && 4 % KVS == 0, "a merge row set fits a buffer, a wave's rows whole ones");
   __shared__ __align__(16) uint8_t s_k0[kTile], s_k1[kTile], s_v0[kTile], s_v1[kTile];
   __shared__ float s_m[KVS > 1 ? KVS * CW * 32 : 1], s_l[KVS > 1 ? KVS * CW * 32 : 1];
   // by 32 tokens from those of *pos on: the tokens that have V chunks which check_v took out
@@ -445,79 +445,65 @@ attn_tree_kernel(const TreeArgs a) {
     }
   }
   l += __shfl_xor(l, 32, kWave);
-  // ---- merge: groups 1 .. KVS - 1 leave maximum and sum per column and the accumulator per lane in LDS (over the K / V
-  // buffers, which every wave has finished reading at the last barrier); group 0 merges them in group order
+  // ---- output: acc[t][4 q + v] = O[column r][dim 32 t + 8 q + 4 h + v], row 4 t + q of a wave's 4 DT rows of float4. The
+  // groups leave theirs in LDS (over the K / V buffers, which every wave has finished reading at the last barrier), with
+  // maximum and sum per column; then each takes 1 / KVS of the rows, over all groups in order.
+  const int waves = (cols + 31) >> 5;
+  const size_t part = ((size_t)split * a.n_kv + kvh) * waves + (cb * CW + gw);
+  if (a.splits > 1 && r0 >= r1) {  // a split without tokens: the join reads no accumulator of it
+    if (grp == 0 && h == 0 && col < cols) a.part_ml[part * 32 + r] = float2{kTreeNoMax, 0.f};
+    return;
+  }
+  constexpr int kRows = 4 * DT / KVS;
+  float mx = mref, L = l, w[KVS];
+  auto own_row = [&](int i) __attribute__((always_inline)) {
+    return float4{acc[i / 4][4 * (i % 4)], acc[i / 4][4 * (i % 4) + 1], acc[i / 4][4 * (i % 4) + 2], acc[i / 4][4 * (i % 4) + 3]};
+  };
+  auto merge_row = [&](int quarter, int i, int g) __attribute__((always_inline)) {  // row DT quarter + i of group g
+    uint8_t* buf = quarter == 0 ? s_k0 : quarter == 1 ? s_k1 : quarter == 2 ? s_v0 : s_v1;
+    return reinterpret_cast<float4*>(buf) + ((i * KVS + g) * CW + gw) * kWave + lane;
+  };
   if constexpr (KVS > 1) {
-    auto merge_row = [&](int row, int g) -> float4* {  // row (of 4 DT) of group g's accumulators, this wave's columns
-      uint8_t* buf = row / DT == 0 ? s_k0 : row / DT == 1 ? s_k1 : row / DT == 2 ? s_v0 : s_v1;
-      return reinterpret_cast<float4*>(buf) + ((row % DT * (KVS - 1) + g - 1) * CW + gw) * kWave + lane;
-    };
     if (h == 0) {
       s_m[(grp * CW + gw) * 32 + r] = mref;
       s_l[(grp * CW + gw) * 32 + r] = l;
     }
-    if (grp > 0) {
 #pragma unroll
-      for (int i = 0; i < 4 * DT; ++i)
-        *merge_row(i, grp) = float4{acc[i / 4][4 * (i % 4)], acc[i / 4][4 * (i % 4) + 1], acc[i / 4][4 * (i % 4) + 2],
-                                    acc[i / 4][4 * (i % 4) + 3]};
-    }
+    for (int i = 0; i < 4 * DT; ++i) *merge_row(i / DT, i % DT, grp) = own_row(i);
     __syncthreads();
-    if (grp > 0) return;  // uniform per wave; no barrier follows
-    float mx = mref;
 #pragma unroll
-    for (int k = 1; k < KVS; ++k) mx = fmaxf(mx, s_m[(k * CW + gw) * 32 + r]);
-    const float w0 = __builtin_amdgcn_exp2f(mref - mx);  // a group that saw no token weighs 0 beside one that did
-    l *= w0;
+    for (int k = 0; k < KVS; ++k) mx = fmaxf(mx, s_m[(k * CW + gw) * 32 + r]);
+    L = 0.f;
 #pragma unroll
-    for (int t = 0; t < DT; ++t) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) acc[t][i] *= w0;
+    for (int k = 0; k < KVS; ++k) {
+      w[k] = __builtin_amdgcn_exp2f(s_m[(k * CW + gw) * 32 + r] - mx);  // a group that saw no token weighs 0 beside one that did
+      L = fmaf(w[k], s_l[(k * CW + gw) * 32 + r], L);
     }
-#pragma unroll
-    for (int k = 1; k < KVS; ++k) {
-      const float wk = __builtin_amdgcn_exp2f(s_m[(k * CW + gw) * 32 + r] - mx);
-      l = fmaf(wk, s_l[(k * CW + gw) * 32 + r], l);
-#pragma unroll
-      for (int i = 0; i < 4 * DT; ++i) {
-        const float4 o = *merge_row(i, k);
-        f32x16& d = acc[i / 4];
-        d[4 * (i % 4)] = fmaf(wk, o.x, d[4 * (i % 4)]);
-        d[4 * (i % 4) + 1] = fmaf(wk, o.y, d[4 * (i % 4) + 1]);
-        d[4 * (i % 4) + 2] = fmaf(wk, o.z, d[4 * (i % 4) + 2]);
-        d[4 * (i % 4) + 3] = fmaf(wk, o.w, d[4 * (i % 4) + 3]);
-      }
-    }
-    mref = mx;
   }
-  // ---- output: acc[t][4 q + v] = O[column r][dim 32 t + 8 q + 4 h + v]
   if (col >= cols) return;
-  const size_t at = (size_t)m * n_q + hd;
-  if (a.splits == 1) {
-    const float inv = l == 0.f ? 0.f : 1.0f / l;  // a NaN stays
-    f16* dst = a.out + at * D + 4 * h;
-#pragma unroll
-    for (int t = 0; t < DT; ++t) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const f16 o0 = (f16)(acc[t][4 * i] * inv), o1 = (f16)(acc[t][4 * i + 1] * inv);
-        const f16 o2 = (f16)(acc[t][4 * i + 2] * inv), o3 = (f16)(acc[t][4 * i + 3] * inv);
-        *reinterpret_cast<u32x2*>(dst + 32 * t + 8 * i) = u32x2{as_u32(f16x2{o0, o1}), as_u32(f16x2{o2, o3})};
-      }
-    }
-    return;
-  }
-  const int waves = (cols + 31) >> 5;
-  const size_t part = ((size_t)split * a.n_kv + kvh) * waves + (cb * CW + gw);
-  if (h == 0) a.part_ml[part * 32 + r] = float2{mref, l};
-  if (r0 >= r1) return;  // a split without tokens: the join reads no accumulator of it
+  if (a.splits > 1 && grp == 0 && h == 0) a.part_ml[part * 32 + r] = float2{mx, L};
+  const float inv = L == 0.f ? 0.f : 1.0f / L;  // a NaN stays
+  f16* out = a.out + ((size_t)m * n_q + hd) * D + 4 * h;
   float4* dst = a.part_o + part * (DT * 4 * kWave);  // uniform per wave
 #pragma unroll
-  for (int t = 0; t < DT; ++t) {
+  for (int i = 0; i < kRows; ++i) {
+    float4 o;
+    if constexpr (KVS > 1) {
+      o = float4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      store_through16(dst, (uint32_t)(((4 * t + i) * kWave + lane) * 16),
-                      __builtin_bit_cast(u32x4, f4{acc[t][4 * i], acc[t][4 * i + 1], acc[t][4 * i + 2], acc[t][4 * i + 3]}));
+      for (int k = 0; k < KVS; ++k) {
+        const float4 x = *merge_row(grp * (4 / KVS) + i / DT, i % DT, k);
+        o = float4{fmaf(w[k], x.x, o.x), fmaf(w[k], x.y, o.y), fmaf(w[k], x.z, o.z), fmaf(w[k], x.w, o.w)};
+      }
+    } else {
+      o = own_row(i);
+    }
+    const int row = grp * kRows + i;
+    if (a.splits == 1)
+      *reinterpret_cast<u32x2*>(out + 32 * (row >> 2) + 8 * (row & 3)) =
+          u32x2{as_u32(f16x2{(f16)(o.x * inv), (f16)(o.y * inv)}), as_u32(f16x2{(f16)(o.z * inv), (f16)(o.w * inv)})};
+    else
+      store_through16(dst, (uint32_t)((row * kWave + lane) * 16), __builtin_bit_cast(u32x4, f4{o.x, o.y, o.z, o.w}));
   }
 }
 
