@@ -31,12 +31,12 @@
 // values in blocks that reach *pos; the latter are added at the end, value by value, for the columns that see their token.
 //
 // What bounds it (250 nodes at 32768 tokens, 8 x 4 heads of 128: 140-146 us against 114 at the rate of a large matrix product,
-// 0.93-0.97 PFLOP/s): the work beside the products, at the 2.0 GHz that the card keeps up under them. Per product a wave issues 4
-// instructions of its softmax, 1.5 LDS reads and its share of the addresses; a loop of nothing but that, two waves per SIMD,
-// runs a product and those in 45 cycles, the product alone in 33. With blocks of 64 tokens, 156 us: without the exponentials
-// it takes 139, without reading V 142, without both 119 and without loads too 100; the products' own time is 62. Barriers
-// and waits taken out changed nothing, 5% fewer cycles save 2% of the time. 64 columns per wave would halve the reads, but then scores lie in accumulation
-// registers, which the softmax cannot use.
+// 0.93-0.97 PFLOP/s): the work beside the products, at the 2.0 GHz that the card keeps up under them. Per product a wave
+// issues 4 instructions of its softmax, 1.5 LDS reads and its share of the addresses; a loop of nothing but that, two waves
+// per SIMD, runs a product and those in 45 cycles, the product alone in 33. With blocks of 64 tokens, 156 us: without the
+// exponentials it takes 139, without reading V 142, without both 119 and without loads too 100; the products' own time is
+// 62. Barriers and waits taken out changed nothing, 5% fewer cycles save 2% of the time. 64 columns per wave would halve
+// the reads, but then scores lie in accumulation registers, which the softmax cannot use.
 // 64 nodes at 16001 take 30 (floor 14), of which about 18 are this and the rest launch, first loads and 17 MB of partials.
 // Small ones are launch, a chain of dependent loads (position, page, K / V: 3 us to the first product), partials and the
 // join: 26 nodes at 4096 16, 5 at 300, unsplit, 6.7.
