@@ -151,7 +151,8 @@ attn_tree_kernel(const TreeArgs a) {
   constexpr int NP = UP ? 1 : LPT;
   const uint64_t page_bytes = (uint64_t)a.n_kv << a.log2P << (D == 128 ? 8 : 7);
   const uint64_t head_bytes = (uint64_t)kvh << a.log2P << (D == 128 ? 8 : 7);
-  const uint8_t *kp = reinterpret_cast<const uint8_t*>(a.kc) + head_bytes, *vp = reinterpret_cast<const uint8_t*>(a.vc) + head_bytes;
+  const uint8_t* kp = reinterpret_cast<const uint8_t*>(a.kc) + head_bytes;
+  const uint8_t* vp = reinterpret_cast<const uint8_t*>(a.vc) + head_bytes;
   // lane j of a load fills bytes [16 j, 16 j + 16) of the load's rows in LDS: with the chunk that belongs there
   const uint32_t row_off = UP ? (lane / CH) * RB : 0;
   const uint32_t k_place = row_off + 16 * (D == 128 ? sch ^ (sr & 15) : sch ^ ((sr >> 1) & 7));
@@ -186,7 +187,8 @@ attn_tree_kernel(const TreeArgs a) {
                     (uint32_t)__builtin_amdgcn_readlane((int)w.base[0], i)
               : w.base[UP ? 0 : i];
   };
-  auto fetch = [&](const uint8_t* cache, const Rows& w, int i, uint32_t place, uint8_t* buf) __attribute__((always_inline)) {  // load i of a round
+  // load i of a round
+  auto fetch = [&](const uint8_t* cache, const Rows& w, int i, uint32_t place, uint8_t* buf) __attribute__((always_inline)) {
     typedef __attribute__((address_space(1))) const void* gptr;
     typedef __attribute__((address_space(3))) void* lptr;
     lptr at = (lptr)(buf + (RPI * i + RPW * wave) * RB);
@@ -256,7 +258,8 @@ attn_tree_kernel(const TreeArgs a) {
     psum[1] = e == 0 ? p1 : psum[1] + p1;
     const h2 p = __builtin_convertvector(f2{p0, p1}, h2);
     uint32_t pair = __builtin_bit_cast(uint32_t, p);
-    asm volatile("" : "+v"(pair), "+v"(psum[0]), "+v"(psum[1]));  // here, beside the products (148.6 us : 145.2), not where they are used
+    // here, beside the products (148.6 -> 145.2 us), not where they are used
+    asm volatile("" : "+v"(pair), "+v"(psum[0]), "+v"(psum[1]));
     pw[e >> 3][(e & 7) >> 1] = pair;
   };
   auto block = [&](int rnd, const uint8_t* kb, const uint8_t* vb, auto send) __attribute__((always_inline)) {
@@ -667,8 +670,8 @@ static void launch_tree(const TreeAttn& t, hipStream_t st) {
       launch_tree_shape<D, 4, 2, 64>(a, cols, st);
   }
   if (t.splits > 1)
-    hipLaunchKernelGGL(attn_tree_join_kernel<D>, dim3(t.n_kv, waves * (D / 8 / kTreeJoinRows)), dim3(kTreeJoinRows * kWave), 0, st, part_o, a.part_ml,
-                       cols, lhpg, t.n_kv, t.splits, (f16*)t.out);
+    hipLaunchKernelGGL(attn_tree_join_kernel<D>, dim3(t.n_kv, waves * (D / 8 / kTreeJoinRows)), dim3(kTreeJoinRows * kWave),
+                       0, st, part_o, a.part_ml, cols, lhpg, t.n_kv, t.splits, (f16*)t.out);
 }
 
 void launch_attention_tree(const TreeAttn& a, hipStream_t st) {

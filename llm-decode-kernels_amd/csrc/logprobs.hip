@@ -173,7 +173,8 @@ __device__ __forceinline__ void rank_list(const uint64_t* list, int n, uint64_t*
   }
 }
 
-// T: the logits' type; NT: threads; CPT: 16-byte chunks per thread and block; TOP: k >= 2 (otherwise each lane keeps its best key).
+// T: the logits' type; NT: threads; CPT: 16-byte chunks per thread and block; TOP: k >= 2 (otherwise each lane keeps its
+// best key).
 template <class T, int NT, int CPT, bool TOP>
 __global__ void __launch_bounds__(NT, 4)
 logprobs_kernel(const void* __restrict__ logits, long long ld, const int64_t* __restrict__ tokens,

@@ -250,6 +250,25 @@ def test_attention_tree_large_scores(K):
     T.within(run_tree(K, qd, words, i32(ctx), btd, kd, vd, ctx + M), want, bound)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("slope,cap", [(0.004, 384), (0.004, 1500), (0.05, 1500), (0.05, 20000), (-0.02, 5000)])
+def test_attention_tree_rising_scores(K, D, slope, cap):
+    """Scores that rise (or fall) steadily with the position: the reference of the weights moves again and again, by small
+    steps and by large ones, and each column's sum and output with it."""
+    M, n_q, n_kv = 70, 8, 2
+    ctx = min(900, cap - M)
+    q, rows, kc, vc, bt = tree_inputs(M, n_q, n_kv, D, 16, ctx, 3, seed=21)
+    q = (q * 0.1 + 0.5).half()
+    kc = kc * 0.2
+    for t in range(ctx + M):
+        c = T.token_row(bt.tolist(), t, 16, kc.size(0))
+        kc[c[0], :, c[1]] += slope * t
+    want, bound = T.attention_tree(q, rows, ctx, bt, kc, vc)
+    qd, words, btd, kd, vd = dev(q, T.mask_words(rows), bt, kc, vc)
+    for ws in ("full", "none"):
+        T.within(run_tree(K, qd, words, i32(ctx), btd, kd, vd, cap, ws), want, bound)
+
+
 def test_attention_tree_replays_at_other_positions(K):
     """One captured call serves every position up to max_ctx, on a side stream's capture, with eager work between."""
     M, n_q, n_kv, D, cap = 24, 32, 8, 128, 3000
