@@ -7,8 +7,9 @@
 // own running (m, l, s), rescaled once per block, and the lanes meet once at the end. The k largest need no second look at
 // the data: in the first block the lanes form 64 groups, and the k-th largest of the groups' maxima is a lower bound T of
 // the k-th largest value, so the values >= T go to a list in LDS, hardly more than k of a block. The list is ranked by
-// counting, and cut to its k largest, at the end and whenever it is half full; T is then what follows the k-th. With more
-// than one slice the (m, l, s) and k keys of each go to the workspace and a second launch joins them in slice order.
+// counting, and cut to its k largest, at the end, whenever it is half full and behind a block whose candidates it could not
+// take; T is then what follows the k-th. With more than one slice the (m, l, s) and k keys of each go to the workspace and
+// a second launch joins them in slice order.
 // Measured (captured, us): 512 x 128256 fp32 45 with one alternative (5.8 TB/s), 63 with 20, 66 with 32; fp16 35, 55, 57;
 // 61 x 128256 fp16 13 with one, 17 with 5, 19 with 20; 1 x 128256 9, 10, 13; 1 x 32000 8 (one launch), 10, 13 (two, of a
 // memory round trip each). What the alternatives cost at 512 rows is the barrier per block that the list needs; one slice per
@@ -322,7 +323,8 @@ logprobs_kernel(const void* __restrict__ logits, long long ld, const int64_t* __
       hits = 0;
 #pragma unroll
       for (int w = 0; w < kLpWaves; ++w) hits += s_hits[b & 1][w];
-      if (n + hits <= kLpList) {  // uniform
+      const bool over = n + hits > kLpList;  // uniform
+      if (!over) {
         n += hits;
       } else {
         // NaN, or more candidates than the list takes (equal values by the hundred): the block's k largest one after the
@@ -356,7 +358,9 @@ logprobs_kernel(const void* __restrict__ logits, long long ld, const int64_t* __
         n += found;
         __syncthreads();
       }
-      if (n > kLpList / 2 || b + 1 == b1 || hits > kLpList) {  // uniform: the list's k largest, and T from the k-th
+      // uniform: the list's k largest, and T from the k-th. Also behind an overflow, which leaves s_n past the list's end:
+      // places in the next block start at the s_n that is set here.
+      if (n > kLpList / 2 || b + 1 == b1 || over) {
         rank_list(s_list, n, s_top, k);
         __syncthreads();
         const uint64_t kth = s_top[k - 1];

@@ -381,6 +381,42 @@ def test_token_logprobs_special_rows(K, dtype):
         check_logprobs(K, x[r:r + 1], tokens[r:r + 1], k)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+def test_token_logprobs_raised_regions(K, dtype):
+    """Rows of several blocks (8192 values each, 1024 or 2048 where they are split) whose candidates come in crowds: some
+    dozens of equal values in the first block, 250 to 520 larger ones in the second, the winners behind them. Whether the
+    second crowd fits the list beside the first or not, none of the winners is lost and none comes twice."""
+    V, counts = 4 * 8192 + 5, list(range(250, 521, 3))
+    g = gen(11)
+    x = torch.randn(len(counts), V, generator=g) * 0.1 - 5
+    for r, c in enumerate(counts):
+        x[r, torch.randperm(8192, generator=g)[:33 + 37 * r % 200]] = 1.0
+        x[r, 8192 + torch.randperm(8192, generator=g)[:c]] = 2.0
+        x[r, 24576 + 80 * r + torch.arange(5)] = torch.arange(20, 25).float()
+        x[r, 16384 + r] = 18.0
+    x = x.to(dtype)
+    tokens = 24576 + 80 * torch.arange(len(counts))
+    given, gb, ent, eb, order, tops, tb = T.token_logprobs(x, tokens, 32)
+    x, tokens = x.to(DEV), tokens.to(DEV)
+    for k in (2, 5, 20, 32):
+        for ws in (True, False):
+            lp, e, ids, top = run_logprobs(K, x, tokens, k, ws)
+            assert torch.equal(ids.cpu(), order[:, :k]), (k, ws)
+            T.within(top, tops[:, :k], tb[:, :k])
+            T.within(lp, given, gb)
+            T.within(e, ent, eb)
+
+
+def test_token_logprobs_rows_whose_level_shifts(K):
+    """Normal rows whose mean moves from region to region, as where a mask or a language favours a range of ids."""
+    V, k = 5 * 8192, 20
+    g = gen(12)
+    shift = (torch.rand(200, V // 4096, generator=g) * 4).repeat_interleave(4096, 1)
+    x = (torch.randn(200, V, generator=g) + shift).to(DEV)
+    tokens = torch.randint(0, V, (200,), generator=g).to(DEV)
+    check_logprobs(K, x, tokens, k)
+
+
 def test_token_logprobs_outputs_alone(K):
     """Any output may be left out."""
     x = (torch.randn(4, 2000, generator=gen(0)) * 3).half().to(DEV)
