@@ -130,7 +130,8 @@ __device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY
 __device__ __forceinline__ void move_sums(Sums& a, float M) {  // M >= a.m
   const float d = a.m == -INFINITY ? 0.f : a.m - finite_or_zero(M);
   const float w = __builtin_amdgcn_exp2f(d * kLog2e);
-  a.s = w * fmaf(d, a.l, a.s);
+  // w is 0 below -200; there d l may pass the range (sums about a mask's lowest value), and 0 times infinity is NaN
+  a.s = w * fmaf(fmaxf(d, -200.f), a.l, a.s);
   a.l *= w;
   a.m = M;
 }

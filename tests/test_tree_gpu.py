@@ -417,6 +417,30 @@ def test_token_logprobs_rows_whose_level_shifts(K):
     check_logprobs(K, x, tokens, k)
 
 
+@pytest.mark.parametrize("dtype,low", [(t, l) for t in (torch.float16, torch.bfloat16, torch.float32)
+                                       for l in (torch.finfo(t).min, -3e4 if t is torch.float16 else -1e38)])
+def test_token_logprobs_masked_regions(K, dtype, low):
+    """Whole regions at the type's lowest value, or near it, as a mask leaves them: a lane, a wave, a block, a slice or all
+    values but one see nothing else, ahead of the finite values or behind them. Each weighs nothing beside a finite value
+    and adds nothing to the entropy."""
+    V = 3 * 8192 + 100
+    x = torch.randn(8, V, generator=gen(9)) * 2
+    x[0, :8192] = low                              # the first block
+    x[1, 8192:] = low                              # all but the first
+    x[2, 1:] = low                                 # all but the first value
+    x[3, :-1] = low                                # all but the last
+    x[4, 9000:20000] = low                         # blocks in part
+    x[5, (torch.arange(V) // 16) % 3 != 0] = low   # by runs of 16
+    x[6, :20000] = low
+    x[6, 7000] = 1.0
+    x[7] = low
+    x[7, 100], x[7, 20000] = 3.0, 2.0
+    x = x.to(dtype).to(DEV)
+    tokens = torch.tensor([8192, 3, 0, V - 1, 10000, 0, 7000, 20000], device=DEV)
+    for k in (0, 1, 5):
+        check_logprobs(K, x, tokens, k)
+
+
 def test_token_logprobs_outputs_alone(K):
     """Any output may be left out."""
     x = (torch.randn(4, 2000, generator=gen(0)) * 3).half().to(DEV)
