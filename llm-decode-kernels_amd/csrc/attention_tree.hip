@@ -15,10 +15,13 @@
 // Per tile of 32 tokens, on v_mfma_f32_32x32x16_f16:
 //   * S^T = K . Q^T: A = the tile's rows of K from LDS, B = the wave's Q columns (registers). Lane (h, r) receives column r,
 //     tokens 8 q + 4 h + v: a column's scores, sum and output live in the lane pair (r, r + 32).
-//   * p = 2^(s - ref + kTreeLift), scale and log2 e in one multiplier, while the next tile's products run. The reference is
-//     a maximum of scores seen so far, not the running one: it moves to the tile's maximum where a lane's sum of p passes
-//     kTreeMost, so that p fits fp16 and no maximum is taken otherwise; what fp16 cannot hold of a small p is 2^-32 of p at
-//     the reference. (With a maximum per block of 64 tokens ahead of its weights 156.7 -> 153.3 us.)
+//   * p = 2^(c2 (s - ref) + kTreeLift), c2 = log2(e) / sqrt(D), as c2 s + lift: one multiply-add, while the next tile's
+//     products run. The reference is a maximum of scores seen so far, not the running one: it moves to the tile's maximum
+//     where a lane's sum of p passes kTreeMost, so that p fits fp16 and no maximum is taken otherwise; what fp16 cannot hold
+//     of a small p is 2^-32 of p at the reference. (With a maximum per block of 64 tokens ahead of its weights 156.7 -> 153.3
+//     us.) lift holds c2 ref to half a step of fp32. From kTreeFar on that would be more than p's own half step in fp16 (and at
+//     2^26 p could overflow at the reference): there lift is infinite, every tile's first weights overflow, and the second
+//     ones are taken from s - ref, exact at the reference.
 //   * O^T += V^T . P^T: the score accumulator, rounded to fp16 to nearest, is the B operand as it is; V^T comes out of the
 //     row-major V tile through the transposing LDS read. One fp16 part of p instead of two: its 2^-11, unbiased and beside
 //     an output that is rounded to fp16 itself, against a half more of the products. The sum of the weights keeps fp32.
@@ -63,6 +66,7 @@ namespace {
 constexpr float kTreeNoMax = -1e30f;
 constexpr float kTreeLift = 7.0f;     // p's exponent at the reference maximum
 constexpr float kTreeMost = 32768.f;  // the reference moves where a lane's sum of p over a tile passes this: p fits fp16
+constexpr float kTreeFar = 4096.f;    // a reference further from 0 than this (log2 units) is taken off the score itself
 
 constexpr int kTreeMaxSplits = 64;
 
@@ -217,7 +221,8 @@ attn_tree_kernel(const TreeArgs a) {
     }
   };
 
-  float mref = kTreeNoMax, l = 0.f;  // the column's reference maximum (log2 units); this lane's half of its sum
+  // the column's reference maximum (a score), kTreeLift less its c2 fold (infinite: far), and this lane's half of its sum
+  float ref = kTreeNoMax, lift = -kTreeNoMax, l = 0.f;
   f32x16 acc[DT];
 #pragma unroll
   for (int t = 0; t < DT; ++t) acc[t] = f32x16{};
@@ -252,8 +257,9 @@ attn_tree_kernel(const TreeArgs a) {
   u32x4 ka[RA + 1];
   h8 va[2][DT];        // V fragments: 16 tokens, in two sets
   float psum[2];       // sums of p over the tile
-  auto weigh = [&](const f32x16& s, int e, float lift) __attribute__((always_inline)) {  // p of scores e, e + 1
-    const float p0 = __builtin_amdgcn_exp2f(fmaf(s[e], a.c2, lift)), p1 = __builtin_amdgcn_exp2f(fmaf(s[e + 1], a.c2, lift));
+  // p of scores x, y, the scores e, e + 1 of a tile
+  auto weigh = [&](float x, float y, int e, float lift) __attribute__((always_inline)) {
+    const float p0 = __builtin_amdgcn_exp2f(fmaf(x, a.c2, lift)), p1 = __builtin_amdgcn_exp2f(fmaf(y, a.c2, lift));
     psum[0] = e == 0 ? p0 : psum[0] + p0;
     psum[1] = e == 0 ? p1 : psum[1] + p1;
     const h2 p = __builtin_convertvector(f2{p0, p1}, h2);
@@ -319,17 +325,16 @@ attn_tree_kernel(const TreeArgs a) {
 #pragma unroll
     for (int tt = 0; tt < NT; ++tt) {
       const f32x16& s = sc[tt & 1];
-      float lift = kTreeLift - mref;
       read_v(2 * tt);
       if (tt + 1 < NT) {
         scores(tt + 1, [&](int k) __attribute__((always_inline)) {
           constexpr int NE = 16 / KS;
 #pragma unroll
-          for (int e = 0; e < NE; e += 2) weigh(s, NE * k + e, lift);
+          for (int e = 0; e < NE; e += 2) weigh(s[NE * k + e], s[NE * k + e + 1], NE * k + e, lift);
         });
       } else {
 #pragma unroll
-        for (int e = 0; e < 16; e += 2) weigh(s, e, lift);
+        for (int e = 0; e < 16; e += 2) weigh(s[e], s[e + 1], e, lift);
       }
       float sum = psum[0] + psum[1];
       if (__any(!(sum <= kTreeMost))) {  // the reference moves to this tile's maximum where that is higher
@@ -337,19 +342,19 @@ attn_tree_kernel(const TreeArgs a) {
         float mx = s[0];
 #pragma unroll
         for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
-        mx = fmaxf(mx, __shfl_xor(mx, 32, kWave)) * a.c2;
-        const float mn = fmaxf(mref, mx);
-        const float alpha = __builtin_amdgcn_exp2f(mref - mn);  // 1 for a column that stays
-        mref = mn;
+        mx = fmaxf(ref, fmaxf(mx, __shfl_xor(mx, 32, kWave)));
+        const float alpha = __builtin_amdgcn_exp2f((ref - mx) * a.c2);  // 1 for a column that stays
+        if (mx != ref) lift = fabsf(mx * a.c2) > kTreeFar ? INFINITY : kTreeLift - mx * a.c2;
+        ref = mx;
+        const float off = lift == INFINITY ? ref : 0.f, up = lift == INFINITY ? kTreeLift : lift;
         l *= alpha;
 #pragma unroll
         for (int t = 0; t < DT; ++t) {
 #pragma unroll
           for (int i = 0; i < 16; ++i) acc[t][i] *= alpha;
         }
-        lift = kTreeLift - mref;
-  #pragma unroll
-        for (int e = 0; e < 16; e += 2) weigh(s, e, lift);
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) weigh(s[e] - off, s[e + 1] - off, e, up);
         sum = psum[0] + psum[1];
       }
       l += sum;
@@ -421,20 +426,22 @@ attn_tree_kernel(const TreeArgs a) {
       uint32_t bad = __builtin_amdgcn_readfirstlane(s_bad[word - tail]);
       if (bad == 0) continue;
       const uint64_t vis = seen_bits(word * 32);
+      // the scores of the 32 tokens, as in the loop and so the same to the last bit (tokens that do not exist: of any row)
+      const int tk = min(word * 32 + r, ctx - 1), pk = a.bt[tk >> a.log2P];
+      const size_t kat = ((((size_t)((unsigned)pk < (unsigned)a.n_pages ? pk : 0) * a.n_kv + kvh) << a.log2P) + (tk & (P - 1))) * D;
+      f32x16 st = {};
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+        st = mfma32x32(__builtin_bit_cast(h8, *reinterpret_cast<const u32x4*>(a.kc + kat + 16 * k + 8 * h)), q[k], st);
       for (; bad != 0; bad &= bad - 1) {
         const int i = __builtin_ctz(bad), t = word * 32 + i;
         const int page = a.bt[t >> a.log2P];  // a token in this set is mapped and inside the context
         const size_t at = ((((size_t)page * a.n_kv + kvh) << a.log2P) + (t & (P - 1))) * D;
-        float dot = 0.f;  // this lane's half of the dims
+        float dot = 0.f;  // in element 4 (i / 8) + i % 4 of the half i / 4 % 2
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          const u32x4 k = *reinterpret_cast<const u32x4*>(a.kc + at + 16 * s + 8 * h);
-          const u32x4 qs = __builtin_bit_cast(u32x4, q[s]);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) dot = dot2(as_f16x2(k[j]), as_f16x2(qs[j]), dot);
-        }
-        dot += __shfl_xor(dot, 32, kWave);
-        const float p = __builtin_amdgcn_exp2f(fmaf(dot, a.c2, kTreeLift - mref));
+        for (int e = 0; e < 16; ++e) dot = e == 4 * (i >> 3) + (i & 3) ? st[e] : dot;
+        dot = __shfl(dot, r + 32 * ((i >> 2) & 1), kWave);
+        const float p = __builtin_amdgcn_exp2f(lift == INFINITY ? fmaf(dot - ref, a.c2, kTreeLift) : fmaf(dot, a.c2, lift));
         const bool see = (vis >> i) & 1;
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
@@ -459,7 +466,7 @@ attn_tree_kernel(const TreeArgs a) {
     return;
   }
   constexpr int kRows = 4 * DT / KVS;
-  float mx = mref, L = l, w[KVS];
+  float mx = ref, L = l, w[KVS];
   auto own_row = [&](int i) __attribute__((always_inline)) {
     return float4{acc[i / 4][4 * (i % 4)], acc[i / 4][4 * (i % 4) + 1], acc[i / 4][4 * (i % 4) + 2], acc[i / 4][4 * (i % 4) + 3]};
   };
@@ -469,7 +476,7 @@ attn_tree_kernel(const TreeArgs a) {
   };
   if constexpr (KVS > 1) {
     if (h == 0) {
-      s_m[(grp * CW + gw) * 32 + r] = mref;
+      s_m[(grp * CW + gw) * 32 + r] = ref;
       s_l[(grp * CW + gw) * 32 + r] = l;
     }
 #pragma unroll
@@ -480,7 +487,8 @@ attn_tree_kernel(const TreeArgs a) {
     L = 0.f;
 #pragma unroll
     for (int k = 0; k < KVS; ++k) {
-      w[k] = __builtin_amdgcn_exp2f(s_m[(k * CW + gw) * 32 + r] - mx);  // a group that saw no token weighs 0 beside one that did
+      // a group that saw no token weighs 0 beside one that did
+      w[k] = __builtin_amdgcn_exp2f((s_m[(k * CW + gw) * 32 + r] - mx) * a.c2);
       L = fmaf(w[k], s_l[(k * CW + gw) * 32 + r], L);
     }
   }
@@ -519,7 +527,7 @@ constexpr int kTreeJoinRows = 4;
 template <int D>
 __global__ void __launch_bounds__(kTreeJoinRows * kWave)
 attn_tree_join_kernel(const float4* __restrict__ part_o, const float2* __restrict__ part_ml, int cols, int lhpg, int n_kv,
-                      int splits, f16* __restrict__ out) {
+                      int splits, float c2, f16* __restrict__ out) {
   constexpr int kRows = kTreeJoinRows, kBatch = 8, kGroups = 2 * kRows;  // kGroups threads share a column's maxima and sums
   __shared__ float s_w[kTreeMaxSplits][32];          // a split's weight in a column, -1 where it saw no token
   __shared__ float s_l[32];
@@ -554,7 +562,7 @@ attn_tree_join_kernel(const float4* __restrict__ part_o, const float2* __restric
     for (int j = 0; j < kMl; ++j) {
       const int s = g + kGroups * j;
       const bool saw = ml[j].x != kTreeNoMax || ml[j].y != 0.f;  // (a NaN sum counts)
-      const float w = __builtin_amdgcn_exp2f(ml[j].x - mx);
+      const float w = __builtin_amdgcn_exp2f((ml[j].x - mx) * c2);
       L = saw ? fmaf(w, ml[j].y, L) : L;
       if (s < splits) s_w[s][c] = saw ? w : -1.f;
     }
@@ -671,7 +679,7 @@ static void launch_tree(const TreeAttn& t, hipStream_t st) {
   }
   if (t.splits > 1)
     hipLaunchKernelGGL(attn_tree_join_kernel<D>, dim3(t.n_kv, waves * (D / 8 / kTreeJoinRows)), dim3(kTreeJoinRows * kWave),
-                       0, st, part_o, a.part_ml, cols, lhpg, t.n_kv, t.splits, (f16*)t.out);
+                       0, st, part_o, a.part_ml, cols, lhpg, t.n_kv, t.splits, a.c2, (f16*)t.out);
 }
 
 void launch_attention_tree(const TreeAttn& a, hipStream_t st) {

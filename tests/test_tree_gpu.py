@@ -269,6 +269,93 @@ def test_attention_tree_rising_scores(K, D, slope, cap):
         T.within(run_tree(K, qd, words, i32(ctx), btd, kd, vd, cap, ws), want, bound)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("M,ctx,cap", [(1, 0, 100), (20, 300, 384), (20, 700, 1500), (20, 700, 5000), (80, 700, 1500),
+                                       (80, 900, 20000)])
+@pytest.mark.parametrize("size", [30.0, 1000.0, 16384.0, 60000.0, -2000.0, -60000.0])
+def test_attention_tree_far_scores(K, D, M, ctx, cap, size):
+    """Scores as large as finite q and K make them, up to 2^36 in units of log2. Equal ones weigh alike, whatever their
+    size: the output is the mean of V over the tokens that a node sees, V itself where it sees one. A token whose score lies
+    as far above them has all the weight, wherever it stands.
+
+    Tolerance: fp16's half step of the output and of the weight (the same one for every token), and the fp32 sums, a chain of
+    at most n + 64 terms of |v| / n."""
+    n_q, n_kv = 8, 2
+    q, rows, kc, vc, bt = tree_inputs(M, n_q, n_kv, D, 16, ctx, 3, seed=31)
+    g = gen(6)
+    q = (abs(size) * (0.5 + 0.5 * torch.rand(q.shape, generator=g))).half()
+    kc = (size * (0.5 + 0.5 * torch.rand(n_kv, 1, D, generator=g))).half().expand_as(kc).contiguous()
+    if M > 1:
+        rows[7] = False
+        rows[7, 7] = True                                      # one node and no other
+    cells = [T.token_row(bt.tolist(), t, 16, kc.size(0)) for t in range(ctx + M)]
+    v = torch.stack([vc[c[0], :, c[1]] for c in cells]).double()                # [tokens, n_kv, D]
+    qd, words, btd = dev(q, T.mask_words(rows), bt)
+
+    def expect(see):                                                            # bool [M, tokens]
+        n = see.sum(1).clamp(min=1)[:, None, None]
+        mean = torch.einsum("mt,thd->mhd", see.double(), v) / n
+        size_ = torch.einsum("mt,thd->mhd", see.double(), v.abs()) / n
+        bound = 2.0 ** -11 * mean.abs() + (2.0 ** -11 + 2.0 ** -24 * (n + 64)) * size_ + 2.0 ** -25
+        wide = lambda x: x.repeat_interleave(n_q // n_kv, 1).reshape(M, -1)
+        return wide(mean), wide(bound)
+
+    see = torch.cat([torch.ones(M, ctx, dtype=torch.bool), rows], 1)
+    for ws in ("full", "none"):
+        T.within(run_tree(K, qd, words, i32(ctx), btd, *dev(kc, vc), cap, ws), *expect(see))
+    for t in ([5, ctx // 2, ctx - 1] if ctx else []):
+        above = kc.clone()
+        above[cells[t][0], :, cells[t][1]] = 65504.0 if size > 0 else 0.0       # the score of one token lies above the others
+        only = torch.zeros_like(see)
+        only[:, t] = True
+        T.within(run_tree(K, qd, words, i32(ctx), btd, *dev(above, vc), cap), *expect(only))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("cap", [384, 1500, 20000])
+@pytest.mark.parametrize("size", [3.0, 30000.0, -30000.0])
+def test_attention_tree_far_scores_beside_nan(K, D, cap, size):
+    """Equal scores, large ones among them, and a NaN in V of one node and an infinity in V of another: only their element is
+    lost to the nodes that see them, the others are the mean. Tolerance as for far scores."""
+    M, n_q, n_kv, ctx = 20, 8, 2, 77
+    q, rows, kc, vc, bt = tree_inputs(M, n_q, n_kv, D, 16, ctx, 3, seed=31)
+    g = gen(7)
+    q = (abs(size) * (0.5 + 0.5 * torch.rand(q.shape, generator=g))).half()
+    kc = (size * (0.5 + 0.5 * torch.rand(n_kv, 1, D, generator=g))).half().expand_as(kc).contiguous()
+    cells = [T.token_row(bt.tolist(), t, 16, kc.size(0)) for t in range(ctx + M)]
+    v = torch.stack([vc[c[0], :, c[1]] for c in cells]).double()
+    for node, bad in ((2, float("nan")), (5, float("inf"))):
+        c = cells[ctx + node]
+        vc[c[0], :, c[1], 9] = bad
+    see = torch.cat([torch.ones(M, ctx, dtype=torch.bool), rows], 1).double()
+    n = see.sum(1)[:, None, None]
+    mean, size_ = (torch.einsum("mt,thd->mhd", see, x).repeat_interleave(n_q // n_kv, 1) / n for x in (v, v.abs()))
+    bound = 2.0 ** -11 * mean.abs() + (2.0 ** -11 + 2.0 ** -24 * (n + 64)) * size_ + 2.0 ** -25
+    mean[rows[:, 5], :, 9] = float("inf")
+    mean[rows[:, 2], :, 9] = float("nan")
+    assert 0 < int(rows[:, 2].sum()) < M and 0 < int(rows[:, 5].sum()) < M
+    for ws in ("full", "none"):
+        out = run_tree(K, *dev(q, T.mask_words(rows)), i32(ctx), *dev(bt, kc, vc), cap, ws)
+        T.within(out, mean.view(M, -1), bound.reshape(M, -1))
+
+
+def test_attention_tree_infinite_scores(K):
+    """A score of +infinity, or NaN, leaves no distribution: NaN for the nodes that see it, and for no other."""
+    M, n_q, n_kv, D, ctx = 40, 8, 2, 64, 200
+    q, rows, kc, vc, bt = tree_inputs(M, n_q, n_kv, D, 16, ctx, 3, seed=5)
+    q = q.abs() + 0.5
+    want, bound = T.attention_tree(q, rows, ctx, bt, kc, vc)
+    for bad in (float("inf"), float("nan")):
+        k = kc.clone()
+        c = T.token_row(bt.tolist(), ctx + 5, 16, kc.size(0))
+        k[c[0], :, c[1], 1] = bad
+        qd, words, btd, kd, vd = dev(q, T.mask_words(rows), bt, k, vc)
+        out = run_tree(K, qd, words, i32(ctx), btd, kd, vd, ctx + M)
+        seen = rows[:, 5]
+        assert 0 < int(seen.sum()) < M and bool(torch.isnan(out[seen.to(DEV)]).all())
+        T.within(out.cpu()[~seen], want[~seen], bound[~seen])
+
+
 def test_attention_tree_replays_at_other_positions(K):
     """One captured call serves every position up to max_ctx, on a side stream's capture, with eager work between."""
     M, n_q, n_kv, D, cap = 24, 32, 8, 128, 3000
