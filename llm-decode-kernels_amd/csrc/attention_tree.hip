@@ -17,11 +17,11 @@
 //     tokens 8 q + 4 h + v: a column's scores, sum and output live in the lane pair (r, r + 32).
 //   * p = 2^(c2 (s - ref) + kTreeLift), c2 = log2(e) / sqrt(D), as c2 s + lift: one multiply-add, while the next tile's
 //     products run. The reference is a maximum of scores seen so far, not the running one: it moves to the tile's maximum
-//     where a lane's sum of p passes kTreeMost, so that p fits fp16 and no maximum is taken otherwise; what fp16 cannot hold
-//     of a small p is 2^-32 of p at the reference. (With a maximum per block of 64 tokens ahead of its weights 156.7 -> 153.3
-//     us.) lift holds c2 ref to half a step of fp32. From kTreeFar on that would be more than p's own half step in fp16 (and at
-//     2^26 p could overflow at the reference): there lift is infinite, every tile's first weights overflow, and the second
-//     ones are taken from s - ref, exact at the reference.
+//     where a sum of p in the column's two lanes passes kTreeMost, so that p fits fp16 and no maximum is taken otherwise;
+//     what fp16 cannot hold of a small p is 2^-32 of p at the reference. (With a maximum per block of 64 tokens ahead of its
+//     weights 156.7 -> 153.3 us.) lift holds c2 ref to half a step of fp32. From kTreeFar on that would be more than p's own
+//     half step in fp16 (and at 2^26 p could overflow at the reference): there lift is infinite, every tile's first weights
+//     overflow, and the second ones are taken from s - ref, exact at the reference.
 //   * O^T += V^T . P^T: the score accumulator, rounded to fp16 to nearest, is the B operand as it is; V^T comes out of the
 //     row-major V tile through the transposing LDS read. One fp16 part of p instead of two: its 2^-11, unbiased and beside
 //     an output that is rounded to fp16 itself, against a half more of the products. The sum of the weights keeps fp32.
@@ -343,6 +343,9 @@ attn_tree_kernel(const TreeArgs a) {
 #pragma unroll
         for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
         mx = fmaxf(ref, fmaxf(mx, __shfl_xor(mx, 32, kWave)));
+        // (a column decides by itself: its result does not depend on what else shares its wave)
+        const int over = !(sum <= kTreeMost);
+        mx = over | __shfl_xor(over, 32, kWave) ? mx : ref;
         const float alpha = __builtin_amdgcn_exp2f((ref - mx) * a.c2);  // 1 for a column that stays
         if (mx != ref) lift = fabsf(mx * a.c2) > kTreeFar ? INFINITY : kTreeLift - mx * a.c2;
         ref = mx;

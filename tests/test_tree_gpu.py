@@ -356,6 +356,33 @@ def test_attention_tree_infinite_scores(K):
         T.within(out.cpu()[~seen], want[~seen], bound[~seen])
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("cap", [384, 1500, 20000])
+def test_attention_tree_node_beside_others(K, D, cap):
+    """A node's output does not depend, not in a bit, on what the nodes hold that it does not attend: their queries, keys and
+    values change (scores that rise much faster than its own), the tokens that it sees do not."""
+    M, n_q, n_kv = 24, 8, 2
+    ctx = min(900, cap - M)
+    q, rows, kc, vc, bt = tree_inputs(M, n_q, n_kv, D, 16, ctx, 3, seed=23)
+    q = (q * 0.1 + 0.5).half()
+    for t in range(ctx + M):
+        c = T.token_row(bt.tolist(), t, 16, kc.size(0))
+        kc[c[0], :, c[1]] = kc[c[0], :, c[1]] * 0.2 + 0.01 * t
+    words, btd = dev(T.mask_words(rows), bt)
+    first = run_tree(K, q.to(DEV), words, i32(ctx), btd, *dev(kc, vc), cap)
+    node = 5
+    other = [j for j in range(M) if not rows[node, j]]
+    for j in other:
+        c = T.token_row(bt.tolist(), ctx + j, 16, kc.size(0))
+        kc[c[0], :, c[1]] *= 3
+        vc[c[0], :, c[1]] += 1
+        q[j] *= 0.05 * (j + 1)
+    second = run_tree(K, q.to(DEV), words, i32(ctx), btd, *dev(kc, vc), cap)
+    same = [i for i in range(M) if not bool(rows[i, other].any())]
+    assert node in same and len(other) > 8
+    assert torch.equal(first[same], second[same]) and not torch.equal(first, second)
+
+
 def test_attention_tree_replays_at_other_positions(K):
     """One captured call serves every position up to max_ctx, on a side stream's capture, with eager work between."""
     M, n_q, n_kv, D, cap = 24, 32, 8, 128, 3000
