@@ -182,7 +182,7 @@ attn_tree_kernel(const TreeArgs a) {
     for (int i = 0; i < NP; ++i) {
       const int t = UP ? rnd * SB + RPW * wave + RPI * (lane % LPT) : rnd * SB + sr + RPI * i;
       w.base[i] = (uint64_t)(uint32_t)((unsigned)pg[i] < (unsigned)a.n_pages ? pg[i] : 0) * page_bytes +
-                  (uint32_t)((t & (P - 1)) * RB);
+                  (uint64_t)(uint32_t)(t & (P - 1)) * RB;  // (a page may pass 4 GiB)
     }
     return w;
   };

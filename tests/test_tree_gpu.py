@@ -712,6 +712,38 @@ def test_caches_past_32_bit_offsets(K):
     assert path.tolist() == want[0] and int(count) > 1 and torch.equal(kv[:, lo:].cpu(), want[3])
 
 
+@pytest.mark.parametrize("D", [64, 128])
+def test_attention_tree_pages_past_32_bit_offsets(K, D):
+    """A page of more than 2^32 bytes per head: K is 0 but for a few tokens on both sides of that offset, so that the exact
+    output is known. Tolerance: fp16's half step of the output and of a weight, the scores' fp32 roundings, and sums whose
+    chains are as long as a split has tiles (2^31 / D tokens in 64 splits and tiles of 32)."""
+    log2P = 33 - (7 if D == 64 else 8)
+    tokens, M = (1 << 32) // (2 * D) + 5000, 3
+    k, v = (torch.zeros(1, 1, 1 << log2P, D, dtype=torch.half, device=DEV) for _ in "kv")
+    at = torch.tensor([7, tokens - 5000 - 1, tokens - 5000 + 7, tokens - 2, tokens + 1])
+    g = gen(D)
+    q = torch.randn(M, 1, D, generator=g).half()
+    kx = ((q[:, 0].float().mean(0) + 0.1 * torch.randn(5, D, generator=g)) * 60 * D ** -0.5).half()   # scores about 20
+    vx = torch.randn(5, D, generator=g).half()
+    k[0, 0, at.to(DEV)], v[0, 0, at.to(DEV)] = kx.to(DEV), vx.to(DEV)
+    rows = torch.eye(M, dtype=torch.bool)
+    rows[:, 1] = True                                          # (node 1 is the last of them)
+    kc, vc = kx.double(), vx.double()
+    sc = q[:, 0].double() @ kc.t() * D ** -0.5
+    n = tokens + rows.sum(1, keepdim=True) - torch.tensor([5.0])[None]
+    w = torch.exp(sc)
+    total = w.sum(1, keepdim=True) + n
+    want = (w @ vc) / total
+    size = (w @ vc.abs()) / total
+    ds = 2.0 ** -24 * ((D + 4) * (q[:, 0].double().abs() @ kc.abs().t()) * D ** -0.5 + 4 * sc.abs()).amax(1, keepdim=True)
+    rel = 2.0 ** -11 + 2 * (ds + 2.0 ** -21) + 2.0 ** -24 * (2.0 ** 31 / D / 32 / 64 + 128)
+    bound = 2.0 ** -11 * want.abs() + rel * size + 2.0 ** -25
+    bt = torch.zeros(1, dtype=torch.int32, device=DEV)
+    out = run_tree(K, q.to(DEV), T.mask_words(rows).to(DEV), i32(tokens), bt, k, v, tokens + M)
+    assert float(want.abs().max()) > 0.05                      # the few weigh against all the others
+    T.within(out, want, bound)
+
+
 # ------------------------------------------------------------------------------------------------ the op module, streams
 def test_op_module_refusals(K):
     """Wrong types, shapes and layouts raise before anything is launched."""
