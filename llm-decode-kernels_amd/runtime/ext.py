@@ -125,6 +125,17 @@ def _workspace(what, device, t):
     return t.data_ptr(), t.nbytes
 
 
+def _ints(*sizes):
+    """Sizes as C ints; ctypes would pass a larger one on without its high bits."""
+    out = []
+    for n in sizes:
+        n = int(n)
+        if not -0x80000000 <= n <= 0x7FFFFFFF:
+            raise RuntimeError(f"a size of {n} does not fit 32 bits")
+        out.append(n)
+    return out
+
+
 LOGITS_DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 
 
@@ -673,7 +684,7 @@ class DecodeKernels:
     # attention of the nodes of a drafted token tree (speculative decoding) over the paged cache
     def attention_tree_workspace_bytes(self, M, n_q, n_kv, head_dim, max_ctx):
         """Bytes of split workspace that attention_tree can use for these sizes (0: it does not split)."""
-        return int(self.lib.dk_attention_tree_workspace_bytes(int(M), int(n_q), int(n_kv), int(head_dim), int(max_ctx)))
+        return int(self.lib.dk_attention_tree_workspace_bytes(*_ints(M, n_q, n_kv, head_dim, max_ctx)))
 
     def attention_tree(self, q, mask, pos, bt, kc, vc, max_ctx, out, workspace=None):
         """q [M, n_q, D] or [M, n_q * D] (rows may be strided, e.g. the q part of qkv rows), rotated; node i attends the
@@ -696,9 +707,12 @@ class DecodeKernels:
             raise RuntimeError(f"{what}: q rows must hold n_q * D values, out be [M, n_q * D] and pos [1]")
         if mask is not None and mask.shape != (M, (M + 63) // 64):
             raise RuntimeError(f"{what}: mask must be int64 [M, ceil(M / 64)]")
+        max_ctx = int(max_ctx)
+        if not -0x80000000 <= max_ctx <= 0x7FFFFFFF:
+            _ints(max_ctx)
         p_ws, ws_bytes = _workspace(what, dev, workspace)
         self._call_on(dev, self.lib.dk_attention_tree, q.data_ptr(), strides[0] if M > 1 else width, p_mask, p_pos, p_bt,
-                      bt.numel(), p_kc, p_vc, cache[0], cache[2], width // D, cache[1], D, M, int(max_ctx), p_out, p_ws,
+                      bt.numel(), p_kc, p_vc, cache[0], cache[2], width // D, cache[1], D, M, max_ctx, p_out, p_ws,
                       ws_bytes)
 
     # log probabilities of given tokens with entropy and top alternatives (the picks of a verified tree, prompt scoring)
@@ -706,7 +720,7 @@ class DecodeKernels:
         """Bytes of split workspace that token_logprobs can use for these sizes (0: it does not split)."""
         if dtype not in LOGITS_DTYPES:
             raise RuntimeError(f"token_logprobs: logits must be fp16, bf16 or fp32, got {dtype}")
-        return int(self.lib.dk_token_logprobs_workspace_bytes(int(M), int(V), int(k), LOGITS_DTYPES[dtype]))
+        return int(self.lib.dk_token_logprobs_workspace_bytes(*_ints(M, V, k), LOGITS_DTYPES[dtype]))
 
     def token_logprobs(self, logits, tokens, logprobs, entropy=None, top_ids=None, top_logprobs=None, workspace=None):
         """logits [M, V] (fp16, bf16 or fp32; rows may be strided): logprobs[m] of the ids tokens[m], entropy[m] and the k
@@ -721,6 +735,8 @@ class DecodeKernels:
         if dev < 0 or dtype is None or len(rows) != 2 or (logits.stride(1) != 1 and rows[1] > 1):
             raise RuntimeError(f"{what}: logits must be a CUDA fp16, bf16 or fp32 [M, V] with contiguous rows")
         M, V = rows
+        if M > 0x7FFFFFFF or V > 0x7FFFFFFF:
+            _ints(M, V)
         for t, name in ((tokens, "tokens"), (logprobs, "logprobs"), (entropy, "entropy")):
             if t is not None and t.numel() != M:
                 raise RuntimeError(f"{what}: {name} must hold M values")

@@ -115,6 +115,16 @@ def test_tree_accept_refusals(lib, kw, code, msg):
     refused(lib, call(lib, "dk_tree_accept", ACC, kw), code, msg)
 
 
+def test_workspace_queries_refuse_sizes_past_32_bits(lib):
+    K = ext.DecodeKernels(lib)
+    for sizes in ((20, 32, 8, 128, (1 << 32) + 9000), ((1 << 32) + 20, 32, 8, 128, 9000)):
+        with pytest.raises(RuntimeError, match="32 bits"):
+            K.attention_tree_workspace_bytes(*sizes)
+    for sizes in ((1, (1 << 32) + 128256, 5), ((1 << 32) + 1, 128256, 5), (1, 128256, 5 - (1 << 32))):
+        with pytest.raises(RuntimeError, match="32 bits"):
+            K.token_logprobs_workspace_bytes(*sizes)
+
+
 def test_op_module_rejects_cpu_tensors(lib):
     K = ext.DecodeKernels(lib)
     h = lambda *s: torch.zeros(*s, dtype=torch.half)

@@ -789,6 +789,22 @@ def test_op_module_refusals(K):
     torch.cuda.synchronize()
 
 
+def test_sizes_past_32_bits_are_refused(K):
+    """Not taken for what their low 32 bits say."""
+    z = lambda *s, t=torch.half: torch.zeros(*s, dtype=t, device=DEV)
+    kc, bt, pos, out = z(4, 2, 16, 64), z(4, t=torch.int32), z(1, t=torch.int32), z(3, 256)
+    for max_ctx in ((1 << 32) + 30, (1 << 60) + 30, 30 - (1 << 32)):
+        with pytest.raises(RuntimeError, match="32 bits"):
+            K.attention_tree(z(3, 4, 64), None, pos, bt, kc, kc, max_ctx, out)
+    logits = torch.empty(1, (1 << 32) + 100, dtype=torch.half, device=DEV)
+    with pytest.raises(RuntimeError, match="32 bits"):
+        K.token_logprobs(logits, None, None, z(1, t=torch.float32))
+    with pytest.raises(RuntimeError, match="32 bits"):
+        K.token_logprobs(logits.view(-1, 1), None, None, z((1 << 32) + 100, t=torch.float32))
+    del logits
+    torch.cuda.empty_cache()
+
+
 def test_graphs_share_a_workspace_and_streams(K):
     """Two captured calls of different sizes with one workspace, replayed in turn with eager work (torch's and the ops' own,
     on another stream with a workspace of its own) between; every replay against the eager result."""
