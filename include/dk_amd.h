@@ -368,7 +368,9 @@ int dk_qk_norm_rope_append_rows(const void* qkv, const void* q_w, const void* k_
  * read as nodes. A node that attends nothing gets zeros. Tokens at positions >= max_ctx (pass *pos + M or more), past the
  * block table or without a mapped page are neither read nor attended, and neither values nor NaN of a token reach a node
  * that does not attend it; *pos < 0: no token is attended. q: row m's heads at q + m q_stride (q_stride % 8 == 0), already
- * rotated; out [M, n_q * head_dim] fp16, not overlapping q or mask. fp32 scores and softmax, scale 1/sqrt(head_dim).
+ * rotated; out [M, n_q * head_dim] fp16, not overlapping q or mask. fp32 scores and softmax sums, scale 1/sqrt(head_dim);
+ * a weight is rounded to fp16 where it meets V. With M, max_ctx and the workspace as they are, a node's output does not
+ * depend, not in a bit, on what the nodes that it does not attend hold.
  * n_q / n_kv in {1, 2, 4, 8}, M 1..1024, max_ctx 1..2^30. q, kc, vc and out 16-byte aligned.
  * The context is split over workgroups whose fp32 partials meet in `workspace` (16-byte aligned, overlapping nothing
  * else) and are joined in split order by a second launch; dk_attention_tree_workspace_bytes gives what the sizes can use

@@ -40,7 +40,8 @@
 // exponentials it takes 139, without reading V 142, without both 119 and without loads too 100; the products' own time is
 // 62. Barriers and waits taken out changed nothing, 5% fewer cycles save 2% of the time. 64 columns per wave would halve
 // the reads, but then scores lie in accumulation registers, which the softmax cannot use.
-// 64 nodes at 16001 take 30 (floor 14), of which about 18 are this and the rest launch, first loads and 17 MB of partials.
+// 64 nodes at 16001 take 30-32 (floor 14; traced 26.5 and 6 for the join), of which about 18 are this and the rest launch,
+// first loads and 17 MB of partials.
 // Small ones are launch, a chain of dependent loads (position, page, K / V: 3 us to the first product), partials and the
 // join: 26 nodes at 4096 16, 5 at 300, unsplit, 6.7.
 // No gain: two halves of the workgroup half a block apart, so that one's softmax meets the other's products; a block's
@@ -65,7 +66,7 @@ namespace {
 // Reference maximum of a column that has seen no token: a finite stand-in for -infinity (no -inf - (-inf)).
 constexpr float kTreeNoMax = -1e30f;
 constexpr float kTreeLift = 7.0f;     // p's exponent at the reference maximum
-constexpr float kTreeMost = 32768.f;  // the reference moves where a lane's sum of p over a tile passes this: p fits fp16
+constexpr float kTreeMost = 32768.f;  // the reference moves where a lane's sum of p over its part of a tile passes this
 constexpr float kTreeFar = 4096.f;    // a reference further from 0 than this (log2 units) is taken off the score itself
 
 constexpr int kTreeMaxSplits = 64;
@@ -628,7 +629,8 @@ TreeShape tree_shape(int M, int n_q, int n_kv, int D, int max_ctx) {
 
 }  // namespace
 
-// One workgroup per CU, in splits of equal length.
+// At most one workgroup per CU, in splits of equal length: exactly one where blocks * n_kv divides 256, and fewer elsewhere
+// (11 blocks of 8 heads: two splits, 176 workgroups).
 int attention_tree_splits(int M, int n_q, int n_kv, int D, int max_ctx) {
   const TreeShape s = tree_shape(M, n_q, n_kv, D, max_ctx);
   if (!s.split) return 1;

@@ -10,11 +10,12 @@
 // counting, and cut to its k largest, at the end, whenever it is half full and behind a block whose candidates it could not
 // take; T is then what follows the k-th. With more than one slice the (m, l, s) and k keys of each go to the workspace and
 // a second launch joins them in slice order.
-// Measured (captured, us): 512 x 128256 fp32 45 with one alternative (5.8 TB/s), 63 with 20, 66 with 32; fp16 35, 55, 57;
-// 61 x 128256 fp16 13 with one, 17 with 5, 19 with 20; 1 x 128256 9, 10, 13; 1 x 32000 8 (one launch), 10, 13 (two, of a
-// memory round trip each). What the alternatives cost at 512 rows is the barrier per block that the list needs; one slice per
-// row is the fastest there (two 65-79, four 68-83, sixteen 96-114 with 2 to 20), eight of two blocks at 61 rows. Two
-// passes (maximum and sums, then one pass per alternative) took 5175 at 512 x 128256 fp32 with 20.
+// Measured (captured, us): 512 x 128256 fp32 46 with one alternative (5.8 TB/s), 57 with 5, 62 with 20, 64 with 32; fp16 35,
+// 50, 55, 57; bf16 32, 50, 55, 57; 61 x 128256 fp16 and bf16 13 with one, 17 with 5, 19 with 20, fp32 14, 18, 20; 1 x 128256
+// 9, 10, 13; 1 x 32000 8 (one launch), 10, 13 (two, of a memory round trip each). What the alternatives cost at 512 rows is
+// the barrier per block that the list needs; one slice per row is the fastest there (two 65-79, four 68-83, sixteen 96-114
+// with 2 to 20), eight of two blocks at 61 rows. Two passes (maximum and sums, then one pass per alternative) took 5175 at
+// 512 x 128256 fp32 with 20.
 // Rows at odd addresses: 16-byte chunks lie on 16-byte boundaries, the first and last one are read value by value.
 #include "common.hpp"
 #include "launch.hpp"
