@@ -1,0 +1,407 @@
+"""The operators of a key / value cache held in 8 bits, and of attention with a sliding window, as cases that can be timed
+and compared.
+
+A cache holds a sequence's K and V in pages: fp16, or 8-bit codes (int8 or e4m3) with one power-of-two scale for each block of
+16 tokens and kv head. A case is a dict of plain values. ``prepare`` makes what the program holds before the call, ``run``
+makes one pass: through ``runtime.ext`` where ``own`` is true, else in plain torch operations in 32 bits. ``exact`` gives the
+same outputs from the definitions in 64 bits.
+
+Definitions:
+  code     a block of values x has the scale s = 2^k, k the smallest in -24 .. 10 with largest |x| <= most s (most: 127, or
+           448 for e4m3); a value's code is x / s rounded to nearest (ties to even), at most 65504 / s in size. Rows that go
+           into a block whose earlier rows are there raise s to the maximum of the old and their own; where that is more than
+           the old, the earlier rows' codes are taken anew from the values that they stand for.
+  attends  the row at position p attends token t where t <= p and (no window, or t > p - window, or t < sinks).
+
+Ranges (``draw`` covers them, ``listed`` has representatives):
+  append   RoPE of q and k, K and V into the 8-bit cache, and the touched blocks read back: 1-4096 rows behind 0-8000 tokens,
+           head dim 64 / 128, 1-8 kv heads, pages of 16 to 64
+  read     1-131072 tokens read back to fp16 rows
+  window   attention of 1-4096 rows over an fp16 cache, windows of 1-8192 tokens, 0-64 sinks
+  kv8      attention of 1-4096 rows over an 8-bit cache of up to 131072 tokens, with or without a window, 1-8 query heads per
+           kv head
+"""
+import math
+import os
+import sys
+
+import torch
+
+own = False
+
+DEV = "cuda"
+THETA = 500000.0
+BLOCK = 16
+CODES = {"int8": (torch.int8, 127.0), "e4m3": (torch.float8_e4m3fn, 448.0)}
+FITS = {"int8": (1024.0, 63.0), "e4m3": (256.0, 240.0)}    # the largest scale, and the largest code whose value then fits fp16
+
+
+def _ops():
+    # the package folder's name is not an identifier: its modules are imported from inside it
+    pkg = os.path.join(os.getcwd(), "llm-decode-kernels_amd")
+    if pkg not in sys.path:
+        sys.path.insert(0, pkg)
+    from runtime import ext
+    return ext.load()
+
+
+def listed():
+    return [
+        # the newest token of a decode step, Llama-3-8B heads, in a block that older tokens share: latency alone
+        {"name": "append_1", "kind": "append", "codes": "e4m3", "M": 1, "n_kv": 8, "hpg": 4, "D": 128, "page": 16,
+         "start": 4091},
+        # an ordinary prompt behind a prefix that ends inside a block, TinyLlama heads
+        {"name": "append_500", "kind": "append", "codes": "int8", "M": 500, "n_kv": 4, "hpg": 8, "D": 64, "page": 16,
+         "start": 777},
+        # a long prompt (a document), Llama-3-8B heads
+        {"name": "append_4096", "kind": "append", "codes": "e4m3", "M": 4096, "n_kv": 8, "hpg": 4, "D": 128, "page": 16,
+         "start": 0},
+        # the rows of a short prefix that another sequence takes over, TinyLlama heads
+        {"name": "read_61", "kind": "read", "codes": "int8", "n": 61, "n_kv": 4, "D": 64, "page": 16, "start": 5},
+        # a long conversation's cache, written out
+        {"name": "read_16001", "kind": "read", "codes": "e4m3", "n": 16001, "n_kv": 8, "D": 128, "page": 32, "start": 0},
+        # one token of an endless conversation: four sinks and the last 2048 tokens, TinyLlama heads
+        {"name": "window_1_16001", "kind": "window", "M": 1, "n_kv": 4, "hpg": 8, "D": 64, "page": 16, "start": 16000,
+         "window": 2048, "sinks": 4},
+        # a long prompt under a window, Llama-3-8B heads
+        {"name": "window_4096", "kind": "window", "M": 4096, "n_kv": 8, "hpg": 4, "D": 128, "page": 16, "start": 0,
+         "window": 1024, "sinks": 4},
+        # one token of a short conversation, TinyLlama heads
+        {"name": "kv8_1_300", "kind": "kv8", "codes": "int8", "M": 1, "n_kv": 4, "hpg": 8, "D": 64, "page": 16, "start": 299,
+         "window": 0, "sinks": 0},
+        # one token at an ordinary context, Llama-3-8B heads
+        {"name": "kv8_1_4096", "kind": "kv8", "codes": "e4m3", "M": 1, "n_kv": 8, "hpg": 4, "D": 128, "page": 16,
+         "start": 4095, "window": 0, "sinks": 0},
+        # one token behind a book, the length that 8 bits are there for
+        {"name": "kv8_1_131072", "kind": "kv8", "codes": "int8", "M": 1, "n_kv": 8, "hpg": 4, "D": 128, "page": 32,
+         "start": 131071, "window": 0, "sinks": 0},
+        # the next question in a conversation: a short prompt behind a long cache
+        {"name": "kv8_100_8000", "kind": "kv8", "codes": "int8", "M": 100, "n_kv": 8, "hpg": 4, "D": 128, "page": 16,
+         "start": 8000, "window": 0, "sinks": 0},
+        # a long prompt
+        {"name": "kv8_4096", "kind": "kv8", "codes": "e4m3", "M": 4096, "n_kv": 8, "hpg": 4, "D": 128, "page": 16, "start": 0,
+         "window": 0, "sinks": 0},
+    ]
+
+
+def _log_int(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    kind = rng.choice(["append", "read", "window", "kv8", "kv8"])
+    n_kv, D, page = rng.choice([1, 2, 4, 8]), rng.choice([64, 128]), rng.choice([16, 16, 32, 64])
+    codes = rng.choice(sorted(CODES))
+    if kind == "append":
+        return {"kind": kind, "codes": codes, "M": rng.choice([1, _log_int(rng, 2, 4096)]), "n_kv": n_kv,
+                "hpg": rng.choice([1, 2, 4]), "D": D, "page": page, "start": rng.choice([0, rng.randint(1, 8000)])}
+    if kind == "read":
+        return {"kind": kind, "codes": codes, "n": _log_int(rng, 1, min(131072, 16001 * 1024 // (n_kv * D))), "n_kv": n_kv, "D": D,
+                "page": page, "start": rng.choice([0, rng.randint(1, 500)])}
+    hpg = rng.choice([1, 2, 4, 8]) if n_kv < 8 else rng.choice([1, 2, 4])
+    M = rng.choice([1, 1, _log_int(rng, 2, 4096)])
+    # (query, token) pairs of a row up to those of the largest listed prompt, tokens up to those of the longest cache
+    most = min(131072, 4096 * 4096 * 32 * 128 // 2 // (M * n_kv * hpg * D))
+    start = max(0, _log_int(rng, 1, max(2, most)) - M)
+    if kind == "window":
+        window, sinks = _log_int(rng, 1, 8192), rng.choice([0, 4, rng.randint(1, 64)])
+        return {"kind": kind, "M": M, "n_kv": n_kv, "hpg": hpg, "D": D, "page": page, "start": start, "window": window,
+                "sinks": sinks}
+    window = rng.choice([0, 0, _log_int(rng, 1, 8192)])
+    return {"kind": kind, "codes": codes, "M": M, "n_kv": n_kv, "hpg": hpg, "D": D, "page": page, "start": start,
+            "window": window, "sinks": rng.choice([0, 4]) if window else 0}
+
+
+# ------------------------------------------------------------------------------------------------ inputs
+def _randn(g, *size, std=1.0):
+    return torch.randn(*size, generator=g, device=DEV) * std
+
+
+def _encode(x, codes):
+    """(codes, scales) of x fp32 [..., 16, D], whose last two axes are a block."""
+    # the next power of two, in the exponent bits (pow and ldexp are not exact on the GPU); a quotient that is none is as far
+    # from one as fp16 values are apart, far more than fp32 rounds off
+    top = (x.abs().amax((-2, -1)) / CODES[codes][1]).clamp(2.0 ** -24, 2.0 ** 10)
+    s = ((top.view(torch.int32) + 0x7FFFFF) & ~0x7FFFFF).view(torch.float32)
+    return _coded(x, s, codes), s
+
+
+def _coded(x, s, codes):
+    dtype, most = CODES[codes]
+    y = x / s[..., None, None]
+    at, fits = FITS[codes]
+    big = torch.where(s == at, fits, most)[..., None, None]
+    y = torch.minimum(torch.maximum(y, -big), big)
+    return (y.round() if dtype == torch.int8 else y).to(dtype)
+
+
+def _rows(g, tokens, n_kv, D, channels):
+    """Rows as a projection leaves them: a common size per channel, a few channels well above the rest (keys have those)."""
+    return (_randn(g, tokens, n_kv, D) * channels).half()
+
+
+def _channels(g, n_kv, D, outliers):
+    size = 0.5 + torch.rand(n_kv, D, generator=g, device=DEV)
+    return torch.where(torch.rand(n_kv, D, generator=g, device=DEV) < outliers, 6 * size, size)
+
+
+def _pages(rows, page, order):
+    """[tokens, n_kv, D] rows in pages [len(order), n_kv, page, D]; page i of the sequence is page order[i] of the cache."""
+    n, (t, n_kv, D) = order.numel(), rows.shape
+    full = torch.zeros(n * page, n_kv, D, dtype=rows.dtype, device=DEV)
+    full[:t] = rows
+    out = torch.empty(n, n_kv, page, D, dtype=rows.dtype, device=DEV)
+    out[order.long()] = full.view(n, page, n_kv, D).transpose(1, 2)
+    return out
+
+
+def prepare(case, seed):
+    kind, n_kv, D, page, start = case["kind"], case["n_kv"], case["D"], case["page"], case["start"]
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    s = {"case": case, "own": own}
+    if own:
+        s["ops"] = _ops()
+    more = case["n"] if kind == "read" else case["M"]
+    held = start if kind == "append" else start + more             # tokens in the cache before the call
+    order = torch.randperm(-(-(start + more) // page) + 1, generator=g, device=DEV)
+    s["bt"] = order.int()
+    chan = {"k": _channels(g, n_kv, D, 0.03), "v": _channels(g, n_kv, D, 0.0)}
+    for c in "kv":
+        pages = _pages(_rows(g, held, n_kv, D, chan[c]), page, order)
+        if kind == "window":
+            s[c + "c"] = pages
+        else:
+            blocks = pages.view(*pages.shape[:2], page // BLOCK, BLOCK, D)
+            code, scale = _encode(blocks.float(), case["codes"])
+            s[c + "c"], s[c + "s"] = code.view(pages.shape), scale
+    if kind == "read":
+        s["k"], s["v"] = (torch.empty(more, n_kv, D, dtype=torch.half, device=DEV) for _ in "kv")
+        return s
+    M, n_q = case["M"], n_kv * case["hpg"]
+    s["pos"] = torch.tensor([start], dtype=torch.int32, device=DEV)
+    if kind == "append":
+        q = _randn(g, M, n_q * D).half()
+        k, v = (_rows(g, M, n_kv, D, chan[c]).view(M, -1) for c in "kv")
+        s["qkv"] = torch.cat([q, k, v], 1)
+        ang = torch.arange(start + M, dtype=torch.float64, device=DEV)[:, None] / \
+            THETA ** (torch.arange(0, D, 2, dtype=torch.float64, device=DEV) / D)
+        s["cos"], s["sin"] = ang.cos().float(), ang.sin().float()
+        s["q_out"] = torch.empty(M, n_q * D, dtype=torch.half, device=DEV)
+        first = start // BLOCK * BLOCK                              # the first token of the first touched block
+        s["first"] = first
+        s["k"], s["v"] = (torch.empty(start + M - first, n_kv, D, dtype=torch.half, device=DEV) for _ in "kv")
+        return s
+    # queries that favour some keys, as trained ones do
+    s["q"] = _randn(g, M, n_q * D, std=1.2).half()
+    s["out"] = torch.empty(M, n_q * D, dtype=torch.half, device=DEV)
+    if own:
+        need = s["ops"].attention_window_workspace_bytes(M, n_q, n_kv, D, start + M, case["window"], case["sinks"],
+                                                         s["kc"].dtype)
+        s["workspace"] = torch.empty(need, dtype=torch.uint8, device=DEV) if need else None
+    return s
+
+
+# ------------------------------------------------------------------------------------------------ the plain forms
+def _at(s, t):
+    """Page and slot of the tokens t."""
+    page = s["case"]["page"]
+    return s["bt"][t // page].long(), t % page
+
+
+def _values(s, c, t):
+    """fp32 [tokens, n_kv, D]: the values of the tokens t in cache c ("k" or "v")."""
+    pg, slot = _at(s, t)
+    if c + "s" not in s:
+        return s[c + "c"][pg, :, slot].float()
+    code = s[c + "c"].view(torch.uint8)[pg, :, slot].view(s[c + "c"].dtype)
+    return code.float() * s[c + "s"][pg, :, slot // BLOCK][..., None]
+
+
+def _plain_append(s):
+    case = s["case"]
+    M, n_kv, D, start, codes = case["M"], case["n_kv"], case["D"], case["start"], case["codes"]
+    n_q = n_kv * case["hpg"]
+    x = s["qkv"].float().view(M, n_q + 2 * n_kv, D)
+    at = s["pos"].long() + torch.arange(M, device=DEV)
+    cos, sin = s["cos"][at][:, None], s["sin"][at][:, None]
+    a, b = x[:, :n_q + n_kv].chunk(2, -1)
+    turned = torch.cat([a * cos - b * sin, b * cos + a * sin], -1).half()
+    s["q_out"].view(M, n_q, D).copy_(turned[:, :n_q])
+    # whole blocks: the rows before the new ones keep their place in the first, nothing is behind them in the last
+    first, n_blocks = s["first"], -(-(start + M) // BLOCK) - start // BLOCK
+    old = torch.arange(first, start, device=DEV)
+    for c, rows in (("k", turned[:, n_q:]), ("v", x[:, n_q + n_kv:].half())):
+        new = torch.zeros(n_blocks * BLOCK, n_kv, D, device=DEV)
+        new[start - first:start - first + M] = rows.float()
+        new = new.view(n_blocks, BLOCK, n_kv, D).transpose(1, 2)
+        scale = _encode(new, codes)[1]
+        pg, slot = _at(s, first + BLOCK * torch.arange(n_blocks, device=DEV))
+        if start > first:
+            scale[0] = torch.maximum(scale[0], s[c + "s"][pg[0], :, slot[0] // BLOCK])
+            new[0, :, :start - first] = _values(s, c, old).transpose(0, 1)
+        code = _coded(new, scale, codes).transpose(1, 2).reshape(-1, n_kv, D)[:start + M - first]
+        tp, ts = _at(s, first + torch.arange(start + M - first, device=DEV))
+        s[c + "c"].view(torch.uint8)[tp, :, ts] = code.view(torch.uint8)
+        s[c + "s"][pg, :, slot // BLOCK] = scale
+    return _plain_read(s, first, start + M - first)
+
+
+def _plain_read(s, start, n):
+    t = start + torch.arange(n, device=DEV)
+    s["k"].copy_(_values(s, "k", t))
+    s["v"].copy_(_values(s, "v", t))
+    return {c: s[c] for c in ("k", "v")}
+
+
+def _plain_attention(s):
+    case = s["case"]
+    M, n_kv, hpg, D, start, window, sinks = (case[k] for k in ("M", "n_kv", "hpg", "D", "start", "window", "sinks"))
+    t = torch.arange(start + M, device=DEV)
+    p = s["pos"].long() + torch.arange(M, device=DEV)[:, None]
+    seen = t <= p
+    if window:
+        seen &= (t > p - window) | (t < sinks)
+    k = _values(s, "k", t).permute(1, 2, 0).contiguous()                                  # [n_kv, D, tokens]
+    v = _values(s, "v", t).transpose(0, 1).contiguous()
+    q = s["q"].float().view(M, n_kv, hpg, D).permute(1, 0, 2, 3).reshape(n_kv, M * hpg, D)
+    sc = torch.bmm(q, k).mul_(1 / math.sqrt(D)).view(n_kv, M, hpg, -1).masked_fill_(~seen[:, None], -math.inf)
+    sc = sc.sub_(sc.amax(-1, keepdim=True)).exp_()
+    total = sc.sum(-1, keepdim=True)
+    o = torch.bmm(sc.view(n_kv, M * hpg, -1), v).view(n_kv, M, hpg, D) / total
+    s["out"].view(M, n_kv, hpg, D).copy_(o.transpose(0, 1))
+    return s["out"]
+
+
+# ------------------------------------------------------------------------------------------------ one pass
+def run(s):
+    case = s["case"]
+    kind = case["kind"]
+    if not s["own"]:
+        if kind == "append":
+            return {"q": s["q_out"], **_plain_append(s)}
+        return _plain_read(s, case["start"], case["n"]) if kind == "read" else _plain_attention(s)
+    ops = s["ops"]
+    if kind == "append":
+        n_kv = case["n_kv"]
+        ops.kv8_append_rows(s["qkv"], s["cos"], s["sin"], s["pos"], s["bt"], s["kc"], s["vc"], s["ks"], s["vs"],
+                            n_kv * case["hpg"], n_kv, s["q_out"])
+        ops.kv8_read(s["bt"], s["kc"], s["vc"], s["ks"], s["vs"], s["first"], s["k"], s["v"])
+        return {"q": s["q_out"], "k": s["k"], "v": s["v"]}
+    if kind == "read":
+        ops.kv8_read(s["bt"], s["kc"], s["vc"], s["ks"], s["vs"], case["start"], s["k"], s["v"])
+        return {"k": s["k"], "v": s["v"]}
+    ctx = case["start"] + case["M"]
+    if kind == "window":
+        ops.attention_window(s["q"], s["pos"], s["bt"], s["kc"], s["vc"], ctx, s["out"], case["window"], case["sinks"],
+                             s["workspace"])
+    else:
+        ops.attention_kv8(s["q"], s["pos"], s["bt"], s["kc"], s["vc"], s["ks"], s["vs"], ctx, s["out"], case["window"],
+                          case["sinks"], s["workspace"])
+    return s["out"]
+
+
+def _pairs(case):
+    """(row, token) pairs that attend, and the tokens that any row attends."""
+    M, start, window, sinks = (case[k] for k in ("M", "start", "window", "sinks"))
+    if not window:
+        return M * start + M * (M + 1) // 2, start + M
+    pairs = sum(min(p + 1, window) + min(sinks, max(0, p + 1 - window)) for p in range(start, start + M))
+    lo = max(0, start - window + 1)
+    return pairs, start + M - lo + min(sinks, lo)
+
+
+def work(case):
+    kind, n_kv, D = case["kind"], case["n_kv"], case["D"]
+    if kind == "read":
+        return {"bytes": case["n"] * n_kv * 2 * (3 * D + 4 / BLOCK), "flops": 2 * case["n"] * n_kv * D}
+    M, n_q = case["M"], n_kv * case["hpg"]
+    if kind == "append":
+        # q and the tables once in and out; K and V in, their codes out, and back as fp16 rows
+        back = M + case["start"] % BLOCK
+        return {"bytes": 4 * M * n_q * D + 4 * M * D + M * n_kv * 2 * (3 * D + 4 / BLOCK) + back * n_kv * 2 * (3 * D + 4 / BLOCK),
+                "flops": 3 * M * (n_q + n_kv) * D + 4 * M * n_kv * D}
+    pairs, tokens = _pairs(case)
+    row = 4 * D if kind == "window" else 2 * D + 8 / BLOCK          # a token's K and V of one kv head
+    return {"bytes": tokens * n_kv * row + 4 * M * n_q * D, "flops": 4 * n_q * D * pairs}
+
+
+# ------------------------------------------------------------------------------------------------ 64-bit references
+def _power(k):
+    """2^k in float64."""
+    return ((k.long() + 1023) << 52).view(torch.float64)
+
+
+def _nearest(y, codes):
+    """y (float64) on the grid of the codes, to nearest, ties to even."""
+    if codes == "int8":
+        return torch.round(y)
+    step = _power((torch.frexp(y)[1] - 4).clamp(min=-9))             # of values in [2^(e - 1), 2^e); 2^-9 below 2^-6
+    return torch.round(y / step) * step
+
+
+def _held(s, c):
+    """float64 [tokens of all pages in sequence order, n_kv, D]: what cache c holds."""
+    order = s["bt"].long()
+    x = s[c + "c"].float()[order].double()
+    if c + "s" in s:
+        x = x * s[c + "s"][order].double().repeat_interleave(BLOCK, 2)[..., None]
+    return x.transpose(1, 2).reshape(-1, x.size(1), x.size(3))
+
+
+def _exact_append(s):
+    case = s["case"]
+    M, n_kv, D, start, codes, first = (*(case[k] for k in ("M", "n_kv", "D", "start", "codes")), s["first"])
+    n_q = n_kv * case["hpg"]
+    most, top_k, top_code = {"int8": (127.0, 10, 63.0), "e4m3": (448.0, 8, 240.0)}[codes]
+    x = s["qkv"].double().view(M, -1, D)
+    ang = torch.complex(s["cos"][start:start + M].double(), s["sin"][start:start + M].double())[:, None]
+
+    def turn(y):
+        z = torch.complex(y[..., :D // 2].contiguous(), y[..., D // 2:].contiguous()) * ang
+        return torch.cat([z.real, z.imag], -1)
+
+    out = {"q": turn(x[:, :n_q]).reshape(M, -1)}
+    for c, rows in (("k", turn(x[:, n_q:n_q + n_kv]).half().double()), ("v", x[:, n_q + n_kv:])):
+        got = torch.cat([_held(s, c)[first:start], rows])
+        scales = s[c + "s"][s["bt"].long()].transpose(1, 2).reshape(-1, n_kv).double()    # [blocks of the sequence, n_kv]
+        parts = []
+        for b in range(0, got.size(0), BLOCK):
+            blk = got[b:b + BLOCK]
+            fresh = blk[start - first:] if b == 0 else blk
+            top = fresh.abs().amax((0, 2))
+            k = torch.frexp(top / most)[1]                           # 2^k > top / most; the one below may hold it too
+            k = torch.where(_power(k - 1) * most >= top, k - 1, k)
+            scale = _power(torch.where(top == 0, -24, k).clamp(-24, 10))
+            if b == 0 and start > first:
+                scale = torch.maximum(scale, scales[first // BLOCK])
+            y = blk / scale[:, None]
+            big = torch.where(scale == 2.0 ** top_k, top_code, most)[:, None]
+            parts.append(_nearest(torch.minimum(torch.maximum(y, -big), big), codes) * scale[:, None])
+        out[c] = torch.cat(parts)
+    return out
+
+
+def _exact_attention(s):
+    case = s["case"]
+    M, hpg, D, start, window, sinks = (case[k] for k in ("M", "hpg", "D", "start", "window", "sinks"))
+    T = start + M
+    k, v = _held(s, "k")[:T], _held(s, "v")[:T]
+    row, tok = torch.arange(start, T, device=DEV)[:, None], torch.arange(T, device=DEV)[None]
+    hidden = tok > row
+    if window:
+        hidden = hidden | ((tok <= row - window) & (tok >= sinks))
+    out = torch.empty(M, case["n_kv"] * hpg, D, dtype=torch.float64, device=DEV)
+    q = s["q"].double().view(M, -1, D)
+    for h in range(out.size(1)):
+        sc = torch.mm(q[:, h].contiguous(), k[:, h // hpg].t().contiguous()) / D ** 0.5
+        out[:, h] = torch.mm(torch.softmax(sc.masked_fill_(hidden, -math.inf), 1), v[:, h // hpg].contiguous())
+    return out.view(M, -1)
+
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    if case["kind"] == "append":
+        return _exact_append(s)
+    if case["kind"] == "read":
+        return {c: _held(s, c)[case["start"]:case["start"] + case["n"]] for c in ("k", "v")}
+    return _exact_attention(s)
