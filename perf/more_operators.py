@@ -96,8 +96,9 @@ def draw(rng):
         return {"kind": kind, "codes": codes, "M": rng.choice([1, _log_int(rng, 2, 4096)]), "n_kv": n_kv,
                 "hpg": rng.choice([1, 2, 4]), "D": D, "page": page, "start": rng.choice([0, rng.randint(1, 8000)])}
     if kind == "read":
-        return {"kind": kind, "codes": codes, "n": _log_int(rng, 1, min(131072, 16001 * 1024 // (n_kv * D))), "n_kv": n_kv, "D": D,
-                "page": page, "start": rng.choice([0, rng.randint(1, 500)])}
+        n = _log_int(rng, 1, min(131072, 16001 * 1024 // (n_kv * D)))
+        return {"kind": kind, "codes": codes, "n": n, "n_kv": n_kv, "D": D, "page": page,
+                "start": rng.choice([0, rng.randint(1, 500)])}
     hpg = rng.choice([1, 2, 4, 8]) if n_kv < 8 else rng.choice([1, 2, 4])
     M = rng.choice([1, 1, _log_int(rng, 2, 4096)])
     # (query, token) pairs of a row up to those of the largest listed prompt, tokens up to those of the longest cache
@@ -318,8 +319,8 @@ def work(case):
     if kind == "append":
         # q and the tables once in and out; K and V in, their codes out, and back as fp16 rows
         back = M + case["start"] % BLOCK
-        return {"bytes": 4 * M * n_q * D + 4 * M * D + M * n_kv * 2 * (3 * D + 4 / BLOCK) + back * n_kv * 2 * (3 * D + 4 / BLOCK),
-                "flops": 3 * M * (n_q + n_kv) * D + 4 * M * n_kv * D}
+        row = n_kv * 2 * (3 * D + 4 / BLOCK)
+        return {"bytes": 4 * M * n_q * D + 4 * M * D + (M + back) * row, "flops": 3 * M * (n_q + n_kv) * D + 4 * M * n_kv * D}
     pairs, tokens = _pairs(case)
     row = 4 * D if kind == "window" else 2 * D + 8 / BLOCK          # a token's K and V of one kv head
     return {"bytes": tokens * n_kv * row + 4 * M * n_q * D, "flops": 4 * n_q * D * pairs}
