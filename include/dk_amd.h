@@ -417,6 +417,61 @@ int dk_tree_accept(const int64_t* tokens, const int32_t* parents, const int64_t*
                    int page, int head_dim, int32_t* path, int32_t* count, int64_t* tok, void* stream);
 
 /*
+ * The 8-bit KV cache. kc, vc hold codes [n_pages, n_kv, page, head_dim], one byte each (page a power of two >= 16), ks, vs
+ * fp32 scales [n_pages, n_kv, page / 16], one for each block of 16 tokens and kv head: a value is code * scale. `cache` names
+ * the codes: DK_CACHE_INT8 (-127 .. 127) or DK_CACHE_E4M3 (the format with 448 as its largest value and no infinities).
+ *
+ * dk_kv8_append_rows: rope_append_rows into that cache. Row m of qkv [M, (n_q + 2 n_kv) head_dim] is token T = *pos + m and
+ * rotates at T as dk_rope_append_rows rotates it (cos_t, sin_t [max_pos, head_dim / 2]; both NULL: no rotation, and max_pos
+ * is not read). q goes to q_out (row stride q_stride values; q_out = qkv with q_stride = (n_q + 2 n_kv) head_dim is in place,
+ * else disjoint from qkv); k and v in qkv stay as they were. K, rotated and rounded to fp16, and V become codes:
+ *   the block's scale s is 2^k with the smallest k >= -24 such that no new value in the block passes most * 2^k (most: 127 or
+ *   448); a code is x / s to nearest, ties to even, and at most 65504 / s. Where rows ahead of the new ones are in the block
+ *   (*pos % 16 != 0: the first block), s is the larger of that and the scale they have; if it grows, their codes are taken anew
+ *   from the values they stand for. Rows behind the new ones count as absent: they are left as they are, and a block that is
+ *   written from its first row on forgets its scale.
+ *   An infinity is stored as the largest fp16 value; NaN stays NaN in e4m3 and becomes 0 in int8.
+ * So an e4m3 value is within 2^-4 of x relative (2^-10 s below 2^-6 s), an int8 one within s / 2, after its block's scale has
+ * grown to s within s. A row whose T is outside [0, max_pos) touches nothing; a T without a mapped page is rotated but not
+ * appended. qkv, q_out, kc, vc and the tables 16-byte aligned, q_stride % 8 == 0, M 1..2^20.
+ *
+ * dk_kv8_read: tokens [start, start + n) as fp16 rows k_out, v_out [n, n_kv, head_dim]; tokens without a mapped page read as
+ * zeros. The scales that dk_kv8_append_rows writes make every value an fp16 number, so nothing is rounded; products of other
+ * scales are rounded, and infinite past 65504. start + n <= 2^30; k_out, v_out, kc and vc 16-byte aligned. No counterparts in
+ * the reference (its cache is fp16, runtime/model.py:117-120).
+ */
+enum dk_cache { DK_CACHE_F16 = 0, DK_CACHE_INT8 = 1, DK_CACHE_E4M3 = 2 };
+int dk_kv8_append_rows(const void* qkv, const float* cos_t, const float* sin_t, const int32_t* pos, const int32_t* bt,
+                       void* kc, void* vc, float* ks, float* vs, int cache, void* q_out, long long q_stride, int M, int n_q,
+                       int n_kv, int head_dim, int page, int max_pos, int n_pages, int n_bt, void* stream);
+int dk_kv8_read(const int32_t* bt, int n_bt, const void* kc, const void* vc, const float* ks, const float* vs, int cache,
+                int n_pages, int page, int n_kv, int head_dim, int start, int n, void* k_out, void* v_out, void* stream);
+
+/*
+ * Attention of M rows over a paged cache under a sliding window with sinks, over fp16 or 8-bit caches. Row m is at position
+ * p = *pos + m and attends the tokens t <= p, and with window > 0 of those the ones with t > p - window or t < sinks; window 0:
+ * all of them. The cache already holds them. A row that attends nothing (its position is negative, or none of its tokens has a
+ * mapped page) gets zeros. Tokens at positions >= max_ctx (pass *pos + M or more), past the block table or without a mapped
+ * page are neither read nor attended, and neither values nor NaN of a token reach a row that does not attend it: pages that lie
+ * behind the window of every row to come may be taken out of the block table and used again.
+ * cache: DK_CACHE_F16 (page any power of two; ks, vs NULL) or the 8-bit caches above (page >= 16; scales powers of two,
+ * 2^-24 .. 2^10, such that code * scale fits fp16). q: row m's heads at q + m q_stride (q_stride % 8 == 0), already rotated;
+ * out [M, n_q * head_dim] fp16, not overlapping q. fp32 scores and softmax sums, scale 1/sqrt(head_dim); a weight is rounded
+ * to fp16 where it meets V. n_q / n_kv in {1, 2, 4, 8}, M 1..2^20, max_ctx 1..2^30, window and sinks 0..2^30. q, kc, vc and out
+ * 16-byte aligned.
+ * The tokens are split over workgroups whose fp32 partials meet in `workspace` (16-byte aligned, overlapping nothing else) and
+ * are joined in split order by a second launch; dk_attention_window_workspace_bytes gives what the sizes can use (0: they do
+ * not split). A smaller workspace runs the most splits it holds, NULL runs unsplit. Calls that may overlap (on two streams)
+ * need a workspace each; captured ones that run in turn can share one. No counterpart in the reference.
+ */
+size_t dk_attention_window_workspace_bytes(int M, int n_q, int n_kv, int head_dim, int max_ctx, int window, int sinks,
+                                           int cache);
+int dk_attention_window(const void* q, long long q_stride, const int32_t* pos, const int32_t* bt, int n_bt, const void* kc,
+                        const void* vc, const float* ks, const float* vs, int cache, int n_pages, int page, int n_q, int n_kv,
+                        int head_dim, int M, int max_ctx, int window, int sinks, void* out, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
+/*
  * INT4 format producer on the GPU: round-to-nearest asymmetric group quantization of fp16 W [N, K] and packing,
  * bit-identical to runtime/quant.py quantize (:42-48, RTN branch of group_params :20-28) + pack (:100-109) +
  * pack_scale_zero (:122-124). Writes packed int32 [N, K/8] and sz fp16 [N, K/G, 2].

@@ -896,6 +896,136 @@ int dk_tree_accept(const int64_t* tokens, const int32_t* parents, const int64_t*
   return launched("tree_accept");
 }
 
+// ---- the 8-bit cache, and attention under a window ---------------------------------------------------------------
+
+static int check_kv8(const char* what, int cache, int head_dim, int n_kv, int page, int n_pages, int n_bt) {
+  if (cache != DK_CACHE_INT8 && cache != DK_CACHE_E4M3)
+    return fail(DK_ERR_DOMAIN, "%s: cache must be int8 or e4m3 codes (1 or 2), got %d", what, cache);
+  if (head_dim != 64 && head_dim != 128) return fail(DK_ERR_SHAPE, "%s: head_dim must be 64 or 128, got %d", what, head_dim);
+  if (n_kv <= 0 || n_kv > 65535) return fail(DK_ERR_SHAPE, "%s: bad kv head count %d", what, n_kv);
+  if (!pow2(page) || page < 16) return fail(DK_ERR_DOMAIN, "%s: page size must be a power of two >= 16, got %d", what, page);
+  if (n_pages < 1 || n_bt < 1) return fail(DK_ERR_SHAPE, "%s: empty cache or block table", what);
+  return DK_OK;
+}
+
+int dk_kv8_append_rows(const void* qkv, const float* cos_t, const float* sin_t, const int32_t* pos, const int32_t* bt,
+                       void* kc, void* vc, float* ks, float* vs, int cache, void* q_out, long long q_stride, int M, int n_q,
+                       int n_kv, int head_dim, int page, int max_pos, int n_pages, int n_bt, void* stream) {
+  if (!qkv || !pos || !bt || !kc || !vc || !ks || !vs || !q_out)
+    return fail(DK_ERR_NULL, "kv8_append_rows: null pointer argument");
+  if ((cos_t == nullptr) != (sin_t == nullptr))
+    return fail(DK_ERR_NULL, "kv8_append_rows: cos_t and sin_t come together or not at all");
+  const int rc = check_kv8("kv8_append_rows", cache, head_dim, n_kv, page, n_pages, n_bt);
+  if (rc != DK_OK) return rc;
+  if (n_q <= 0 || n_q > 65535) return fail(DK_ERR_SHAPE, "kv8_append_rows: bad query head count %d", n_q);
+  if (M < 1 || M > (1 << 20)) return fail(DK_ERR_SHAPE, "kv8_append_rows: M must be 1..2^20, got %d", M);
+  if (cos_t && max_pos < 1) return fail(DK_ERR_SHAPE, "kv8_append_rows: empty rope table");
+  if (!aligned16(qkv) || !aligned16(q_out) || !aligned16(kc) || !aligned16(vc) || !aligned16(cos_t) || !aligned16(sin_t))
+    return fail(DK_ERR_ALIGN, "kv8_append_rows: qkv, q_out, kc, vc and the tables must be 16B aligned");
+  if (!aligned4(pos) || !aligned4(bt) || !aligned4(ks) || !aligned4(vs))
+    return fail(DK_ERR_ALIGN, "kv8_append_rows: pos, bt, ks and vs must be 4B aligned");
+  const long long row = ((long long)n_q + 2LL * n_kv) * head_dim, q_row = (long long)n_q * head_dim;
+  if (q_stride % 8 != 0 || q_stride < q_row || q_stride > (1LL << 40))
+    return fail(DK_ERR_SHAPE, "kv8_append_rows: q_stride must be a multiple of 8 and >= n_q * head_dim, got %lld", q_stride);
+  // waves of the launch: two per kv head and block, one per 512 values of q
+  if (2LL * n_kv * ((M + 30LL) / 16) + M * q_row / 512 >= (1LL << 25))
+    return fail(DK_ERR_SHAPE, "kv8_append_rows: too many rows and heads for one call (M=%d n_q=%d n_kv=%d)", M, n_q, n_kv);
+  const bool in_place = q_out == qkv && q_stride == row;
+  if (!in_place && ranges_overlap(qkv, (size_t)(M * row) * 2, q_out, (size_t)((M - 1) * q_stride + q_row) * 2))
+    return fail(DK_ERR_DOMAIN, "kv8_append_rows: q_out must be qkv itself (with its row stride) or disjoint from it");
+  clear_error();
+  dk::launch_kv8_append({(const _Float16*)qkv, cos_t, sin_t, pos, bt, (uint8_t*)kc, (uint8_t*)vc, ks, vs, (_Float16*)q_out,
+                         q_stride, M, n_q, n_kv, ilog2(page), cos_t ? max_pos : 0x7fffffff, n_pages, n_bt},
+                        head_dim, cache, (hipStream_t)stream);
+  return launched("kv8_append_rows");
+}
+
+int dk_kv8_read(const int32_t* bt, int n_bt, const void* kc, const void* vc, const float* ks, const float* vs, int cache,
+                int n_pages, int page, int n_kv, int head_dim, int start, int n, void* k_out, void* v_out, void* stream) {
+  if (!bt || !kc || !vc || !ks || !vs || !k_out || !v_out) return fail(DK_ERR_NULL, "kv8_read: null pointer argument");
+  const int rc = check_kv8("kv8_read", cache, head_dim, n_kv, page, n_pages, n_bt);
+  if (rc != DK_OK) return rc;
+  if (start < 0 || n < 1 || (long long)start + n > (1LL << 30))
+    return fail(DK_ERR_SHAPE, "kv8_read: tokens must be a range inside [0, 2^30), got start %d and n %d", start, n);
+  const long long values = (long long)n * n_kv * head_dim;
+  if (values > (1LL << 34)) return fail(DK_ERR_SHAPE, "kv8_read: too many values for one call (n=%d n_kv=%d)", n, n_kv);
+  if (!aligned16(kc) || !aligned16(vc) || !aligned16(k_out) || !aligned16(v_out))
+    return fail(DK_ERR_ALIGN, "kv8_read: kc, vc, k_out and v_out must be 16B aligned");
+  if (!aligned4(bt) || !aligned4(ks) || !aligned4(vs)) return fail(DK_ERR_ALIGN, "kv8_read: bt, ks and vs must be 4B aligned");
+  if (ranges_overlap(k_out, (size_t)values * 2, v_out, (size_t)values * 2))
+    return fail(DK_ERR_DOMAIN, "kv8_read: k_out must not overlap v_out");
+  clear_error();
+  dk::launch_kv8_read({bt, (const uint8_t*)kc, (const uint8_t*)vc, ks, vs, (_Float16*)k_out, (_Float16*)v_out, n_bt, n_pages,
+                       ilog2(page), n_kv, start, n}, head_dim, cache, (hipStream_t)stream);
+  return launched("kv8_read");
+}
+
+static bool window_sizes(int M, int n_q, int n_kv, int head_dim, int max_ctx, int window, int sinks, int cache) {
+  if (M < 1 || M > (1 << 20) || n_kv < 1 || n_kv > 65535 || n_q < 1 || n_q % n_kv != 0) return false;
+  const int hpg = n_q / n_kv;
+  return (hpg == 1 || hpg == 2 || hpg == 4 || hpg == 8) && (head_dim == 64 || head_dim == 128) && max_ctx >= 1 &&
+         max_ctx <= dk::kWindowMaxCtx && window >= 0 && window <= dk::kWindowMaxCtx && sinks >= 0 &&
+         sinks <= dk::kWindowMaxCtx && cache >= DK_CACHE_F16 && cache <= DK_CACHE_E4M3;
+}
+
+size_t dk_attention_window_workspace_bytes(int M, int n_q, int n_kv, int head_dim, int max_ctx, int window, int sinks,
+                                           int cache) {
+  if (!window_sizes(M, n_q, n_kv, head_dim, max_ctx, window, sinks, cache)) return 0;
+  const int s = dk::attention_window_splits(M, n_q, n_kv, head_dim, max_ctx, window, sinks, cache);
+  return s > 1 ? (size_t)s * dk::attention_window_part_bytes(M, n_q, n_kv, head_dim) : 0;
+}
+
+int dk_attention_window(const void* q, long long q_stride, const int32_t* pos, const int32_t* bt, int n_bt, const void* kc,
+                        const void* vc, const float* ks, const float* vs, int cache, int n_pages, int page, int n_q, int n_kv,
+                        int head_dim, int M, int max_ctx, int window, int sinks, void* out, void* workspace,
+                        size_t workspace_bytes, void* stream) {
+  if (!q || !pos || !bt || !kc || !vc || !out) return fail(DK_ERR_NULL, "attention_window: null pointer argument");
+  if (cache < DK_CACHE_F16 || cache > DK_CACHE_E4M3)
+    return fail(DK_ERR_DOMAIN, "attention_window: cache must be 0, 1 or 2, got %d", cache);
+  if ((cache != DK_CACHE_F16) != (ks != nullptr) || (cache != DK_CACHE_F16) != (vs != nullptr))
+    return fail(DK_ERR_NULL, "attention_window: scales belong to 8-bit caches, and to each of them");
+  if (head_dim != 64 && head_dim != 128)
+    return fail(DK_ERR_SHAPE, "attention_window: head_dim must be 64 or 128, got %d", head_dim);
+  if (M < 1 || M > (1 << 20)) return fail(DK_ERR_SHAPE, "attention_window: M must be 1..2^20, got %d", M);
+  if (max_ctx < 1 || max_ctx > dk::kWindowMaxCtx)
+    return fail(DK_ERR_DOMAIN, "attention_window: max_ctx must be 1..%d, got %d", dk::kWindowMaxCtx, max_ctx);
+  if (window < 0 || window > dk::kWindowMaxCtx || sinks < 0 || sinks > dk::kWindowMaxCtx)
+    return fail(DK_ERR_DOMAIN, "attention_window: window and sinks must be 0..%d, got %d and %d", dk::kWindowMaxCtx, window,
+                sinks);
+  if (!window_sizes(M, n_q, n_kv, head_dim, max_ctx, window, sinks, cache))
+    return fail(DK_ERR_SHAPE, "heads-per-group must be 1/2/4/8 (n_q=%d n_kv=%d)", n_q, n_kv);
+  if (!pow2(page)) return fail(DK_ERR_DOMAIN, "page size must be a power of two, got %d", page);
+  if (cache != DK_CACHE_F16 && page < 16)
+    return fail(DK_ERR_DOMAIN, "attention_window: pages of an 8-bit cache hold 16 tokens or more, got %d", page);
+  if (n_pages < 1 || n_bt < 1) return fail(DK_ERR_SHAPE, "attention_window: empty cache or block table");
+  const long long row = (long long)n_q * head_dim;
+  // (workgroups of one launch, in the smallest shape)
+  if (M * row > (1LL << 31)) return fail(DK_ERR_SHAPE, "attention_window: too many rows and heads (M=%d n_q=%d)", M, n_q);
+  if (q_stride % 8 != 0 || q_stride < row || q_stride > (1LL << 40))
+    return fail(DK_ERR_SHAPE, "attention_window: q_stride must be a multiple of 8 and >= n_q * head_dim, got %lld", q_stride);
+  if (!aligned16(q) || !aligned16(kc) || !aligned16(vc) || !aligned16(out))
+    return fail(DK_ERR_ALIGN, "attention_window: q, kc, vc and out must be 16B aligned");
+  if (!aligned4(pos) || !aligned4(bt) || !aligned4(ks) || !aligned4(vs))
+    return fail(DK_ERR_ALIGN, "attention_window: pos, bt, ks and vs must be 4B aligned");
+  const size_t q_bytes = (size_t)((M - 1) * q_stride + row) * 2, out_bytes = (size_t)(M * row) * 2;
+  if (ranges_overlap(q, q_bytes, out, out_bytes))
+    return fail(DK_ERR_DOMAIN, "attention_window: out must not overlap q");
+  int splits = 1;
+  if (workspace != nullptr) {
+    if (!aligned16(workspace)) return fail(DK_ERR_ALIGN, "attention_window: workspace must be 16B aligned");
+    const size_t part = dk::attention_window_part_bytes(M, n_q, n_kv, head_dim);
+    splits = dk::attention_window_splits(M, n_q, n_kv, head_dim, max_ctx, window, sinks, cache);
+    if (workspace_bytes / part < (size_t)splits) splits = workspace_bytes / part < 2 ? 1 : (int)(workspace_bytes / part);
+    const size_t used = splits > 1 ? (size_t)splits * part : 0;
+    if (used > 0 && (ranges_overlap(workspace, used, q, q_bytes) || ranges_overlap(workspace, used, out, out_bytes)))
+      return fail(DK_ERR_DOMAIN, "attention_window: workspace must not overlap q or out");
+  }
+  clear_error();
+  dk::launch_attention_window({q, q_stride, pos, bt, n_bt, kc, vc, ks, vs, cache, n_pages, ilog2(page), n_q, n_kv, head_dim,
+                               M, max_ctx, window, sinks, out, splits, workspace}, (hipStream_t)stream);
+  return launched("attention_window");
+}
+
 int dk_quantize_w4(const void* w, void* packed, void* sz, int N, int K, int group, int clip, void* stream) {
   if (!w || !packed || !sz) return fail(DK_ERR_NULL, "quantize_w4: null pointer argument");
   if (N <= 0 || K <= 0) return fail(DK_ERR_SHAPE, "quantize_w4: N and K must be positive");

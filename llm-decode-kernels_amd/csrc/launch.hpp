@@ -237,6 +237,61 @@ struct TreeAccept {
 };
 void launch_tree_accept(const TreeAccept& a, hipStream_t st);
 
+// How a cache holds its values: fp16, or 8-bit codes with a scale for each 16 tokens and kv head (kv8.hpp).
+constexpr int kCacheF16 = 0, kCacheInt8 = 1, kCacheE4m3 = 2;
+
+// RoPE of M rows (cos_t null: none) and their K / V into the 8-bit cache; q to q_out (row stride q_stride).
+struct Kv8Append {
+  const _Float16* qkv;
+  const float* cos_t;
+  const float* sin_t;
+  const int32_t* pos;
+  const int32_t* bt;
+  uint8_t* kc;
+  uint8_t* vc;
+  float* ks;  // [n_pages, n_kv, page / 16]
+  float* vs;
+  _Float16* q_out;
+  long long q_stride;
+  int M, n_q, n_kv, log2P, max_pos, n_pages, n_bt;
+};
+void launch_kv8_append(const Kv8Append& a, int head_dim, int cache, hipStream_t st);
+
+// The tokens [start, start + n) of the 8-bit cache as fp16 rows [n, n_kv, head_dim].
+struct Kv8Read {
+  const int32_t* bt;
+  const uint8_t* kc;
+  const uint8_t* vc;
+  const float* ks;
+  const float* vs;
+  _Float16* k_out;
+  _Float16* v_out;
+  int n_bt, n_pages, log2P, n_kv, start, n;
+};
+void launch_kv8_read(const Kv8Read& a, int head_dim, int cache, hipStream_t st);
+
+// Attention of M rows (row m at position *pos + m) over a paged cache of any kind, under a window with sinks (window 0:
+// none), the tokens in `splits` parts (1: no workspace).
+constexpr int kWindowMaxCtx = 1 << 30;
+struct WindowAttn {
+  const void* q;
+  long long q_stride;
+  const int32_t* pos;
+  const int32_t* bt;
+  int n_bt;
+  const void* kc;
+  const void* vc;
+  const float* ks;
+  const float* vs;
+  int cache, n_pages, log2P, n_q, n_kv, head_dim, M, max_ctx, window, sinks;
+  void* out;
+  int splits;
+  void* ws;
+};
+int attention_window_splits(int M, int n_q, int n_kv, int head_dim, int max_ctx, int window, int sinks, int cache);
+size_t attention_window_part_bytes(int M, int n_q, int n_kv, int head_dim);
+void launch_attention_window(const WindowAttn& a, hipStream_t st);
+
 void launch_quantize_w4(const void* w, void* packed, void* sz, int N, int K, int log2G, int clip, hipStream_t st);
 
 

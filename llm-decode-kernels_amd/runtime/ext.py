@@ -60,6 +60,11 @@ SIGNATURES = {
     "dk_token_logprobs_workspace_bytes": ([_I, _I, _I, _I], _Z),
     "dk_token_logprobs": ([_P, _I, _L, _P, _P, _P, _P, _P, _I, _I, _I, _P, _Z, _P], _I),
     "dk_tree_accept": ([_P, _P, _P, _L, _I, _P, _P, _I, _P, _I, _I, _I, _I, _I, _P, _P, _P, _P], _I),
+    "dk_kv8_append_rows": ([_P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _P, _L, _I, _I, _I, _I, _I, _I, _I, _I, _P], _I),
+    "dk_kv8_read": ([_P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P, _P], _I),
+    "dk_attention_window_workspace_bytes": ([_I, _I, _I, _I, _I, _I, _I, _I], _Z),
+    "dk_attention_window": ([_P, _L, _P, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P, _Z, _P],
+                            _I),
     "dk_quantize_w4": ([_P, _P, _P, _I, _I, _I, _I, _P], _I),
 }
 
@@ -137,6 +142,8 @@ def _ints(*sizes):
 
 
 LOGITS_DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+CACHE_DTYPES = {torch.float16: 0, torch.int8: 1, torch.float8_e4m3fn: 2}
+KV8_BLOCK = 16  # tokens that share a scale
 
 
 class DecodeKernels:
@@ -774,6 +781,107 @@ class DecodeKernels:
         self._call_on(dev, self.lib.dk_tree_accept, p_tokens, p_parents, picks.data_ptr(), picks.stride(0) if M > 1 else 1, M,
                       p_pos, p_bt, 0 if bt is None else bt.numel(), p_kv, n_caches, cache[0], cache[1], cache[2], cache[3],
                       p_path, p_count, p_tok)
+
+    def _kv8_cache(self, what, kc, vc, ks, vs):
+        """Shape and type of an 8-bit cache: (its type's number, [pages, n_kv, P, D])."""
+        cache, dtype = kc.shape, CACHE_DTYPES.get(kc.dtype, 0)
+        if dtype == 0:
+            raise RuntimeError(f"{what}: kc and vc must be int8 or float8_e4m3fn, got {kc.dtype}")
+        if len(cache) != 4 or cache[3] not in (64, 128) or vc.shape != cache or cache[2] % KV8_BLOCK:
+            raise RuntimeError("cache must be [pages, n_kv, P, 64|128], of an 8-bit cache P a multiple of 16")
+        scales = (cache[0], cache[1], cache[2] // KV8_BLOCK)
+        if ks.shape != scales or vs.shape != scales:
+            raise RuntimeError(f"{what}: ks and vs must be [pages, n_kv, P / {KV8_BLOCK}]")
+        return dtype, cache
+
+    # rows of a prompt, or one token, rotated and appended to a cache of 8-bit codes
+    def kv8_append_rows(self, qkv, cos_t, sin_t, pos, bt, kc, vc, ks, vs, n_q, n_kv, q_out=None):
+        """rope_append_rows into an 8-bit cache: row m of qkv [M, (n_q + 2 n_kv) * D] is token *pos + m. kc, vc int8 or
+        float8_e4m3fn [pages, n_kv, P, D], ks, vs fp32 [pages, n_kv, P / 16]: a value is code * scale, one power-of-two
+        scale for 16 tokens. The rotated q goes to q_out [M, n_q * D] (rows may be strided; None: in place in qkv). cos_t
+        and sin_t None: no rotation. Rows behind the new ones in a block count as absent."""
+        what, dev = "kv8_append_rows", qkv.get_device()
+        dtype, cache = self._kv8_cache(what, kc, vc, ks, vs)
+        p_qkv, p_cos, p_sin, p_pos, p_bt, p_kc, p_vc, p_ks, p_vs = _check_all(
+            what, dev, (qkv, "qkv", torch.float16), (cos_t, "cos_t", torch.float32), (sin_t, "sin_t", torch.float32),
+            (pos, "pos", torch.int32), (bt, "bt", torch.int32), (kc, "kc", kc.dtype), (vc, "vc", kc.dtype),
+            (ks, "ks", torch.float32), (vs, "vs", torch.float32))
+        rows, D = qkv.shape, cache[3]
+        row = (n_q + 2 * n_kv) * D
+        if len(rows) != 2 or rows[1] != row or cache[1] != n_kv or pos.numel() < 1:
+            raise RuntimeError(f"{what}: qkv must be [M, (n_q + 2 n_kv) * D], pos [1]")
+        if (cos_t is None) != (sin_t is None) \
+                or (cos_t is not None and (cos_t.dim() != 2 or cos_t.size(1) * 2 != D or sin_t.shape != cos_t.shape)):
+            raise RuntimeError(f"{what}: cos_t and sin_t must both be [max_pos, D/2] or both None")
+        M = rows[0]
+        if q_out is None:
+            p_out, q_stride = p_qkv, row
+        else:
+            if q_out.dtype is not torch.float16 or q_out.get_device() != dev or q_out.shape != (M, n_q * D) \
+                    or q_out.stride(1) != 1:
+                raise RuntimeError(f"{what}: q_out must be a CUDA fp16 [M, n_q * D] with contiguous rows")
+            p_out = q_out.data_ptr()
+            q_stride = q_out.stride(0) if M > 1 else row if p_out == p_qkv else n_q * D
+        self._call_on(dev, self.lib.dk_kv8_append_rows, p_qkv, p_cos, p_sin, p_pos, p_bt, p_kc, p_vc, p_ks, p_vs, dtype, p_out,
+                      q_stride, M, int(n_q), int(n_kv), D, cache[2], 0 if cos_t is None else cos_t.size(0), cache[0],
+                      bt.numel())
+
+    # tokens of an 8-bit cache as fp16 rows
+    def kv8_read(self, bt, kc, vc, ks, vs, start, k_out, v_out):
+        """Tokens [start, start + n) of the 8-bit cache as fp16 rows k_out, v_out [n, n_kv, D] (or [n, n_kv * D]); tokens
+        without a mapped page read as zeros."""
+        what, dev = "kv8_read", k_out.get_device()
+        dtype, cache = self._kv8_cache(what, kc, vc, ks, vs)
+        p_bt, p_kc, p_vc, p_ks, p_vs, p_k, p_v = _check_all(
+            what, dev, (bt, "bt", torch.int32), (kc, "kc", kc.dtype), (vc, "vc", kc.dtype), (ks, "ks", torch.float32),
+            (vs, "vs", torch.float32), (k_out, "k_out", torch.float16), (v_out, "v_out", torch.float16))
+        n = k_out.size(0) if k_out.dim() else 0
+        if n < 1 or k_out.numel() != n * cache[1] * cache[3] or v_out.shape != k_out.shape:
+            raise RuntimeError(f"{what}: k_out and v_out must be [n, n_kv, D], n >= 1")
+        self._call_on(dev, self.lib.dk_kv8_read, p_bt, bt.numel(), p_kc, p_vc, p_ks, p_vs, dtype, cache[0], cache[2], cache[1],
+                      cache[3], *_ints(start, n), p_k, p_v)
+
+    # attention of rows under a sliding window with sinks, over fp16 or 8-bit caches
+    def attention_window_workspace_bytes(self, M, n_q, n_kv, head_dim, max_ctx, window=0, sinks=0, dtype=torch.float16):
+        """Bytes of split workspace that attention_window (dtype of the cache fp16) or attention_kv8 (int8, float8_e4m3fn)
+        can use for these sizes (0: it does not split)."""
+        if dtype not in CACHE_DTYPES:
+            raise RuntimeError(f"attention_window: the cache must be fp16, int8 or float8_e4m3fn, got {dtype}")
+        return int(self.lib.dk_attention_window_workspace_bytes(*_ints(M, n_q, n_kv, head_dim, max_ctx, window, sinks),
+                                                                CACHE_DTYPES[dtype]))
+
+    def _attention_window(self, what, q, pos, bt, kc, vc, ks, vs, dtype, max_ctx, out, window, sinks, workspace):
+        dev = q.get_device()
+        p_pos, p_bt, p_kc, p_vc, p_ks, p_vs, p_out = _check_all(
+            what, dev, (pos, "pos", torch.int32), (bt, "bt", torch.int32), (kc, "kc", kc.dtype), (vc, "vc", kc.dtype),
+            (ks, "ks", torch.float32), (vs, "vs", torch.float32), (out, "out", torch.float16))
+        cache, rows, strides = kc.shape, q.shape, q.stride()
+        D = cache[3]
+        if q.dtype is not torch.float16 or len(rows) not in (2, 3) or strides[-1] != 1 \
+                or (len(rows) == 3 and (rows[2] != D or (rows[1] > 1 and strides[1] != D))):
+            raise RuntimeError(f"{what}: q must be a CUDA fp16 [M, n_q, D] or [M, n_q * D] with contiguous rows")
+        M = rows[0]
+        width = rows[1] if len(rows) == 2 else rows[1] * D
+        if width % D != 0 or out.shape != (M, width) or pos.numel() < 1:
+            raise RuntimeError(f"{what}: q rows must hold n_q * D values, out be [M, n_q * D] and pos [1]")
+        max_ctx, window, sinks = _ints(max_ctx, window, sinks)
+        p_ws, ws_bytes = _workspace(what, dev, workspace)
+        self._call_on(dev, self.lib.dk_attention_window, q.data_ptr(), strides[0] if M > 1 else width, p_pos, p_bt, bt.numel(),
+                      p_kc, p_vc, p_ks, p_vs, dtype, cache[0], cache[2], width // D, cache[1], D, M, max_ctx, window, sinks,
+                      p_out, p_ws, ws_bytes)
+
+    def attention_window(self, q, pos, bt, kc, vc, max_ctx, out, window=0, sinks=0, workspace=None):
+        """q [M, n_q, D] or [M, n_q * D] (rows may be strided), rotated; row m is at position p = *pos + m and attends the
+        tokens t <= p of the cache that are in its window (t > p - window; 0: no window) or sinks (t < sinks). max_ctx:
+        *pos + M or more. out [M, n_q * D]."""
+        if kc.dtype is not torch.float16 or kc.dim() != 4 or kc.size(3) not in (64, 128) or vc.shape != kc.shape:
+            raise RuntimeError("cache must be fp16 [pages, n_kv, P, 64|128]")
+        self._attention_window("attention_window", q, pos, bt, kc, vc, None, None, 0, max_ctx, out, window, sinks, workspace)
+
+    def attention_kv8(self, q, pos, bt, kc, vc, ks, vs, max_ctx, out, window=0, sinks=0, workspace=None):
+        """attention_window over an 8-bit cache (kv8_append_rows), by default without a window."""
+        dtype, _ = self._kv8_cache("attention_kv8", kc, vc, ks, vs)
+        self._attention_window("attention_kv8", q, pos, bt, kc, vc, ks, vs, dtype, max_ctx, out, window, sinks, workspace)
 
     # runtime/quant.py:42-48,100-124 on the GPU
     def quantize_w4(self, w, packed, sz, group, clip=False):
