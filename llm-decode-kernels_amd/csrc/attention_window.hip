@@ -600,6 +600,380 @@ attn_window_join_kernel(const float4* __restrict__ part_o, const float2* __restr
       u32x2{as_u32(f16x2{(f16)(o.x * inv), (f16)(o.y * inv)}), as_u32(f16x2{(f16)(o.z * inv), (f16)(o.w * inv)})};
 }
 
+// ---------------------------------------------------------------------------------------------------------------
+// Few columns: at most 16 (row, query head) pairs of a kv head, as in a decode step. Nothing is shared between waves, so K
+// and V go from the cache to registers. A wave takes every kFewWaves-th tile of 32 tokens of its split:
+//   * S^T = K . Q^T on v_mfma_f32_16x16x32_f16, 16 tokens at a time: lane (g, c) feeds token c of K and column c of Q over the
+//     same dims (any order of the dims serves that both operands keep): 16 bytes of a row are one k step of fp16 values or
+//     two of codes. It receives the scores of tokens 4 g + v for column c.
+//   * O^T += V^T . P^T over the 32 tokens: those scores' weights, in fp16, are the B operand as they are (k slot 4 s + v of
+//     lane group g is token 16 s + 4 g + v). For A lane (g, r) loads dims [r D / 16, (r + 1) D / 16) of those 8 tokens' rows
+//     and transposes them in registers; output tile t holds dim r D / 16 + t, so that lane (g, c) ends with D / 4 dims in a
+//     row of column c.
+constexpr int kFewWaves = 8;
+constexpr int kFewCols = 16;
+constexpr int kFewTile = 32;
+
+template <int D, int CACHE>
+struct FewShape {
+  static constexpr bool F16 = CACHE == kCacheF16;
+  static constexpr int ES = F16 ? 2 : 1;        // bytes of a value in the cache
+  static constexpr int KW = D * ES / 64;        // 16-byte loads of a K row per lane
+  static constexpr int DPL = D / 16;            // dims of a V row per lane
+  static constexpr int VW = DPL * ES / 4;       // their words
+};
+
+template <int D, int CACHE>
+__global__ void __launch_bounds__(kFewWaves * kWave)
+attn_few_kernel(const WinArgs a) {
+  using S = FewShape<D, CACHE>;
+  constexpr bool F16 = S::F16;
+  constexpr int NW = kFewWaves, ES = S::ES, KW = S::KW, DPL = S::DPL, VW = S::VW, KS = D / 32;
+  __shared__ float s_m[NW][kFewCols], s_l[NW][kFewCols];
+  __shared__ __align__(16) float s_o[NW][kFewCols][D];
+  const int kvh = blockIdx.x, split = blockIdx.y;
+  const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int P = 1 << a.log2P;
+  const long long pos = *a.pos;
+  const int n_q = a.n_kv << a.lhpg, cols = a.M << a.lhpg;
+  const int cc = min(c, cols - 1);              // columns past the last repeat it
+  const int m = cc >> a.lhpg, hd = (kvh << a.lhpg) + (cc & ((1 << a.lhpg) - 1));
+  const Sight mine = sight_of(pos, m, a.window, a.cap);
+  const Sight s0 = sight_of(pos, 0, a.window, a.cap), s1 = sight_of(pos, a.M - 1, a.window, a.cap);
+  const int ctx = s1.lim + 1;                   // tokens [0, ctx) are read
+  // tiles: those of the sinks, then those of the window; this split's [i0, i1)
+  const int all = (ctx + kFewTile - 1) / kFewTile, wt = min(s0.lo / kFewTile, all);
+  const int ns = a.window > 0 ? min((min(a.sinks, ctx) + kFewTile - 1) / kFewTile, wt) : 0;
+  const unsigned nt = (unsigned)(ns + all - wt), per = nt / (unsigned)a.splits, more = nt - per * (unsigned)a.splits;
+  const int i0 = (int)(split * per + min((unsigned)split, more)), i1 = i0 + (int)per + ((unsigned)split < more);
+  auto tile_at = [&](int i) __attribute__((always_inline)) { return kFewTile * (i < ns ? i : i + (wt - ns)); };
+
+  h8 q[KS];
+  {
+    const f16* qh = a.q + (size_t)m * a.q_stride + (size_t)hd * D;
+#pragma unroll
+    for (int k = 0; k < KS; ++k)  // the dims of K's k step
+      q[k] = __builtin_bit_cast(
+          h8, *reinterpret_cast<const u32x4*>(qh + (F16 ? 32 * k + 8 * g : 64 * (k >> 1) + 16 * g + 8 * (k & 1))));
+  }
+  typedef uint32_t vrow __attribute__((ext_vector_type(VW)));
+  struct Tile {
+    int t0;
+    u32x4 k[2][KW];   // by 16 tokens
+    vrow v[2][4];
+    float ks[2], vs[2];
+    bool ok[2];       // the page is mapped; uniform
+  };
+  struct Pages {
+    int p[2];
+  };
+  auto lookup = [&](int i) __attribute__((always_inline)) {
+    Pages w;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) w.p[s] = a.bt[min(tile_at(i) + 16 * s, ctx - 1) >> a.log2P];
+    return w;
+  };
+  auto load = [&](int i, const Pages& w) __attribute__((always_inline)) {
+    Tile x;
+    x.t0 = tile_at(i);
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      x.ok[s] = (unsigned)w.p[s] < (unsigned)a.n_pages;
+      // (16 tokens lie in one page; without one, rows of a page that exists)
+      const size_t row = (((size_t)(x.ok[s] ? w.p[s] : 0) * a.n_kv + kvh) << a.log2P) + ((x.t0 + 16 * s) & (P - 1));
+      const uint8_t* kr = a.kc + row * (D * ES) + c * (D * ES) + 16 * g;
+      const uint8_t* vr = a.vc + row * (D * ES) + 4 * g * (D * ES) + c * (DPL * ES);
+#pragma unroll
+      for (int j = 0; j < KW; ++j) x.k[s][j] = load_stream(reinterpret_cast<const u32x4*>(kr + 64 * j));
+#pragma unroll
+      for (int v = 0; v < 4; ++v)
+        x.v[s][v] = __builtin_nontemporal_load(reinterpret_cast<const vrow*>(vr + v * (D * ES)));
+      if constexpr (!F16) {
+        x.ks[s] = a.ks[row >> 4];
+        x.vs[s] = a.vs[row >> 4];
+      }
+    }
+    return x;
+  };
+
+  float ref = kWinNoMax, lift = -kWinNoMax, l = 0.f;  // as in the kernel of many columns
+  f4 acc[DPL];
+#pragma unroll
+  for (int t = 0; t < DPL; ++t) acc[t] = f4{0.f, 0.f, 0.f, 0.f};
+
+  // the V operand of output tile t: dim DPL r + t of the 8 tokens
+  auto operand = [&](const Tile& x, const uint32_t (&tr)[2][VW][4], int t) __attribute__((always_inline)) -> u32x4 {
+    if constexpr (F16) {
+      const uint32_t sel = (t & 1) ? 0x07060302u : 0x05040100u;
+      u32x4 r;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        r[2 * s] = __builtin_amdgcn_perm(x.v[s][1][t >> 1], x.v[s][0][t >> 1], sel);
+        r[2 * s + 1] = __builtin_amdgcn_perm(x.v[s][3][t >> 1], x.v[s][2][t >> 1], sel);
+      }
+      return r;
+    } else {
+      const u32x2 lo = kv8_decode4<CACHE>(tr[0][t >> 2][t & 3], x.vs[0]), hi = kv8_decode4<CACHE>(tr[1][t >> 2][t & 3], x.vs[1]);
+      return u32x4{lo[0], lo[1], hi[0], hi[1]};
+    }
+  };
+  auto finite = [](u32x4 x) __attribute__((always_inline)) -> u32x4 {  // zero for what is no finite number
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if ((x[i] & 0x7C00u) == 0x7C00u) x[i] &= 0xFFFF0000u;
+      if ((x[i] & 0x7C000000u) == 0x7C000000u) x[i] &= 0xFFFFu;
+    }
+    return x;
+  };
+  auto compute = [&](Tile& x) __attribute__((always_inline)) {
+    const int t0 = x.t0;
+    // every column sees every token; uniform per wave
+    const bool plain = x.ok[0] && x.ok[1] && t0 + kFewTile - 1 <= s0.lim && (t0 >= s1.lo || t0 + kFewTile <= a.sinks);
+    f4 sc[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      sc[s] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < KW; ++j) {
+        if constexpr (F16) {
+          sc[s] = mfma16x32(__builtin_bit_cast(h8, x.k[s][j]), q[j], sc[s]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            sc[s] = mfma16x32(__builtin_bit_cast(h8, kv8_decode8<CACHE>(u32x2{x.k[s][j][2 * e], x.k[s][j][2 * e + 1]}, x.ks[s])),
+                              q[2 * j + e], sc[s]);
+        }
+      }
+    }
+    if (!plain) {
+      asm volatile("");  // stays a branch
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          const int t = t0 + 16 * s + 4 * g + v;
+          if (!(x.ok[s] && t <= mine.lim && (t >= mine.lo || t < a.sinks))) sc[s][v] = -INFINITY;
+          if (!(x.ok[s] && t < ctx)) x.v[s][v] = vrow(0u);  // (a token that does not exist: its V must not meet a p of 0)
+        }
+        if constexpr (!F16) x.vs[s] = x.ok[s] && t0 + 16 * s < ctx ? x.vs[s] : 1.f;
+      }
+    }
+    float p[2][4];
+    auto weigh = [&](float off, float lift) __attribute__((always_inline)) -> float {
+      float sum = 0.f;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          p[s][v] = __builtin_amdgcn_exp2f(fmaf(sc[s][v] - off, a.c2, lift));
+          sum += p[s][v];
+        }
+      }
+      return sum;
+    };
+    float sum = weigh(0.f, lift);
+    if (__any(!(sum <= kWinMost))) {  // the reference moves to this tile's maximum where that is higher
+      asm volatile("");
+      float mx = sc[0][0];
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+#pragma unroll
+        for (int v = 0; v < 4; ++v) mx = fmaxf(mx, sc[s][v]);
+      }
+      mx = fmaxf(ref, rows_max(mx));
+      int over = !(sum <= kWinMost);  // in any of the column's four lanes
+      over |= __shfl_xor(over, 16, kWave);
+      over |= __shfl_xor(over, 32, kWave);
+      mx = over ? mx : ref;
+      const float alpha = __builtin_amdgcn_exp2f((ref - mx) * a.c2);  // 1 for a column that stays
+      if (mx != ref) lift = fabsf(mx * a.c2) > kWinFar ? INFINITY : kWinLift - mx * a.c2;
+      ref = mx;
+      l *= alpha;
+#pragma unroll
+      for (int t = 0; t < DPL; ++t) acc[t] *= alpha;
+      sum = weigh(lift == INFINITY ? ref : 0.f, lift == INFINITY ? kWinLift : lift);
+    }
+    l += sum;
+    h8 ph;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+#pragma unroll
+      for (int v = 0; v < 4; ++v) ph[4 * s + v] = (f16)p[s][v];
+    }
+    // codes: bytes of four tokens' words to words of four tokens
+    uint32_t tr[2][VW][4];
+    if constexpr (!F16) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+#pragma unroll
+        for (int w = 0; w < VW; ++w) {
+          const uint32_t al = __builtin_amdgcn_perm(x.v[s][1][w], x.v[s][0][w], 0x05010400u);
+          const uint32_t ah = __builtin_amdgcn_perm(x.v[s][1][w], x.v[s][0][w], 0x07030602u);
+          const uint32_t bl = __builtin_amdgcn_perm(x.v[s][3][w], x.v[s][2][w], 0x05010400u);
+          const uint32_t bh = __builtin_amdgcn_perm(x.v[s][3][w], x.v[s][2][w], 0x07030602u);
+          tr[s][w][0] = __builtin_amdgcn_perm(bl, al, 0x05040100u);
+          tr[s][w][1] = __builtin_amdgcn_perm(bl, al, 0x07060302u);
+          tr[s][w][2] = __builtin_amdgcn_perm(bh, ah, 0x05040100u);
+          tr[s][w][3] = __builtin_amdgcn_perm(bh, ah, 0x07060302u);
+        }
+      }
+    }
+    bool dirty = false;  // NaN or infinity in V of a tile that not every column sees whole; uniform
+    if (!plain) {
+      asm volatile("");
+#pragma unroll
+      for (int t = 0; t < DPL; ++t) dirty = dirty || has_nonfinite(operand(x, tr, t));
+      dirty = __any(dirty);
+    }
+    if (!dirty) {
+#pragma unroll
+      for (int t = 0; t < DPL; ++t) acc[t] = mfma16x32(__builtin_bit_cast(h8, operand(x, tr, t)), ph, acc[t]);
+      return;
+    }
+    asm volatile("");
+#pragma unroll
+    for (int t = 0; t < DPL; ++t) acc[t] = mfma16x32(__builtin_bit_cast(h8, finite(operand(x, tr, t))), ph, acc[t]);
+    // the values left out, for the columns that see their token
+    for (int i = 0; i < kFewTile; ++i) {
+      const int t = t0 + i, s = i >> 4;
+      if (!((s ? x.ok[1] : x.ok[0]) && t < ctx)) continue;  // uniform
+      const bool see = t <= mine.lim && (t >= mine.lo || t < a.sinks);
+      float w = 0.f;                        // p of token i: in lane group i / 4 % 4, element (s, i % 4)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w = e == 4 * s + (i & 3) ? p[e >> 2][e & 3] : w;
+      w = __shfl(w, 16 * ((i >> 2) & 3) + c, kWave);
+      const size_t at = (((size_t)a.bt[t >> a.log2P] * a.n_kv + kvh) << a.log2P) + (t & (P - 1));
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+#pragma unroll
+        for (int d = 0; d < DPL; d += 4) {
+          const size_t off = at * D + (size_t)(4 * g + v) * DPL + d;
+          u32x2 b;
+          if constexpr (F16)
+            b = *reinterpret_cast<const u32x2*>(a.vc + 2 * off);
+          else
+            b = kv8_decode4<CACHE>(*reinterpret_cast<const uint32_t*>(a.vc + off), a.vs[at >> 4]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float f = (float)as_f16x2(b[e >> 1])[e & 1];
+            if (see && !(fabsf(f) <= 65504.f)) acc[d + e][v] = fmaf(w, f, acc[d + e][v]);
+          }
+        }
+      }
+    }
+  };
+
+  int i = i0 + wave;
+  if (i < i1) {  // uniform per wave
+    Pages pg = lookup(i);
+    Tile x = load(i, pg);
+    pg = lookup(i + NW);
+    for (; i < i1; i += 2 * NW) {
+      Tile y = load(i + NW, pg);  // past the end: rows that are never computed on
+      pg = lookup(i + 2 * NW);
+      compute(x);
+      if (i + NW >= i1) break;
+      x = load(i + 2 * NW, pg);
+      pg = lookup(i + 3 * NW);
+      compute(y);
+    }
+  }
+  l = rows_sum(l);
+  // ---- the waves meet in LDS, in order: column c's dims [D / 4 g, + D / 4), acc[t][v] dim D / 4 g + DPL v + t
+  if (g == 0) {
+    s_m[wave][c] = ref;
+    s_l[wave][c] = l;
+  }
+  if (c < cols) {
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+#pragma unroll
+      for (int t = 0; t < DPL; t += 4)
+        *reinterpret_cast<f4*>(&s_o[wave][c][D / 4 * g + DPL * v + t]) = f4{acc[t][v], acc[t + 1][v], acc[t + 2][v], acc[t + 3][v]};
+    }
+  }
+  __syncthreads();
+  const size_t part = (size_t)split * a.n_kv + kvh;
+  const bool none = i0 >= i1;  // a split without tokens: the join reads no output of it
+  for (int j = tid; j < cols * (D / 4); j += NW * kWave) {
+    const int col = j / (D / 4), d = 4 * (j % (D / 4));
+    float mx = kWinNoMax, L = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) mx = fmaxf(mx, s_m[w][col]);
+    f4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      // a wave that saw no token weighs 0 beside one that did
+      const float f = __builtin_amdgcn_exp2f((s_m[w][col] - mx) * a.c2);
+      L = fmaf(f, s_l[w][col], L);
+      const f4 y = *reinterpret_cast<const f4*>(&s_o[w][col][d]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = fmaf(f, y[e], o[e]);
+    }
+    if (a.splits > 1) {
+      if (d == 0) a.part_ml[part * kFewCols + col] = none ? float2{kWinNoMax, 0.f} : float2{mx, L};
+      if (!none) store_through16(a.part_o + part * kFewCols * (D / 4), 4 * (col * D + d), __builtin_bit_cast(u32x4, o));
+      continue;
+    }
+    const float inv = L == 0.f ? 0.f : 1.0f / L;  // a NaN stays
+    const int mo = col >> a.lhpg, ho = (kvh << a.lhpg) + (col & ((1 << a.lhpg) - 1));
+    *reinterpret_cast<u32x2*>(a.out + ((size_t)mo * n_q + ho) * D + d) =
+        u32x2{as_u32(f16x2{(f16)(o[0] * inv), (f16)(o[1] * inv)}), as_u32(f16x2{(f16)(o[2] * inv), (f16)(o[3] * inv)})};
+  }
+}
+
+// Joins the splits of one column, in split order: groups of D / 4 threads take the splits i, i + G, ..., then meet in LDS.
+template <int D>
+__global__ void __launch_bounds__(256)
+attn_few_join_kernel(const f4* __restrict__ part_o, const float2* __restrict__ part_ml, int lhpg, int n_kv, int splits,
+                     float c2, f16* __restrict__ out) {
+  constexpr int T = D / 4, G = 256 / T;
+  __shared__ float s_w[kWinMaxSplits];
+  __shared__ float s_l;
+  __shared__ f4 s_o[G][T];
+  const int kvh = blockIdx.x, col = blockIdx.y, tid = threadIdx.x, d = tid % T, grp = tid / T;
+  const size_t step = (size_t)n_kv * kFewCols, first = (size_t)kvh * kFewCols + col;
+  constexpr int NB = kWinMaxSplits / G;
+  f4 x[NB];
+#pragma unroll
+  for (int k = 0; k < NB; ++k) {
+    const int s = grp + G * k;
+    if (s < splits) x[k] = part_o[((size_t)s * step + first) * T + d];
+  }
+  if (tid < kWave) {
+    const float2 ml = tid < splits ? part_ml[(size_t)tid * step + first] : float2{kWinNoMax, 0.f};
+    const bool saw = ml.x != kWinNoMax || ml.y != 0.f;  // (a NaN sum counts)
+    const float mx = group_max<kWave>(ml.x);
+    const float w = __builtin_amdgcn_exp2f((ml.x - mx) * c2);
+    const float L = group_sum<kWave>(saw ? w * ml.y : 0.f);
+    s_w[tid] = saw ? w : -1.f;
+    if (tid == 0) s_l = L;
+  }
+  __syncthreads();
+  f4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int k = 0; k < NB; ++k) {
+    const int s = grp + G * k;
+    const float w = s < splits ? s_w[s] : -1.f;
+    if (w < 0.f) continue;  // (its output was not written)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = fmaf(w, x[k][e], o[e]);
+  }
+  s_o[grp][d] = o;
+  __syncthreads();
+  if (grp > 0) return;
+#pragma unroll
+  for (int k = 1; k < G; ++k) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] += s_o[k][d][e];
+  }
+  const float inv = s_l == 0.f ? 0.f : 1.0f / s_l;  // a NaN stays
+  const int m = col >> lhpg, hd = (kvh << lhpg) + (col & ((1 << lhpg) - 1));
+  *reinterpret_cast<u32x2*>(out + ((size_t)m * (n_kv << lhpg) + hd) * D + 4 * d) =
+      u32x2{as_u32(f16x2{(f16)(o[0] * inv), (f16)(o[1] * inv)}), as_u32(f16x2{(f16)(o[2] * inv), (f16)(o[3] * inv)})};
+}
+
 // Workgroup shape (CW, KVS, BT) by the column waves of a kv head.
 struct WinShape {
   int cw, kvs, bt;
@@ -610,6 +984,8 @@ WinShape win_shape(int M, int n_q, int n_kv) {
   if (waves <= 32) return {4, 2, 64};
   return {8, 1, 128};
 }
+// Whether the kernel of few columns takes a call. Pages of fewer than 16 tokens are left to the other one.
+bool win_few(int M, int n_q, int n_kv, int log2P) { return (long long)M * (n_q / n_kv) <= kFewCols && log2P >= 4; }
 // The tokens that a block of columns can see at most.
 long long win_tokens(int rows, int max_ctx, int window, int sinks) {
   if (window == 0) return max_ctx;
@@ -618,8 +994,16 @@ long long win_tokens(int rows, int max_ctx, int window, int sinks) {
 
 }  // namespace
 
-// At most one workgroup per CU, in splits of equal length.
+// At most one workgroup per CU, in splits of equal length. (The query does not know the page: where a cache of small pages
+// keeps few columns from their kernel, the other one runs that many splits.)
 int attention_window_splits(int M, int n_q, int n_kv, int D, int max_ctx, int window, int sinks, int cache) {
+  if (win_few(M, n_q, n_kv, 4)) {
+    const long long tiles = (win_tokens(M, max_ctx, window, sinks) + kFewTile - 1) / kFewTile + 2;
+    if (tiles <= 2 * kFewWaves) return 1;
+    const long long want = max(1LL, min((long long)kWinMaxSplits, 256LL / n_kv));
+    const long long per = max((tiles + want - 1) / want, (long long)kFewWaves);
+    return (int)((tiles + per - 1) / per);
+  }
   const WinShape s = win_shape(M, n_q, n_kv);
   const long long cols = (long long)M * (n_q / n_kv);
   const long long blocks = (cols + 32 * s.cw - 1) / (32 * s.cw), round = s.bt * s.kvs;
@@ -655,6 +1039,15 @@ void launch(const WindowAttn& w, hipStream_t st) {
                   w.log2P, w.n_kv, lhpg, w.M, (int)min((long long)w.max_ctx, (long long)w.n_bt << w.log2P), w.window, w.sinks,
                   w.splits, (float)(1.4426950408889634 / sqrt((double)D)), (f16*)w.out, part_o,
                   (float2*)(part_o + (size_t)w.splits * w.n_kv * waves * 8 * D)};
+  if (win_few(w.M, w.n_q, w.n_kv, w.log2P)) {
+    WinArgs f = a;
+    f.part_ml = (float2*)(part_o + (size_t)w.splits * w.n_kv * kFewCols * (D / 4));
+    hipLaunchKernelGGL((attn_few_kernel<D, CACHE>), dim3(w.n_kv, w.splits), dim3(kFewWaves * kWave), 0, st, f);
+    if (w.splits > 1)
+      hipLaunchKernelGGL(attn_few_join_kernel<D>, dim3(w.n_kv, (unsigned)cols), dim3(256), 0, st, (const f4*)part_o, f.part_ml,
+                         lhpg, w.n_kv, w.splits, a.c2, (f16*)w.out);
+    return;
+  }
   const WinShape s = win_shape(w.M, w.n_q, w.n_kv);
   if (s.cw == 2)
     launch_shape<D, CACHE, 2, 4, 32>(a, cols, st);

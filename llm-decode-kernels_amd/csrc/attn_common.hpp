@@ -65,6 +65,8 @@ __device__ __forceinline__ f32x16 mfma32x32(h8 a, h8 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
 
+__device__ __forceinline__ f4 mfma16x32(h8 a, h8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+
 // Keeps loads where they are written (no sinking to their first use).
 __device__ __forceinline__ void pf_fence() { asm volatile("" ::: "memory"); }
 

@@ -58,27 +58,24 @@ __device__ __forceinline__ uint32_t kv8_encode4(const float (&y)[4], float big) 
   }
 }
 
-// The values of eight codes in fp16. A product that passes fp16 (codes that this library did not write) is infinite.
+// The values of four codes in fp16. A product that passes fp16 (codes that this library did not write) is infinite.
 template <int CACHE>
-__device__ __forceinline__ u32x4 kv8_decode8(u32x2 w, float s) {
-  u32x4 r;
+__device__ __forceinline__ u32x2 kv8_decode4(uint32_t w, float s) {
   if constexpr (CACHE == kCacheInt8) {
     const f16 sh = (f16)s;
     const f16x2 sc = {sh, sh}, bias = {(f16)-1152.f, (f16)-1152.f};
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint32_t u = w[i] ^ 0x80808080u;  // code + 128; as the low byte of 0x6400 it is 1024 + code + 128
-      r[2 * i] = as_u32((as_f16x2(__builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) + bias) * sc);
-      r[2 * i + 1] = as_u32((as_f16x2(__builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) + bias) * sc);
-    }
+    const uint32_t u = w ^ 0x80808080u;  // code + 128; as the low byte of 0x6400 it is 1024 + code + 128
+    return u32x2{as_u32((as_f16x2(__builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) + bias) * sc),
+                 as_u32((as_f16x2(__builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) + bias) * sc)};
   } else {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      r[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[i], s, false));
-      r[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[i], s, true));
-    }
+    return u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, s, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, s, true))};
   }
-  return r;
+}
+template <int CACHE>
+__device__ __forceinline__ u32x4 kv8_decode8(u32x2 w, float s) {
+  const u32x2 lo = kv8_decode4<CACHE>(w[0], s), hi = kv8_decode4<CACHE>(w[1], s);
+  return u32x4{lo[0], lo[1], hi[0], hi[1]};
 }
 
 }  // namespace dk
