@@ -24,7 +24,7 @@ struct WinArgs {
   const uint8_t* vc;
   const float* ks;
   const float* vs;
-  int n_pages, log2P, n_kv, lhpg, M, cap;  // cap: tokens at and past it do not exist
+  int n_pages, n_bt, log2P, n_kv, lhpg, M, cap;  // cap: tokens at and past it do not exist
   int window, sinks, splits;
   float c2;  // log2(e) / sqrt(D)
   f16* out;  // [M, n_q D]
@@ -97,12 +97,13 @@ __global__ void __launch_bounds__(CW * KVS * kWave, 2) attn_window_kernel(const 
   const Sight g0 = sight_of(pos, row_of(cb * CW * 32), a.window, a.cap);              // the workgroup's
   const Sight g1 = sight_of(pos, row_of((cb + 1) * CW * 32 - 1), a.window, a.cap);
   const int ctx = g1.lim + 1;                   // tokens [0, ctx) are read
-  // rounds: those of the sinks, then those of the window
-  const int all = (ctx + SB - 1) / SB, wr = min(g0.lo / SB, all);
-  const int ns = a.window > 0 ? min((min(a.sinks, ctx) + SB - 1) / SB, wr) : 0;
-  auto round_at = [&](int v) __attribute__((always_inline)) { return v < ns ? v : v + (wr - ns); };
-  // this split's [r0, r1): the first nr % splits splits have one more
-  const unsigned nr = (unsigned)(ns + all - wr), per = nr / (unsigned)a.splits, more = nr - per * (unsigned)a.splits;
+  // The tokens in the order in which they are taken ("places"): the sinks, in whole tiles of 32, then those from the window's
+  // first tile on; place v is token v below ns and v + gap from there.
+  const int all = (ctx + 31) / 32, wt = min(g0.lo / 32, all);
+  const int ns = a.window > 0 ? 32 * min((min(a.sinks, ctx) + 31) / 32, wt) : 0, gap = 32 * wt - ns;
+  auto token = [&](int v) __attribute__((always_inline)) { return v < ns ? v : v + gap; };
+  // this split's rounds [r0, r1): the first nr % splits splits have one more
+  const unsigned nr = (unsigned)(32 * all - gap + SB - 1) / SB, per = nr / (unsigned)a.splits, more = nr - per * (unsigned)a.splits;
   const int r0 = (int)(split * per + min((unsigned)split, more)), r1 = r0 + (int)per + ((unsigned)split < more);
   h8 q[KS];
   auto load_q = [&]() __attribute__((always_inline)) {
@@ -133,18 +134,18 @@ __global__ void __launch_bounds__(CW * KVS * kWave, 2) attn_window_kernel(const 
   };
   bool whole = true;      // every page with a token of this split that some column can see is mapped; uniform
   auto mapped = [&](int t) __attribute__((always_inline)) { return (unsigned)a.bt[t >> a.log2P] < (unsigned)a.n_pages; };
-  auto first_row = [&](int rr, int i) __attribute__((always_inline)) { return rr * SB + (UP ? RPW * wave : sr) + RPI * i; };
+  auto first_row = [&](int rnd, int i) __attribute__((always_inline)) {  // (a load's rows lie in one tile)
+    return token(rnd * SB + (UP ? RPW * wave : sr) + RPI * i);
+  };
   auto lookup = [&](int rnd) __attribute__((always_inline)) {
-    const int rr = round_at(rnd);
 #pragma unroll
-    for (int i = 0; i < NP; ++i) pg[i] = a.bt[min(first_row(rr, UP ? lane % LPT : i), ctx - 1) >> a.log2P];
+    for (int i = 0; i < NP; ++i) pg[i] = a.bt[min(first_row(rnd, UP ? lane % LPT : i), ctx - 1) >> a.log2P];
   };
   auto locate = [&](int rnd) __attribute__((always_inline)) {  // from the looked-up pages
     Rows w;
-    const int rr = round_at(rnd);
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-      const int t = first_row(rr, UP ? lane % LPT : i);
+      const int t = first_row(rnd, UP ? lane % LPT : i);
       const uint64_t page = (uint64_t)(uint32_t)((unsigned)pg[i] < (unsigned)a.n_pages ? pg[i] : 0);
       w.base[i] = page * page_bytes + (uint64_t)(uint32_t)(t & (P - 1)) * GB;  // (a page may pass 4 GiB)
       if constexpr (!F16) {
@@ -180,16 +181,17 @@ __global__ void __launch_bounds__(CW * KVS * kWave, 2) attn_window_kernel(const 
     }
   };
   // A round in which some column does not see some token (uniform in the workgroup).
-  auto partial = [&](int rr) __attribute__((always_inline)) {
-    const int t0 = rr * SB, t1 = t0 + SB;
-    return t1 > g0.lim + 1 || (t0 < g1.lo && t1 > a.sinks);
+  auto partial = [&](int rnd) __attribute__((always_inline)) {
+    const int t0 = rnd * SB + gap, t1 = t0 + SB;
+    return rnd * SB < ns || t1 > g0.lim + 1 || (t0 < g1.lo && t1 > a.sinks);
   };
   // A V chunk (8 dims of token t) that must not meet a p of 0 is taken out: one of a token that does not exist, and one with
   // NaN or infinity in a round that not every column sees whole.
-  auto checked = [&](u32x4 x, int rnd, int rr, int t) __attribute__((always_inline)) -> u32x4 {
+  auto checked = [&](u32x4 x, int rnd, int row) __attribute__((always_inline)) -> u32x4 {
+    const int t = token(rnd * SB + row);
     const bool ok = t < ctx && (whole || mapped(t));
     const bool bad = ok && has_nonfinite(x);
-    if (bad) atomicOr(&s_bad[(unsigned)rnd % 3u][(t - rr * SB) / 32], 1u << (t % 32));
+    if (bad) atomicOr(&s_bad[(unsigned)rnd % 3u][row / 32], 1u << (row % 32));
     return ok && !bad ? x : u32x4{0u, 0u, 0u, 0u};
   };
 
@@ -205,9 +207,9 @@ __global__ void __launch_bounds__(CW * KVS * kWave, 2) attn_window_kernel(const 
   const int vd = 32 * ((lane >> 4) & 1) + 8 * (lane & 3);  // byte of its 4 dims within the 64-byte unit
   const int vrow = (grp * BT + vt) * RB + vd, vsw = D == 128 ? vt & 3 : (vt >> 1) & 1;
 
-  // bits of tokens [t0, t0 + 64) that this lane's column sees by position
-  auto seen_bits = [&](int t0) __attribute__((always_inline)) -> uint64_t {
-    auto low = [](int n) -> uint64_t { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1; };
+  // bits of tokens [t0, t0 + 32) that this lane's column sees by position
+  auto seen_bits = [&](int t0) __attribute__((always_inline)) -> uint32_t {
+    auto low = [](int n) -> uint32_t { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; };
     return low(mine.lim + 1 - t0) & (~low(mine.lo - t0) | low(a.sinks - t0));
   };
   // ---- a block, by tiles of 32 tokens
@@ -228,17 +230,16 @@ __global__ void __launch_bounds__(CW * KVS * kWave, 2) attn_window_kernel(const 
     pw[e >> 3][(e & 7) >> 1] = pair;
   };
   auto block = [&](int rnd, const uint8_t* kb, const uint8_t* vb, auto send) __attribute__((always_inline)) {
-    const int t0 = (round_at(rnd) * KVS + grp) * BT;
-    // every token is seen; uniform per wave
-    const bool plain = whole && t0 + BT - 1 <= w0.lim && (t0 >= w1.lo || t0 + BT <= a.sinks);
-    constexpr int NB = (BT + 63) / 64;
-    uint64_t vis[NB];
+    const int v0 = (rnd * KVS + grp) * BT, t0 = v0 + gap;
+    // every token is seen; uniform per wave (a block with sinks counts as one that is not seen whole)
+    const bool plain = whole && v0 >= ns && t0 + BT - 1 <= w0.lim && (t0 >= w1.lo || t0 + BT <= a.sinks);
+    uint32_t vis[NT];
     if (!plain) {
       asm volatile("");  // stays a branch
 #pragma unroll
-      for (int c = 0; c < NB; ++c) {
-        const int t = t0 + 64 * c + lane % BT;
-        vis[c] = __ballot(t < ctx && lane < BT && (whole || mapped(t))) & seen_bits(t0 + 64 * c);
+      for (int c = 0; c < NT; ++c) {
+        const int ts = token(v0 + 32 * c);
+        vis[c] = (uint32_t)__ballot(ts + r < ctx && (whole || mapped(ts + r))) & seen_bits(ts);
       }
     }
     int kat = krow + ((h ^ ksw) << 4), vat = vrow + (vsw << 6);
@@ -268,7 +269,7 @@ __global__ void __launch_bounds__(CW * KVS * kWave, 2) attn_window_kernel(const 
       }
       if (!plain) {
         asm volatile("");
-        const uint32_t bits = (uint32_t)(vis[tt / 2] >> (32 * (tt & 1))) >> (4 * h);
+        const uint32_t bits = vis[tt] >> (4 * h);
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           if (!(bits & (1u << (8 * (i >> 2) + (i & 3))))) sc[tt & 1][i] = -INFINITY;
@@ -328,19 +329,20 @@ __global__ void __launch_bounds__(CW * KVS * kWave, 2) attn_window_kernel(const 
         for (int t = 0; t < DT; ++t) acc[t] = mfma32x32(va[ks][t], __builtin_bit_cast(h8, pw[ks]), acc[t]);
       }
     }
-    if (!whole || partial(round_at(rnd))) {  // uniform in the workgroup
+    if (!whole || partial(rnd)) {  // uniform in the workgroup
       // the chunks that were taken out, from the cache, for the columns that see their token; its weight once more from q and
       // k, as in the loop and so the same to the last bit
       for (int w = 0; w < BT / 32; ++w) {
         uint32_t bad = __builtin_amdgcn_readfirstlane(s_bad[(unsigned)rnd % 3u][grp * (BT / 32) + w]);
         if (bad == 0) continue;
-        const uint64_t seen = plain ? ~0ull : vis[w / 2] >> (32 * (w & 1));
+        const int ts = token(v0 + 32 * w);
+        const uint32_t seen = seen_bits(ts);
         f32x16 st = {};
 #pragma unroll
         for (int k = 0; k < KS; ++k)
           st = mfma32x32(__builtin_bit_cast(h8, *reinterpret_cast<const u32x4*>(kb + w * 32 * RB + (kat ^ (k << 5)))), q[k], st);
         for (; bad != 0; bad &= bad - 1) {
-          const int i = __builtin_ctz(bad), t = t0 + 32 * w + i;  // a token in this set is inside the context
+          const int i = __builtin_ctz(bad), t = ts + i;            // a token in this set is inside the context
           const int page = a.bt[t >> a.log2P];
           if ((unsigned)page >= (unsigned)a.n_pages) continue;     // (nobody sees it)
           const size_t at = (((size_t)page * a.n_kv + kvh) << a.log2P) + (t & (P - 1));
@@ -378,8 +380,7 @@ __global__ void __launch_bounds__(CW * KVS * kWave, 2) attn_window_kernel(const 
       fetch(vp, rows, j - LPT, v_place, v, vv);
   };
   auto finish = [&](int rnd, uint8_t* k, uint8_t* v) __attribute__((always_inline)) {
-    const int rr = round_at(rnd);
-    const bool check = rnd < r1 && (!whole || partial(rr));  // uniform
+    const bool check = rnd < r1 && (!whole || partial(rnd));  // uniform
     if constexpr (F16) {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       if (check) {
@@ -388,7 +389,7 @@ __global__ void __launch_bounds__(CW * KVS * kWave, 2) attn_window_kernel(const 
         for (int i = 0; i < LPT; ++i) {
           const int row = sr + RPI * i;
           u32x4* x = reinterpret_cast<u32x4*>(v + row * RB + 16 * sch);
-          *x = checked(*x, rnd, rr, rr * SB + row);
+          *x = checked(*x, rnd, row);
         }
       }
     } else {
@@ -411,7 +412,7 @@ __global__ void __launch_bounds__(CW * KVS * kWave, 2) attn_window_kernel(const 
         for (int e = 0; e < 2; ++e) x[e] = kv8_decode8<CACHE>(u32x2{vv[i][2 * e], vv[i][2 * e + 1]}, s);
         if (check) {
           asm volatile("");  // stays a branch
-          for (int e = 0; e < 2; ++e) x[e] = checked(x[e], rnd, rr, rr * SB + sr + RPI * i);
+          for (int e = 0; e < 2; ++e) x[e] = checked(x[e], rnd, sr + RPI * i);
         }
         at[0] = x[0];
         at[1] = x[1];
@@ -452,8 +453,8 @@ __global__ void __launch_bounds__(CW * KVS * kWave, 2) attn_window_kernel(const 
         whole = whole && (unsigned)a.bt[p] < (unsigned)a.n_pages;
     };
     // (pages between the sinks and the window may be gone)
-    if (r0 < ns) scan(r0 * SB, min(min(r1, ns) * SB, min(a.sinks, ctx)));
-    if (r1 > ns) scan(max(round_at(max(r0, ns)) * SB, min(g0.lo, ctx)), min(round_at(r1) * SB, ctx));
+    if (r0 * SB < ns) scan(r0 * SB, min(min(r1 * SB, ns), min(a.sinks, ctx)));
+    if (r1 * SB > ns) scan(max(max(r0 * SB, ns) + gap, min(g0.lo, ctx)), min(r1 * SB + gap, ctx));
     __syncthreads();  // (s_bad, s_holes)
     if (!whole) s_holes = 1;
     __syncthreads();
@@ -602,7 +603,8 @@ attn_window_join_kernel(const float4* __restrict__ part_o, const float2* __restr
 
 // ---------------------------------------------------------------------------------------------------------------
 // Few columns: at most 16 (row, query head) pairs of a kv head, as in a decode step. Nothing is shared between waves, so K
-// and V go from the cache to registers. A wave takes every kFewWaves-th tile of 32 tokens of its split:
+// and V go from the cache to registers. The waves of all splits take the tiles of 32 tokens in turn, so that a page can be
+// looked up before the position is known. Per tile:
 //   * S^T = K . Q^T on v_mfma_f32_16x16x32_f16, 16 tokens at a time: lane (g, c) feeds token c of K and column c of Q over the
 //     same dims (any order of the dims serves that both operands keep): 16 bytes of a row are one k step of fp16 values or
 //     two of codes. It receives the scores of tokens 4 g + v for column c.
@@ -642,11 +644,10 @@ attn_few_kernel(const WinArgs a) {
   const Sight mine = sight_of(pos, m, a.window, a.cap);
   const Sight s0 = sight_of(pos, 0, a.window, a.cap), s1 = sight_of(pos, a.M - 1, a.window, a.cap);
   const int ctx = s1.lim + 1;                   // tokens [0, ctx) are read
-  // tiles: those of the sinks, then those of the window; this split's [i0, i1)
+  // tiles: those of the sinks, then those of the window, nt in all; this wave's are i0 and every step-th from there
   const int all = (ctx + kFewTile - 1) / kFewTile, wt = min(s0.lo / kFewTile, all);
   const int ns = a.window > 0 ? min((min(a.sinks, ctx) + kFewTile - 1) / kFewTile, wt) : 0;
-  const unsigned nt = (unsigned)(ns + all - wt), per = nt / (unsigned)a.splits, more = nt - per * (unsigned)a.splits;
-  const int i0 = (int)(split * per + min((unsigned)split, more)), i1 = i0 + (int)per + ((unsigned)split < more);
+  const int nt = ns + all - wt, i0 = split * NW + wave, step = a.splits * NW;
   auto tile_at = [&](int i) __attribute__((always_inline)) { return kFewTile * (i < ns ? i : i + (wt - ns)); };
 
   h8 q[KS];
@@ -671,7 +672,7 @@ attn_few_kernel(const WinArgs a) {
   auto lookup = [&](int i) __attribute__((always_inline)) {
     Pages w;
 #pragma unroll
-    for (int s = 0; s < 2; ++s) w.p[s] = a.bt[min(tile_at(i) + 16 * s, ctx - 1) >> a.log2P];
+    for (int s = 0; s < 2; ++s) w.p[s] = a.bt[min((tile_at(i) + 16 * s) >> a.log2P, a.n_bt - 1)];
     return w;
   };
   auto load = [&](int i, const Pages& w) __attribute__((always_inline)) {
@@ -864,18 +865,17 @@ attn_few_kernel(const WinArgs a) {
     }
   };
 
-  int i = i0 + wave;
-  if (i < i1) {  // uniform per wave
-    Pages pg = lookup(i);
-    Tile x = load(i, pg);
-    pg = lookup(i + NW);
-    for (; i < i1; i += 2 * NW) {
-      Tile y = load(i + NW, pg);  // past the end: rows that are never computed on
-      pg = lookup(i + 2 * NW);
+  Pages pg = lookup(i0);
+  if (i0 < nt) {  // uniform per wave
+    Tile x = load(i0, pg);
+    pg = lookup(i0 + step);
+    for (int i = i0; i < nt; i += 2 * step) {
+      Tile y = load(i + step, pg);  // past the end: rows that are never computed on
+      pg = lookup(i + 2 * step);
       compute(x);
-      if (i + NW >= i1) break;
-      x = load(i + 2 * NW, pg);
-      pg = lookup(i + 3 * NW);
+      if (i + step >= nt) break;
+      x = load(i + 2 * step, pg);
+      pg = lookup(i + 3 * step);
       compute(y);
     }
   }
@@ -895,7 +895,7 @@ attn_few_kernel(const WinArgs a) {
   }
   __syncthreads();
   const size_t part = (size_t)split * a.n_kv + kvh;
-  const bool none = i0 >= i1;  // a split without tokens: the join reads no output of it
+  const bool none = split * NW >= nt;  // a split without tokens: the join reads no output of it
   for (int j = tid; j < cols * (D / 4); j += NW * kWave) {
     const int col = j / (D / 4), d = 4 * (j % (D / 4));
     float mx = kWinNoMax, L = 0.f;
@@ -974,45 +974,72 @@ attn_few_join_kernel(const f4* __restrict__ part_o, const float2* __restrict__ p
       u32x2{as_u32(f16x2{(f16)(o[0] * inv), (f16)(o[1] * inv)}), as_u32(f16x2{(f16)(o[2] * inv), (f16)(o[3] * inv)})};
 }
 
-// Workgroup shape (CW, KVS, BT) by the column waves of a kv head.
+// The tokens that a block of `rows` rows can see at most.
+long long win_tokens(long long rows, int max_ctx, int window, int sinks) {
+  return window == 0 ? max_ctx : min((long long)max_ctx, (long long)window + rows + sinks + 32);
+}
+// Shape of the workgroup (CW, KVS, BT), and the splits that it can use: at most one workgroup per CU, of equal length.
 struct WinShape {
-  int cw, kvs, bt;
+  int cw, kvs, bt, splits;
 };
-WinShape win_shape(int M, int n_q, int n_kv) {
-  const long long waves = ((long long)M * (n_q / n_kv) + 31) / 32;
-  if (waves <= 4) return {2, 4, 32};
-  if (waves <= 32) return {4, 2, 64};
-  return {8, 1, 128};
+constexpr WinShape kWinShapes[4] = {{2, 4, 32, 1}, {4, 1, 64, 1}, {4, 2, 64, 1}, {8, 1, 128, 1}};
+
+// The shape with the least estimated time: a fixed part, a round's time times the rounds of the longest workgroup, or of all
+// of them over the CUs with what it takes to start each. Fitted to the times of all four shapes in 75 cases (8 to 4096 rows
+// behind 0 to 30000 tokens, windows of 256 to 2048 and none, five head layouts); the choice is 0.8% above the best of the four
+// in the geometric mean, 15% at worst. In us, D 128 (e4m3, 8 x 4 heads):
+//                              (2,4,32) (4,1,64) (4,2,64) (8,1,128)
+//   512 rows at 0                15.3     19.2     19.3     20.5
+//   64 behind 4000               18.4     19.3     19.7     23.7
+//   1024 at 0                    30.2     32.1     28.1     33.5
+//   256 behind 8000              62.9     59.5     52.0     49.1
+//   4096 at 0                   262      171      185      150
+//   4096, window 1024           172       97      121      103
+WinShape win_shape(int M, int n_q, int n_kv, int D, int max_ctx, int window, int sinks) {
+  const double rounds[2][4] = {{0.96, 1.0, 1.42, 2.39}, {1.62, 1.49, 2.52, 4.3}};  // us of a round, D 64 and 128
+  const double paired[2] = {1.24, 2.32};                                            // (4,1,64): of two workgroups of a CU
+  const double fixed[4] = {7.89, 8.49, 8.88, 10.19}, join = 2.9, start = 7.68;
+  const int hpg = n_q / n_kv, d = D == 128;
+  const long long waves = ((long long)M * hpg + 31) / 32;
+  WinShape best = {};
+  double least = 0;
+  for (int i = 0; i < 4; ++i) {
+    WinShape s = kWinShapes[i];
+    const long long blocks = (waves + s.cw - 1) / s.cw * n_kv, round = s.bt * s.kvs;
+    const long long span = win_tokens(min((long long)M, 32LL * s.cw / hpg), max_ctx, window, sinks);
+    const long long all = (span + round - 1) / round, want = max(1LL, min((long long)kWinMaxSplits, 256 / blocks));
+    const long long per = (all + want - 1) / want;
+    s.splits = (int)((all + per - 1) / per);
+    // tokens of a row in the mean: min(p, span) over the positions p of the rows
+    const double lo = max(0, max_ctx - M), hi = max_ctx, w = (double)span;
+    const double mean = w >= hi ? (lo + hi) / 2 : w <= lo ? w : ((w * w - lo * lo) / 2 + w * (hi - w)) / (hi - lo);
+    const double groups = (double)blocks * s.splits;
+    const bool two = i == 1 && groups > 256;
+    const double us = two ? paired[d] : rounds[d][i];
+    double turns = groups / (two ? 512 : 256);
+    if (w < 1.3 * mean) turns = ceil(turns);  // workgroups alike end together
+    const double time = fixed[i] + (s.splits > 1 ? join : 0) +
+                        max(us * per, turns * (us * (mean / round / s.splits + 0.5) + start) - start);
+    if (i == 0 || time < least) {
+      least = time;
+      best = s;
+    }
+  }
+  return best;
 }
 // Whether the kernel of few columns takes a call. Pages of fewer than 16 tokens are left to the other one.
 bool win_few(int M, int n_q, int n_kv, int log2P) { return (long long)M * (n_q / n_kv) <= kFewCols && log2P >= 4; }
-// The tokens that a block of columns can see at most.
-long long win_tokens(int rows, int max_ctx, int window, int sinks) {
-  if (window == 0) return max_ctx;
-  return min((long long)max_ctx, (long long)window + rows + sinks);
-}
-
 }  // namespace
 
-// At most one workgroup per CU, in splits of equal length. (The query does not know the page: where a cache of small pages
-// keeps few columns from their kernel, the other one runs that many splits.)
-int attention_window_splits(int M, int n_q, int n_kv, int D, int max_ctx, int window, int sinks, int cache) {
-  if (win_few(M, n_q, n_kv, 4)) {
-    const long long tiles = (win_tokens(M, max_ctx, window, sinks) + kFewTile - 1) / kFewTile + 2;
-    if (tiles <= 2 * kFewWaves) return 1;
-    const long long want = max(1LL, min((long long)kWinMaxSplits, 256LL / n_kv));
-    const long long per = max((tiles + want - 1) / want, (long long)kFewWaves);
-    return (int)((tiles + per - 1) / per);
-  }
-  const WinShape s = win_shape(M, n_q, n_kv);
-  const long long cols = (long long)M * (n_q / n_kv);
-  const long long blocks = (cols + 32 * s.cw - 1) / (32 * s.cw), round = s.bt * s.kvs;
-  const long long tokens = win_tokens((int)min(cols, 32LL * s.cw) / (n_q / n_kv), max_ctx, window, sinks);
-  const long long rounds = (tokens + round - 1) / round;
-  long long want = 256 / (blocks * n_kv);
-  want = want < 1 ? 1 : want > kWinMaxSplits ? kWinMaxSplits : want;
-  const long long per = (rounds + want - 1) / want;
-  return (int)((rounds + per - 1) / per);
+// (The query does not know the page: where a cache of small pages keeps few columns from their kernel, the other one runs that
+// many splits.)
+int attention_window_splits(int M, int n_q, int n_kv, int D, int max_ctx, int window, int sinks, int) {
+  if (!win_few(M, n_q, n_kv, 4)) return win_shape(M, n_q, n_kv, D, max_ctx, window, sinks).splits;
+  const long long tiles = (win_tokens(M, max_ctx, window, sinks) + kFewTile - 1) / kFewTile + (window > 0);
+  if (tiles <= 2 * kFewWaves) return 1;
+  const long long want = max(1LL, min((long long)kWinMaxSplits, 256LL / n_kv));
+  const long long per = max((tiles + want - 1) / want, (long long)kFewWaves);
+  return (int)((tiles + per - 1) / per);
 }
 size_t attention_window_part_bytes(int M, int n_q, int n_kv, int head_dim) {
   return (size_t)n_kv * (((size_t)M * (n_q / n_kv) + 31) / 32) * 32 * (head_dim + 2) * sizeof(float);
@@ -1036,7 +1063,7 @@ void launch(const WindowAttn& w, hipStream_t st) {
   const long long cols = (long long)w.M << lhpg, waves = (cols + 31) / 32;
   float4* part_o = (float4*)w.ws;
   const WinArgs a{(const f16*)w.q, w.q_stride, w.pos, w.bt, (const uint8_t*)w.kc, (const uint8_t*)w.vc, w.ks, w.vs, w.n_pages,
-                  w.log2P, w.n_kv, lhpg, w.M, (int)min((long long)w.max_ctx, (long long)w.n_bt << w.log2P), w.window, w.sinks,
+                  w.n_bt, w.log2P, w.n_kv, lhpg, w.M, (int)min((long long)w.max_ctx, (long long)w.n_bt << w.log2P), w.window, w.sinks,
                   w.splits, (float)(1.4426950408889634 / sqrt((double)D)), (f16*)w.out, part_o,
                   (float2*)(part_o + (size_t)w.splits * w.n_kv * waves * 8 * D)};
   if (win_few(w.M, w.n_q, w.n_kv, w.log2P)) {
@@ -1048,13 +1075,15 @@ void launch(const WindowAttn& w, hipStream_t st) {
                          lhpg, w.n_kv, w.splits, a.c2, (f16*)w.out);
     return;
   }
-  const WinShape s = win_shape(w.M, w.n_q, w.n_kv);
+  const WinShape s = win_shape(w.M, w.n_q, w.n_kv, D, w.max_ctx, w.window, w.sinks);
   if (s.cw == 2)
     launch_shape<D, CACHE, 2, 4, 32>(a, cols, st);
-  else if (s.cw == 4)
-    launch_shape<D, CACHE, 4, 2, 64>(a, cols, st);
-  else
+  else if (s.cw == 8)
     launch_shape<D, CACHE, 8, 1, 128>(a, cols, st);
+  else if (s.kvs == 1)
+    launch_shape<D, CACHE, 4, 1, 64>(a, cols, st);
+  else
+    launch_shape<D, CACHE, 4, 2, 64>(a, cols, st);
   if (w.splits > 1)
     hipLaunchKernelGGL(attn_window_join_kernel<D>, dim3(w.n_kv, (unsigned)(waves * (D / 8 / kWinJoinRows))),
                        dim3(kWinJoinRows * kWave), 0, st, part_o, a.part_ml, (int)cols, lhpg, w.n_kv, w.splits, a.c2,
