@@ -23,8 +23,10 @@ Knobs (DecodeConfig): weights "int4" | "fp16"; group; quant "rtn" | "clip" | "pr
 from runtime.gptq.calibrate); lm_head "auto" | "fp16" | "int4"; fused (False runs the
 HF-style torch op sequences for norm and SwiGLU on the GPU, the reference's unfused comparison point); max_ctx, page,
 part_size (0 -> attention policy table), attn_version, gemv_stage ((stage, R, warps, pf) forced everywhere, or None for
-the tuning table), autotune_path, attn_policy_path, shuffle_pages, device; fused_attention, fused_gemv and swiglu
-select the MI355X launch fusions (each one is checked against the unfused composition by the GPU tests).
+the tuning table), autotune_path, attn_policy_path, shuffle_pages, device; kv "fp16" | "int8" | "e4m3" (the cache in 8-bit
+codes: half the memory and half of what attention reads); window and sinks (a token attends the last `window` ones and the
+first `sinks`); fused_attention, fused_gemv and swiglu select the MI355X launch fusions (each one is checked against the
+unfused composition by the GPU tests).
 """
 import json
 from dataclasses import dataclass, field
@@ -37,6 +39,7 @@ from .quant import QuantLinear
 from .tree import MAX_NODES, tree_layout
 
 PKG = Path(__file__).resolve().parents[1]
+KV_DTYPES = {"fp16": torch.half, "int8": torch.int8, "e4m3": torch.float8_e4m3fn}
 
 
 @dataclass
@@ -47,6 +50,10 @@ class DecodeConfig:
     qparams: dict = field(default=None, repr=False)  # "layers.{i}.{qkv,o,gu,down}" / "lm_head" -> (q, scale, zero),
                                                      # e.g. runtime.gptq.calibrate
     lm_head: str = "auto"
+    kv: str = "fp16"               # the cache: "fp16", or codes "int8" | "e4m3" with a scale for each 16 tokens and kv head
+                                   # (pages of a multiple of 16 tokens); with codes rope_epilogue and combine_in_o are off
+    window: int = 0                # > 0: a token attends the last `window` tokens, itself among them,
+    sinks: int = 0                 # and the first `sinks` of the sequence
     fused: bool = True
     backend: str = "hip"
     max_ctx: int = 2048
@@ -219,9 +226,17 @@ class Model:
         quant = cfg.weights == "int4"
         if cfg.swiglu not in ("epilogue", "kernel"):
             raise ValueError(f"swiglu {cfg.swiglu!r}: 'epilogue' or 'kernel'")
+        if cfg.kv not in KV_DTYPES:
+            raise ValueError(f"kv {cfg.kv!r}: 'fp16', 'int8' or 'e4m3'")
+        if cfg.window < 0 or cfg.sinks < 0 or (cfg.sinks and not cfg.window):
+            raise ValueError(f"window {cfg.window}, sinks {cfg.sinks}: both >= 0, and sinks belong to a window")
+        self.kv8 = cfg.kv != "fp16"
+        if self.kv8 and cfg.page % ext.KV8_BLOCK:
+            raise ValueError(f"page {cfg.page}: an 8-bit cache takes pages of a multiple of {ext.KV8_BLOCK} tokens")
+        self.window_attention = self.kv8 or cfg.window > 0     # attention by attention_window / attention_kv8
         self.use_fused_gemv = (cfg.fused and cfg.fused_gemv and quant and self.H <= 32768 and self.I <= 32768)
         self.gate_up_epilogue = self.use_fused_gemv and cfg.swiglu == "epilogue"
-        self.rope_epilogue = self.use_fused_gemv and cfg.rope_epilogue
+        self.rope_epilogue = self.use_fused_gemv and cfg.rope_epilogue and not self.kv8
         sd = hf_state
         g = lambda k: sd[k].half()
         self.emb = g("model.embed_tokens.weight").to(dev).contiguous()
@@ -262,9 +277,12 @@ class Model:
             # configurations chosen by the decode step time (runtime.autotune.tune_step), ahead of the isolated tables
             self.step_cfg_override = {k: tuple(v) for k, v in t["best_step"].items()}
 
-        # paged KV cache [L, 2, pages, n_kv, P, D]; one block table shared by all layers (one sequence)
+        # paged KV cache [L, 2, pages, n_kv, P, D]; one block table shared by all layers (one sequence); of codes, their
+        # scales [L, 2, pages, n_kv, P / 16]
         self.n_pages = (cfg.max_ctx + cfg.page - 1) // cfg.page + 1
-        self.kv = torch.zeros(self.L, 2, self.n_pages, self.n_kv, cfg.page, self.D, dtype=torch.half, device=dev)
+        self.kv = torch.zeros(self.L, 2, self.n_pages, self.n_kv, cfg.page, self.D, dtype=KV_DTYPES[cfg.kv], device=dev)
+        self.kv_scale = torch.zeros(*self.kv.shape[:4], cfg.page // ext.KV8_BLOCK, dtype=torch.float32, device=dev) \
+            if self.kv8 else None
         gen = torch.Generator().manual_seed(cfg.seed)
         perm = torch.randperm(self.n_pages, generator=gen) if cfg.shuffle_pages else torch.arange(self.n_pages)
         self.bt = perm.int().to(dev)
@@ -311,12 +329,14 @@ class Model:
         # the o projection merges the split partials itself (one thread per 8 values of x, at most 8 waves) while
         # the partials one of its workgroups reads (every split of all of x) stay small
         self.attn_in_o = (self.cfg.combine_in_o and self.rope_epilogue and self.layers[0]["o"].quant
+                          and not self.window_attention
                           and self.max_splits <= self.COMBINE_MAX_SPLITS and self.n_q * self.D <= 4096
                           and self.max_splits * self.n_q * self.D * 4 <= self.COMBINE_MAX_BYTES)
         dev = self.cfg.device
         self.o_part, self.m_part, self.l_part = (
             torch.empty(*shape, dtype=torch.float32, device=dev)
             for shape in ((self.n_q, self.max_splits, self.D), (self.n_q, self.max_splits), (self.n_q, self.max_splits)))
+        self.attn_ws = self._window_workspace(1, self.ctx_cap) if self.window_attention else None
         self.graph = None
 
     def prepare(self, ctx_cap, use_graph=True, part_size=None, impl=None):
@@ -481,8 +501,47 @@ class Model:
                                    self.sin, self.pos, self.bt, self.kv[li, 0], self.kv[li, 1], self.n_q, self.n_kv,
                                    self.cfg.group)
 
+    def _window_workspace(self, M, max_ctx):
+        need = self.K.attention_window_workspace_bytes(M, self.n_q, self.n_kv, self.D, max_ctx, self.cfg.window,
+                                                       self.cfg.sinks, self.kv.dtype)
+        return torch.empty(need, dtype=torch.uint8, device=self.cfg.device) if need else None
+
+    def append_rows(self, li, qkv):
+        """Rows of qkv [M, ...] from position *pos on: q rotated in place, K and V into layer li's cache."""
+        kc, vc = self.kv[li]
+        if self.kv8:
+            self.K.kv8_append_rows(qkv, self.cos, self.sin, self.pos, self.bt, kc, vc, *self.kv_scale[li], self.n_q, self.n_kv)
+        else:
+            self.K.rope_append_rows(qkv, self.cos, self.sin, self.pos, self.bt, kc, vc, self.n_q, self.n_kv)
+
+    def attend_rows(self, li, q, max_ctx, out, workspace):
+        """Attention of rotated rows q [M, n_q * D] from position *pos on over layer li's cache, under the config's window."""
+        kc, vc = self.kv[li]
+        if self.kv8:
+            self.K.attention_kv8(q, self.pos, self.bt, kc, vc, *self.kv_scale[li], max_ctx, out, self.cfg.window,
+                                 self.cfg.sinks, workspace)
+        else:
+            self.K.attention_window(q, self.pos, self.bt, kc, vc, max_ctx, out, self.cfg.window, self.cfg.sinks, workspace)
+
+    def read_cache(self, li, start, n):
+        """K and V of the tokens [start, start + n) of layer li as fp16 rows [n, n_kv, D], from a cache of any kind."""
+        if not (0 <= start and 0 < n and start + n <= self.cfg.max_ctx):
+            raise ValueError(f"read_cache: tokens [{start}, {start + n}) of a cache of {self.cfg.max_ctx}")
+        if self.kv8:
+            k, v = (torch.empty(n, self.n_kv, self.D, dtype=torch.half, device=self.cfg.device) for _ in "kv")
+            self.K.kv8_read(self.bt, *self.kv[li], *self.kv_scale[li], start, k, v)
+            return k, v
+        t = torch.arange(start, start + n, device=self.cfg.device)
+        rows = self.kv[li][:, self.bt[t // self.cfg.page].long(), :, t % self.cfg.page]     # [n, 2, n_kv, D]
+        return rows[:, 0], rows[:, 1]
+
     def attention(self, li):
         kc, vc = self.kv[li, 0], self.kv[li, 1]
+        if self.window_attention:
+            if not self.rope_epilogue:
+                self.append_rows(li, self.qkv.view(1, -1))
+            self.attend_rows(li, self.qkv[: self.n_q * self.D].view(1, -1), self.ctx_cap, self.attn.view(1, -1), self.attn_ws)
+            return
         if self.rope_epilogue:  # q rotated and k, v appended by the qkv GEMV
             version = 5 if self.attn_impl == 3 else 4     # the policy's kernel, explicitly
             if self.attn_in_o:  # the o projection merges the partials
@@ -741,8 +800,13 @@ class Model:
         B = self._prefill_buffers(M)
         B["tok"].copy_(toks)
 
+        ws = self._window_workspace(M, start + M) if self.window_attention else None
+
         def attend(li, kc, vc):
-            self.K.rope_append_rows(B["qkv"], self.cos, self.sin, self.pos, self.bt, kc, vc, self.n_q, self.n_kv)
+            self.append_rows(li, B["qkv"])
+            if self.window_attention:
+                self.attend_rows(li, B["qkv"][:, : self.n_q * self.D], start + M, B["attn"], ws)
+                return
             self.K.attention_prefill(B["qkv"], self.pos, self.bt, kc, vc, self.n_q, self.n_kv, start + M, B["attn"])
 
         x, xn, delta = self._layers_rows(B, attend)
@@ -767,6 +831,10 @@ class Model:
             self._tree_ws = torch.empty(need, dtype=torch.uint8, device=self.cfg.device)
         return self._tree_logits[:M], self._tree_results[: 4 * M + 1], getattr(self, "_tree_ws", None)
 
+    def _no_tree_cache(self, what):
+        if self.window_attention:
+            raise NotImplementedError(f"{what}: tree attention and the move of accepted rows take an fp16 cache and no window")
+
     def verify(self, draft, parents=None):
         """One step of speculative decoding: the pending token and n drafted ones run through the model in one pass, as
         the nodes of a tree, and the path that greedy decoding takes is kept. draft: n token ids (0 .. 1023 of them),
@@ -776,6 +844,7 @@ class Model:
         Leaves the state of as many steps: their cache rows, the logits of the last one, tok = tokens[-1] and
         pos += len(tokens), up to the summation order of the projections, as prefill does. The cache needs room for all
         n + 1 nodes."""
+        self._no_tree_cache("verify")
         ids = torch.as_tensor(draft, dtype=torch.long).reshape(-1).cpu()
         M = ids.numel() + 1
         if M > 1 and (int(ids.min()) < 0 or int(ids.max()) >= self.V):
@@ -841,6 +910,7 @@ class Model:
         1690 -> 1416, 249 2570 -> 2540; a decode step takes 493). Token, position
         and cache stay as they are: the warm-up runs at a position ahead of the cache, where no row is appended, attended
         or moved. INT4 weights and head only: library products stay out of the recorded pass."""
+        self._no_tree_cache("capture_verify")
         if not (self.lm_head.quant and self.layers[0]["gu"].quant):
             raise NotImplementedError("capture_verify: INT4 weights and LM head only")
         if not 0 <= n < MAX_NODES:
@@ -899,9 +969,13 @@ class Model:
                 "embedding_row": self.emb[0].numel() * self.emb.element_size()}
 
     def kv_bytes_per_token(self, ctx):
-        """K and V bytes of all layers that one token moves: ctx cached rows read, one new row written."""
+        """K and V bytes of all layers that one token moves: the cached rows that it attends read, one new row written. Of a
+        cache of codes, a row has its share of the scales."""
         row = self.kv[0, 0, 0, :, 0].numel() * self.kv.element_size()    # one token's K (or V) of one layer
-        return 2 * row * self.L * (ctx + 1)
+        if self.kv8:
+            row += self.n_kv * 4 // ext.KV8_BLOCK
+        seen = min(ctx, self.cfg.window + self.cfg.sinks) if self.cfg.window else ctx
+        return 2 * row * self.L * (seen + 1)
 
     def activation_bytes(self):
         """fp16 activation vectors read/written per token (bench/analyze.py:40 of the reference)."""
