@@ -315,6 +315,40 @@ def test_attention_caps_and_holes(K, dtype, D, M, cap):
     check(K, q, -(1 << 31), bt, caches, scales, vals, cap, 3, 4, ws=("full",))
 
 
+@pytest.mark.parametrize("dtype", CACHES, ids=name)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("M,pos,cap,window,sinks,hpg,n_kv", [
+    (60, 440, 500, 0, 0, 4, 2), (700, 0, 700, 100, 20, 1, 16), (40, 700, 1 << 20, 0, 0, 4, 2), (800, 0, 800, 0, 0, 8, 8),
+    (1500, 0, 1500, 30, 4, 8, 8), (1200, 0, 1200, 200, 70, 1, 32), (130, 900, 60000, 0, 0, 8, 8), (300, 500, 20000, 400, 4, 4, 2)])
+def test_attention_every_workgroup_shape(K, dtype, D, M, pos, cap, window, sinks, hpg, n_kv):
+    """The sizes choose among the shapes of a workgroup, split and not: rows spread over all of them, heads of the first and
+    the last kv head, with a page that is not mapped and (fp16, e4m3) a NaN in V of a token that some of the rows attend."""
+    page, n_q = 16, hpg * n_kv
+    caches, scales, bt, vals = paged_kv(pos + M, n_kv, D, page, dtype, gen(M + D))
+    q = torch.randn(M, n_q, D, generator=gen(7)).half()
+    bt[(pos + M // 3) // page] = -1
+    bad = pos + M // 2 + 30
+    if dtype != torch.int8:
+        c = R.token_row(bt.tolist(), bad, page, caches[0].size(0))
+        for v in (caches, vals):
+            v[1][c[0], :, c[1], 9] = float("nan")
+    a = dev(q, bt, *caches, *scales)
+    half = M // 2
+    rows = sorted({0, 1, M // 3 - 1, M // 3, half, half + 29, half + 30, half + 31, M - 1, *range(5, M, max(1, M // 16))})
+    for ws in ("full", "none"):
+        out = run(K, a[0], i32(pos), a[1], a[2:4], a[4:6], cap, window, sinks, ws).view(M, n_q, D)
+        for h in (0, n_kv - 1):
+            heads = slice(h * hpg, (h + 1) * hpg)
+            for m in (r for r in rows if r < M):
+                sees = dtype != torch.int8 and pos + m >= bad and (not window or bad > pos + m - window)
+                of = [v[:, h:h + 1] for v in vals]
+                want, bound = R.attention(q[m:m + 1, heads], pos + m, bt, *of, cap, window, sinks)
+                if sees:
+                    assert bool(torch.isnan(out[m, heads, 9]).all()) and bool(torch.isfinite(out[m, heads, :9]).all())
+                else:
+                    R.within(out[m:m + 1, heads].reshape(1, -1), want, bound)
+
+
 @pytest.mark.parametrize("dtype", [torch.half, torch.float8_e4m3fn], ids=name)
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("M,pos,window,sinks,cap", [

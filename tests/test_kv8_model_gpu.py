@@ -125,7 +125,7 @@ def test_window_wider_than_the_sequence_changes_only_the_kernel():
 
 
 def test_a_window_forgets():
-    """Two prompts that differ in a token that no window on the way to the last row holds: its logits are the same to the bit."""
+    """Two prompts that differ in a token that no window on the way to the last row holds: the same logits to the bit."""
     m = model(kv="e4m3", window=8, sinks=2)
     out = []
     for edit in (3, 700):
