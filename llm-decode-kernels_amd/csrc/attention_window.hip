@@ -32,13 +32,16 @@ struct WinArgs {
   float2* part_ml;  // [splits][n_kv][column waves][32]: reference maximum, sum
 };
 
-// The tokens of one row: [lo, lim] and [0, sinks).
+// The tokens of one row: [lo, lim] and [0, sinks). (The position of a row that exists fits 32 bits without a sign.)
 struct Sight {
   int lim, lo;
 };
-__device__ __forceinline__ Sight sight_of(long long pos, int m, int window, int cap) {
-  const long long p = pos + m;
-  return {(int)max(-1LL, min(p, (long long)cap - 1)), window > 0 ? (int)min(max(0LL, p - window + 1), (long long)cap) : 0};
+__device__ __forceinline__ Sight sight_of(int pos, int m, int window, int cap) {
+  const uint32_t p = (uint32_t)pos + (uint32_t)m;
+  const bool none = pos < 0 && (int)p < 0;
+  const int lim = none ? -1 : (int)min(p, (uint32_t)cap - 1);
+  const int lo = none || window == 0 || p < (uint32_t)window ? 0 : (int)min(p + 1 - (uint32_t)window, (uint32_t)cap);
+  return {lim, lo};
 }
 
 // 16 bytes with a half that is no finite number.
@@ -84,7 +87,7 @@ __global__ void __launch_bounds__(CW * KVS * kWave, 2) attn_window_kernel(const 
   const int grp = wave / CW, gw = wave % CW;  // group, and the wave's columns within it
   const int r = lane & 31, h = lane >> 5;
   const int P = 1 << a.log2P;
-  const long long pos = *a.pos;
+  const int pos = *a.pos;
   const int n_q = a.n_kv << a.lhpg, cols = a.M << a.lhpg;
   // this lane's column: row m, head hd; columns past the last repeat it
   const int col = (cb * CW + gw) * 32 + r;
@@ -612,8 +615,8 @@ attn_window_join_kernel(const float4* __restrict__ part_o, const float2* __restr
 //     lane group g is token 16 s + 4 g + v). For A lane (g, r) loads dims [r D / 16, (r + 1) D / 16) of those 8 tokens' rows
 //     and transposes them in registers; output tile t holds dim r D / 16 + t, so that lane (g, c) ends with D / 4 dims in a
 //     row of column c.
-constexpr int kFewWaves = 8;
 constexpr int kFewCols = 16;
+constexpr long long kFewUnsplit = 16, kFewLong = 4096, kFewGroups = 256;
 constexpr int kFewTile = 32;
 
 template <int D, int CACHE>
@@ -625,31 +628,31 @@ struct FewShape {
   static constexpr int VW = DPL * ES / 4;       // their words
 };
 
-template <int D, int CACHE>
-__global__ void __launch_bounds__(kFewWaves * kWave)
+template <int D, int CACHE, int NW>
+__global__ void __launch_bounds__(NW * kWave, 2)
 attn_few_kernel(const WinArgs a) {
   using S = FewShape<D, CACHE>;
   constexpr bool F16 = S::F16;
-  constexpr int NW = kFewWaves, ES = S::ES, KW = S::KW, DPL = S::DPL, VW = S::VW, KS = D / 32;
+  constexpr int ES = S::ES, KW = S::KW, DPL = S::DPL, VW = S::VW, KS = D / 32;
   __shared__ float s_m[NW][kFewCols], s_l[NW][kFewCols];
   __shared__ __align__(16) float s_o[NW][kFewCols][D];
   const int kvh = blockIdx.x, split = blockIdx.y;
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int P = 1 << a.log2P;
-  const long long pos = *a.pos;
+  const int i0 = split * NW + wave, step = a.splits * NW;  // the wave's tiles: i0 and every step-th from there
+  // pages of tile i0 as they are without a window, beside the position
+  struct Pages {
+    int p[2];
+  };
+  auto pages_at = [&](int t) __attribute__((always_inline)) {
+    return Pages{{a.bt[min(t >> a.log2P, a.n_bt - 1)], a.bt[min((t + 16) >> a.log2P, a.n_bt - 1)]}};
+  };
+  const int pos = *a.pos;
+  Pages pg = pages_at(kFewTile * i0);
   const int n_q = a.n_kv << a.lhpg, cols = a.M << a.lhpg;
   const int cc = min(c, cols - 1);              // columns past the last repeat it
   const int m = cc >> a.lhpg, hd = (kvh << a.lhpg) + (cc & ((1 << a.lhpg) - 1));
-  const Sight mine = sight_of(pos, m, a.window, a.cap);
-  const Sight s0 = sight_of(pos, 0, a.window, a.cap), s1 = sight_of(pos, a.M - 1, a.window, a.cap);
-  const int ctx = s1.lim + 1;                   // tokens [0, ctx) are read
-  // tiles: those of the sinks, then those of the window, nt in all; this wave's are i0 and every step-th from there
-  const int all = (ctx + kFewTile - 1) / kFewTile, wt = min(s0.lo / kFewTile, all);
-  const int ns = a.window > 0 ? min((min(a.sinks, ctx) + kFewTile - 1) / kFewTile, wt) : 0;
-  const int nt = ns + all - wt, i0 = split * NW + wave, step = a.splits * NW;
-  auto tile_at = [&](int i) __attribute__((always_inline)) { return kFewTile * (i < ns ? i : i + (wt - ns)); };
-
   h8 q[KS];
   {
     const f16* qh = a.q + (size_t)m * a.q_stride + (size_t)hd * D;
@@ -658,6 +661,16 @@ attn_few_kernel(const WinArgs a) {
       q[k] = __builtin_bit_cast(
           h8, *reinterpret_cast<const u32x4*>(qh + (F16 ? 32 * k + 8 * g : 64 * (k >> 1) + 16 * g + 8 * (k & 1))));
   }
+  __builtin_amdgcn_sched_barrier(0);            // (those loads go out before the position is waited for)
+  const Sight mine = sight_of(pos, m, a.window, a.cap);
+  const Sight s0 = sight_of(pos, 0, a.window, a.cap), s1 = sight_of(pos, a.M - 1, a.window, a.cap);
+  const int ctx = s1.lim + 1;                   // tokens [0, ctx) are read
+  // tiles: those of the sinks, then those of the window, nt in all
+  const int all = (ctx + kFewTile - 1) / kFewTile, wt = min(s0.lo / kFewTile, all);
+  const int ns = a.window > 0 ? min((min(a.sinks, ctx) + kFewTile - 1) / kFewTile, wt) : 0;
+  const int nt = ns + all - wt;
+  auto tile_at = [&](int i) __attribute__((always_inline)) { return kFewTile * (i < ns ? i : i + (wt - ns)); };
+
   typedef uint32_t vrow __attribute__((ext_vector_type(VW)));
   struct Tile {
     int t0;
@@ -666,15 +679,7 @@ attn_few_kernel(const WinArgs a) {
     float ks[2], vs[2];
     bool ok[2];       // the page is mapped; uniform
   };
-  struct Pages {
-    int p[2];
-  };
-  auto lookup = [&](int i) __attribute__((always_inline)) {
-    Pages w;
-#pragma unroll
-    for (int s = 0; s < 2; ++s) w.p[s] = a.bt[min((tile_at(i) + 16 * s) >> a.log2P, a.n_bt - 1)];
-    return w;
-  };
+  auto lookup = [&](int i) __attribute__((always_inline)) { return pages_at(tile_at(i)); };
   auto load = [&](int i, const Pages& w) __attribute__((always_inline)) {
     Tile x;
     x.t0 = tile_at(i);
@@ -686,10 +691,9 @@ attn_few_kernel(const WinArgs a) {
       const uint8_t* kr = a.kc + row * (D * ES) + c * (D * ES) + 16 * g;
       const uint8_t* vr = a.vc + row * (D * ES) + 4 * g * (D * ES) + c * (DPL * ES);
 #pragma unroll
-      for (int j = 0; j < KW; ++j) x.k[s][j] = load_stream(reinterpret_cast<const u32x4*>(kr + 64 * j));
+      for (int j = 0; j < KW; ++j) x.k[s][j] = *reinterpret_cast<const u32x4*>(kr + 64 * j);
 #pragma unroll
-      for (int v = 0; v < 4; ++v)
-        x.v[s][v] = __builtin_nontemporal_load(reinterpret_cast<const vrow*>(vr + v * (D * ES)));
+      for (int v = 0; v < 4; ++v) x.v[s][v] = *reinterpret_cast<const vrow*>(vr + v * (D * ES));
       if constexpr (!F16) {
         x.ks[s] = a.ks[row >> 4];
         x.vs[s] = a.vs[row >> 4];
@@ -865,18 +869,18 @@ attn_few_kernel(const WinArgs a) {
     }
   };
 
-  Pages pg = lookup(i0);
   if (i0 < nt) {  // uniform per wave
+    if (a.window > 0) pg = lookup(i0);
+    // the next tile's loads go out ahead of a tile's products; behind the last one every wave's are of tile 0, from a cache
+    auto live = [&](int i) __attribute__((always_inline)) { return i < nt ? i : 0; };
     Tile x = load(i0, pg);
-    pg = lookup(i0 + step);
-    for (int i = i0; i < nt; i += 2 * step) {
-      Tile y = load(i + step, pg);  // past the end: rows that are never computed on
-      pg = lookup(i + 2 * step);
+    pg = lookup(live(i0 + step));
+#pragma unroll 1
+    for (int i = i0; i < nt; i += step) {
+      const Tile y = load(live(i + step), pg);
+      pg = lookup(live(i + 2 * step));
       compute(x);
-      if (i + step >= nt) break;
-      x = load(i + 2 * step, pg);
-      pg = lookup(i + 3 * step);
-      compute(y);
+      x = y;
     }
   }
   l = rows_sum(l);
@@ -1029,17 +1033,26 @@ WinShape win_shape(int M, int n_q, int n_kv, int D, int max_ctx, int window, int
 }
 // Whether the kernel of few columns takes a call. Pages of fewer than 16 tokens are left to the other one.
 bool win_few(int M, int n_q, int n_kv, int log2P) { return (long long)M * (n_q / n_kv) <= kFewCols && log2P >= 4; }
+// Waves of a workgroup and splits of a call of few columns.
+struct FewPlan {
+  int waves, splits;
+};
+FewPlan few_plan(int M, int n_kv, int max_ctx, int window, int sinks) {
+  const long long tiles = (win_tokens(M, max_ctx, window, sinks) + kFewTile - 1) / kFewTile;
+  if (tiles <= kFewUnsplit) return {8, 1};
+  const int waves = tiles * n_kv < kFewLong ? 4 : 8;
+  const long long want = max(1LL, min((long long)kWinMaxSplits, kFewGroups / n_kv));
+  const long long per = max((tiles + want - 1) / want, (long long)waves);
+  return {waves, (int)((tiles + per - 1) / per)};
+}
+
 }  // namespace
 
 // (The query does not know the page: where a cache of small pages keeps few columns from their kernel, the other one runs that
 // many splits.)
 int attention_window_splits(int M, int n_q, int n_kv, int D, int max_ctx, int window, int sinks, int) {
-  if (!win_few(M, n_q, n_kv, 4)) return win_shape(M, n_q, n_kv, D, max_ctx, window, sinks).splits;
-  const long long tiles = (win_tokens(M, max_ctx, window, sinks) + kFewTile - 1) / kFewTile + (window > 0);
-  if (tiles <= 2 * kFewWaves) return 1;
-  const long long want = max(1LL, min((long long)kWinMaxSplits, 256LL / n_kv));
-  const long long per = max((tiles + want - 1) / want, (long long)kFewWaves);
-  return (int)((tiles + per - 1) / per);
+  return win_few(M, n_q, n_kv, 4) ? few_plan(M, n_kv, max_ctx, window, sinks).splits
+                                  : win_shape(M, n_q, n_kv, D, max_ctx, window, sinks).splits;
 }
 size_t attention_window_part_bytes(int M, int n_q, int n_kv, int head_dim) {
   return (size_t)n_kv * (((size_t)M * (n_q / n_kv) + 31) / 32) * 32 * (head_dim + 2) * sizeof(float);
@@ -1069,7 +1082,10 @@ void launch(const WindowAttn& w, hipStream_t st) {
   if (win_few(w.M, w.n_q, w.n_kv, w.log2P)) {
     WinArgs f = a;
     f.part_ml = (float2*)(part_o + (size_t)w.splits * w.n_kv * kFewCols * (D / 4));
-    hipLaunchKernelGGL((attn_few_kernel<D, CACHE>), dim3(w.n_kv, w.splits), dim3(kFewWaves * kWave), 0, st, f);
+    if (few_plan(w.M, w.n_kv, w.max_ctx, w.window, w.sinks).waves == 4)
+      hipLaunchKernelGGL((attn_few_kernel<D, CACHE, 4>), dim3(w.n_kv, w.splits), dim3(4 * kWave), 0, st, f);
+    else
+      hipLaunchKernelGGL((attn_few_kernel<D, CACHE, 8>), dim3(w.n_kv, w.splits), dim3(8 * kWave), 0, st, f);
     if (w.splits > 1)
       hipLaunchKernelGGL(attn_few_join_kernel<D>, dim3(w.n_kv, (unsigned)cols), dim3(256), 0, st, (const f4*)part_o, f.part_ml,
                          lhpg, w.n_kv, w.splits, a.c2, (f16*)w.out);
