@@ -619,6 +619,18 @@ constexpr int kFewCols = 16;
 constexpr long long kFewUnsplit = 16, kFewLong = 4096, kFewGroups = 256;
 constexpr int kFewTile = 32;
 
+// Over the lanes c, c + 16, c + 32, c + 48 of a wave, by swapping rows and halves of two registers (LDS is not touched).
+template <class F>
+__device__ __forceinline__ float over_rows(float v, F f) {
+  const uint32_t u = __float_as_uint(v);
+  const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const uint32_t a0 = a[0], a1 = a[1];
+  const uint32_t w = __float_as_uint(f(__uint_as_float(a0), __uint_as_float(a1)));
+  const auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+  const uint32_t b0 = b[0], b1 = b[1];
+  return f(__uint_as_float(b0), __uint_as_float(b1));
+}
+
 template <int D, int CACHE>
 struct FewShape {
   static constexpr bool F16 = CACHE == kCacheF16;
@@ -731,7 +743,7 @@ attn_few_kernel(const WinArgs a) {
     }
     return x;
   };
-  auto compute = [&](Tile& x) __attribute__((always_inline)) {
+  auto compute = [&](Tile& x, bool first) __attribute__((always_inline)) {
     const int t0 = x.t0;
     // every column sees every token; uniform per wave
     const bool plain = x.ok[0] && x.ok[1] && t0 + kFewTile - 1 <= s0.lim && (t0 >= s1.lo || t0 + kFewTile <= a.sinks);
@@ -753,15 +765,19 @@ attn_few_kernel(const WinArgs a) {
     }
     if (!plain) {
       asm volatile("");  // stays a branch
+      auto low = [](int n) __attribute__((always_inline)) -> uint32_t { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; };
+      // tokens of the tile that exist (uniform), and those that the column sees, from this lane's first one on
+      const uint32_t there = low(ctx - t0) & ((x.ok[0] ? 0xFFFFu : 0u) | (x.ok[1] ? 0xFFFF0000u : 0u));
+      const uint32_t seen = (there & low(mine.lim + 1 - t0) & (~low(mine.lo - t0) | low(a.sinks - t0))) >> (4 * g);
+      const uint32_t real = there >> (4 * g);
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
-          const int t = t0 + 16 * s + 4 * g + v;
-          if (!(x.ok[s] && t <= mine.lim && (t >= mine.lo || t < a.sinks))) sc[s][v] = -INFINITY;
-          if (!(x.ok[s] && t < ctx)) x.v[s][v] = vrow(0u);  // (a token that does not exist: its V must not meet a p of 0)
+          if (!(seen & (1u << (16 * s + v)))) sc[s][v] = -INFINITY;
+          if (!(real & (1u << (16 * s + v)))) x.v[s][v] = vrow(0u);  // (its V must not meet a p of 0)
         }
-        if constexpr (!F16) x.vs[s] = x.ok[s] && t0 + 16 * s < ctx ? x.vs[s] : 1.f;
+        if constexpr (!F16) x.vs[s] = there & (1u << (16 * s)) ? x.vs[s] : 1.f;
       }
     }
     float p[2][4];
@@ -777,7 +793,8 @@ attn_few_kernel(const WinArgs a) {
       }
       return sum;
     };
-    float sum = weigh(0.f, lift);
+    float sum = INFINITY;            // (the first tile brings the reference)
+    if (!first) sum = weigh(0.f, lift);
     if (__any(!(sum <= kWinMost))) {  // the reference moves to this tile's maximum where that is higher
       asm volatile("");
       float mx = sc[0][0];
@@ -786,11 +803,9 @@ attn_few_kernel(const WinArgs a) {
 #pragma unroll
         for (int v = 0; v < 4; ++v) mx = fmaxf(mx, sc[s][v]);
       }
-      mx = fmaxf(ref, rows_max(mx));
-      int over = !(sum <= kWinMost);  // in any of the column's four lanes
-      over |= __shfl_xor(over, 16, kWave);
-      over |= __shfl_xor(over, 32, kWave);
-      mx = over ? mx : ref;
+      const auto larger = [](float x, float y) { return fmaxf(x, y); };
+      mx = fmaxf(ref, over_rows(mx, larger));
+      mx = over_rows(sum <= kWinMost ? 0.f : 1.f, larger) != 0.f ? mx : ref;  // in any of the column's four lanes
       const float alpha = __builtin_amdgcn_exp2f((ref - mx) * a.c2);  // 1 for a column that stays
       if (mx != ref) lift = fabsf(mx * a.c2) > kWinFar ? INFINITY : kWinLift - mx * a.c2;
       ref = mx;
@@ -827,9 +842,28 @@ attn_few_kernel(const WinArgs a) {
     bool dirty = false;  // NaN or infinity in V of a tile that not every column sees whole; uniform
     if (!plain) {
       asm volatile("");
+      // a look at the words first: fp16 with all exponent bits, e4m3's NaN, a scale that takes a code past fp16
+      uint32_t odd = 0;
 #pragma unroll
-      for (int t = 0; t < DPL; ++t) dirty = dirty || has_nonfinite(operand(x, tr, t));
-      dirty = __any(dirty);
+      for (int s = 0; s < 2; ++s) {
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+#pragma unroll
+          for (int w = 0; w < VW; ++w) {
+            if constexpr (F16)
+              odd |= ((x.v[s][v][w] & 0x7C007C00u) + 0x04000400u) & 0x80008000u;
+            else if constexpr (CACHE == kCacheE4m3)
+              odd |= ((x.v[s][v][w] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+          }
+        }
+        if constexpr (!F16) odd |= x.vs[s] <= (CACHE == kCacheInt8 ? 512.f : 128.f) ? 0u : 1u;
+      }
+      if (__any(odd != 0)) {
+        asm volatile("");
+#pragma unroll
+        for (int t = 0; t < DPL; ++t) dirty = dirty || has_nonfinite(operand(x, tr, t));
+        dirty = __any(dirty);
+      }
     }
     if (!dirty) {
 #pragma unroll
@@ -879,11 +913,11 @@ attn_few_kernel(const WinArgs a) {
     for (int i = i0; i < nt; i += step) {
       const Tile y = load(live(i + step), pg);
       pg = lookup(live(i + 2 * step));
-      compute(x);
+      compute(x, i == i0);
       x = y;
     }
   }
-  l = rows_sum(l);
+  l = over_rows(l, [](float x, float y) { return x + y; });
   // ---- the waves meet in LDS, in order: column c's dims [D / 4 g, + D / 4), acc[t][v] dim D / 4 g + DPL v + t
   if (g == 0) {
     s_m[wave][c] = ref;
