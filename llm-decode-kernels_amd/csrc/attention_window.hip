@@ -616,7 +616,6 @@ attn_window_join_kernel(const float4* __restrict__ part_o, const float2* __restr
 //     and transposes them in registers; output tile t holds dim r D / 16 + t, so that lane (g, c) ends with D / 4 dims in a
 //     row of column c.
 constexpr int kFewCols = 16;
-constexpr long long kFewUnsplit = 16, kFewLong = 4096, kFewGroups = 256;
 constexpr int kFewTile = 32;
 
 // Over the lanes c, c + 16, c + 32, c + 48 of a wave, by swapping rows and halves of two registers (LDS is not touched).
@@ -1067,15 +1066,21 @@ WinShape win_shape(int M, int n_q, int n_kv, int D, int max_ctx, int window, int
 }
 // Whether the kernel of few columns takes a call. Pages of fewer than 16 tokens are left to the other one.
 bool win_few(int M, int n_q, int n_kv, int log2P) { return (long long)M * (n_q / n_kv) <= kFewCols && log2P >= 4; }
-// Waves of a workgroup and splits of a call of few columns.
+// Waves of a workgroup and splits of a call of few columns. A context that eight waves get through in two tiles each (D 128)
+// or four (D 64) is not split: one launch instead of two. From there to 4096 tiles over all kv heads workgroups of four waves,
+// so that one tile per wave reaches twice the CUs; then of eight. At most one workgroup per CU, none with less than a tile per
+// wave. Captured, in us, one token, e4m3:
+//   8 x 4 heads of 128   300 tokens unsplit 6.9, split 7.7 | 600: 8.5, 7.6 | 4096: waves 4 8.2, 8 10.5 | 32768: 18.8, eight
+//                        in 512 workgroups 23.2, four in 256 18.4
+//   4 x 8 heads of 64    600 tokens unsplit 5.4, split 6.9 | 900: 6.8, 6.8 | 16384: waves 4 7.8, 8 8.4 | 32768: 9.4, 8.9
 struct FewPlan {
   int waves, splits;
 };
-FewPlan few_plan(int M, int n_kv, int max_ctx, int window, int sinks) {
+FewPlan few_plan(int M, int n_kv, int D, int max_ctx, int window, int sinks) {
   const long long tiles = (win_tokens(M, max_ctx, window, sinks) + kFewTile - 1) / kFewTile;
-  if (tiles <= kFewUnsplit) return {8, 1};
-  const int waves = tiles * n_kv < kFewLong ? 4 : 8;
-  const long long want = max(1LL, min((long long)kWinMaxSplits, kFewGroups / n_kv));
+  if (tiles <= (D == 128 ? 16 : 32)) return {8, 1};
+  const int waves = tiles * n_kv < 4096 ? 4 : 8;
+  const long long want = max(1LL, min((long long)kWinMaxSplits, 256LL / n_kv));
   const long long per = max((tiles + want - 1) / want, (long long)waves);
   return {waves, (int)((tiles + per - 1) / per)};
 }
@@ -1085,7 +1090,7 @@ FewPlan few_plan(int M, int n_kv, int max_ctx, int window, int sinks) {
 // (The query does not know the page: where a cache of small pages keeps few columns from their kernel, the other one runs that
 // many splits.)
 int attention_window_splits(int M, int n_q, int n_kv, int D, int max_ctx, int window, int sinks, int) {
-  return win_few(M, n_q, n_kv, 4) ? few_plan(M, n_kv, max_ctx, window, sinks).splits
+  return win_few(M, n_q, n_kv, 4) ? few_plan(M, n_kv, D, max_ctx, window, sinks).splits
                                   : win_shape(M, n_q, n_kv, D, max_ctx, window, sinks).splits;
 }
 size_t attention_window_part_bytes(int M, int n_q, int n_kv, int head_dim) {
@@ -1116,7 +1121,7 @@ void launch(const WindowAttn& w, hipStream_t st) {
   if (win_few(w.M, w.n_q, w.n_kv, w.log2P)) {
     WinArgs f = a;
     f.part_ml = (float2*)(part_o + (size_t)w.splits * w.n_kv * kFewCols * (D / 4));
-    if (few_plan(w.M, w.n_kv, w.max_ctx, w.window, w.sinks).waves == 4)
+    if (few_plan(w.M, w.n_kv, D, w.max_ctx, w.window, w.sinks).waves == 4)
       hipLaunchKernelGGL((attn_few_kernel<D, CACHE, 4>), dim3(w.n_kv, w.splits), dim3(4 * kWave), 0, st, f);
     else
       hipLaunchKernelGGL((attn_few_kernel<D, CACHE, 8>), dim3(w.n_kv, w.splits), dim3(8 * kWave), 0, st, f);
