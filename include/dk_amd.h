@@ -418,8 +418,9 @@ int dk_tree_accept(const int64_t* tokens, const int32_t* parents, const int64_t*
 
 /*
  * The 8-bit KV cache. kc, vc hold codes [n_pages, n_kv, page, head_dim], one byte each (page a power of two >= 16), ks, vs
- * fp32 scales [n_pages, n_kv, page / 16], one for each block of 16 tokens and kv head: a value is code * scale. `cache` names
- * the codes: DK_CACHE_INT8 (-127 .. 127) or DK_CACHE_E4M3 (the format with 448 as its largest value and no infinities).
+ * fp32 scales [n_pages, n_kv, page / 16], one for each block of 16 tokens and kv head: a value is code * scale, and a scale is a
+ * power of two, 2^-24 .. 2^10 (readers may take no more of it than its exponent). `cache` names the codes: DK_CACHE_INT8
+ * (-127 .. 127) or DK_CACHE_E4M3 (the format with 448 as its largest value and no infinities).
  *
  * dk_kv8_append_rows: rope_append_rows into that cache. Row m of qkv [M, (n_q + 2 n_kv) head_dim] is token T = *pos + m and
  * rotates at T as dk_rope_append_rows rotates it (cos_t, sin_t [max_pos, head_dim / 2]; both NULL: no rotation, and max_pos
@@ -433,11 +434,12 @@ int dk_tree_accept(const int64_t* tokens, const int32_t* parents, const int64_t*
  *   An infinity is stored as the largest fp16 value; NaN stays NaN in e4m3 and becomes 0 in int8.
  * So an e4m3 value is within 2^-4 of x relative (2^-10 s below 2^-6 s), an int8 one within s / 2, after its block's scale has
  * grown to s within s. A row whose T is outside [0, max_pos) touches nothing; a T without a mapped page is rotated but not
- * appended. qkv, q_out, kc, vc and the tables 16-byte aligned, q_stride % 8 == 0, M 1..2^20.
+ * appended. A page that the call appends to is listed once in the block table. qkv, q_out, kc, vc and the tables 16-byte
+ * aligned, q_stride % 8 == 0, M 1..2^20.
  *
  * dk_kv8_read: tokens [start, start + n) as fp16 rows k_out, v_out [n, n_kv, head_dim]; tokens without a mapped page read as
- * zeros. The scales that dk_kv8_append_rows writes make every value an fp16 number, so nothing is rounded; products of other
- * scales are rounded, and infinite past 65504. start + n <= 2^30; k_out, v_out, kc and vc 16-byte aligned. No counterparts in
+ * zeros. Every value that dk_kv8_append_rows stores is an fp16 number, so nothing is rounded; of other codes and scales, products
+ * below 2^-14 may be, and those past 65504 are infinite. start + n <= 2^30; k_out, v_out, kc and vc 16-byte aligned. No counterparts in
  * the reference (its cache is fp16, runtime/model.py:117-120).
  */
 enum dk_cache { DK_CACHE_F16 = 0, DK_CACHE_INT8 = 1, DK_CACHE_E4M3 = 2 };

@@ -639,7 +639,7 @@ struct FewShape {
   static constexpr int VW = DPL * ES / 4;       // their words
 };
 
-template <int D, int CACHE, int NW>
+template <int D, int CACHE, int NW, bool NT>
 __global__ void __launch_bounds__(NW * kWave, 2)
 attn_few_kernel(const WinArgs a) {
   using S = FewShape<D, CACHE>;
@@ -702,9 +702,15 @@ attn_few_kernel(const WinArgs a) {
       const uint8_t* kr = a.kc + row * (D * ES) + c * (D * ES) + 16 * g;
       const uint8_t* vr = a.vc + row * (D * ES) + 4 * g * (D * ES) + c * (DPL * ES);
 #pragma unroll
-      for (int j = 0; j < KW; ++j) x.k[s][j] = *reinterpret_cast<const u32x4*>(kr + 64 * j);
+      for (int j = 0; j < KW; ++j) {
+        const u32x4* p = reinterpret_cast<const u32x4*>(kr + 64 * j);
+        x.k[s][j] = NT ? load_stream(p) : *p;
+      }
 #pragma unroll
-      for (int v = 0; v < 4; ++v) x.v[s][v] = *reinterpret_cast<const vrow*>(vr + v * (D * ES));
+      for (int v = 0; v < 4; ++v) {
+        const vrow* p = reinterpret_cast<const vrow*>(vr + v * (D * ES));
+        x.v[s][v] = NT ? __builtin_nontemporal_load(p) : *p;
+      }
       if constexpr (!F16) {
         x.ks[s] = a.ks[row >> 4];
         x.vs[s] = a.vs[row >> 4];
@@ -1121,10 +1127,16 @@ void launch(const WindowAttn& w, hipStream_t st) {
   if (win_few(w.M, w.n_q, w.n_kv, w.log2P)) {
     WinArgs f = a;
     f.part_ml = (float2*)(part_o + (size_t)w.splits * w.n_kv * kFewCols * (D / 4));
-    if (few_plan(w.M, w.n_kv, D, w.max_ctx, w.window, w.sinks).waves == 4)
-      hipLaunchKernelGGL((attn_few_kernel<D, CACHE, 4>), dim3(w.n_kv, w.splits), dim3(4 * kWave), 0, st, f);
+    const FewPlan p = few_plan(w.M, w.n_kv, D, w.max_ctx, w.window, w.sinks);
+    // K and V that fill half of the last cache (256 MB) are not kept there for the next call. (8 x 4 heads of 128: one token at
+    // 131072, int8, cold 55.1 -> 51.2 us; at 16384, e4m3, from the cache 12.1, past it 14.0)
+    const long long bytes = win_tokens(w.M, w.max_ctx, w.window, w.sinks) * w.n_kv * 2 * D * (CACHE == kCacheF16 ? 2 : 1);
+    if (p.waves == 4)
+      hipLaunchKernelGGL((attn_few_kernel<D, CACHE, 4, false>), dim3(w.n_kv, w.splits), dim3(4 * kWave), 0, st, f);
+    else if (bytes < (128LL << 20))
+      hipLaunchKernelGGL((attn_few_kernel<D, CACHE, 8, false>), dim3(w.n_kv, w.splits), dim3(8 * kWave), 0, st, f);
     else
-      hipLaunchKernelGGL((attn_few_kernel<D, CACHE, 8>), dim3(w.n_kv, w.splits), dim3(8 * kWave), 0, st, f);
+      hipLaunchKernelGGL((attn_few_kernel<D, CACHE, 8, true>), dim3(w.n_kv, w.splits), dim3(8 * kWave), 0, st, f);
     if (w.splits > 1)
       hipLaunchKernelGGL(attn_few_join_kernel<D>, dim3(w.n_kv, (unsigned)cols), dim3(256), 0, st, (const f4*)part_o, f.part_ml,
                          lhpg, w.n_kv, w.splits, a.c2, (f16*)w.out);

@@ -824,8 +824,8 @@ class DecodeKernels:
     # rows of a prompt, or one token, rotated and appended to a cache of 8-bit codes
     def kv8_append_rows(self, qkv, cos_t, sin_t, pos, bt, kc, vc, ks, vs, n_q, n_kv, q_out=None):
         """rope_append_rows into an 8-bit cache: row m of qkv [M, (n_q + 2 n_kv) * D] is token *pos + m. kc, vc int8 or
-        float8_e4m3fn [pages, n_kv, P, D], ks, vs fp32 [pages, n_kv, P / 16]: a value is code * scale, one power-of-two
-        scale for 16 tokens. The rotated q goes to q_out [M, n_q * D] (rows may be strided; None: in place in qkv). cos_t
+        float8_e4m3fn [pages, n_kv, P, D], ks, vs fp32 [pages, n_kv, P / 16]: a value is code * scale, one scale for 16
+        tokens, a power of two. The rotated q goes to q_out [M, n_q * D] (rows may be strided; None: in place in qkv). cos_t
         and sin_t None: no rotation. Rows behind the new ones in a block count as absent."""
         what, dev = "kv8_append_rows", qkv.get_device()
         dtype, cache = self._kv8_cache(what, kc, vc, ks, vs)

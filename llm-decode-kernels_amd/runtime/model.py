@@ -648,6 +648,9 @@ class Model:
         position could exceed; the K/V the warm-up writes sit at positions every real step overwrites before reading),
         then one step is recorded. Token and position are left as they were."""
         with self._keep_state():
+            # in a cache of codes the block of the warm-up's rows takes their scale: its page is put back
+            page = int(self.bt[0]) if self.kv8 else 0
+            kept = [t[:, :, page].clone() for t in (self.kv, self.kv_scale)] if self.kv8 else []
             self.pos.zero_()
             side = torch.cuda.Stream()
             side.wait_stream(torch.cuda.current_stream())
@@ -659,6 +662,8 @@ class Model:
             with torch.cuda.graph(graph):
                 self.step()
             self.graph = graph
+            for t, was in zip((self.kv, self.kv_scale), kept):
+                t[:, :, page] = was
         torch.cuda.synchronize()
 
     def _claim_positions(self, n):

@@ -287,6 +287,18 @@ def test_attention(K, dtype, M, n_q, n_kv, D, page, pos, window, sinks):
 
 
 @pytest.mark.parametrize("dtype", CACHES, ids=name)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("M,pos,cap,window", [(1, 900, 900, 0), (1, 900, 5000, 0), (1, 900, 60000, 0), (1, 900, 1 << 22, 0),
+                                              (3, 2000, 1 << 22, 700)])
+def test_attention_every_plan_of_few_columns(K, dtype, D, M, pos, cap, window):
+    """max_ctx and the window choose whether a call of few columns is split, by how many waves, and how K and V are loaded."""
+    cap = max(cap, pos + M)
+    caches, scales, bt, vals = paged_kv(pos + M, 2, D, 16, dtype, gen(D + M))
+    q = torch.randn(M, 8, D, generator=gen(1)).half()
+    check(K, q, pos, bt, caches, scales, vals, cap, window, 4 if window else 0)
+
+
+@pytest.mark.parametrize("dtype", CACHES, ids=name)
 @pytest.mark.parametrize("M,pos,window,sinks", [(1, 40, 1 << 30, 0), (3, 40, 43, 0), (3, 40, 5, 1 << 30), (3, 40, 5, 36),
                                                 (3, 2, 3, 3), (40, 0, 1, 1), (40, 0, 40, 9), (40, 25, 7, 30)])
 def test_attention_windows_that_meet_their_sinks(K, dtype, M, pos, window, sinks):
@@ -387,6 +399,23 @@ def test_attention_keeps_unattended_values_out(K, dtype, D, M, pos, window, sink
     keep = [d for d in range(D) if d != 9]
     shape = lambda x: x.view(M, n_q, D)[hit][:, n_q // n_kv:][..., keep]
     R.within(shape(out), shape(want), shape(bound))
+
+
+@pytest.mark.parametrize("dtype", [torch.half, torch.float8_e4m3fn], ids=name)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("M,pos,window,sinks", [(1, 200, 50, 4), (3, 200, 50, 4), (1, 97, 33, 0), (40, 500, 70, 9),
+                                                (200, 600, 100, 3)])
+def test_attention_nan_outside_every_window(K, dtype, D, M, pos, window, sinks):
+    """Tokens that no row attends, next to the windows and the sinks, hold NaN in K and V: in the tiles that the kernels read."""
+    n_q, n_kv, page = 8, 2, 16
+    caches, scales, bt, vals = paged_kv(pos + M, n_kv, D, page, dtype, gen(pos + D))
+    q = torch.randn(M, n_q, D, generator=gen(4)).half()
+    lo = pos - window + 1
+    for t in {lo - 1, lo - 2, lo - 17, sinks, sinks + 1, sinks + 20}:
+        c = R.token_row(bt.tolist(), t, page, caches[0].size(0))
+        for x in (*caches, *vals):
+            x[c[0], :, c[1]] = float("nan")
+    check(K, q, pos, bt, caches, scales, vals, pos + M, window, sinks)
 
 
 @pytest.mark.parametrize("dtype", CACHES, ids=name)

@@ -110,6 +110,22 @@ def test_replayed_steps_are_the_eager_ones(cfg):
     assert torch.equal(*got) and a.host_pos == int(a.pos) == 45
 
 
+@pytest.mark.parametrize("kv", ["int8", "e4m3"])
+def test_preparing_again_keeps_a_sequence_in_codes(kv):
+    """The captured step is recorded anew in the middle of a sequence: what follows is what follows without it."""
+    a, b = model(kv=kv), model(kv=kv)
+    got = []
+    for m in (a, b):
+        m.reset(0)
+        m.prefill(tokens(30))
+        if m is b:
+            before = [t.clone() for t in (m.kv.view(torch.uint8), m.kv_scale)]
+            m.prepare(256)
+            assert all(torch.equal(x, y) for x, y in zip(before, (m.kv.view(torch.uint8), m.kv_scale)))
+        got.append(m.teacher_force(tokens(10, 5), collect_logits=True))
+    assert torch.equal(*got)
+
+
 def test_window_wider_than_the_sequence_changes_only_the_kernel():
     """The same attention by other kernels: logits within the 2e-2 of the largest that two summation orders of one model are
     given elsewhere."""
