@@ -1,0 +1,477 @@
+// Windowed attention of few columns: at most 16 (row, query head) pairs of a kv head, as in a decode step.
+// Nothing is shared between waves, so K
+// and V go from the cache to registers. The waves of all splits take the tiles of 32 tokens in turn, so that a page can be
+// looked up before the position is known. Per tile:
+//   * S^T = K . Q^T on v_mfma_f32_16x16x32_f16, 16 tokens at a time: lane (g, c) feeds token c of K and column c of Q over the
+//     same dims (any order of the dims serves that both operands keep): 16 bytes of a row are one k step of fp16 values or
+//     two of codes. It receives the scores of tokens 4 g + v for column c.
+//   * O^T += V^T . P^T over the 32 tokens: those scores' weights, in fp16, are the B operand as they are (k slot 4 s + v of
+//     lane group g is token 16 s + 4 g + v). For A lane (g, r) loads dims [r D / 16, (r + 1) D / 16) of those 8 tokens' rows
+//     and transposes them in registers; output tile t holds dim r D / 16 + t, so that lane (g, c) ends with D / 4 dims in a
+//     row of column c.
+#include "attn_window.hpp"
+
+namespace dk {
+namespace {
+
+// Over the lanes c, c + 16, c + 32, c + 48 of a wave, by swapping rows and halves of two registers (LDS is not touched).
+template <class F>
+__device__ __forceinline__ float over_rows(float v, F f) {
+  const uint32_t u = __float_as_uint(v);
+  const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const uint32_t a0 = a[0], a1 = a[1];
+  const uint32_t w = __float_as_uint(f(__uint_as_float(a0), __uint_as_float(a1)));
+  const auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+  const uint32_t b0 = b[0], b1 = b[1];
+  return f(__uint_as_float(b0), __uint_as_float(b1));
+}
+
+template <int D, int CACHE>
+struct FewShape {
+  static constexpr bool F16 = CACHE == kCacheF16;
+  static constexpr int ES = F16 ? 2 : 1;        // bytes of a value in the cache
+  static constexpr int KW = D * ES / 64;        // 16-byte loads of a K row per lane
+  static constexpr int DPL = D / 16;            // dims of a V row per lane
+  static constexpr int VW = DPL * ES / 4;       // their words
+};
+
+template <int D, int CACHE, int NW, bool NT>
+__global__ void __launch_bounds__(NW * kWave, 2)
+attn_few_kernel(const WinArgs a) {
+  using S = FewShape<D, CACHE>;
+  constexpr bool F16 = S::F16;
+  constexpr int ES = S::ES, KW = S::KW, DPL = S::DPL, VW = S::VW, KS = D / 32;
+  __shared__ float s_m[NW][kFewCols], s_l[NW][kFewCols];
+  __shared__ __align__(16) float s_o[NW][kFewCols][D];
+  const int kvh = blockIdx.x, split = blockIdx.y;
+  const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int P = 1 << a.log2P;
+  const int i0 = split * NW + wave, step = a.splits * NW;  // the wave's tiles: i0 and every step-th from there
+  // pages of tile i0 as they are without a window, beside the position
+  struct Pages {
+    int p[2];
+  };
+  auto pages_at = [&](int t) __attribute__((always_inline)) {
+    return Pages{{a.bt[min(t >> a.log2P, a.n_bt - 1)], a.bt[min((t + 16) >> a.log2P, a.n_bt - 1)]}};
+  };
+  const int pos = *a.pos;
+  Pages pg = pages_at(kFewTile * i0);
+  const int n_q = a.n_kv << a.lhpg, cols = a.M << a.lhpg;
+  const int cc = min(c, cols - 1);              // columns past the last repeat it
+  const int m = cc >> a.lhpg, hd = (kvh << a.lhpg) + (cc & ((1 << a.lhpg) - 1));
+  h8 q[KS];
+  {
+    const f16* qh = a.q + (size_t)m * a.q_stride + (size_t)hd * D;
+#pragma unroll
+    for (int k = 0; k < KS; ++k)  // the dims of K's k step
+      q[k] = __builtin_bit_cast(
+          h8, *reinterpret_cast<const u32x4*>(qh + (F16 ? 32 * k + 8 * g : 64 * (k >> 1) + 16 * g + 8 * (k & 1))));
+  }
+  __builtin_amdgcn_sched_barrier(0);            // (those loads go out before the position is waited for)
+  const Sight mine = sight_of(pos, m, a.window, a.cap);
+  const Sight s0 = sight_of(pos, 0, a.window, a.cap), s1 = sight_of(pos, a.M - 1, a.window, a.cap);
+  const int ctx = s1.lim + 1;                   // tokens [0, ctx) are read
+  // tiles: those of the sinks, then those of the window, nt in all
+  const int all = (ctx + kFewTile - 1) / kFewTile, wt = min(s0.lo / kFewTile, all);
+  const int ns = a.window > 0 ? min((min(a.sinks, ctx) + kFewTile - 1) / kFewTile, wt) : 0;
+  const int nt = ns + all - wt;
+  auto tile_at = [&](int i) __attribute__((always_inline)) { return kFewTile * (i < ns ? i : i + (wt - ns)); };
+
+  typedef uint32_t vrow __attribute__((ext_vector_type(VW)));
+  struct Tile {
+    int t0;
+    u32x4 k[2][KW];   // by 16 tokens
+    vrow v[2][4];
+    float ks[2], vs[2];
+    bool ok[2];       // the page is mapped; uniform
+  };
+  auto lookup = [&](int i) __attribute__((always_inline)) { return pages_at(tile_at(i)); };
+  auto load = [&](int i, const Pages& w) __attribute__((always_inline)) {
+    Tile x;
+    x.t0 = tile_at(i);
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      x.ok[s] = (unsigned)w.p[s] < (unsigned)a.n_pages;
+      // (16 tokens lie in one page; without one, rows of a page that exists)
+      const size_t row = (((size_t)(x.ok[s] ? w.p[s] : 0) * a.n_kv + kvh) << a.log2P) + ((x.t0 + 16 * s) & (P - 1));
+      const uint8_t* kr = a.kc + row * (D * ES) + c * (D * ES) + 16 * g;
+      const uint8_t* vr = a.vc + row * (D * ES) + 4 * g * (D * ES) + c * (DPL * ES);
+#pragma unroll
+      for (int j = 0; j < KW; ++j) {
+        const u32x4* p = reinterpret_cast<const u32x4*>(kr + 64 * j);
+        x.k[s][j] = NT ? load_stream(p) : *p;
+      }
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const vrow* p = reinterpret_cast<const vrow*>(vr + v * (D * ES));
+        x.v[s][v] = NT ? __builtin_nontemporal_load(p) : *p;
+      }
+      if constexpr (!F16) {
+        x.ks[s] = a.ks[row >> 4];
+        x.vs[s] = a.vs[row >> 4];
+      }
+    }
+    return x;
+  };
+
+  float ref = kWinNoMax, lift = -kWinNoMax, l = 0.f;  // as in the kernel of many columns
+  f4 acc[DPL];
+#pragma unroll
+  for (int t = 0; t < DPL; ++t) acc[t] = f4{0.f, 0.f, 0.f, 0.f};
+
+  // the V operand of output tile t: dim DPL r + t of the 8 tokens
+  auto operand = [&](const Tile& x, const uint32_t (&tr)[2][VW][4], int t) __attribute__((always_inline)) -> u32x4 {
+    if constexpr (F16) {
+      const uint32_t sel = (t & 1) ? 0x07060302u : 0x05040100u;
+      u32x4 r;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        r[2 * s] = __builtin_amdgcn_perm(x.v[s][1][t >> 1], x.v[s][0][t >> 1], sel);
+        r[2 * s + 1] = __builtin_amdgcn_perm(x.v[s][3][t >> 1], x.v[s][2][t >> 1], sel);
+      }
+      return r;
+    } else {
+      const u32x2 lo = kv8_decode4<CACHE>(tr[0][t >> 2][t & 3], x.vs[0]), hi = kv8_decode4<CACHE>(tr[1][t >> 2][t & 3], x.vs[1]);
+      return u32x4{lo[0], lo[1], hi[0], hi[1]};
+    }
+  };
+  auto finite = [](u32x4 x) __attribute__((always_inline)) -> u32x4 {  // zero for what is no finite number
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if ((x[i] & 0x7C00u) == 0x7C00u) x[i] &= 0xFFFF0000u;
+      if ((x[i] & 0x7C000000u) == 0x7C000000u) x[i] &= 0xFFFFu;
+    }
+    return x;
+  };
+  auto compute = [&](Tile& x, bool first) __attribute__((always_inline)) {
+    const int t0 = x.t0;
+    // every column sees every token; uniform per wave
+    const bool plain = x.ok[0] && x.ok[1] && t0 + kFewTile - 1 <= s0.lim && (t0 >= s1.lo || t0 + kFewTile <= a.sinks);
+    f4 sc[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      sc[s] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < KW; ++j) {
+        if constexpr (F16) {
+          sc[s] = mfma16x32(__builtin_bit_cast(h8, x.k[s][j]), q[j], sc[s]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            sc[s] = mfma16x32(__builtin_bit_cast(h8, kv8_decode8<CACHE>(u32x2{x.k[s][j][2 * e], x.k[s][j][2 * e + 1]}, x.ks[s])),
+                              q[2 * j + e], sc[s]);
+        }
+      }
+    }
+    if (!plain) {
+      asm volatile("");  // stays a branch
+      auto low = [](int n) __attribute__((always_inline)) -> uint32_t { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; };
+      // tokens of the tile that exist (uniform), and those that the column sees, from this lane's first one on
+      const uint32_t there = low(ctx - t0) & ((x.ok[0] ? 0xFFFFu : 0u) | (x.ok[1] ? 0xFFFF0000u : 0u));
+      const uint32_t seen = (there & low(mine.lim + 1 - t0) & (~low(mine.lo - t0) | low(a.sinks - t0))) >> (4 * g);
+      const uint32_t real = there >> (4 * g);
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          if (!(seen & (1u << (16 * s + v)))) sc[s][v] = -INFINITY;
+          if (!(real & (1u << (16 * s + v)))) x.v[s][v] = vrow(0u);  // (its V must not meet a p of 0)
+        }
+        if constexpr (!F16) x.vs[s] = there & (1u << (16 * s)) ? x.vs[s] : 1.f;
+      }
+    }
+    float p[2][4];
+    auto weigh = [&](float off, float lift) __attribute__((always_inline)) -> float {
+      float sum = 0.f;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          p[s][v] = __builtin_amdgcn_exp2f(fmaf(sc[s][v] - off, a.c2, lift));
+          sum += p[s][v];
+        }
+      }
+      return sum;
+    };
+    float sum = INFINITY;            // (the first tile brings the reference)
+    if (!first) sum = weigh(0.f, lift);
+    if (__any(!(sum <= kWinMost))) {  // the reference moves to this tile's maximum where that is higher
+      asm volatile("");
+      float mx = sc[0][0];
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+#pragma unroll
+        for (int v = 0; v < 4; ++v) mx = fmaxf(mx, sc[s][v]);
+      }
+      const auto larger = [](float x, float y) { return fmaxf(x, y); };
+      mx = fmaxf(ref, over_rows(mx, larger));
+      mx = over_rows(sum <= kWinMost ? 0.f : 1.f, larger) != 0.f ? mx : ref;  // in any of the column's four lanes
+      const float alpha = __builtin_amdgcn_exp2f((ref - mx) * a.c2);  // 1 for a column that stays
+      if (mx != ref) lift = fabsf(mx * a.c2) > kWinFar ? INFINITY : kWinLift - mx * a.c2;
+      ref = mx;
+      l *= alpha;
+#pragma unroll
+      for (int t = 0; t < DPL; ++t) acc[t] *= alpha;
+      sum = weigh(lift == INFINITY ? ref : 0.f, lift == INFINITY ? kWinLift : lift);
+    }
+    l += sum;
+    h8 ph;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+#pragma unroll
+      for (int v = 0; v < 4; ++v) ph[4 * s + v] = (f16)p[s][v];
+    }
+    // codes: bytes of four tokens' words to words of four tokens
+    uint32_t tr[2][VW][4];
+    if constexpr (!F16) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+#pragma unroll
+        for (int w = 0; w < VW; ++w) {
+          const uint32_t al = __builtin_amdgcn_perm(x.v[s][1][w], x.v[s][0][w], 0x05010400u);
+          const uint32_t ah = __builtin_amdgcn_perm(x.v[s][1][w], x.v[s][0][w], 0x07030602u);
+          const uint32_t bl = __builtin_amdgcn_perm(x.v[s][3][w], x.v[s][2][w], 0x05010400u);
+          const uint32_t bh = __builtin_amdgcn_perm(x.v[s][3][w], x.v[s][2][w], 0x07030602u);
+          tr[s][w][0] = __builtin_amdgcn_perm(bl, al, 0x05040100u);
+          tr[s][w][1] = __builtin_amdgcn_perm(bl, al, 0x07060302u);
+          tr[s][w][2] = __builtin_amdgcn_perm(bh, ah, 0x05040100u);
+          tr[s][w][3] = __builtin_amdgcn_perm(bh, ah, 0x07060302u);
+        }
+      }
+    }
+    bool dirty = false;  // NaN or infinity in V of a tile that not every column sees whole; uniform
+    if (!plain) {
+      asm volatile("");
+      // a look at the words first: fp16 with all exponent bits, e4m3's NaN, a scale that takes a code past fp16
+      uint32_t odd = 0;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+#pragma unroll
+          for (int w = 0; w < VW; ++w) {
+            if constexpr (F16)
+              odd |= ((x.v[s][v][w] & 0x7C007C00u) + 0x04000400u) & 0x80008000u;
+            else if constexpr (CACHE == kCacheE4m3)
+              odd |= ((x.v[s][v][w] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+          }
+        }
+        if constexpr (!F16) odd |= x.vs[s] <= (CACHE == kCacheInt8 ? 512.f : 128.f) ? 0u : 1u;
+      }
+      if (__any(odd != 0)) {
+        asm volatile("");
+#pragma unroll
+        for (int t = 0; t < DPL; ++t) dirty = dirty || has_nonfinite(operand(x, tr, t));
+        dirty = __any(dirty);
+      }
+    }
+    if (!dirty) {
+#pragma unroll
+      for (int t = 0; t < DPL; ++t) acc[t] = mfma16x32(__builtin_bit_cast(h8, operand(x, tr, t)), ph, acc[t]);
+      return;
+    }
+    asm volatile("");
+#pragma unroll
+    for (int t = 0; t < DPL; ++t) acc[t] = mfma16x32(__builtin_bit_cast(h8, finite(operand(x, tr, t))), ph, acc[t]);
+    // the values left out, for the columns that see their token
+    for (int i = 0; i < kFewTile; ++i) {
+      const int t = t0 + i, s = i >> 4;
+      if (!((s ? x.ok[1] : x.ok[0]) && t < ctx)) continue;  // uniform
+      const bool see = t <= mine.lim && (t >= mine.lo || t < a.sinks);
+      float w = 0.f;                        // p of token i: in lane group i / 4 % 4, element (s, i % 4)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w = e == 4 * s + (i & 3) ? p[e >> 2][e & 3] : w;
+      w = __shfl(w, 16 * ((i >> 2) & 3) + c, kWave);
+      const size_t at = (((size_t)a.bt[t >> a.log2P] * a.n_kv + kvh) << a.log2P) + (t & (P - 1));
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+#pragma unroll
+        for (int d = 0; d < DPL; d += 4) {
+          const size_t off = at * D + (size_t)(4 * g + v) * DPL + d;
+          u32x2 b;
+          if constexpr (F16)
+            b = *reinterpret_cast<const u32x2*>(a.vc + 2 * off);
+          else
+            b = kv8_decode4<CACHE>(*reinterpret_cast<const uint32_t*>(a.vc + off), a.vs[at >> 4]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float f = (float)as_f16x2(b[e >> 1])[e & 1];
+            if (see && !(fabsf(f) <= 65504.f)) acc[d + e][v] = fmaf(w, f, acc[d + e][v]);
+          }
+        }
+      }
+    }
+  };
+
+  if (i0 < nt) {  // uniform per wave
+    if (a.window > 0) pg = lookup(i0);
+    // the next tile's loads go out ahead of a tile's products; behind the last one every wave's are of tile 0, from a cache
+    auto live = [&](int i) __attribute__((always_inline)) { return i < nt ? i : 0; };
+    Tile x = load(i0, pg);
+    pg = lookup(live(i0 + step));
+#pragma unroll 1
+    for (int i = i0; i < nt; i += step) {
+      const Tile y = load(live(i + step), pg);
+      pg = lookup(live(i + 2 * step));
+      compute(x, i == i0);
+      x = y;
+    }
+  }
+  l = over_rows(l, [](float x, float y) { return x + y; });
+  // ---- the waves meet in LDS, in order: column c's dims [D / 4 g, + D / 4), acc[t][v] dim D / 4 g + DPL v + t
+  if (g == 0) {
+    s_m[wave][c] = ref;
+    s_l[wave][c] = l;
+  }
+  if (c < cols) {
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+#pragma unroll
+      for (int t = 0; t < DPL; t += 4)
+        *reinterpret_cast<f4*>(&s_o[wave][c][D / 4 * g + DPL * v + t]) = f4{acc[t][v], acc[t + 1][v], acc[t + 2][v], acc[t + 3][v]};
+    }
+  }
+  __syncthreads();
+  const size_t part = (size_t)split * a.n_kv + kvh;
+  const bool none = split * NW >= nt;  // a split without tokens: the join reads no output of it
+  for (int j = tid; j < cols * (D / 4); j += NW * kWave) {
+    const int col = j / (D / 4), d = 4 * (j % (D / 4));
+    float mx = kWinNoMax, L = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) mx = fmaxf(mx, s_m[w][col]);
+    f4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      // a wave that saw no token weighs 0 beside one that did
+      const float f = __builtin_amdgcn_exp2f((s_m[w][col] - mx) * a.c2);
+      L = fmaf(f, s_l[w][col], L);
+      const f4 y = *reinterpret_cast<const f4*>(&s_o[w][col][d]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = fmaf(f, y[e], o[e]);
+    }
+    if (a.splits > 1) {
+      if (d == 0) a.part_ml[part * kFewCols + col] = none ? float2{kWinNoMax, 0.f} : float2{mx, L};
+      if (!none) store_through16(a.part_o + part * kFewCols * (D / 4), 4 * (col * D + d), __builtin_bit_cast(u32x4, o));
+      continue;
+    }
+    const float inv = L == 0.f ? 0.f : 1.0f / L;  // a NaN stays
+    const int mo = col >> a.lhpg, ho = (kvh << a.lhpg) + (col & ((1 << a.lhpg) - 1));
+    *reinterpret_cast<u32x2*>(a.out + ((size_t)mo * n_q + ho) * D + d) =
+        u32x2{as_u32(f16x2{(f16)(o[0] * inv), (f16)(o[1] * inv)}), as_u32(f16x2{(f16)(o[2] * inv), (f16)(o[3] * inv)})};
+  }
+}
+
+// Joins the splits of one column, in split order: groups of D / 4 threads take the splits i, i + G, ..., then meet in LDS.
+template <int D>
+__global__ void __launch_bounds__(256)
+attn_few_join_kernel(const f4* __restrict__ part_o, const float2* __restrict__ part_ml, int lhpg, int n_kv, int splits,
+                     float c2, f16* __restrict__ out) {
+  constexpr int T = D / 4, G = 256 / T;
+  __shared__ float s_w[kWinMaxSplits];
+  __shared__ float s_l;
+  __shared__ f4 s_o[G][T];
+  const int kvh = blockIdx.x, col = blockIdx.y, tid = threadIdx.x, d = tid % T, grp = tid / T;
+  const size_t step = (size_t)n_kv * kFewCols, first = (size_t)kvh * kFewCols + col;
+  constexpr int NB = kWinMaxSplits / G;
+  f4 x[NB];
+#pragma unroll
+  for (int k = 0; k < NB; ++k) {
+    const int s = grp + G * k;
+    if (s < splits) x[k] = part_o[((size_t)s * step + first) * T + d];
+  }
+  if (tid < kWave) {
+    const float2 ml = tid < splits ? part_ml[(size_t)tid * step + first] : float2{kWinNoMax, 0.f};
+    const bool saw = ml.x != kWinNoMax || ml.y != 0.f;  // (a NaN sum counts)
+    const float mx = group_max<kWave>(ml.x);
+    const float w = __builtin_amdgcn_exp2f((ml.x - mx) * c2);
+    const float L = group_sum<kWave>(saw ? w * ml.y : 0.f);
+    s_w[tid] = saw ? w : -1.f;
+    if (tid == 0) s_l = L;
+  }
+  __syncthreads();
+  f4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int k = 0; k < NB; ++k) {
+    const int s = grp + G * k;
+    const float w = s < splits ? s_w[s] : -1.f;
+    if (w < 0.f) continue;  // (its output was not written)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = fmaf(w, x[k][e], o[e]);
+  }
+  s_o[grp][d] = o;
+  __syncthreads();
+  if (grp > 0) return;
+#pragma unroll
+  for (int k = 1; k < G; ++k) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] += s_o[k][d][e];
+  }
+  const float inv = s_l == 0.f ? 0.f : 1.0f / s_l;  // a NaN stays
+  const int m = col >> lhpg, hd = (kvh << lhpg) + (col & ((1 << lhpg) - 1));
+  *reinterpret_cast<u32x2*>(out + ((size_t)m * (n_kv << lhpg) + hd) * D + 4 * d) =
+      u32x2{as_u32(f16x2{(f16)(o[0] * inv), (f16)(o[1] * inv)}), as_u32(f16x2{(f16)(o[2] * inv), (f16)(o[3] * inv)})};
+}
+
+// Waves of a workgroup and splits of a call of few columns. A context that eight waves get through in two tiles each (D 128)
+// or four (D 64) is not split: one launch instead of two. From there to 4096 tiles over all kv heads workgroups of four waves,
+// so that one tile per wave reaches twice the CUs; then of eight. At most one workgroup per CU, none with less than a tile per
+// wave. Captured, in us, one token, e4m3:
+//   8 x 4 heads of 128   300 tokens unsplit 6.9, split 7.7 | 600: 8.5, 7.6 | 4096: waves 4 8.2, 8 10.5 | 32768: 18.8, eight
+//                        in 512 workgroups 23.2, four in 256 18.4
+//   4 x 8 heads of 64    600 tokens unsplit 5.4, split 6.9 | 900: 6.8, 6.8 | 16384: waves 4 7.8, 8 8.4 | 32768: 9.4, 8.9
+struct FewPlan {
+  int waves, splits;
+};
+FewPlan few_plan(int M, int n_kv, int D, int max_ctx, int window, int sinks) {
+  const long long tiles = (win_tokens(M, max_ctx, window, sinks) + kFewTile - 1) / kFewTile;
+  if (tiles <= (D == 128 ? 16 : 32)) return {8, 1};
+  const int waves = tiles * n_kv < 4096 ? 4 : 8;
+  const long long want = max(1LL, min((long long)kWinMaxSplits, 256LL / n_kv));
+  const long long per = max((tiles + want - 1) / want, (long long)waves);
+  return {waves, (int)((tiles + per - 1) / per)};
+}
+
+template <int D, int CACHE>
+void launch(const WindowAttn& w, WinArgs a, hipStream_t st) {
+  a.part_ml = (float2*)(a.part_o + (size_t)w.splits * w.n_kv * kFewCols * (D / 4));
+  const FewPlan p = few_plan(w.M, w.n_kv, D, w.max_ctx, w.window, w.sinks);
+  // K and V that fill half of the last cache (256 MB) are not kept there for the next call. (8 x 4 heads of 128: one token at
+  // 131072, int8, cold 55.1 -> 51.2 us; at 16384, e4m3, from the cache 12.1, past it 14.0)
+  const long long bytes = win_tokens(w.M, w.max_ctx, w.window, w.sinks) * w.n_kv * 2 * D * (CACHE == kCacheF16 ? 2 : 1);
+  const dim3 grid(w.n_kv, w.splits);
+  if (p.waves == 4)
+    hipLaunchKernelGGL((attn_few_kernel<D, CACHE, 4, false>), grid, dim3(4 * kWave), 0, st, a);
+  else if (bytes < (128LL << 20))
+    hipLaunchKernelGGL((attn_few_kernel<D, CACHE, 8, false>), grid, dim3(8 * kWave), 0, st, a);
+  else
+    hipLaunchKernelGGL((attn_few_kernel<D, CACHE, 8, true>), grid, dim3(8 * kWave), 0, st, a);
+  if (w.splits > 1)
+    hipLaunchKernelGGL(attn_few_join_kernel<D>, dim3(w.n_kv, (unsigned)(w.M << a.lhpg)), dim3(256), 0, st,
+                       (const f4*)a.part_o, a.part_ml, a.lhpg, w.n_kv, w.splits, a.c2, (f16*)w.out);
+}
+
+template <int D>
+void launch_cache(const WindowAttn& w, const WinArgs& a, hipStream_t st) {
+  if (w.cache == kCacheF16)
+    launch<D, kCacheF16>(w, a, st);
+  else if (w.cache == kCacheInt8)
+    launch<D, kCacheInt8>(w, a, st);
+  else
+    launch<D, kCacheE4m3>(w, a, st);
+}
+
+}  // namespace
+
+int attention_few_splits(int M, int n_kv, int D, int max_ctx, int window, int sinks) {
+  return few_plan(M, n_kv, D, max_ctx, window, sinks).splits;
+}
+
+void launch_attention_few(const WindowAttn& w, const WinArgs& a, hipStream_t st) {
+  if (w.head_dim == 64)
+    launch_cache<64>(w, a, st);
+  else
+    launch_cache<128>(w, a, st);
+}
+
+}  // namespace dk
