@@ -1,14 +1,24 @@
 // Windowed attention of few columns: at most 16 (row, query head) pairs of a kv head, as in a decode step.
-// Nothing is shared between waves, so K
-// and V go from the cache to registers. The waves of all splits take the tiles of 32 tokens in turn, so that a page can be
-// looked up before the position is known. Per tile:
+//
+// Nothing is shared between waves, so K and V go from the cache to registers, a tile ahead of its products. The waves of all
+// splits take the tiles of 32 tokens in turn, so that without a window the first tile's pages are looked up beside the position
+// instead of behind it, and any context spreads evenly. Per tile:
 //   * S^T = K . Q^T on v_mfma_f32_16x16x32_f16, 16 tokens at a time: lane (g, c) feeds token c of K and column c of Q over the
 //     same dims (any order of the dims serves that both operands keep): 16 bytes of a row are one k step of fp16 values or
-//     two of codes. It receives the scores of tokens 4 g + v for column c.
-//   * O^T += V^T . P^T over the 32 tokens: those scores' weights, in fp16, are the B operand as they are (k slot 4 s + v of
-//     lane group g is token 16 s + 4 g + v). For A lane (g, r) loads dims [r D / 16, (r + 1) D / 16) of those 8 tokens' rows
-//     and transposes them in registers; output tile t holds dim r D / 16 + t, so that lane (g, c) ends with D / 4 dims in a
-//     row of column c.
+//     two of codes, which become fp16 with their scale here. It receives the scores of tokens 4 g + v for column c.
+//   * the weights (attn_window.hpp); the first tile brings the reference at once.
+//   * O^T += V^T . P^T over the 32 tokens: the weights, in fp16, are the B operand as they are (k slot 4 s + v of lane group g
+//     is token 16 s + 4 g + v). For A lane (g, r) loads dims [r D / 16, (r + 1) D / 16) of those 8 tokens' rows and transposes
+//     them in registers; output tile t holds dim r D / 16 + t, so that lane (g, c) ends with D / 4 dims in a row of column c.
+// Tiles that some column does not see whole: 32 token bits per column; V of tokens that do not exist is zeroed, and where the
+// words hold anything that may be NaN or infinite such values are taken out of the products and added one by one for the
+// columns that see their token.
+//
+// What bounds it: one int8 token at 131072, 8 x 4 heads of 128, takes 47 us for 269 MB, 5.7 TB/s. Small ones are launch and a
+// chain of dependent loads (position and page, K / V), the waves' merge in LDS, and where they are split the join: captured,
+// 4.9 us at 300 tokens of 4 x 8 heads of 64 (one launch), 8.1 at 4096 of 8 x 4 heads of 128 (5.5 and 2.6). Of those, masks
+// as compares and the look for NaN on unpacked values cost 1 us (every decode step's last tile takes that path), reductions
+// through LDS and a second copy of the tile's code 0.2. No gain: 16 waves (the registers of a tile do not fit).
 #include "attn_window.hpp"
 
 namespace dk {
@@ -132,7 +142,8 @@ attn_few_kernel(const WinArgs a) {
       }
       return r;
     } else {
-      const u32x2 lo = kv8_decode4<CACHE>(tr[0][t >> 2][t & 3], x.vs[0]), hi = kv8_decode4<CACHE>(tr[1][t >> 2][t & 3], x.vs[1]);
+      const u32x2 lo = kv8_decode4<CACHE>(tr[0][t >> 2][t & 3], x.vs[0]);
+      const u32x2 hi = kv8_decode4<CACHE>(tr[1][t >> 2][t & 3], x.vs[1]);
       return u32x4{lo[0], lo[1], hi[0], hi[1]};
     }
   };
@@ -158,9 +169,10 @@ attn_few_kernel(const WinArgs a) {
           sc[s] = mfma16x32(__builtin_bit_cast(h8, x.k[s][j]), q[j], sc[s]);
         } else {
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
-            sc[s] = mfma16x32(__builtin_bit_cast(h8, kv8_decode8<CACHE>(u32x2{x.k[s][j][2 * e], x.k[s][j][2 * e + 1]}, x.ks[s])),
-                              q[2 * j + e], sc[s]);
+          for (int e = 0; e < 2; ++e) {
+            const u32x4 k = kv8_decode8<CACHE>(u32x2{x.k[s][j][2 * e], x.k[s][j][2 * e + 1]}, x.ks[s]);
+            sc[s] = mfma16x32(__builtin_bit_cast(h8, k), q[2 * j + e], sc[s]);
+          }
         }
       }
     }
@@ -329,7 +341,8 @@ attn_few_kernel(const WinArgs a) {
     for (int v = 0; v < 4; ++v) {
 #pragma unroll
       for (int t = 0; t < DPL; t += 4)
-        *reinterpret_cast<f4*>(&s_o[wave][c][D / 4 * g + DPL * v + t]) = f4{acc[t][v], acc[t + 1][v], acc[t + 2][v], acc[t + 3][v]};
+        *reinterpret_cast<f4*>(&s_o[wave][c][D / 4 * g + DPL * v + t]) =
+            f4{acc[t][v], acc[t + 1][v], acc[t + 2][v], acc[t + 3][v]};
     }
   }
   __syncthreads();

@@ -1,4 +1,41 @@
-// Windowed attention of many columns.
+// Windowed attention of many columns. A wave has 32 columns, so every column does work at any GQA ratio. A workgroup has CW
+// waves of columns, KVS times: group g of KVS takes the blocks of BT tokens with index % KVS == g, so that K / V in LDS once
+// serve CW waves, and few columns still fill a workgroup. The tokens are further split over `splits` workgroups in whole rounds
+// of KVS blocks; the ends follow *pos, so one captured launch serves every position. The kv head is the fastest grid index: with
+// 8 of them each XCD's L2 holds one head's K / V for all its workgroups.
+//
+// The tokens of a workgroup are those of its rows' windows behind those of the sinks, as one list of 32-token tiles ("places"):
+// a round is taken from the list, so a handful of sinks costs one tile, and the window's start is aligned to a tile. (As whole
+// rounds of their own 4 sinks cost a round of 128 tokens: 4096 rows under a window of 1024 took 110 us instead of 102 in that
+// shape.)
+// A round's K / V lie in LDS as fp16, double-buffered. fp16 caches are loaded straight into LDS (buffer loads, spread over the
+// products of the round before); codes go to registers in the first half of that round's products and are turned to fp16, with
+// their scale, on the way to LDS behind them: CW waves share that work, 1 / CW of a conversion per weight and wave. 4096 rows
+// take 149 us over e4m3, 148 over fp16.
+//
+// Per tile of 32 tokens, on v_mfma_f32_32x32x16_f16:
+//   * S^T = K . Q^T: A = the tile's rows of K from LDS, B = the wave's Q columns (registers). Lane (h, r) receives column r,
+//     tokens 8 q + 4 h + v: a column's scores, sum and output live in the lane pair (r, r + 32).
+//   * the weights (attn_window.hpp), while the next tile's products run;
+//   * O^T += V^T . P^T: the score accumulator, rounded to fp16, is the B operand as it is; V^T comes out of the row-major V tile
+//     through the transposing LDS read.
+// Masks cost nothing where every column of the wave sees the whole block and every page of the split is mapped (asked once).
+// Elsewhere a lane compares its column's bounds to 32 token bits per tile. Scores of tokens that are not seen become -inf
+// whatever K holds; their p is an exact 0. Since 0 times NaN or infinity is NaN, V chunks of tokens that do not exist are zeroed
+// on the way, and those with such values in rounds that some column does not see whole; the latter are added behind the block,
+// value by value, for the columns that see their token.
+//
+// What bounds it: 4096 rows at 0, 8 x 4 heads of 128, take 148-155 us, 0.89-0.93 PFLOP/s of what they need, against 117 at the
+// rate of a large matrix product: the softmax and LDS reads beside the products at the clock that the card keeps up under
+// them, and blocks on the diagonal that are computed whole. Under a window of 1024 they take 93-95 (floor 51): two turns of 18
+// rounds of 64 tokens, 16 of them needed, and about 8 us each to start. 100 rows behind 8000 tokens take 31 (floor 11): 78% of
+// the columns are real, four rounds in 256 workgroups (17 us), 10 for launch and first loads, 28 MB of partials.
+// No gain: tiles that no column of a wave sees left out (the accumulators meet at the branch: 10 to 250 registers spilled); blocks
+// of 64 tokens for eight waves (157 us instead of 150).
+//
+// LDS: rows of 2 D bytes without padding. K chunk q (16 bytes) of row t at q ^ (t & 15) (D 128) or q ^ ((t >> 1) & 7) (D 64),
+// V in 64-byte units, unit u of row t at u ^ (t & 3) (D 128) or u ^ ((t >> 1) & 1) (D 64): reads fall in distinct banks.
+// The groups of a workgroup meet in LDS, the splits in the workspace and a second launch, both in order.
 #include <type_traits>
 
 #include "attn_window.hpp"
@@ -6,8 +43,6 @@
 namespace dk {
 namespace {
 
-// Many columns. A column is a (row, query head) pair of one kv head; a wave has 32 columns. A workgroup has CW waves of
-// columns, KVS times: group g of KVS takes the blocks of BT tokens with index % KVS == g.
 template <int D, int CACHE, int CW, int KVS, int BT, bool UP>
 __global__ void __launch_bounds__(CW * KVS * kWave, 2) attn_window_kernel(const WinArgs a) {
   constexpr bool F16 = CACHE == kCacheF16;
@@ -24,7 +59,8 @@ __global__ void __launch_bounds__(CW * KVS * kWave, 2) attn_window_kernel(const 
   static_assert(LPT >= 1 && LPT * RPI == SB && RPI % 16 == 0, "staging covers a round");
   static_assert(F16 || UP, "8-bit pages hold 16 tokens or more");
   constexpr int kTile = SB * RB;                // bytes of one K (or V) buffer
-  static_assert((KVS == 1 || KVS * CW * kWave * 16 * DT <= kTile) && 4 % KVS == 0, "a merge row set fits a buffer, a wave's rows whole ones");
+  static_assert((KVS == 1 || KVS * CW * kWave * 16 * DT <= kTile) && 4 % KVS == 0,
+                "a merge row set fits a buffer, a wave's rows whole ones");
   __shared__ __align__(16) uint8_t s_k0[kTile], s_k1[kTile], s_v0[kTile], s_v1[kTile];
   __shared__ float s_m[KVS > 1 ? KVS * CW * 32 : 1], s_l[KVS > 1 ? KVS * CW * 32 : 1];
   // tokens of a round (by 32, in the slot of the round's number modulo 3) of which V chunks were taken out (checked)
@@ -58,7 +94,8 @@ __global__ void __launch_bounds__(CW * KVS * kWave, 2) attn_window_kernel(const 
   const int ns = a.window > 0 ? 32 * min((min(a.sinks, ctx) + 31) / 32, wt) : 0, gap = 32 * wt - ns;
   auto token = [&](int v) __attribute__((always_inline)) { return v < ns ? v : v + gap; };
   // this split's rounds [r0, r1): the first nr % splits splits have one more
-  const unsigned nr = (unsigned)(32 * all - gap + SB - 1) / SB, per = nr / (unsigned)a.splits, more = nr - per * (unsigned)a.splits;
+  const unsigned nr = (unsigned)(32 * all - gap + SB - 1) / SB;
+  const unsigned per = nr / (unsigned)a.splits, more = nr - per * (unsigned)a.splits;
   const int r0 = (int)(split * per + min((unsigned)split, more)), r1 = r0 + (int)per + ((unsigned)split < more);
   h8 q[KS];
   auto load_q = [&]() __attribute__((always_inline)) {
@@ -295,7 +332,8 @@ __global__ void __launch_bounds__(CW * KVS * kWave, 2) attn_window_kernel(const 
         f32x16 st = {};
 #pragma unroll
         for (int k = 0; k < KS; ++k)
-          st = mfma32x32(__builtin_bit_cast(h8, *reinterpret_cast<const u32x4*>(kb + w * 32 * RB + (kat ^ (k << 5)))), q[k], st);
+          st = mfma32x32(__builtin_bit_cast(h8, *reinterpret_cast<const u32x4*>(kb + w * 32 * RB + (kat ^ (k << 5)))), q[k],
+                         st);
         for (; bad != 0; bad &= bad - 1) {
           const int i = __builtin_ctz(bad), t = ts + i;            // a token in this set is inside the context
           const int page = a.bt[t >> a.log2P];
@@ -433,7 +471,8 @@ __global__ void __launch_bounds__(CW * KVS * kWave, 2) attn_window_kernel(const 
   constexpr int kRows = 4 * DT / KVS;
   float mx = ref, L = l, w[KVS];
   auto own_row = [&](int i) __attribute__((always_inline)) {
-    return float4{acc[i / 4][4 * (i % 4)], acc[i / 4][4 * (i % 4) + 1], acc[i / 4][4 * (i % 4) + 2], acc[i / 4][4 * (i % 4) + 3]};
+    const f32x16& x = acc[i / 4];
+    return float4{x[4 * (i % 4)], x[4 * (i % 4) + 1], x[4 * (i % 4) + 2], x[4 * (i % 4) + 3]};
   };
   auto merge_row = [&](int quarter, int i, int g) __attribute__((always_inline)) {  // row DT quarter + i of group g
     uint8_t* buf = quarter == 0 ? s_k0 : quarter == 1 ? s_k1 : quarter == 2 ? s_v0 : s_v1;
@@ -636,8 +675,8 @@ void launch(const WindowAttn& w, hipStream_t st) {
   const long long cols = (long long)w.M << lhpg, waves = (cols + 31) / 32;
   float4* part_o = (float4*)w.ws;
   const WinArgs a{(const f16*)w.q, w.q_stride, w.pos, w.bt, (const uint8_t*)w.kc, (const uint8_t*)w.vc, w.ks, w.vs, w.n_pages,
-                  w.n_bt, w.log2P, w.n_kv, lhpg, w.M, (int)min((long long)w.max_ctx, (long long)w.n_bt << w.log2P), w.window, w.sinks,
-                  w.splits, (float)(1.4426950408889634 / sqrt((double)D)), (f16*)w.out, part_o,
+                  w.n_bt, w.log2P, w.n_kv, lhpg, w.M, (int)min((long long)w.max_ctx, (long long)w.n_bt << w.log2P), w.window,
+                  w.sinks, w.splits, (float)(1.4426950408889634 / sqrt((double)D)), (f16*)w.out, part_o,
                   (float2*)(part_o + (size_t)w.splits * w.n_kv * waves * 8 * D)};
   if (win_few(w.M, w.n_q, w.n_kv, w.log2P)) {
     launch_attention_few(w, a, st);

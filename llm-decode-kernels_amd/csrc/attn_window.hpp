@@ -5,8 +5,8 @@
 // Both hold a column's weights as p = 2^(c2 (s - ref) + kWinLift), c2 = log2(e) / sqrt(D), computed as c2 s + lift: one
 // multiply-add. The reference is a maximum of scores seen so far, not the running one: it moves to a tile's maximum where a sum
 // of p passes kWinMost, so that p fits fp16 and no maximum is taken otherwise; what fp16 cannot hold of a small p is 2^-32 of p
-// at the reference. lift holds c2 ref to half a step of fp32. From kWinFar on that would be more than p's own half step in fp16:
-// there lift is infinite, every tile's first weights overflow, and the second ones are taken from s - ref, exact at the
+// at the reference. lift holds c2 ref to half a step of fp32. From kWinFar on that would be more than p's own half step in
+// fp16: there lift is infinite, every tile's first weights overflow, and the second ones are taken from s - ref, exact at the
 // reference. Scores, sums and outputs are fp32; a weight is rounded to fp16, to nearest, where it meets V (2^-11, unbiased,
 // beside an output that is rounded to fp16 itself; its sum is taken unrounded).
 #pragma once

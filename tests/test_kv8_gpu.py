@@ -331,7 +331,8 @@ def test_attention_caps_and_holes(K, dtype, D, M, cap):
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("M,pos,cap,window,sinks,hpg,n_kv", [
     (60, 440, 500, 0, 0, 4, 2), (700, 0, 700, 100, 20, 1, 16), (40, 700, 1 << 20, 0, 0, 4, 2), (800, 0, 800, 0, 0, 8, 8),
-    (1500, 0, 1500, 30, 4, 8, 8), (1200, 0, 1200, 200, 70, 1, 32), (130, 900, 60000, 0, 0, 8, 8), (300, 500, 20000, 400, 4, 4, 2)])
+    (1500, 0, 1500, 30, 4, 8, 8), (1200, 0, 1200, 200, 70, 1, 32), (130, 900, 60000, 0, 0, 8, 8),
+    (300, 500, 20000, 400, 4, 4, 2)])
 def test_attention_every_workgroup_shape(K, dtype, D, M, pos, cap, window, sinks, hpg, n_kv):
     """The sizes choose among the shapes of a workgroup, split and not: rows spread over all of them, heads of the first and
     the last kv head, with a page that is not mapped and (fp16, e4m3) a NaN in V of a token that some of the rows attend."""
@@ -406,7 +407,7 @@ def test_attention_keeps_unattended_values_out(K, dtype, D, M, pos, window, sink
 @pytest.mark.parametrize("M,pos,window,sinks", [(1, 200, 50, 4), (3, 200, 50, 4), (1, 97, 33, 0), (40, 500, 70, 9),
                                                 (200, 600, 100, 3)])
 def test_attention_nan_outside_every_window(K, dtype, D, M, pos, window, sinks):
-    """Tokens that no row attends, next to the windows and the sinks, hold NaN in K and V: in the tiles that the kernels read."""
+    """Tokens that no row attends, next to the windows and the sinks and in the tiles that are read, hold NaN in K and V."""
     n_q, n_kv, page = 8, 2, 16
     caches, scales, bt, vals = paged_kv(pos + M, n_kv, D, page, dtype, gen(pos + D))
     q = torch.randn(M, n_q, D, generator=gen(4)).half()
