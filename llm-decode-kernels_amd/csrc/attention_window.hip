@@ -1,13 +1,13 @@
 // Windowed attention of many columns. A wave has 32 columns, so every column does work at any GQA ratio. A workgroup has CW
 // waves of columns, KVS times: group g of KVS takes the blocks of BT tokens with index % KVS == g, so that K / V in LDS once
-// serve CW waves, and few columns still fill a workgroup. The tokens are further split over `splits` workgroups in whole rounds
-// of KVS blocks; the ends follow *pos, so one captured launch serves every position. The kv head is the fastest grid index: with
-// 8 of them each XCD's L2 holds one head's K / V for all its workgroups.
+// serve CW waves, and few columns still fill a workgroup. The tokens are further split over `splits` workgroups in whole
+// rounds of KVS blocks; the ends follow *pos, so one captured launch serves every position. The kv head is the fastest grid
+// index: with 8 of them each XCD's L2 holds one head's K / V for all its workgroups.
 //
-// The tokens of a workgroup are those of its rows' windows behind those of the sinks, as one list of 32-token tiles ("places"):
-// a round is taken from the list, so a handful of sinks costs one tile, and the window's start is aligned to a tile. (As whole
-// rounds of their own 4 sinks cost a round of 128 tokens: 4096 rows under a window of 1024 took 110 us instead of 102 in that
-// shape.)
+// The tokens of a workgroup are those of its rows' windows behind those of the sinks, as one list of 32-token tiles
+// ("places"): a round is taken from the list, so a handful of sinks costs one tile, and the window's start is aligned to a
+// tile. (As whole rounds of their own 4 sinks cost a round of 128 tokens: 4096 rows under a window of 1024 took 110 us instead
+// of 102 in that shape.)
 // A round's K / V lie in LDS as fp16, double-buffered. fp16 caches are loaded straight into LDS (buffer loads, spread over the
 // products of the round before); codes go to registers in the first half of that round's products and are turned to fp16, with
 // their scale, on the way to LDS behind them: CW waves share that work, 1 / CW of a conversion per weight and wave. 4096 rows
@@ -17,21 +17,21 @@
 //   * S^T = K . Q^T: A = the tile's rows of K from LDS, B = the wave's Q columns (registers). Lane (h, r) receives column r,
 //     tokens 8 q + 4 h + v: a column's scores, sum and output live in the lane pair (r, r + 32).
 //   * the weights (attn_window.hpp), while the next tile's products run;
-//   * O^T += V^T . P^T: the score accumulator, rounded to fp16, is the B operand as it is; V^T comes out of the row-major V tile
-//     through the transposing LDS read.
+//   * O^T += V^T . P^T: the score accumulator, rounded to fp16, is the B operand as it is; V^T comes out of the row-major V
+//     tile through the transposing LDS read.
 // Masks cost nothing where every column of the wave sees the whole block and every page of the split is mapped (asked once).
 // Elsewhere a lane compares its column's bounds to 32 token bits per tile. Scores of tokens that are not seen become -inf
-// whatever K holds; their p is an exact 0. Since 0 times NaN or infinity is NaN, V chunks of tokens that do not exist are zeroed
-// on the way, and those with such values in rounds that some column does not see whole; the latter are added behind the block,
-// value by value, for the columns that see their token.
+// whatever K holds; their p is an exact 0. Since 0 times NaN or infinity is NaN, V chunks of tokens that do not exist are
+// zeroed on the way, and those with such values in rounds that some column does not see whole; the latter are added behind the
+// block, value by value, for the columns that see their token.
 //
 // What bounds it: 4096 rows at 0, 8 x 4 heads of 128, take 148-155 us, 0.89-0.93 PFLOP/s of what they need, against 117 at the
 // rate of a large matrix product: the softmax and LDS reads beside the products at the clock that the card keeps up under
 // them, and blocks on the diagonal that are computed whole. Under a window of 1024 they take 93-95 (floor 51): two turns of 18
 // rounds of 64 tokens, 16 of them needed, and about 8 us each to start. 100 rows behind 8000 tokens take 31 (floor 11): 78% of
 // the columns are real, four rounds in 256 workgroups (17 us), 10 for launch and first loads, 28 MB of partials.
-// No gain: tiles that no column of a wave sees left out (the accumulators meet at the branch: 10 to 250 registers spilled); blocks
-// of 64 tokens for eight waves (157 us instead of 150).
+// No gain: tiles that no column of a wave sees left out (the accumulators meet at the branch: 10 to 250 registers spilled);
+// blocks of 64 tokens for eight waves (157 us instead of 150).
 //
 // LDS: rows of 2 D bytes without padding. K chunk q (16 bytes) of row t at q ^ (t & 15) (D 128) or q ^ ((t >> 1) & 7) (D 64),
 // V in 64-byte units, unit u of row t at u ^ (t & 3) (D 128) or u ^ ((t >> 1) & 1) (D 64): reads fall in distinct banks.

@@ -169,8 +169,8 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(const Kv8Append a, int 
 
 // ---------------------------------------------------------------------------------------------------------------
 // Read back: a lane turns eight codes into 16 bytes of an fp16 row, SETS times, 256 chunks apart. Tokens without a page read
-// as zeros. 16001 tokens of 8 heads of 128 take 17 us warm, 20 cold (98 MB, at the rate of a large copy; with one chunk per lane
-// 23); 61 of 4 heads of 64 take 2.6.
+// as zeros. 16001 tokens of 8 heads of 128 take 17 us warm, 20 cold (98 MB, at the rate of a large copy; with one chunk per
+// lane 23); 61 of 4 heads of 64 take 2.6.
 template <int D, int CACHE, int SETS>
 __global__ void __launch_bounds__(256) kv8_read_kernel(const Kv8Read a, long long chunks) {
   constexpr int CPL = D / 8;
