@@ -474,6 +474,19 @@ int dk_attention_window(const void* q, long long q_stride, const int32_t* pos, c
                         size_t workspace_bytes, void* stream);
 
 /*
+ * One decode token over the 8-bit cache: dk_kv8_append_rows of the fused qkv vector [(n_q + 2 n_kv) head_dim] at *pos and
+ * dk_attention_window of its rotated q, in the attention's launches (the workgroup that attends the token's block appends it).
+ * The cache is left as those two leave it and out [n_q * head_dim] is what they give; qkv stays as it was. A *pos outside
+ * [0, max_pos) touches nothing, out included; one at or past max_ctx is appended and attends the tokens before max_ctx.
+ * Workspace as for dk_attention_window with M = 1; qkv and the tables 16-byte aligned, out not overlapping qkv. The 8-bit
+ * counterpart of dk_attention_decode.
+ */
+int dk_attention_kv8_decode(const void* qkv, const float* cos_t, const float* sin_t, int max_pos, const int32_t* pos,
+                            const int32_t* bt, int n_bt, void* kc, void* vc, float* ks, float* vs, int cache, int n_pages,
+                            int page, int n_q, int n_kv, int head_dim, int max_ctx, int window, int sinks, void* out,
+                            void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * INT4 format producer on the GPU: round-to-nearest asymmetric group quantization of fp16 W [N, K] and packing,
  * bit-identical to runtime/quant.py quantize (:42-48, RTN branch of group_params :20-28) + pack (:100-109) +
  * pack_scale_zero (:122-124). Writes packed int32 [N, K/8] and sz fp16 [N, K/G, 2].

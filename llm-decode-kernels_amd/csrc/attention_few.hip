@@ -45,9 +45,21 @@ struct FewShape {
   static constexpr int VW = DPL * ES / 4;       // their words
 };
 
-template <int D, int CACHE, int NW, bool NT>
+// Largest value over the 16 lanes of a row.
+__device__ __forceinline__ float over_lanes16(float v) {
+  v = fmaxf(v, DK_DPP_F32(v, 0xB1, 0xF));   // quad_perm [1,0,3,2]
+  v = fmaxf(v, DK_DPP_F32(v, 0x4E, 0xF));   // quad_perm [2,3,0,1]
+  v = fmaxf(v, DK_DPP_F32(v, 0x141, 0xF));  // row_half_mirror
+  return fmaxf(v, DK_DPP_F32(v, 0x140, 0xF));
+}
+
+// DECODE: one row, whose q is rotated here and whose K / V are appended by the wave that has their tile: it takes the new
+// row's codes into the tile that it has loaded, takes the block's others anew where its scale grows, and stores them. So the
+// append adds no launch and no round trip to the cache, only this wave's arithmetic: in a decode step of 8 layers of 8 x 4
+// heads of 128 at 512 tokens, e4m3, the step takes 342 us, with the append in a launch of its own 358 (at 65536 531 and 535).
+template <int D, int CACHE, int NW, bool NT, bool DECODE>
 __global__ void __launch_bounds__(NW * kWave, 2)
-attn_few_kernel(const WinArgs a) {
+attn_few_kernel(const WinArgs a, const WinDecode dec) {
   using S = FewShape<D, CACHE>;
   constexpr bool F16 = S::F16;
   constexpr int ES = S::ES, KW = S::KW, DPL = S::DPL, VW = S::VW, KS = D / 32;
@@ -79,6 +91,7 @@ attn_few_kernel(const WinArgs a) {
           h8, *reinterpret_cast<const u32x4*>(qh + (F16 ? 32 * k + 8 * g : 64 * (k >> 1) + 16 * g + 8 * (k & 1))));
   }
   __builtin_amdgcn_sched_barrier(0);            // (those loads go out before the position is waited for)
+  if (DECODE && (pos < 0 || pos >= dec.max_pos)) return;  // uniform: nothing is touched
   const Sight mine = sight_of(pos, m, a.window, a.cap);
   const Sight s0 = sight_of(pos, 0, a.window, a.cap), s1 = sight_of(pos, a.M - 1, a.window, a.cap);
   const int ctx = s1.lim + 1;                   // tokens [0, ctx) are read
@@ -86,7 +99,11 @@ attn_few_kernel(const WinArgs a) {
   const int all = (ctx + kFewTile - 1) / kFewTile, wt = min(s0.lo / kFewTile, all);
   const int ns = a.window > 0 ? min((min(a.sinks, ctx) + kFewTile - 1) / kFewTile, wt) : 0;
   const int nt = ns + all - wt;
-  auto tile_at = [&](int i) __attribute__((always_inline)) { return kFewTile * (i < ns ? i : i + (wt - ns)); };
+  // DECODE: one more where the position is past all of them (max_ctx is): a tile that is not attended
+  const int nd = DECODE && pos / kFewTile >= all ? nt + 1 : nt;
+  auto tile_at = [&](int i) __attribute__((always_inline)) {
+    return DECODE && i == nd - 1 ? pos & -kFewTile : kFewTile * (i < ns ? i : i + (wt - ns));
+  };
 
   typedef uint32_t vrow __attribute__((ext_vector_type(VW)));
   struct Tile {
@@ -154,6 +171,130 @@ attn_few_kernel(const WinArgs a) {
       if ((x[i] & 0x7C000000u) == 0x7C000000u) x[i] &= 0xFFFFu;
     }
     return x;
+  };
+  // ---- DECODE: q's rotation, and this token's K and V in the layouts of the operands
+  const bool owner = DECODE && i0 == (nd - 1) % step;  // uniform per wave
+  h8 kn[DECODE ? KS : 1];
+  typedef uint32_t vnew __attribute__((ext_vector_type(DPL / 2)));
+  vnew vn;
+  if constexpr (DECODE) {
+    static_assert(!F16, "the append is the 8-bit one");
+    if (owner) {
+      const f16* kr = a.q + (size_t)(n_q + kvh) * D;
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+        kn[k] = __builtin_bit_cast(h8, *reinterpret_cast<const u32x4*>(kr + 64 * (k >> 1) + 16 * g + 8 * (k & 1)));
+      vn = *reinterpret_cast<const vnew*>(a.q + (size_t)(n_q + a.n_kv + kvh) * D + DPL * c);
+    }
+    // dims 64 (k / 2) + 16 g + 8 (k % 2): the partner D / 2 further is k ^ 2 of the lane (D 128) or k of lane group g ^ 2 (D 64)
+    float cs[2][8], sn[2][8];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const size_t at = (size_t)pos * (D / 2) + (16 * g + 8 * k) % (D / 2);
+#pragma unroll
+      for (int e = 0; e < 8; e += 4) {
+        *reinterpret_cast<f4*>(&cs[k][e]) = *reinterpret_cast<const f4*>(dec.cos_t + at + e);
+        *reinterpret_cast<f4*>(&sn[k][e]) = *reinterpret_cast<const f4*>(dec.sin_t + at + e);
+      }
+    }
+    auto turn = [&](h8* f) __attribute__((always_inline)) {
+      u32x4 own[KS], other[KS];
+#pragma unroll
+      for (int k = 0; k < KS; ++k) own[k] = __builtin_bit_cast(u32x4, f[k]);
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        if constexpr (D == 128) {
+          other[k] = own[k ^ 2];
+        } else {
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const uint32_t u = own[k][w];
+            const auto both = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+            const uint32_t lo = both[0], hi = both[1];
+            other[k][w] = lane < 32 ? hi : lo;
+          }
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+        f[k] = __builtin_bit_cast(h8, rope_slice<D>(own[k], other[k], cs[k & 1], sn[k & 1], D == 128 ? k < 2 : g < 2));
+    };
+    turn(q);
+    if (owner) turn(kn);
+  }
+  auto append = [&](Tile& x) __attribute__((always_inline)) {
+    if constexpr (DECODE) {
+      const int row = pos & 15, page = a.bt[min(pos >> a.log2P, a.n_bt - 1)];
+      if (pos >> a.log2P >= a.n_bt || (unsigned)page >= (unsigned)a.n_pages) return;  // uniform
+      const size_t at = (((size_t)page * a.n_kv + kvh) << a.log2P) + (pos & (P - 1) & ~15);  // the block's first row
+      uint8_t* kb = const_cast<uint8_t*>(a.kc) + at * D + c * D + 16 * g;
+      uint8_t* vb = const_cast<uint8_t*>(a.vc) + at * D + c * DPL;
+      const auto larger = [](float x, float y) { return fmaxf(x, y); };
+      uint32_t tk = 0, tv = 0;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        const u32x4 w = __builtin_bit_cast(u32x4, kn[k]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) tk = kv8_top(w[j], tk);
+      }
+#pragma unroll
+      for (int j = 0; j < DPL / 2; ++j) tv = kv8_top(vn[j], tv);
+      const float need_k = kv8_scale<CACHE>(over_rows((float)as_f16x2(tk)[0], larger));
+      const float need_v = kv8_scale<CACHE>(over_lanes16((float)as_f16x2(tv)[0]));
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        if (((pos >> 4) & 1) != s) continue;  // uniform
+        const float had_k = row ? x.ks[s] : 0.f, had_v = row ? x.vs[s] : 0.f;
+        const float sk = kv8_grown(had_k, need_k), sv = kv8_grown(had_v, need_v);
+        const float ik = 1.0f / sk, iv = 1.0f / sv, big_k = kv8_big<CACHE>(sk), big_v = kv8_big<CACHE>(sv);
+        if (row && had_k != sk) {             // uniform
+          const float ratio = had_k * ik;
+#pragma unroll
+          for (int j = 0; j < KW; ++j) {
+            if (c < row) {
+#pragma unroll
+              for (int w = 0; w < 4; ++w) x.k[s][j][w] = kv8_recode4<CACHE>(x.k[s][j][w], ratio, big_k);
+              *reinterpret_cast<u32x4*>(kb + 64 * j) = x.k[s][j];
+            }
+          }
+        }
+        if (row && had_v != sv) {
+          const float ratio = had_v * iv;
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            if (4 * g + v < row) {
+#pragma unroll
+              for (int w = 0; w < VW; ++w) x.v[s][v][w] = kv8_recode4<CACHE>(x.v[s][v][w], ratio, big_v);
+              *reinterpret_cast<vrow*>(vb + (4 * g + v) * D) = x.v[s][v];
+            }
+          }
+        }
+        if (c == row) {
+#pragma unroll
+          for (int j = 0; j < KW; ++j) {
+            const u32x4 lo = __builtin_bit_cast(u32x4, kn[2 * j]), hi = __builtin_bit_cast(u32x4, kn[2 * j + 1]);
+            x.k[s][j] = u32x4{kv8_code4<CACHE>(lo[0], lo[1], ik, big_k), kv8_code4<CACHE>(lo[2], lo[3], ik, big_k),
+                              kv8_code4<CACHE>(hi[0], hi[1], ik, big_k), kv8_code4<CACHE>(hi[2], hi[3], ik, big_k)};
+            *reinterpret_cast<u32x4*>(kb + 64 * j) = x.k[s][j];
+          }
+        }
+        vrow code;
+#pragma unroll
+        for (int w = 0; w < VW; ++w) code[w] = kv8_code4<CACHE>(vn[2 * w], vn[2 * w + 1], iv, big_v);
+#pragma unroll
+        for (int v = 0; v < 4; ++v)
+          if (4 * g + v == row) {
+            x.v[s][v] = code;
+            *reinterpret_cast<vrow*>(vb + row * D) = code;
+          }
+        x.ks[s] = sk;
+        x.vs[s] = sv;
+        if (lane == 0) {
+          const_cast<float*>(a.ks)[at >> 4] = sk;
+          const_cast<float*>(a.vs)[at >> 4] = sv;
+        }
+      }
+    }
   };
   auto compute = [&](Tile& x, bool first) __attribute__((always_inline)) {
     const int t0 = x.t0;
@@ -284,6 +425,7 @@ attn_few_kernel(const WinArgs a) {
       return;
     }
     asm volatile("");
+    if constexpr (DECODE) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "agent");  // V is read again, the appended row with it
 #pragma unroll
     for (int t = 0; t < DPL; ++t) acc[t] = mfma16x32(__builtin_bit_cast(h8, finite(operand(x, tr, t))), ph, acc[t]);
     // the values left out, for the columns that see their token
@@ -305,7 +447,7 @@ attn_few_kernel(const WinArgs a) {
           if constexpr (F16)
             b = *reinterpret_cast<const u32x2*>(a.vc + 2 * off);
           else
-            b = kv8_decode4<CACHE>(*reinterpret_cast<const uint32_t*>(a.vc + off), a.vs[at >> 4]);
+            b = kv8_decode4<CACHE>(*reinterpret_cast<const uint32_t*>(a.vc + off), s ? x.vs[1] : x.vs[0]);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float f = (float)as_f16x2(b[e >> 1])[e & 1];
@@ -316,16 +458,17 @@ attn_few_kernel(const WinArgs a) {
     }
   };
 
-  if (i0 < nt) {  // uniform per wave
-    if (a.window > 0) pg = lookup(i0);
+  if (i0 < nd) {  // uniform per wave
+    if (a.window > 0 || (DECODE && i0 >= nt)) pg = lookup(i0);
     // the next tile's loads go out ahead of a tile's products; behind the last one every wave's are of tile 0, from a cache
-    auto live = [&](int i) __attribute__((always_inline)) { return i < nt ? i : 0; };
+    auto live = [&](int i) __attribute__((always_inline)) { return i < nd ? i : 0; };
     Tile x = load(i0, pg);
     pg = lookup(live(i0 + step));
 #pragma unroll 1
-    for (int i = i0; i < nt; i += step) {
+    for (int i = i0; i < nd; i += step) {
       const Tile y = load(live(i + step), pg);
       pg = lookup(live(i + 2 * step));
+      if (DECODE && i == nd - 1) append(x);
       compute(x, i == i0);
       x = y;
     }
@@ -379,7 +522,8 @@ attn_few_kernel(const WinArgs a) {
 template <int D>
 __global__ void __launch_bounds__(256)
 attn_few_join_kernel(const f4* __restrict__ part_o, const float2* __restrict__ part_ml, int lhpg, int n_kv, int splits,
-                     float c2, f16* __restrict__ out) {
+                     float c2, f16* __restrict__ out, const int32_t* __restrict__ pos, int max_pos) {
+  if (pos && (*pos < 0 || *pos >= max_pos)) return;  // uniform: nothing was written
   constexpr int T = D / 4, G = 256 / T;
   __shared__ float s_w[kWinMaxSplits];
   __shared__ float s_l;
@@ -445,8 +589,8 @@ FewPlan few_plan(int M, int n_kv, int D, int max_ctx, int window, int sinks) {
   return {waves, (int)((tiles + per - 1) / per)};
 }
 
-template <int D, int CACHE>
-void launch(const WindowAttn& w, WinArgs a, hipStream_t st) {
+template <int D, int CACHE, bool DECODE>
+void launch(const WindowAttn& w, WinArgs a, const WinDecode& dec, hipStream_t st) {
   a.part_ml = (float2*)(a.part_o + (size_t)w.splits * w.n_kv * kFewCols * (D / 4));
   const FewPlan p = few_plan(w.M, w.n_kv, D, w.max_ctx, w.window, w.sinks);
   // K and V that fill half of the last cache (256 MB) are not kept there for the next call. (8 x 4 heads of 128: one token at
@@ -454,24 +598,29 @@ void launch(const WindowAttn& w, WinArgs a, hipStream_t st) {
   const long long bytes = win_tokens(w.M, w.max_ctx, w.window, w.sinks) * w.n_kv * 2 * D * (CACHE == kCacheF16 ? 2 : 1);
   const dim3 grid(w.n_kv, w.splits);
   if (p.waves == 4)
-    hipLaunchKernelGGL((attn_few_kernel<D, CACHE, 4, false>), grid, dim3(4 * kWave), 0, st, a);
+    hipLaunchKernelGGL((attn_few_kernel<D, CACHE, 4, false, DECODE>), grid, dim3(4 * kWave), 0, st, a, dec);
   else if (bytes < (128LL << 20))
-    hipLaunchKernelGGL((attn_few_kernel<D, CACHE, 8, false>), grid, dim3(8 * kWave), 0, st, a);
+    hipLaunchKernelGGL((attn_few_kernel<D, CACHE, 8, false, DECODE>), grid, dim3(8 * kWave), 0, st, a, dec);
   else
-    hipLaunchKernelGGL((attn_few_kernel<D, CACHE, 8, true>), grid, dim3(8 * kWave), 0, st, a);
+    hipLaunchKernelGGL((attn_few_kernel<D, CACHE, 8, true, DECODE>), grid, dim3(8 * kWave), 0, st, a, dec);
   if (w.splits > 1)
     hipLaunchKernelGGL(attn_few_join_kernel<D>, dim3(w.n_kv, (unsigned)(w.M << a.lhpg)), dim3(256), 0, st,
-                       (const f4*)a.part_o, a.part_ml, a.lhpg, w.n_kv, w.splits, a.c2, (f16*)w.out);
+                       (const f4*)a.part_o, a.part_ml, a.lhpg, w.n_kv, w.splits, a.c2, (f16*)w.out,
+                       DECODE ? a.pos : nullptr, dec.max_pos);
 }
 
 template <int D>
-void launch_cache(const WindowAttn& w, const WinArgs& a, hipStream_t st) {
-  if (w.cache == kCacheF16)
-    launch<D, kCacheF16>(w, a, st);
+void launch_cache(const WindowAttn& w, const WinArgs& a, const WinDecode* dec, hipStream_t st) {
+  if (dec && w.cache == kCacheInt8)
+    launch<D, kCacheInt8, true>(w, a, *dec, st);
+  else if (dec)
+    launch<D, kCacheE4m3, true>(w, a, *dec, st);
+  else if (w.cache == kCacheF16)
+    launch<D, kCacheF16, false>(w, a, {}, st);
   else if (w.cache == kCacheInt8)
-    launch<D, kCacheInt8>(w, a, st);
+    launch<D, kCacheInt8, false>(w, a, {}, st);
   else
-    launch<D, kCacheE4m3>(w, a, st);
+    launch<D, kCacheE4m3, false>(w, a, {}, st);
 }
 
 }  // namespace
@@ -480,11 +629,11 @@ int attention_few_splits(int M, int n_kv, int D, int max_ctx, int window, int si
   return few_plan(M, n_kv, D, max_ctx, window, sinks).splits;
 }
 
-void launch_attention_few(const WindowAttn& w, const WinArgs& a, hipStream_t st) {
+void launch_attention_few(const WindowAttn& w, const WinArgs& a, const WinDecode* dec, hipStream_t st) {
   if (w.head_dim == 64)
-    launch_cache<64>(w, a, st);
+    launch_cache<64>(w, a, dec, st);
   else
-    launch_cache<128>(w, a, st);
+    launch_cache<128>(w, a, dec, st);
 }
 
 }  // namespace dk

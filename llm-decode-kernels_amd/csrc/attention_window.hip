@@ -668,20 +668,21 @@ void launch_shape(const WinArgs& a, long long cols, hipStream_t st) {
     hipLaunchKernelGGL((attn_window_kernel<D, CACHE, CW, KVS, BT, false>), grid, block, 0, st, a);
 }
 
-template <int D, int CACHE>
-void launch(const WindowAttn& w, hipStream_t st) {
+template <int D>
+WinArgs window_args(const WindowAttn& w) {
   int lhpg = 0;
   while ((w.n_kv << lhpg) < w.n_q) ++lhpg;
-  const long long cols = (long long)w.M << lhpg, waves = (cols + 31) / 32;
+  const long long waves = (((long long)w.M << lhpg) + 31) / 32;
   float4* part_o = (float4*)w.ws;
-  const WinArgs a{(const f16*)w.q, w.q_stride, w.pos, w.bt, (const uint8_t*)w.kc, (const uint8_t*)w.vc, w.ks, w.vs, w.n_pages,
+  return {(const f16*)w.q, w.q_stride, w.pos, w.bt, (const uint8_t*)w.kc, (const uint8_t*)w.vc, w.ks, w.vs, w.n_pages,
                   w.n_bt, w.log2P, w.n_kv, lhpg, w.M, (int)min((long long)w.max_ctx, (long long)w.n_bt << w.log2P), w.window,
                   w.sinks, w.splits, (float)(1.4426950408889634 / sqrt((double)D)), (f16*)w.out, part_o,
                   (float2*)(part_o + (size_t)w.splits * w.n_kv * waves * 8 * D)};
-  if (win_few(w.M, w.n_q, w.n_kv, w.log2P)) {
-    launch_attention_few(w, a, st);
-    return;
-  }
+}
+
+template <int D, int CACHE>
+void launch(const WindowAttn& w, const WinArgs& a, hipStream_t st) {
+  const long long cols = (long long)w.M << a.lhpg, waves = (cols + 31) / 32;
   const WinShape s = win_shape(w.M, w.n_q, w.n_kv, D, w.max_ctx, w.window, w.sinks);
   if (s.cw == 2)
     launch_shape<D, CACHE, 2, 4, 32>(a, cols, st);
@@ -693,27 +694,38 @@ void launch(const WindowAttn& w, hipStream_t st) {
     launch_shape<D, CACHE, 4, 2, 64>(a, cols, st);
   if (w.splits > 1)
     hipLaunchKernelGGL(attn_window_join_kernel<D>, dim3(w.n_kv, (unsigned)(waves * (D / 8 / kWinJoinRows))),
-                       dim3(kWinJoinRows * kWave), 0, st, part_o, a.part_ml, (int)cols, lhpg, w.n_kv, w.splits, a.c2,
+                       dim3(kWinJoinRows * kWave), 0, st, a.part_o, a.part_ml, (int)cols, a.lhpg, w.n_kv, w.splits, a.c2,
                        (f16*)w.out);
 }
 
 template <int D>
-void launch_cache(const WindowAttn& w, hipStream_t st) {
-  if (w.cache == kCacheF16)
-    launch<D, kCacheF16>(w, st);
+void launch_cache(const WindowAttn& w, const WinDecode* dec, hipStream_t st) {
+  const WinArgs a = window_args<D>(w);
+  if (dec || win_few(w.M, w.n_q, w.n_kv, w.log2P))
+    launch_attention_few(w, a, dec, st);
+  else if (w.cache == kCacheF16)
+    launch<D, kCacheF16>(w, a, st);
   else if (w.cache == kCacheInt8)
-    launch<D, kCacheInt8>(w, st);
+    launch<D, kCacheInt8>(w, a, st);
   else
-    launch<D, kCacheE4m3>(w, st);
+    launch<D, kCacheE4m3>(w, a, st);
 }
 
 }  // namespace
 
 void launch_attention_window(const WindowAttn& a, hipStream_t st) {
   if (a.head_dim == 64)
-    launch_cache<64>(a, st);
+    launch_cache<64>(a, nullptr, st);
   else
-    launch_cache<128>(a, st);
+    launch_cache<128>(a, nullptr, st);
+}
+
+void launch_attention_kv8_decode(const WindowAttn& a, const float* cos_t, const float* sin_t, int max_pos, hipStream_t st) {
+  const WinDecode dec{cos_t, sin_t, max_pos};
+  if (a.head_dim == 64)
+    launch_cache<64>(a, &dec, st);
+  else
+    launch_cache<128>(a, &dec, st);
 }
 
 }  // namespace dk

@@ -71,8 +71,14 @@ constexpr int kFewTile = 32;
 // Whether the kernel of few columns takes a call. Pages of fewer than 16 tokens are left to the other one.
 inline bool win_few(int M, int n_q, int n_kv, int log2P) { return (long long)M * (n_q / n_kv) <= kFewCols && log2P >= 4; }
 
-// attention_few.hip: the splits that a call can use, and its launch.
+// The RoPE of one token and its append, in front of its attention (8-bit caches, one row; a.q is then the fused qkv vector).
+struct WinDecode {
+  const float* cos_t;
+  const float* sin_t;
+  int max_pos;
+};
+// attention_few.hip: the splits that a call can use, and its launch (dec null: attention alone).
 int attention_few_splits(int M, int n_kv, int head_dim, int max_ctx, int window, int sinks);
-void launch_attention_few(const WindowAttn& w, const WinArgs& a, hipStream_t st);
+void launch_attention_few(const WindowAttn& w, const WinArgs& a, const WinDecode* dec, hipStream_t st);
 
 }  // namespace dk

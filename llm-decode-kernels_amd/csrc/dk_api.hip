@@ -975,6 +975,23 @@ size_t dk_attention_window_workspace_bytes(int M, int n_q, int n_kv, int head_di
   return s > 1 ? (size_t)s * dk::attention_window_part_bytes(M, n_q, n_kv, head_dim) : 0;
 }
 
+// Splits that a workspace holds, and whether it is one that the call can use.
+static int window_splits(const char* what, const void* q, size_t q_bytes, const void* out, size_t out_bytes, void* workspace,
+                         size_t workspace_bytes, int M, int n_q, int n_kv, int head_dim, int max_ctx, int window, int sinks,
+                         int cache, int* splits) {
+  if (ranges_overlap(q, q_bytes, out, out_bytes)) return fail(DK_ERR_DOMAIN, "%s: out must not overlap q", what);
+  *splits = 1;
+  if (workspace == nullptr) return DK_OK;
+  if (!aligned16(workspace)) return fail(DK_ERR_ALIGN, "%s: workspace must be 16B aligned", what);
+  const size_t part = dk::attention_window_part_bytes(M, n_q, n_kv, head_dim);
+  *splits = dk::attention_window_splits(M, n_q, n_kv, head_dim, max_ctx, window, sinks, cache);
+  if (workspace_bytes / part < (size_t)*splits) *splits = workspace_bytes / part < 2 ? 1 : (int)(workspace_bytes / part);
+  const size_t used = *splits > 1 ? (size_t)*splits * part : 0;
+  if (used > 0 && (ranges_overlap(workspace, used, q, q_bytes) || ranges_overlap(workspace, used, out, out_bytes)))
+    return fail(DK_ERR_DOMAIN, "%s: workspace must not overlap q or out", what);
+  return DK_OK;
+}
+
 int dk_attention_window(const void* q, long long q_stride, const int32_t* pos, const int32_t* bt, int n_bt, const void* kc,
                         const void* vc, const float* ks, const float* vs, int cache, int n_pages, int page, int n_q, int n_kv,
                         int head_dim, int M, int max_ctx, int window, int sinks, void* out, void* workspace,
@@ -1008,22 +1025,46 @@ int dk_attention_window(const void* q, long long q_stride, const int32_t* pos, c
   if (!aligned4(pos) || !aligned4(bt) || !aligned4(ks) || !aligned4(vs))
     return fail(DK_ERR_ALIGN, "attention_window: pos, bt, ks and vs must be 4B aligned");
   const size_t q_bytes = (size_t)((M - 1) * q_stride + row) * 2, out_bytes = (size_t)(M * row) * 2;
-  if (ranges_overlap(q, q_bytes, out, out_bytes))
-    return fail(DK_ERR_DOMAIN, "attention_window: out must not overlap q");
   int splits = 1;
-  if (workspace != nullptr) {
-    if (!aligned16(workspace)) return fail(DK_ERR_ALIGN, "attention_window: workspace must be 16B aligned");
-    const size_t part = dk::attention_window_part_bytes(M, n_q, n_kv, head_dim);
-    splits = dk::attention_window_splits(M, n_q, n_kv, head_dim, max_ctx, window, sinks, cache);
-    if (workspace_bytes / part < (size_t)splits) splits = workspace_bytes / part < 2 ? 1 : (int)(workspace_bytes / part);
-    const size_t used = splits > 1 ? (size_t)splits * part : 0;
-    if (used > 0 && (ranges_overlap(workspace, used, q, q_bytes) || ranges_overlap(workspace, used, out, out_bytes)))
-      return fail(DK_ERR_DOMAIN, "attention_window: workspace must not overlap q or out");
-  }
+  const int rc = window_splits("attention_window", q, q_bytes, out, out_bytes, workspace, workspace_bytes, M, n_q, n_kv,
+                               head_dim, max_ctx, window, sinks, cache, &splits);
+  if (rc != DK_OK) return rc;
   clear_error();
   dk::launch_attention_window({q, q_stride, pos, bt, n_bt, kc, vc, ks, vs, cache, n_pages, ilog2(page), n_q, n_kv, head_dim,
                                M, max_ctx, window, sinks, out, splits, workspace}, (hipStream_t)stream);
   return launched("attention_window");
+}
+
+int dk_attention_kv8_decode(const void* qkv, const float* cos_t, const float* sin_t, int max_pos, const int32_t* pos,
+                            const int32_t* bt, int n_bt, void* kc, void* vc, float* ks, float* vs, int cache, int n_pages,
+                            int page, int n_q, int n_kv, int head_dim, int max_ctx, int window, int sinks, void* out,
+                            void* workspace, size_t workspace_bytes, void* stream) {
+  const char* what = "attention_kv8_decode";
+  if (!qkv || !cos_t || !sin_t || !pos || !bt || !kc || !vc || !ks || !vs || !out)
+    return fail(DK_ERR_NULL, "%s: null pointer argument", what);
+  int rc = check_kv8(what, cache, head_dim, n_kv, page, n_pages, n_bt);
+  if (rc != DK_OK) return rc;
+  if (max_pos < 1) return fail(DK_ERR_SHAPE, "%s: empty rope table", what);
+  if (max_ctx < 1 || max_ctx > dk::kWindowMaxCtx)
+    return fail(DK_ERR_DOMAIN, "%s: max_ctx must be 1..%d, got %d", what, dk::kWindowMaxCtx, max_ctx);
+  if (window < 0 || window > dk::kWindowMaxCtx || sinks < 0 || sinks > dk::kWindowMaxCtx)
+    return fail(DK_ERR_DOMAIN, "%s: window and sinks must be 0..%d, got %d and %d", what, dk::kWindowMaxCtx, window, sinks);
+  if (!window_sizes(1, n_q, n_kv, head_dim, max_ctx, window, sinks, cache))
+    return fail(DK_ERR_SHAPE, "heads-per-group must be 1/2/4/8 (n_q=%d n_kv=%d)", n_q, n_kv);
+  if (!aligned16(qkv) || !aligned16(cos_t) || !aligned16(sin_t) || !aligned16(kc) || !aligned16(vc) || !aligned16(out))
+    return fail(DK_ERR_ALIGN, "%s: qkv, the tables, kc, vc and out must be 16B aligned", what);
+  if (!aligned4(pos) || !aligned4(bt) || !aligned4(ks) || !aligned4(vs))
+    return fail(DK_ERR_ALIGN, "%s: pos, bt, ks and vs must be 4B aligned", what);
+  const size_t q_bytes = ((size_t)n_q + 2 * (size_t)n_kv) * head_dim * 2, out_bytes = (size_t)n_q * head_dim * 2;
+  int splits = 1;
+  rc = window_splits(what, qkv, q_bytes, out, out_bytes, workspace, workspace_bytes, 1, n_q, n_kv, head_dim, max_ctx, window,
+                     sinks, cache, &splits);
+  if (rc != DK_OK) return rc;
+  clear_error();
+  dk::launch_attention_kv8_decode({qkv, (long long)n_q * head_dim, pos, bt, n_bt, kc, vc, ks, vs, cache, n_pages, ilog2(page),
+                                   n_q, n_kv, head_dim, 1, max_ctx, window, sinks, out, splits, workspace},
+                                  cos_t, sin_t, max_pos, (hipStream_t)stream);
+  return launched(what);
 }
 
 int dk_quantize_w4(const void* w, void* packed, void* sz, int N, int K, int group, int clip, void* stream) {

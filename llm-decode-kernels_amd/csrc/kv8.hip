@@ -81,41 +81,34 @@ __device__ __forceinline__ void append_block(const Kv8Append& a, long long pos, 
 #pragma unroll
   for (int i = 0; i < NP; ++i) {
     if (!is_v && a.cos_t) rotate(lo[i], hi[i], turn[i]);
+    uint32_t most = 0;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      uint32_t m = ((j < 8 ? lo[i][j / 2] : hi[i][j / 2 - 4]) >> (16 * (j & 1))) & 0x7FFFu;
-      m = m == 0x7C00u ? 0x7BFFu : m;  // an infinity is stored as the largest fp16 value
-      if (m < 0x7C00u && mine[i]) top = max(top, m);
-    }
+    for (int j = 0; j < 4; ++j) most = kv8_top(hi[i][j], kv8_top(lo[i][j], most));
+    top = max(top, mine[i] ? most : 0u);
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, kWave));
   const float need = kv8_scale<CACHE>((float)as_f16x2(top)[0]);
-  // (a scale that this library did not write is not taken further than its own go)
-  const float s = had > need && had <= kKv8MaxScale ? had : need, inv = 1.0f / s;
-  using Codes = Kv8Codes<CACHE>;
-  const float big = s == Codes::top_scale ? Codes::top_code : Codes::most;
+  const float s = kv8_grown(had, need), inv = 1.0f / s, big = kv8_big<CACHE>(s);
   const bool grows = first < pos && had != s;  // uniform: the rows before pos take the new scale
   const float ratio = had * inv;
-  auto put = [&](uint8_t* at, const u32x4& x, float by) __attribute__((always_inline)) {
-    float v[8];
-    unpack8(x, v);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] *= by;
-    const float v0[4] = {v[0], v[1], v[2], v[3]}, v1[4] = {v[4], v[5], v[6], v[7]};
-    *reinterpret_cast<u32x2*>(at) = u32x2{kv8_encode4<CACHE>(v0, big), kv8_encode4<CACHE>(v1, big)};
+  auto put = [&](uint8_t* at, const u32x4& x) __attribute__((always_inline)) {
+    *reinterpret_cast<u32x2*>(at) = u32x2{kv8_code4<CACHE>(x[0], x[1], inv, big), kv8_code4<CACHE>(x[2], x[3], inv, big)};
+  };
+  auto again = [&](uint8_t* at) __attribute__((always_inline)) {
+    const u32x2 w = *reinterpret_cast<const u32x2*>(at);
+    *reinterpret_cast<u32x2*>(at) = u32x2{kv8_recode4<CACHE>(w[0], ratio, big), kv8_recode4<CACHE>(w[1], ratio, big)};
   };
 #pragma unroll
   for (int i = 0; i < NP; ++i) {
     const int row = RPP * i + lane / LPR;
     uint8_t* at = codes + row * D;
     if (mine[i]) {
-      put(at, lo[i], inv);
-      put(at + D / 2, hi[i], inv);
+      put(at, lo[i]);
+      put(at + D / 2, hi[i]);
     } else if (grows && first + row < pos) {
-      const u32x2 x = *reinterpret_cast<const u32x2*>(at), y = *reinterpret_cast<const u32x2*>(at + D / 2);
-      put(at, kv8_decode8<CACHE>(x, 1.0f), ratio);  // (by 1: the codes themselves)
-      put(at + D / 2, kv8_decode8<CACHE>(y, 1.0f), ratio);
+      again(at);
+      again(at + D / 2);
     }
   }
   if (lane == 0) *scale = s;

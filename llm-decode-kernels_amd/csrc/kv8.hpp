@@ -78,4 +78,36 @@ __device__ __forceinline__ u32x4 kv8_decode8(u32x2 w, float s) {
   return u32x4{lo[0], lo[1], hi[0], hi[1]};
 }
 
+// The scale of a block that had `had` (0: no rows ahead of the new ones) and whose new rows need `need`: the larger one. (A
+// scale that this library did not write is not taken further than its own go.)
+__device__ __forceinline__ float kv8_grown(float had, float need) { return had > need && had <= kKv8MaxScale ? had : need; }
+template <int CACHE>
+__device__ __forceinline__ float kv8_big(float s) {  // the largest code at scale s
+  return s == Kv8Codes<CACHE>::top_scale ? Kv8Codes<CACHE>::top_code : Kv8Codes<CACHE>::most;
+}
+// The largest finite magnitude of eight fp16 values, as fp16 bits (an infinity is stored as the largest fp16 value, NaN counts
+// for nothing), and of fewer.
+__device__ __forceinline__ uint32_t kv8_top(uint32_t w, uint32_t top) {
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    uint32_t m = (w >> (16 * e)) & 0x7FFFu;
+    m = m == 0x7C00u ? 0x7BFFu : m;
+    top = max(top, m < 0x7C00u ? m : 0u);
+  }
+  return top;
+}
+// Codes of four fp16 values times `by`.
+template <int CACHE>
+__device__ __forceinline__ uint32_t kv8_code4(uint32_t lo, uint32_t hi, float by, float big) {
+  const f16x2 a = as_f16x2(lo), b = as_f16x2(hi);
+  const float y[4] = {(float)a[0] * by, (float)a[1] * by, (float)b[0] * by, (float)b[1] * by};
+  return kv8_encode4<CACHE>(y, big);
+}
+// Codes at another scale, `ratio` the old one over the new.
+template <int CACHE>
+__device__ __forceinline__ uint32_t kv8_recode4(uint32_t w, float ratio, float big) {
+  const u32x2 x = kv8_decode4<CACHE>(w, 1.0f);  // (times 1: the codes themselves)
+  return kv8_code4<CACHE>(x[0], x[1], ratio, big);
+}
+
 }  // namespace dk

@@ -291,6 +291,8 @@ struct WindowAttn {
 int attention_window_splits(int M, int n_q, int n_kv, int head_dim, int max_ctx, int window, int sinks, int cache);
 size_t attention_window_part_bytes(int M, int n_q, int n_kv, int head_dim);
 void launch_attention_window(const WindowAttn& a, hipStream_t st);
+// One token (M 1, an 8-bit cache): its RoPE and append in front of its attention; q is the fused qkv vector.
+void launch_attention_kv8_decode(const WindowAttn& a, const float* cos_t, const float* sin_t, int max_pos, hipStream_t st);
 
 void launch_quantize_w4(const void* w, void* packed, void* sz, int N, int K, int log2G, int clip, hipStream_t st);
 

@@ -63,6 +63,8 @@ SIGNATURES = {
     "dk_kv8_append_rows": ([_P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _P, _L, _I, _I, _I, _I, _I, _I, _I, _I, _P], _I),
     "dk_kv8_read": ([_P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P, _P], _I),
     "dk_attention_window_workspace_bytes": ([_I, _I, _I, _I, _I, _I, _I, _I], _Z),
+    "dk_attention_kv8_decode": ([_P, _P, _P, _I, _P, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P, _Z,
+                                 _P], _I),
     "dk_attention_window": ([_P, _L, _P, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P, _P, _Z, _P],
                             _I),
     "dk_quantize_w4": ([_P, _P, _P, _I, _I, _I, _I, _P], _I),
@@ -169,6 +171,8 @@ _APPEND_SPEC = _kv8_specs(("qkv", torch.float16), ("cos_t", torch.float32), ("si
                           *_CACHE_SPEC)
 _READ_SPEC = _kv8_specs(*_CACHE_SPEC, ("k_out", torch.float16), ("v_out", torch.float16))
 _KV8_SPEC = _kv8_specs(("pos", torch.int32), *_CACHE_SPEC, ("out", torch.float16))
+_DECODE_SPEC = _kv8_specs(("qkv", torch.float16), ("cos_t", torch.float32), ("sin_t", torch.float32), ("pos", torch.int32),
+                          *_CACHE_SPEC, ("out", torch.float16))
 _WINDOW_SPEC = (("pos", torch.int32), ("bt", torch.int32), ("kc", torch.float16), ("vc", torch.float16), ("ks", torch.float32),
                 ("vs", torch.float32), ("out", torch.float16))
 
@@ -907,6 +911,24 @@ class DecodeKernels:
         dtype, cache = self._kv8_cache("attention_kv8", kc, vc, ks, vs)
         self._attention_window("attention_kv8", _KV8_SPEC[kc.dtype], q, pos, bt, kc, vc, ks, vs, dtype, cache, max_ctx, out,
                                window, sinks, workspace)
+
+    def attention_kv8_decode(self, qkv, cos_t, sin_t, pos, bt, kc, vc, ks, vs, n_q, n_kv, max_ctx, out, window=0, sinks=0,
+                             workspace=None):
+        """kv8_append_rows of one token, the fused qkv vector [(n_q + 2 n_kv) * D] (which stays as it is), and attention_kv8
+        of its rotated q, in the launches of the attention. out [n_q * D]; workspace as for attention_kv8 with M = 1."""
+        what, dev = "attention_kv8_decode", qkv.get_device()
+        dtype, cache = self._kv8_cache(what, kc, vc, ks, vs)
+        p_qkv, p_cos, p_sin, p_pos, p_bt, p_kc, p_vc, p_ks, p_vs, p_out = _addresses(
+            what, dev, _DECODE_SPEC[kc.dtype], qkv, cos_t, sin_t, pos, bt, kc, vc, ks, vs, out)
+        D = cache[3]
+        if cos_t is None or sin_t is None or cos_t.dim() != 2 or cos_t.size(1) * 2 != D or sin_t.shape != cos_t.shape:
+            raise RuntimeError(f"{what}: cos_t and sin_t must be [max_pos, D/2]")
+        if qkv.numel() != (n_q + 2 * n_kv) * D or cache[1] != n_kv or out.numel() != n_q * D or pos.numel() < 1:
+            raise RuntimeError(f"{what}: qkv must hold (n_q + 2 n_kv) * D values, out n_q * D and pos one")
+        p_ws, ws_bytes = _workspace(what, dev, workspace)
+        self._call_on(dev, self.lib.dk_attention_kv8_decode, p_qkv, p_cos, p_sin, cos_t.size(0), p_pos, p_bt, bt.numel(), p_kc,
+                      p_vc, p_ks, p_vs, dtype, cache[0], cache[2], *_ints(n_q, n_kv), D, *_ints(max_ctx, window, sinks), p_out,
+                      p_ws, ws_bytes)
 
     # runtime/quant.py:42-48,100-124 on the GPU
     def quantize_w4(self, w, packed, sz, group, clip=False):

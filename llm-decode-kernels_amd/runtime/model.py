@@ -69,7 +69,8 @@ class DecodeConfig:
     device: str = "cuda"
     seed: int = 0            # block-table permutation seed
     fused_attention: bool = True   # rope_epilogue off: dk_attention_decode (RoPE + append in the split kernel) vs
-                                   # rope_append + paged_attention
+                                   # rope_append + paged_attention; kv of codes: dk_attention_kv8_decode vs
+                                   # kv8_append_rows + attention_kv8
     argmax_split_min_v: int = 16384  # vocabularies at least this large pick the next token with the multi-workgroup
                                      # argmax (dk_argmax_advance_split); smaller ones with the one-workgroup kernel
     fused_gemv: bool = True        # residual + RMSNorm (and the embedding gather) computed inside the INT4 GEMV that
@@ -538,6 +539,11 @@ class Model:
     def attention(self, li):
         kc, vc = self.kv[li, 0], self.kv[li, 1]
         if self.window_attention:
+            if self.kv8 and self.cfg.fused_attention:
+                self.K.attention_kv8_decode(self.qkv, self.cos, self.sin, self.pos, self.bt, kc, vc, *self.kv_scale[li],
+                                            self.n_q, self.n_kv, self.ctx_cap, self.attn, self.cfg.window, self.cfg.sinks,
+                                            self.attn_ws)
+                return
             if not self.rope_epilogue:
                 self.append_rows(li, self.qkv.view(1, -1))
             self.attend_rows(li, self.qkv[: self.n_q * self.D].view(1, -1), self.ctx_cap, self.attn.view(1, -1), self.attn_ws)

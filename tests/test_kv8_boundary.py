@@ -75,6 +75,25 @@ def test_attention_window_refusals(lib, kw, code, msg):
     refused(lib, "dk_attention_window", WIN, kw, code, msg)
 
 
+DEC = dict(qkv=AT[0], cos=AT[1], sin=AT[2], max_pos=64, pos=AT[3], bt=AT[4], n_bt=8, kc=AT[5], vc=AT[6], ks=AT[7], vs=AT[8],
+           cache=1, n_pages=8, page=16, n_q=8, n_kv=2, head_dim=64, max_ctx=64, window=0, sinks=0, out=AT[9], ws=None,
+           ws_bytes=0)
+
+
+@pytest.mark.parametrize("kw,code,msg", [
+    (dict(qkv=None), 1, "null"), (dict(cos=None), 1, "null"), (dict(sin=None), 1, "null"), (dict(ks=None), 1, "null"),
+    (dict(out=None), 1, "null"), (dict(cache=0), 4, "int8 or e4m3"), (dict(head_dim=96), 3, "head_dim"),
+    (dict(n_kv=0), 3, "kv head count"), (dict(page=8), 4, "power of two >= 16"), (dict(n_pages=0), 3, "empty"),
+    (dict(max_pos=0), 3, "empty rope"), (dict(max_ctx=0), 4, "max_ctx"), (dict(max_ctx=(1 << 30) + 1), 4, "max_ctx"),
+    (dict(window=-1), 4, "window and sinks"), (dict(sinks=(1 << 30) + 1), 4, "window and sinks"),
+    (dict(n_q=6), 3, "heads-per-group"), (dict(n_q=32), 3, "heads-per-group"), (dict(qkv=AT[0] + 8), 2, "16B"),
+    (dict(cos=AT[1] + 4), 2, "16B"), (dict(out=AT[9] + 2), 2, "16B"), (dict(bt=AT[4] + 2), 2, "4B"),
+    (dict(out=AT[0] + 1024), 4, "overlap q"), (dict(ws=AT[9] + 8, ws_bytes=64), 2, "workspace must be 16B"),
+    (dict(max_ctx=1 << 20, ws=AT[0] + 160, ws_bytes=1 << 24), 4, "workspace must not overlap")])
+def test_attention_kv8_decode_refusals(lib, kw, code, msg):
+    refused(lib, "dk_attention_kv8_decode", DEC, kw, code, msg)
+
+
 def test_attention_window_workspace(lib):
     need = lib.dk_attention_window_workspace_bytes
     for bad in ((0, 8, 2, 128, 100, 0, 0, 0), (20, 6, 2, 128, 100, 0, 0, 0), (20, 8, 2, 96, 100, 0, 0, 0),
@@ -101,6 +120,8 @@ def test_op_module_refusals_on_the_cpu(lib):
         K.attention_window(h(3, 2, 64), pos, bt, h(4, 2, 16, 64), h(4, 2, 16, 64), 10, h(3, 128))
     with pytest.raises(RuntimeError, match="contiguous CUDA tensor"):
         K.attention_kv8(h(3, 2, 64), pos, bt, c8, c8, s8, s8, 10, h(3, 128))
+    with pytest.raises(RuntimeError, match="contiguous CUDA tensor"):
+        K.attention_kv8_decode(h(384), f(8, 32), f(8, 32), pos, bt, c8, c8, s8, s8, 2, 2, 10, h(128))
     with pytest.raises(RuntimeError, match="int8 or float8_e4m3fn"):
         K.attention_kv8(h(3, 2, 64), pos, bt, h(4, 2, 16, 64), h(4, 2, 16, 64), s8, s8, 10, h(3, 128))
     with pytest.raises(RuntimeError, match="must be fp16"):

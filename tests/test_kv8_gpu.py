@@ -602,6 +602,142 @@ def test_append_read_and_attend_as_a_sequence(K, dtype):
         assert torch.equal(got.cpu().double(), torch.stack([val[a, :, s] for a, s in cells]))
 
 
+def decode(K, row, cos, sin, pos, bt, c, n_q, n_kv, cap, window=0, sinks=0, ws=True, fill=float("nan")):
+    """attention_kv8_decode, in place in the cache c."""
+    D = c[0].size(3)
+    out = torch.full((n_q * D,), fill, dtype=torch.half, device=DEV)
+    need = K.attention_window_workspace_bytes(1, n_q, n_kv, D, cap, window, sinks, c[0].dtype)
+    w = torch.full((need,), 255, dtype=torch.uint8, device=DEV) if need and ws else None
+    K.attention_kv8_decode(row, cos, sin, i32(pos), bt, *c, n_q, n_kv, cap, out, window, sinks, w)
+    return out
+
+
+@pytest.mark.parametrize("dtype", CODES, ids=name)
+@pytest.mark.parametrize("n_q,n_kv,D,page,start,cap,window,sinks", [
+    (32, 4, 64, 16, 0, 64, 0, 0), (32, 8, 128, 16, 290, 350, 0, 0), (8, 1, 128, 32, 500, 5000, 0, 0),
+    (4, 4, 64, 64, 1000, 1 << 17, 0, 0), (2, 1, 128, 16, 300, 1 << 22, 0, 0), (8, 2, 128, 16, 250, 400, 40, 3),
+    (8, 4, 64, 32, 25, 100, 1, 0), (4, 2, 64, 16, 700, 5000, 200, 40), (2, 2, 128, 128, 90, 200, 1000, 4)])
+def test_decode_appends_and_attends(K, dtype, n_q, n_kv, D, page, start, cap, window, sinks):
+    """Tokens one by one, their sizes going up and down so that blocks grow in the middle: the cache bit for bit the
+    reference's, attention within its bound, with and without a workspace, qkv and the pages of others as they were."""
+    g, n = gen(start + D + page), 40
+    caches, scales, bt, _ = paged_kv(start + n, n_kv, D, page, dtype, g)
+    ref = [*caches, *scales]
+    size = torch.exp2(torch.randint(-12, 7, (n, 1), generator=g).float())
+    size[:3] = 1.0
+    rows = (torch.randn(n, (n_q + 2 * n_kv) * D, generator=g) * size).half()
+    rows[:, :n_q * D] = torch.randn(n, n_q * D, generator=g).half()
+    cos, sin = rope_tables(start + n, D)
+    cosd, sind, btd, rd, *c = dev(cos, sin, bt, rows, *ref)
+    other = [t.clone() for t in c]
+    for i in range(n):
+        t = start + i
+        q, ref = R.append(rows[i:i + 1], cos, sin, t, bt, *ref, n_q)
+        out = decode(K, rd[i], cosd, sind, t, btd, c, n_q, n_kv, cap, window, sinks)
+        alone = decode(K, rd[i], cosd, sind, t, btd, other, n_q, n_kv, cap, window, sinks, ws=False)
+        if i in (0, 1, 15, 16, 17, 31, 39):
+            want, bound = R.attention(q, t, bt, R.values(ref[0], ref[2]), R.values(ref[1], ref[3]), cap, window, sinks)
+            R.within(out.view(1, -1), want, bound)
+            R.within(alone.view(1, -1), want, bound)
+        assert all(same(a, b) for a, b in zip(c, ref)), t
+    assert all(same(a, b) for a, b in zip(other, ref)) and same(rd, rows)
+
+
+@pytest.mark.parametrize("dtype", CODES, ids=name)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("pos,cap,window", [(5, 100, 0), (31, 100, 0), (200, 4000, 0), (200, 4000, 30), (48, 100, 1)])
+def test_decode_of_values_that_are_not_finite(K, dtype, D, pos, cap, window):
+    """Infinities and NaN in the new K and V, and NaN in codes behind the window: what append and attention give."""
+    n_q, n_kv, page = 8, 2, 16
+    caches, scales, bt, _ = paged_kv(pos + 1, n_kv, D, page, dtype, gen(pos + D))
+    if dtype == torch.float8_e4m3fn and window:
+        for t in (0, max(0, pos - 60), max(0, pos - window)):
+            i, slot = R.token_row(bt.tolist(), t, page, caches[0].size(0))
+            for x in caches:
+                x.view(torch.uint8)[i, 0, slot, 3] = 127
+    cos, sin = (t.to(DEV) for t in rope_tables(pos + 1, D))
+    for edit in range(4):
+        row = torch.randn((n_q + 2 * n_kv) * D, generator=gen(edit)).half()
+        kv = row[n_q * D:].view(2, n_kv, D)
+        if edit == 1:
+            kv[1, 0, 5], kv[1, 1, 7] = float("inf"), float("-inf")
+        elif edit == 2:
+            kv[1, 0, D - 1] = float("nan")
+        elif edit == 3:
+            kv[0, 1, 2] = float("nan")
+        row = row.to(DEV)
+        btd, *a = dev(bt, *caches, *scales)
+        b = [t.clone() for t in a]
+        out = decode(K, row, cos, sin, pos, btd, a, n_q, n_kv, cap, window, 0)
+        q = torch.empty(1, n_q * D, dtype=torch.half, device=DEV)
+        K.kv8_append_rows(row.view(1, -1), cos, sin, i32(pos), btd, *b, n_q, n_kv, q)
+        want = run(K, q, i32(pos), btd, b[:2], b[2:], cap, window, 0)
+        assert all(same(x, y) for x, y in zip(a, b))
+        torch.testing.assert_close(out, want[0], rtol=0, atol=0, equal_nan=True)
+
+
+@pytest.mark.parametrize("dtype", CODES, ids=name)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("window", [0, 50])
+def test_decode_positions_and_pages(K, dtype, D, window):
+    """Positions outside the table touch nothing; one past max_ctx, one without a page and one past the block table attend what
+    there is."""
+    n_q, n_kv, page, tokens = 8, 2, 16, 400
+    caches, scales, bt, _ = paged_kv(tokens, n_kv, D, page, dtype, gen(D), extra=0)
+    row = torch.randn((n_q + 2 * n_kv) * D, generator=gen(2)).half()
+    cos, sin = rope_tables(500, D)
+    cosd, sind, rd = dev(cos, sin, row)
+    for pos, cap, hole in ((-1, 400, None), (500, 400, None), (1 << 30, 400, None), (399, 100, None), (130, 128, None),
+                           (399, 128, None), (399, 5000, 399), (399, 400, 0), (130, 131, 129), (400, 600, None),
+                           (499, 600, None), (499, 100, None), (10, 4000, 3)):
+        t = bt.clone()
+        if hole is not None:
+            t[hole // page] = -1 if hole % 2 else caches[0].size(0)
+        td, *c = dev(t, *caches, *scales)
+        q, ref = R.append(row.view(1, -1), cos, sin, pos, t, *caches, *scales, n_q)
+        for ws in (True, False):
+            c = dev(*caches, *scales)
+            out = decode(K, rd, cosd, sind, pos, td, c, n_q, n_kv, cap, window, 4 if window else 0, ws, fill=7.0)
+            assert all(same(a, b) for a, b in zip(c, ref)), pos
+            if not 0 <= pos < 500:
+                assert bool((out == 7.0).all())
+                continue
+            want, bound = R.attention(q, pos, t, R.values(ref[0], ref[2]), R.values(ref[1], ref[3]), cap, window,
+                                      4 if window else 0)
+            R.within(out.view(1, -1), want, bound)
+
+
+@pytest.mark.parametrize("dtype", CODES, ids=name)
+def test_decode_replayed(K, dtype):
+    """One captured call over a sequence of tokens, with eager work between, beside the append and the attention as two."""
+    n_q, n_kv, D, page, cap, start = 32, 8, 128, 16, 1000, 45
+    caches, scales, bt, _ = paged_kv(cap, n_kv, D, page, dtype, gen(8))
+    cos, sin = (t.to(DEV) for t in rope_tables(cap, D))
+    rows = (torch.randn(40, (n_q + 2 * n_kv) * D, generator=gen(9))
+            * torch.exp2(torch.arange(40).float()[:, None] % 7)).half().to(DEV)
+    btd, *a = dev(bt, *caches, *scales)
+    b = [t.clone() for t in a]
+    pos, row, out = i32(start), rows[0].clone(), torch.empty(n_q * D, dtype=torch.half, device=DEV)
+    ws = torch.empty(K.attention_window_workspace_bytes(1, n_q, n_kv, D, cap, 0, 0, dtype) or 16, dtype=torch.uint8, device=DEV)
+    call = lambda: K.attention_kv8_decode(row, cos, sin, pos, btd, *a, n_q, n_kv, cap, out, workspace=ws)
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    for t, was in zip(a, b):
+        t.copy_(was)
+    for i in range(40):
+        row.copy_(rows[i])
+        pos.fill_(start + i)
+        graph.replay()
+        torch.cuda.synchronize()
+        q = torch.empty(1, n_q * D, dtype=torch.half, device=DEV)
+        K.kv8_append_rows(rows[i:i + 1], cos, sin, pos, btd, *b, n_q, n_kv, q)
+        want = run(K, q, pos, btd, b[:2], b[2:], cap)
+        assert all(same(x, y) for x, y in zip(a, b)) and torch.equal(out, want[0]), i
+
+
 @pytest.mark.parametrize("dtype", CACHES, ids=name)
 def test_graphs_share_a_workspace_and_streams(K, dtype):
     """Two captured calls of different sizes with one workspace, replayed in turn, another call on another stream with a
@@ -700,6 +836,14 @@ def test_op_module_refusals(K):
         K.kv8_read(bt, c8, c8, s8, s8, 0, z(3, 2, 64), z(3, 64))
     with pytest.raises(RuntimeError, match="range"):
         K.kv8_read(bt, c8, c8, s8, s8, -1, z(3, 2, 64), z(3, 2, 64))
+    dec = lambda **k: K.attention_kv8_decode(**dict(dict(qkv=z(6 * 64), cos_t=f, sin_t=f, pos=pos, bt=bt, kc=c8, vc=c8.clone(),
+                                                         ks=s8, vs=s8.clone(), n_q=2, n_kv=2, max_ctx=10, out=z(128)), **k))
+    for kw, msg in ((dict(qkv=z(5 * 64)), "qkv must hold"), (dict(out=z(64)), "qkv must hold"), (dict(cos_t=None), "cos_t and"),
+                    (dict(sin_t=z(8, 16, t=torch.float32)), "cos_t and"), (dict(max_ctx=0), "max_ctx"),
+                    (dict(max_ctx=1 << 32), "32 bits"), (dict(n_kv=1, n_q=4), "qkv must hold"),
+                    (dict(kc=z(4, 2, 16, 64)), "int8 or float8"), (dict(window=-1), "window and sinks|32 bits")):
+        with pytest.raises(RuntimeError, match=msg):
+            dec(**kw)
     win = lambda **k: K.attention_kv8(**dict(dict(q=z(3, 4, 64), pos=pos, bt=bt, kc=c8, vc=c8, ks=s8, vs=s8, max_ctx=10,
                                                   out=z(3, 256)), **k))
     for kw, msg in ((dict(q=z(3, 6, 64), out=z(3, 384)), "heads-per-group"), (dict(out=z(3, 128)), "out be"),

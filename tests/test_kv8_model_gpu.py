@@ -33,6 +33,8 @@ class Recorder:
 
     def __getattr__(self, name):
         fn = getattr(self.ops, name)
+        if name == "attention_kv8_decode":
+            return self.decode
         if name not in ("attention_kv8", "attention_window"):
             return fn
 
@@ -45,6 +47,16 @@ class Recorder:
 
         return call
 
+    def decode(self, qkv, cos, sin, pos, bt, kc, vc, ks, vs, n_q, n_kv, max_ctx, out, *rest):
+        """One token appended and attended: the cache as it is afterwards, which is the reference's append."""
+        was = [t.cpu() for t in (kc, vc, ks, vs)]
+        q, want = R.append(qkv.cpu().view(1, -1), cos.cpu(), sin.cpu(), int(pos), bt.cpu(), *was, n_q)
+        self.ops.attention_kv8_decode(qkv, cos, sin, pos, bt, kc, vc, ks, vs, n_q, n_kv, max_ctx, out, *rest)
+        raw = lambda t: t.cpu().contiguous().view(torch.uint8)
+        assert all(torch.equal(raw(t), raw(w)) for t, w in zip((kc, vc, ks, vs), want))
+        self.calls.append((q.view(1, -1), int(pos), R.values(kc.cpu(), ks.cpu()), R.values(vc.cpu(), vs.cpu()),
+                           out.view(1, -1).clone().cpu()))
+
 
 CASES = [dict(kv="int8"), dict(kv="e4m3"), dict(kv="e4m3", window=20, sinks=3), dict(window=25, sinks=2), dict(window=9)]
 ids = lambda c: "-".join(f"{k}{v}" for k, v in c.items())
@@ -52,9 +64,10 @@ ids = lambda c: "-".join(f"{k}{v}" for k, v in c.items())
 
 @pytest.mark.parametrize("cfg", CASES, ids=ids)
 @pytest.mark.parametrize("D,page,fused", [(64, 16, True), (128, 32, True), (64, 16, False)])
-def test_decode_and_prefill_attend_their_cache(cfg, D, page, fused):
+@pytest.mark.parametrize("one", [True, False])
+def test_decode_and_prefill_attend_their_cache(cfg, D, page, fused, one):
     """Every attention call of a prefill and of steps behind it, against the reference over the cache as it is."""
-    m = model(D, page=page, fused_gemv=fused, **cfg)
+    m = model(D, page=page, fused_gemv=fused, fused_attention=one, **cfg)
     m.K = rec = Recorder(m.K)
     m.reset(0)
     m.prefill(tokens(37))
