@@ -570,19 +570,22 @@ attn_few_join_kernel(const f4* __restrict__ part_o, const float2* __restrict__ p
       u32x2{as_u32(f16x2{(f16)(o[0] * inv), (f16)(o[1] * inv)}), as_u32(f16x2{(f16)(o[2] * inv), (f16)(o[3] * inv)})};
 }
 
-// Waves of a workgroup and splits of a call of few columns. A context that eight waves get through in two tiles each (D 128)
-// or four (D 64) is not split: one launch instead of two. From there to 4096 tiles over all kv heads workgroups of four waves,
-// so that one tile per wave reaches twice the CUs; then of eight. At most one workgroup per CU, none with less than a tile per
-// wave. Captured, in us, one token, e4m3:
-//   8 x 4 heads of 128   300 tokens unsplit 6.9, split 7.7 | 600: 8.5, 7.6 | 4096: waves 4 8.2, 8 10.5 | 32768: 18.8, eight
+// Waves of a workgroup and splits of a call of few columns. A short context is not split, one launch instead of two: up to 512
+// tokens in e4m3, 384 in int8 (more arithmetic per code) and 256 in fp16 (twice the bytes) at D 128, twice that at D 64. From
+// there to 4096 tiles over all kv heads workgroups of four waves, so that one tile per wave reaches twice the CUs; then of
+// eight. At most one workgroup per CU, none with less than a tile per wave. Captured, in us, one token, e4m3 if nothing else:
+//   8 x 4 heads of 128   384 tokens unsplit 7.0, split 7.8 | 512: 7.7, 7.8 | int8 384: 7.6, 8.0 | 448: 8.6, 8.0
+//                        fp16 256: 7.9, 8.3 | 320: 8.6, 8.4 | 4096: waves 4 8.2, 8 10.5 | 32768: 18.8, eight
 //                        in 512 workgroups 23.2, four in 256 18.4
-//   4 x 8 heads of 64    600 tokens unsplit 5.4, split 6.9 | 900: 6.8, 6.8 | 16384: waves 4 7.8, 8 8.4 | 32768: 9.4, 8.9
+//   4 x 8 heads of 64    768 tokens unsplit 6.0, split 6.9 | 1024: 6.7, 6.8 | int8 768: 6.7, 7.0 | 1024: 7.8, 7.0
+//                        fp16 512: 7.1, 7.4 | 640: 7.8, 7.4 | 16384: waves 4 7.8, 8 8.4 | 32768: 9.4, 8.9
 struct FewPlan {
   int waves, splits;
 };
-FewPlan few_plan(int M, int n_kv, int D, int max_ctx, int window, int sinks) {
+FewPlan few_plan(int M, int n_kv, int D, int max_ctx, int window, int sinks, int cache) {
   const long long tiles = (win_tokens(M, max_ctx, window, sinks) + kFewTile - 1) / kFewTile;
-  if (tiles <= (D == 128 ? 16 : 32)) return {8, 1};
+  const int alone = cache == kCacheE4m3 ? 16 : cache == kCacheInt8 ? 12 : 8;
+  if (tiles * D <= alone * 128) return {8, 1};
   const int waves = tiles * n_kv < 4096 ? 4 : 8;
   const long long want = max(1LL, min((long long)kWinMaxSplits, 256LL / n_kv));
   const long long per = max((tiles + want - 1) / want, (long long)waves);
@@ -592,7 +595,7 @@ FewPlan few_plan(int M, int n_kv, int D, int max_ctx, int window, int sinks) {
 template <int D, int CACHE, bool DECODE>
 void launch(const WindowAttn& w, WinArgs a, const WinDecode& dec, hipStream_t st) {
   a.part_ml = (float2*)(a.part_o + (size_t)w.splits * w.n_kv * kFewCols * (D / 4));
-  const FewPlan p = few_plan(w.M, w.n_kv, D, w.max_ctx, w.window, w.sinks);
+  const FewPlan p = few_plan(w.M, w.n_kv, D, w.max_ctx, w.window, w.sinks, w.cache);
   // K and V that fill half of the last cache (256 MB) are not kept there for the next call. (8 x 4 heads of 128: one token at
   // 131072, int8, cold 55.1 -> 51.2 us; at 16384, e4m3, from the cache 12.1, past it 14.0)
   const long long bytes = win_tokens(w.M, w.max_ctx, w.window, w.sinks) * w.n_kv * 2 * D * (CACHE == kCacheF16 ? 2 : 1);
@@ -625,8 +628,8 @@ void launch_cache(const WindowAttn& w, const WinArgs& a, const WinDecode* dec, h
 
 }  // namespace
 
-int attention_few_splits(int M, int n_kv, int D, int max_ctx, int window, int sinks) {
-  return few_plan(M, n_kv, D, max_ctx, window, sinks).splits;
+int attention_few_splits(int M, int n_kv, int D, int max_ctx, int window, int sinks, int cache) {
+  return few_plan(M, n_kv, D, max_ctx, window, sinks, cache).splits;
 }
 
 void launch_attention_few(const WindowAttn& w, const WinArgs& a, const WinDecode* dec, hipStream_t st) {

@@ -650,8 +650,8 @@ WinShape win_shape(int M, int n_q, int n_kv, int D, int max_ctx, int window, int
 
 // (The query does not know the page: where a cache of small pages keeps few columns from their kernel, the other one runs that
 // many splits.)
-int attention_window_splits(int M, int n_q, int n_kv, int D, int max_ctx, int window, int sinks, int) {
-  return win_few(M, n_q, n_kv, 4) ? attention_few_splits(M, n_kv, D, max_ctx, window, sinks)
+int attention_window_splits(int M, int n_q, int n_kv, int D, int max_ctx, int window, int sinks, int cache) {
+  return win_few(M, n_q, n_kv, 4) ? attention_few_splits(M, n_kv, D, max_ctx, window, sinks, cache)
                                   : win_shape(M, n_q, n_kv, D, max_ctx, window, sinks).splits;
 }
 size_t attention_window_part_bytes(int M, int n_q, int n_kv, int head_dim) {

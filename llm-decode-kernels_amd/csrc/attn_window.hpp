@@ -78,7 +78,7 @@ struct WinDecode {
   int max_pos;
 };
 // attention_few.hip: the splits that a call can use, and its launch (dec null: attention alone).
-int attention_few_splits(int M, int n_kv, int head_dim, int max_ctx, int window, int sinks);
+int attention_few_splits(int M, int n_kv, int head_dim, int max_ctx, int window, int sinks, int cache);
 void launch_attention_few(const WindowAttn& w, const WinArgs& a, const WinDecode* dec, hipStream_t st);
 
 }  // namespace dk
