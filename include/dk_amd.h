@@ -438,9 +438,9 @@ int dk_tree_accept(const int64_t* tokens, const int32_t* parents, const int64_t*
  * aligned, q_stride % 8 == 0, M 1..2^20.
  *
  * dk_kv8_read: tokens [start, start + n) as fp16 rows k_out, v_out [n, n_kv, head_dim]; tokens without a mapped page read as
- * zeros. Every value that dk_kv8_append_rows stores is an fp16 number, so nothing is rounded; of other codes and scales, products
- * below 2^-14 may be, and those past 65504 are infinite. start + n <= 2^30; k_out, v_out, kc and vc 16-byte aligned. No counterparts in
- * the reference (its cache is fp16, runtime/model.py:117-120).
+ * zeros. Every value that dk_kv8_append_rows stores is an fp16 number, so nothing is rounded; of other codes and scales,
+ * products below 2^-14 may be, and those past 65504 are infinite. start + n <= 2^30; k_out, v_out, kc and vc 16-byte aligned.
+ * No counterparts in the reference (its cache is fp16, runtime/model.py:117-120).
  */
 enum dk_cache { DK_CACHE_F16 = 0, DK_CACHE_INT8 = 1, DK_CACHE_E4M3 = 2 };
 int dk_kv8_append_rows(const void* qkv, const float* cos_t, const float* sin_t, const int32_t* pos, const int32_t* bt,
@@ -478,8 +478,8 @@ int dk_attention_window(const void* q, long long q_stride, const int32_t* pos, c
  * dk_attention_window of its rotated q, in the attention's launches (the workgroup that attends the token's block appends it).
  * The cache is left as those two leave it and out [n_q * head_dim] is what they give; qkv stays as it was. A *pos outside
  * [0, max_pos) touches nothing, out included; one at or past max_ctx is appended and attends the tokens before max_ctx.
- * Workspace as for dk_attention_window with M = 1; qkv and the tables 16-byte aligned, out not overlapping qkv. The 8-bit
- * counterpart of dk_attention_decode.
+ * The page of *pos is listed once in the block table. Workspace as for dk_attention_window with M = 1; qkv and the tables
+ * 16-byte aligned, out not overlapping qkv. The 8-bit counterpart of dk_attention_decode.
  */
 int dk_attention_kv8_decode(const void* qkv, const float* cos_t, const float* sin_t, int max_pos, const int32_t* pos,
                             const int32_t* bt, int n_bt, void* kc, void* vc, float* ks, float* vs, int cache, int n_pages,
