@@ -708,6 +708,34 @@ def test_decode_positions_and_pages(K, dtype, D, window):
 
 
 @pytest.mark.parametrize("dtype", CODES, ids=name)
+def test_decode_on_two_streams(K, dtype):
+    """Two sequences in one cache, each with its block table and workspace, decoded at once: what they give in turn."""
+    n_q, n_kv, D, page, cap, n = 32, 8, 128, 16, 2000, 12
+    caches, scales, bt, _ = paged_kv(2 * cap, n_kv, D, page, dtype, gen(6))
+    tables = [t.contiguous().to(DEV) for t in bt[:2 * (cap // page)].view(2, -1)]
+    cos, sin = (t.to(DEV) for t in rope_tables(cap, D))
+    rows = (torch.randn(2, n, (n_q + 2 * n_kv) * D, generator=gen(7))
+            * torch.exp2(torch.arange(n).float()[:, None] % 5)).half().to(DEV)
+    got = []
+    for together in (True, False):
+        c = dev(*caches, *scales)
+        out = torch.empty(2, n, n_q * D, dtype=torch.half, device=DEV)
+        pos = torch.arange(1500, 1500 + n, dtype=torch.int32, device=DEV)
+        need = K.attention_window_workspace_bytes(1, n_q, n_kv, D, cap, 0, 0, dtype)
+        ws = [torch.full((max(need, 16),), 255, dtype=torch.uint8, device=DEV) for _ in range(2)]
+        streams = [torch.cuda.Stream() for _ in range(2)] if together else [torch.cuda.current_stream()] * 2
+        torch.cuda.synchronize()
+        for i in range(n):
+            for j, st in enumerate(streams):
+                with torch.cuda.stream(st):
+                    K.attention_kv8_decode(rows[j, i], cos, sin, pos[i:], tables[j], *c, n_q, n_kv, cap, out[j, i],
+                                           workspace=ws[j])
+        torch.cuda.synchronize()
+        got.append((out, c))
+    assert torch.equal(got[0][0], got[1][0]) and all(same(a, b) for a, b in zip(got[0][1], got[1][1]))
+
+
+@pytest.mark.parametrize("dtype", CODES, ids=name)
 def test_decode_replayed(K, dtype):
     """One captured call over a sequence of tokens, with eager work between, beside the append and the attention as two."""
     n_q, n_kv, D, page, cap, start = 32, 8, 128, 16, 1000, 45
@@ -815,6 +843,14 @@ def test_caches_past_32_bit_offsets(K, dtype):
     val = R.values(ref[0], ref[2])
     assert torch.equal(k.cpu().double(), torch.stack([val[a, :, s] for a, s in
                                                       (R.token_row([2, 0], t, page, 3) for t in range(pos + M))]))
+    row, t = qkv_rows(1, n_q, n_kv, D, g), pos + M
+    cos, sin = rope_tables(t + 1, D)
+    q, ref = R.append(row, cos, sin, t, small_bt, *ref, n_q)
+    out = decode(K, row.view(-1).to(DEV), cos.to(DEV), sin.to(DEV), t, btd, big, n_q, n_kv, t + 1)
+    for a, b in zip(big, ref):
+        assert same(a[lo:], b)
+    want, bound = R.attention(q, t, small_bt, R.values(ref[0], ref[2]), R.values(ref[1], ref[3]), t + 1)
+    R.within(out.view(1, -1), want, bound)
 
 
 def test_op_module_refusals(K):
