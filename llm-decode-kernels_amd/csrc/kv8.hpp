@@ -85,8 +85,8 @@ template <int CACHE>
 __device__ __forceinline__ float kv8_big(float s) {  // the largest code at scale s
   return s == Kv8Codes<CACHE>::top_scale ? Kv8Codes<CACHE>::top_code : Kv8Codes<CACHE>::most;
 }
-// The largest finite magnitude of eight fp16 values, as fp16 bits (an infinity is stored as the largest fp16 value, NaN counts
-// for nothing), and of fewer.
+// The larger of `top` and the magnitudes of two fp16 values, as fp16 bits (an infinity counts as the largest fp16 value, as
+// which it is stored, NaN for nothing).
 __device__ __forceinline__ uint32_t kv8_top(uint32_t w, uint32_t top) {
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
