@@ -446,9 +446,10 @@ __global__ void __launch_bounds__(CW * KVS * kWave, 2) attn_window_kernel(const 
       for (int p = (t0 >> a.log2P) + tid; p <= (t1 - 1) >> a.log2P; p += NTH)
         whole = whole && (unsigned)a.bt[p] < (unsigned)a.n_pages;
     };
-    // (pages between the sinks and the window may be gone)
+    // (pages between the sinks and the window may be gone; sinks that reach past 32 wt are in the window's places)
     if (r0 * SB < ns) scan(r0 * SB, min(min(r1 * SB, ns), min(a.sinks, ctx)));
-    if (r1 * SB > ns) scan(max(max(r0 * SB, ns) + gap, min(g0.lo, ctx)), min(r1 * SB + gap, ctx));
+    const int from = a.sinks > 32 * wt ? 0 : min(g0.lo, ctx);
+    if (r1 * SB > ns) scan(max(max(r0 * SB, ns) + gap, from), min(r1 * SB + gap, ctx));
     __syncthreads();  // (s_bad, s_holes)
     if (!whole) s_holes = 1;
     __syncthreads();

@@ -888,3 +888,17 @@ def test_op_module_refusals(K):
                     (dict(workspace=z(64, t=torch.uint8).cpu()), "CUDA tensor")):
         with pytest.raises(RuntimeError, match=msg):
             win(**kw)
+
+
+@pytest.mark.parametrize("dtype", CACHES, ids=name)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("M,pos,cap,window,sinks,hole", [(40, 100, 140, 75, 4, 0), (20, 51, 71, 1, 82, 2),
+                                                         (40, 100, 140, 41, 50, 2), (40, 100, 20000, 41, 50, 3),
+                                                         (300, 120, 420, 60, 35, 2), (3, 100, 103, 75, 4, 0)])
+def test_attention_holes_among_the_sinks(K, dtype, D, M, pos, cap, window, sinks, hole):
+    """A page of the sinks is not mapped, and the window begins in the sinks' last tile or ahead of their end: its tokens are
+    attended by no row, whatever the cache's first page holds."""
+    caches, scales, bt, vals = paged_kv(pos + M, 2, D, 16, dtype, gen(M + D))
+    bt[hole] = -1
+    q = torch.randn(M, 8, D, generator=gen(3)).half()
+    check(K, q, pos, bt, caches, scales, vals, cap, window, sinks)
