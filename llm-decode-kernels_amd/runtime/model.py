@@ -648,28 +648,44 @@ class Model:
 
         return _Keep()
 
+    def _rows_kept(self, n):
+        """Context manager: the pages of the first n positions, put back on exit (the scales of codes with them)."""
+        model = self
+
+        class _Keep:
+            def __enter__(self):
+                pages = model.bt[: -(-n // model.cfg.page)].tolist()
+                self.pages = sorted({p for p in pages if 0 <= p < model.n_pages})
+                self.held = [(t, t[:, :, self.pages].clone()) for t in (model.kv, model.kv_scale) if t is not None]
+                return self
+
+            def __exit__(self, *exc):
+                for t, was in self.held:
+                    for i, p in enumerate(self.pages):
+                        t[:, :, p] = was[:, :, i]
+                return False
+
+        return _Keep()
+
     def capture(self):
         """Record step() into a hipGraph (torch.cuda.CUDAGraph), the role of runtime/model.py:235-251: two warm-up
         steps run on a side stream at position 0 (the split buffers are sized for the prepared cap, which a stale
-        position could exceed; the K/V the warm-up writes sit at positions every real step overwrites before reading),
-        then one step is recorded. Token and position are left as they were."""
-        with self._keep_state():
-            # in a cache of codes the block of the warm-up's rows takes their scale: its page is put back
-            page = int(self.bt[0]) if self.kv8 else 0
-            kept = [t[:, :, page].clone() for t in (self.kv, self.kv_scale)] if self.kv8 else []
+        position could exceed), then one step is recorded. Token, position and the cache rows that the warm-up writes
+        are put back: in the middle of a sequence they are its first ones, which a window's sinks attend for ever."""
+        with self._keep_state(), self._rows_kept(2):
             self.pos.zero_()
             side = torch.cuda.Stream()
             side.wait_stream(torch.cuda.current_stream())
-            with torch.cuda.stream(side):
-                self.step()
-                self.step()
-            torch.cuda.current_stream().wait_stream(side)
+            try:
+                with torch.cuda.stream(side):
+                    self.step()
+                    self.step()
+            finally:
+                torch.cuda.current_stream().wait_stream(side)
             graph = torch.cuda.CUDAGraph()
             with torch.cuda.graph(graph):
                 self.step()
             self.graph = graph
-            for t, was in zip((self.kv, self.kv_scale), kept):
-                t[:, :, page] = was
         torch.cuda.synchronize()
 
     def _claim_positions(self, n):

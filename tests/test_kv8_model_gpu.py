@@ -179,3 +179,36 @@ def test_config_refusals():
     with pytest.raises(ValueError, match="read_cache"):
         m.read_cache(0, 250, 10)
     assert m.kv.element_size() == 1 and m.kv_bytes_per_token(100) == 2 * 2 * 101 * (2 * 64 + 2 * 4 // 16)
+
+
+@pytest.mark.parametrize("cfg", [dict(), dict(window=25), dict(window=25, sinks=2), dict(page=1), dict(page=1, window=9, sinks=2),
+                                 dict(kv="int8", window=25, sinks=2)], ids=ids)
+@pytest.mark.parametrize("fails", [False, True])
+def test_preparing_again_keeps_a_sequence(cfg, fails):
+    """The captured step is recorded anew, or its recording fails, in the middle of a sequence: the cache, token and position
+    are as they were, and what follows is what follows without it."""
+    a, b = model(**cfg), model(**cfg)
+    got = []
+    for m in (a, b):
+        m.reset(0)
+        m.prefill(tokens(30))
+        if m is b:
+            held = [t for t in (m.kv.view(torch.uint8), m.kv_scale, m.tok, m.pos) if t is not None]
+            before, step = [t.clone() for t in held], m.step
+
+            def broken():
+                step()
+                raise RuntimeError("a step that fails")
+
+            if fails:
+                m.step = broken
+                with pytest.raises(RuntimeError, match="a step that fails"):
+                    m.prepare(256)
+                del m.step
+            else:
+                m.prepare(256)
+            torch.cuda.synchronize()
+            assert all(torch.equal(x, y) for x, y in zip(before, held))
+            m.prepare(256)
+        got.append(m.teacher_force(tokens(10, 5), collect_logits=True))
+    assert torch.equal(*got)
