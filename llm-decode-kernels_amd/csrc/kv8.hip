@@ -55,7 +55,7 @@ __device__ __forceinline__ void append_block(const Kv8Append& a, long long pos, 
   const int c = lane % LPR;
   const long long first = (pos & ~15LL) + 16LL * blk;             // the block's first token
   const long long end = min(pos + a.M, (long long)a.max_pos);     // tokens that are appended: [max(pos, 0), end)
-  if (first < 0 || first >= end) return;                          // uniform
+  if (first < 0 || max(first, pos) >= end) return;                // uniform: none of its tokens is new
   // the page, whose scale waits for it, then rows and tables, which do not
   const long long lp = first >> a.log2P;
   const int page = lp < a.n_bt ? a.bt[lp] : -1;

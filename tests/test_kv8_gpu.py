@@ -902,3 +902,20 @@ def test_attention_holes_among_the_sinks(K, dtype, D, M, pos, cap, window, sinks
     bt[hole] = -1
     q = torch.randn(M, 8, D, generator=gen(3)).half()
     check(K, q, pos, bt, caches, scales, vals, cap, window, sinks)
+
+
+@pytest.mark.parametrize("dtype", CODES, ids=name)
+@pytest.mark.parametrize("pos,max_pos,M", [(45, 42, 3), (45, 33, 40), (47, 47, 1), (40, 40, 2)])
+@pytest.mark.parametrize("scale", [float("nan"), 0.0, 2.0 ** -30])
+def test_append_past_the_tables_touches_nothing(K, dtype, pos, max_pos, M, scale):
+    """The tables end inside the position's block, whose scale is none that an append leaves: no row is new, and neither the
+    scale nor the codes of the rows ahead are taken anew."""
+    n_q, n_kv, D, page = 4, 2, 64, 16
+    g = gen(pos)
+    kc, vc, ks, vs = empty_cache(6, n_kv, page, D, dtype, g, scale)
+    bt = torch.tensor([5, 2, 1, 0, 4, 3], dtype=torch.int32)
+    qkv = qkv_rows(M, n_q, n_kv, D, g)
+    x, cos, sin, btd, *c = dev(qkv, *rope_tables(max_pos, D), bt, kc, vc, ks, vs)
+    out = torch.full((M, n_q * D), 7.0, dtype=torch.half, device=DEV)
+    K.kv8_append_rows(x, cos, sin, i32(pos), btd, *c, n_q, n_kv, out)
+    assert bool((out == 7.0).all()) and all(same(a, b) for a, b in zip(c, (kc, vc, ks, vs)))
