@@ -246,7 +246,7 @@ attn_few_kernel(const WinArgs a, const WinDecode dec) {
         if (((pos >> 4) & 1) != s) continue;  // uniform
         const float had_k = row ? x.ks[s] : 0.f, had_v = row ? x.vs[s] : 0.f;
         const float sk = kv8_grown(had_k, need_k), sv = kv8_grown(had_v, need_v);
-        const float ik = 1.0f / sk, iv = 1.0f / sv, big_k = kv8_big<CACHE>(sk), big_v = kv8_big<CACHE>(sv);
+        const float ik = 1.0f / sk, iv = 1.0f / sv, big_k = kv8_big<CACHE>(sk, ik), big_v = kv8_big<CACHE>(sv, iv);
         if (row && had_k != sk) {             // uniform
           const float ratio = had_k * ik;
 #pragma unroll

@@ -89,7 +89,7 @@ __device__ __forceinline__ void append_block(const Kv8Append& a, long long pos, 
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, kWave));
   const float need = kv8_scale<CACHE>((float)as_f16x2(top)[0]);
-  const float s = kv8_grown(had, need), inv = 1.0f / s, big = kv8_big<CACHE>(s);
+  const float s = kv8_grown(had, need), inv = 1.0f / s, big = kv8_big<CACHE>(s, inv);
   const bool grows = first < pos && had != s;  // uniform: the rows before pos take the new scale
   const float ratio = had * inv;
   auto put = [&](uint8_t* at, const u32x4& x) __attribute__((always_inline)) {

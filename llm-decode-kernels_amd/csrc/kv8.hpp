@@ -18,14 +18,14 @@ template <>
 struct Kv8Codes<kCacheInt8> {
   static constexpr float most = 127.f;
   static constexpr int most_exp = 6, most_mant = 0x7E0000;  // 127 = 1.984375 * 2^6
-  // at this scale the largest code is one whose value fits fp16: 63 * 1024
+  // from this scale on the largest code is one whose value fits fp16: 63 * 1024
   static constexpr float top_scale = 1024.f, top_code = 63.f;
 };
 template <>
 struct Kv8Codes<kCacheE4m3> {
   static constexpr float most = 448.f;
   static constexpr int most_exp = 8, most_mant = 0x600000;  // 448 = 1.75 * 2^8
-  static constexpr float top_scale = 256.f, top_code = 240.f;
+  static constexpr float top_scale = 256.f, top_code = 240.f;  // 240 * 256 = 120 * 512 = 60 * 1024
 };
 
 // The scale of a block whose largest finite |x| is `top` (a non-negative fp16 value): 2^k with the smallest k >= -24 such
@@ -82,8 +82,8 @@ __device__ __forceinline__ u32x4 kv8_decode8(u32x2 w, float s) {
 // scale that this library did not write is not taken further than its own go.)
 __device__ __forceinline__ float kv8_grown(float had, float need) { return had > need && had <= kKv8MaxScale ? had : need; }
 template <int CACHE>
-__device__ __forceinline__ float kv8_big(float s) {  // the largest code at scale s
-  return s == Kv8Codes<CACHE>::top_scale ? Kv8Codes<CACHE>::top_code : Kv8Codes<CACHE>::most;
+__device__ __forceinline__ float kv8_big(float s, float inv) {  // the largest code at scale s (inv = 1 / s)
+  return s < Kv8Codes<CACHE>::top_scale ? Kv8Codes<CACHE>::most : Kv8Codes<CACHE>::top_code * Kv8Codes<CACHE>::top_scale * inv;
 }
 // The larger of `top` and the magnitudes of two fp16 values, as fp16 bits (an infinity counts as the largest fp16 value, as
 // which it is stored, NaN for nothing).

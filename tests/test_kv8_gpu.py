@@ -919,3 +919,27 @@ def test_append_past_the_tables_touches_nothing(K, dtype, pos, max_pos, M, scale
     out = torch.full((M, n_q * D), 7.0, dtype=torch.half, device=DEV)
     K.kv8_append_rows(x, cos, sin, i32(pos), btd, *c, n_q, n_kv, out)
     assert bool((out == 7.0).all()) and all(same(a, b) for a, b in zip(c, (kc, vc, ks, vs)))
+
+
+@pytest.mark.parametrize("dtype", CODES, ids=name)
+@pytest.mark.parametrize("scale", [128.0, 256.0, 512.0, 1024.0])
+@pytest.mark.parametrize("D", [64, 128])
+def test_append_into_a_block_of_a_large_scale(K, dtype, scale, D):
+    """A block of any valid scale takes the largest fp16 values as codes whose values fit fp16, by either way of appending."""
+    n_q, n_kv, page, pos = 4, 2, 16, 21
+    g = gen(int(scale))
+    kc, vc = (R.to_codes(R.codes_of(torch.randn(2, n_kv, page, D, generator=g) * 20000, scale, dtype), dtype) for _ in "kv")
+    ks, vs = (torch.full((2, n_kv, 1), scale) for _ in "kv")
+    row = torch.randn(1, (n_q + 2 * n_kv) * D, generator=g).half()
+    row[0, n_q * D::3], row[0, n_q * D + 1::3], row[0, (n_q + n_kv) * D + 2::9] = 65504.0, -65504.0, float("inf")
+    bt, cos, sin = torch.tensor([1, 0], dtype=torch.int32), torch.ones(30, D // 2), torch.zeros(30, D // 2)
+    _, want = R.append(row, cos, sin, pos, bt, kc, vc, ks, vs, n_q)
+    x, cosd, sind, btd, *a = dev(row, cos, sin, bt, kc, vc, ks, vs)
+    b = [t.clone() for t in a]
+    decode(K, x[0], cosd, sind, pos, btd, b, n_q, n_kv, pos + 1)
+    K.kv8_append_rows(x, cosd, sind, i32(pos), btd, *a, n_q, n_kv)
+    for got in (a, b):
+        assert all(same(u, v) for u, v in zip(got, want))
+    back = [torch.empty(pos + 1, n_kv, D, dtype=torch.half, device=DEV) for _ in "kv"]
+    K.kv8_read(btd, *a, 0, *back)
+    assert all(bool(torch.isfinite(t).all()) for t in back)
