@@ -525,7 +525,8 @@ class Model:
             self.K.attention_window(q, self.pos, self.bt, kc, vc, max_ctx, out, self.cfg.window, self.cfg.sinks, workspace)
 
     def read_cache(self, li, start, n):
-        """K and V of the tokens [start, start + n) of layer li as fp16 rows [n, n_kv, D], from a cache of any kind."""
+        """K and V of the tokens [start, start + n) of layer li as fp16 rows [n, n_kv, D], from a cache of any kind; tokens
+        whose page is not in the block table read as zeros."""
         if not (0 <= start and 0 < n and start + n <= self.cfg.max_ctx):
             raise ValueError(f"read_cache: tokens [{start}, {start + n}) of a cache of {self.cfg.max_ctx}")
         if self.kv8:
@@ -533,7 +534,10 @@ class Model:
             self.K.kv8_read(self.bt, *self.kv[li], *self.kv_scale[li], start, k, v)
             return k, v
         t = torch.arange(start, start + n, device=self.cfg.device)
-        rows = self.kv[li][:, self.bt[t // self.cfg.page].long(), :, t % self.cfg.page]     # [n, 2, n_kv, D]
+        page = self.bt[t // self.cfg.page].long()
+        held = (page >= 0) & (page < self.n_pages)
+        rows = self.kv[li][:, torch.where(held, page, 0), :, t % self.cfg.page]             # [n, 2, n_kv, D]
+        rows = torch.where(held[:, None, None, None], rows, torch.zeros_like(rows))
         return rows[:, 0], rows[:, 1]
 
     def attention(self, li):

@@ -212,3 +212,17 @@ def test_preparing_again_keeps_a_sequence(cfg, fails):
             m.prepare(256)
         got.append(m.teacher_force(tokens(10, 5), collect_logits=True))
     assert torch.equal(*got)
+
+
+@pytest.mark.parametrize("kv", ["fp16", "int8", "e4m3"])
+def test_read_cache_of_pages_taken_out(kv):
+    """Tokens whose page is no longer in the block table read as zeros, from a cache of any kind; the others as before."""
+    m = model(kv=kv)
+    m.reset(0)
+    m.prefill(tokens(70))
+    before = m.read_cache(1, 3, 60)
+    P = m.cfg.page
+    m.bt[1] = -1
+    for t, was in zip(m.read_cache(1, 3, 60), before):
+        gone = (torch.arange(3, 63, device=DEV) // P == 1)[:, None, None]
+        assert bool((was != 0).any()) and torch.equal(t, torch.where(gone, 0.0, was).half())
