@@ -1000,12 +1000,13 @@ class Model:
                 "embedding_row": self.emb[0].numel() * self.emb.element_size()}
 
     def kv_bytes_per_token(self, ctx):
-        """K and V bytes of all layers that one token moves: the cached rows that it attends read, one new row written. Of a
-        cache of codes, a row has its share of the scales."""
+        """K and V bytes of all layers that one token moves behind ctx cached ones: the cached rows that it attends read
+        (under a window the last window - 1 and the sinks), one new row written. Of a cache of codes a row has its share of
+        the scales, n_kv / 4 bytes, counted in whole ones (none for fewer than 4 kv heads, 0.4% of a row of 64 dims)."""
         row = self.kv[0, 0, 0, :, 0].numel() * self.kv.element_size()    # one token's K (or V) of one layer
         if self.kv8:
             row += self.n_kv * 4 // ext.KV8_BLOCK
-        seen = min(ctx, self.cfg.window + self.cfg.sinks) if self.cfg.window else ctx
+        seen = min(ctx, self.cfg.window - 1 + self.cfg.sinks) if self.cfg.window else ctx
         return 2 * row * self.L * (seen + 1)
 
     def activation_bytes(self):

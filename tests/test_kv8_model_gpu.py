@@ -226,3 +226,11 @@ def test_read_cache_of_pages_taken_out(kv):
     for t, was in zip(m.read_cache(1, 3, 60), before):
         gone = (torch.arange(3, 63, device=DEV) // P == 1)[:, None, None]
         assert bool((was != 0).any()) and torch.equal(t, torch.where(gone, 0.0, was).half())
+
+
+def test_bytes_of_a_step_under_a_window():
+    """A token reads the cached rows that it attends, window - 1 ahead of it and the sinks, and writes its own."""
+    m = model(window=20, sinks=3)
+    row = 2 * 2 * 2 * 64 * 2                       # K and V, layers, kv heads, head dim, fp16
+    for ctx, rows in ((0, 1), (10, 11), (22, 23), (23, 23), (200, 23)):
+        assert m.kv_bytes_per_token(ctx) == row * rows
