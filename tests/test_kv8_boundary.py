@@ -135,3 +135,13 @@ def test_op_module_refusals_on_the_cpu(lib):
     for sizes in ((1, 8, 2, 64, 1 << 32), ((1 << 32) + 1, 8, 2, 64, 100), (1, 8, 2, 64, 100, 1 << 32)):
         with pytest.raises(RuntimeError, match="32 bits"):
             K.attention_window_workspace_bytes(*sizes)
+
+
+@pytest.mark.parametrize("M,n_q,n_kv,max_ctx", [(64, 32, 8, 1 << 20), (1, 32, 8, 1 << 20), (1, 8, 2, 1 << 14)])
+def test_attention_window_workspace_overlaps_nothing(lib, M, n_q, n_kv, max_ctx):
+    """Sizes that split, with many columns and with few: the workspace that the call would use is disjoint from q and out."""
+    need = lib.dk_attention_window_workspace_bytes(M, n_q, n_kv, 128, max_ctx, 0, 0, 2)
+    assert need > 0 and need % 16 == 0
+    kw = dict(M=M, n_q=n_q, n_kv=n_kv, q_stride=n_q * 128, max_ctx=max_ctx, ws_bytes=need)
+    for ws in (AT[0] + 160, AT[7] + 16, AT[0] - need + 16, AT[7] - need + 16):
+        refused(lib, "dk_attention_window", WIN, dict(kw, ws=ws), 4, "workspace must not overlap")
