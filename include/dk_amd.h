@@ -453,9 +453,10 @@ int dk_kv8_read(const int32_t* bt, int n_bt, const void* kc, const void* vc, con
  * Attention of M rows over a paged cache under a sliding window with sinks, over fp16 or 8-bit caches. Row m is at position
  * p = *pos + m and attends the tokens t <= p, and with window > 0 of those the ones with t > p - window or t < sinks; window 0:
  * all of them. The cache already holds them. A row that attends nothing (its position is negative, or none of its tokens has a
- * mapped page) gets zeros. Tokens at positions >= max_ctx (pass *pos + M or more), past the block table or without a mapped
- * page are neither read nor attended, and neither values nor NaN of a token reach a row that does not attend it: pages that lie
- * behind the window of every row to come may be taken out of the block table and used again.
+ * mapped page) gets zeros, and so does one whose scores are all -infinity. Tokens at positions >= max_ctx (pass *pos + M or
+ * more), past the block table or without a mapped page are neither read nor attended, and neither values nor NaN of a token
+ * reach a row that does not attend it: pages that lie behind the window of every row to come may be taken out of the block
+ * table and used again.
  * cache: DK_CACHE_F16 (page any power of two; ks, vs NULL) or the 8-bit caches above (page >= 16; scales powers of two,
  * 2^-24 .. 2^10, such that code * scale fits fp16). q: row m's heads at q + m q_stride (q_stride % 8 == 0), already rotated;
  * out [M, n_q * head_dim] fp16, not overlapping q. fp32 scores and softmax sums, scale 1/sqrt(head_dim); a weight is rounded

@@ -943,3 +943,28 @@ def test_append_into_a_block_of_a_large_scale(K, dtype, scale, D):
     back = [torch.empty(pos + 1, n_kv, D, dtype=torch.half, device=DEV) for _ in "kv"]
     K.kv8_read(btd, *a, 0, *back)
     assert all(bool(torch.isfinite(t).all()) for t in back)
+
+
+@pytest.mark.parametrize("M,pos,cap", [(1, 300, 301), (1, 300, 5000), (3, 90, 93), (40, 300, 2000)])
+def test_attention_of_tokens_without_weight(K, M, pos, cap):
+    """A score of -infinity weighs nothing beside others: as if its token were not there. A row that has only such ones gets
+    zeros, as one that attends nothing."""
+    n_q, n_kv, D, page = 8, 2, 64, 16
+    caches, scales, bt, vals = paged_kv(pos + M, n_kv, D, page, torch.half, gen(5))
+    q = (torch.randn(M, n_q, D, generator=gen(5)).abs() + 0.5).half()
+    a = dev(q, bt, *caches)
+    cells = [R.token_row(bt.tolist(), t, page, caches[0].size(0)) for t in range(pos + M)]
+    for step in (3, 1):
+        k = caches[0].clone()
+        for c in cells[::step]:
+            k[c[0], :, c[1], 1] = float("-inf")
+        for ws in ("full", "none"):
+            out = run(K, a[0], i32(pos), a[1], [k.to(DEV), a[3]], scales, cap, ws=ws)
+            if step == 1:
+                assert bool((out == 0).all())
+                continue
+            for m in {0, M // 2, M - 1}:
+                left = [c for t, c in enumerate(cells[:pos + m + 1]) if t % step]
+                kv = [torch.stack([x[c[0], :, c[1]] for c in left], 1)[None] for x in vals]   # one page of the tokens left
+                want, bound = R.attention(q[m:m + 1], len(left) - 1, torch.zeros(1, dtype=torch.int32), *kv, len(left))
+                R.within(out[m:m + 1], want, bound)
