@@ -459,9 +459,9 @@ int dk_kv8_read(const int32_t* bt, int n_bt, const void* kc, const void* vc, con
  * table and used again.
  * cache: DK_CACHE_F16 (page any power of two; ks, vs NULL) or the 8-bit caches above (page >= 16; scales powers of two,
  * 2^-24 .. 2^10, such that code * scale fits fp16). q: row m's heads at q + m q_stride (q_stride % 8 == 0), already rotated;
- * out [M, n_q * head_dim] fp16, not overlapping q. fp32 scores and softmax sums, scale 1/sqrt(head_dim); a weight is rounded
- * to fp16 where it meets V. n_q / n_kv in {1, 2, 4, 8}, M 1..2^20, max_ctx 1..2^30, window and sinks 0..2^30. q, kc, vc and out
- * 16-byte aligned.
+ * out [M, n_q * head_dim] fp16, not overlapping q. fp32 scores and softmax sums, scale 1/sqrt(head_dim); where a
+ * weight meets V it is held to 22 bits, over 8-bit caches with more than 16 rows times n_q / n_kv to fp16's 11. n_q / n_kv in
+ * {1, 2, 4, 8}, M 1..2^20, max_ctx 1..2^30, window and sinks 0..2^30. q, kc, vc and out 16-byte aligned.
  * The tokens are split over workgroups whose fp32 partials meet in `workspace` (16-byte aligned, overlapping nothing else) and
  * are joined in split order by a second launch; dk_attention_window_workspace_bytes gives what the sizes can use (0: they do
  * not split). A smaller workspace runs the most splits it holds, NULL runs unsplit. Calls that may overlap (on two streams)

@@ -7,8 +7,8 @@
 //     same dims (any order of the dims serves that both operands keep): 16 bytes of a row are one k step of fp16 values or
 //     two of codes, which become fp16 with their scale here. It receives the scores of tokens 4 g + v for column c.
 //   * the weights (attn_window.hpp); the first tile brings the reference at once.
-//   * O^T += V^T . P^T over the 32 tokens: the weights, in fp16, are the B operand as they are (k slot 4 s + v of lane group g
-//     is token 16 s + 4 g + v). For A lane (g, r) loads dims [r D / 16, (r + 1) D / 16) of those 8 tokens' rows and transposes
+//   * O^T += V^T . P^T over the 32 tokens: the weights, as two fp16 numbers, are the B operands as they are (k slot 4 s + v of
+//     lane group g is token 16 s + 4 g + v). For A lane (g, r) loads dims [r D / 16, (r + 1) D / 16) of those 8 tokens' rows and transposes
 //     them in registers; output tile t holds dim r D / 16 + t, so that lane (g, c) ends with D / 4 dims in a row of column c.
 // Tiles that some column does not see whole: 32 token bits per column; V of tokens that do not exist is zeroed, and where the
 // words hold anything that may be NaN or infinite such values are taken out of the products and added one by one for the
@@ -369,12 +369,23 @@ attn_few_kernel(const WinArgs a, const WinDecode dec) {
       sum = weigh(lift == INFINITY ? ref : 0.f, lift == INFINITY ? kWinLift : lift);
     }
     l += sum;
-    h8 ph;
+    h8 ph, pl;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
 #pragma unroll
-      for (int v = 0; v < 4; ++v) ph[4 * s + v] = (f16)p[s][v];
+      for (int v = 0; v < 4; v += 2) {
+        const h2 hi = __builtin_convertvector(f2{p[s][v], p[s][v + 1]}, h2);
+        const uint32_t pair = __builtin_bit_cast(uint32_t, hi);
+        const h2 lo = __builtin_convertvector(f2{minus_lo(p[s][v], pair), minus_hi(p[s][v + 1], pair)}, h2);
+        ph[4 * s + v] = hi[0];
+        ph[4 * s + v + 1] = hi[1];
+        pl[4 * s + v] = lo[0];
+        pl[4 * s + v + 1] = lo[1];
+      }
     }
+    auto weighted = [&](u32x4 v, f4 c) __attribute__((always_inline)) {
+      return mfma16x32(__builtin_bit_cast(h8, v), pl, mfma16x32(__builtin_bit_cast(h8, v), ph, c));
+    };
     // codes: bytes of four tokens' words to words of four tokens
     uint32_t tr[2][VW][4];
     if constexpr (!F16) {
@@ -421,13 +432,13 @@ attn_few_kernel(const WinArgs a, const WinDecode dec) {
     }
     if (!dirty) {
 #pragma unroll
-      for (int t = 0; t < DPL; ++t) acc[t] = mfma16x32(__builtin_bit_cast(h8, operand(x, tr, t)), ph, acc[t]);
+      for (int t = 0; t < DPL; ++t) acc[t] = weighted(operand(x, tr, t), acc[t]);
       return;
     }
     asm volatile("");
     if constexpr (DECODE) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "agent");  // V is read again, the appended row with it
 #pragma unroll
-    for (int t = 0; t < DPL; ++t) acc[t] = mfma16x32(__builtin_bit_cast(h8, finite(operand(x, tr, t))), ph, acc[t]);
+    for (int t = 0; t < DPL; ++t) acc[t] = weighted(finite(operand(x, tr, t)), acc[t]);
     // the values left out, for the columns that see their token
     for (int i = 0; i < kFewTile; ++i) {
       const int t = t0 + i, s = i >> 4;

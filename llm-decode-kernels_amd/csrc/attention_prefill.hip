@@ -49,18 +49,6 @@ constexpr float kLazy = 8.0f;  // log2 units
 constexpr float kLift = 7.0f;  // p's exponent at the reference maximum
 static_assert(kLazy + kLift <= 15.0f, "p fits fp16");
 
-// p - (float)(low / high half of an fp16 pair), one instruction each (the compiler converts and subtracts)
-__device__ __forceinline__ float minus_lo(float p, uint32_t pair) {
-  float r;
-  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(pair), "v"(p));
-  return r;
-}
-__device__ __forceinline__ float minus_hi(float p, uint32_t pair) {
-  float r;
-  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(pair), "v"(p));
-  return r;
-}
-
 template <int D, int CW, int KVS, int BT, bool UP>
 __global__ void __launch_bounds__(CW * KVS * kWave, 2)
 attn_prefill_kernel(const f16* __restrict__ qkv, const int32_t* __restrict__ pos_ptr, const int32_t* __restrict__ bt,

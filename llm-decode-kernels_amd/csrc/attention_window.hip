@@ -11,14 +11,14 @@
 // A round's K / V lie in LDS as fp16, double-buffered. fp16 caches are loaded straight into LDS (buffer loads, spread over the
 // products of the round before); codes go to registers in the first half of that round's products and are turned to fp16, with
 // their scale, on the way to LDS behind them: CW waves share that work, 1 / CW of a conversion per weight and wave. 4096 rows
-// take 149 us over e4m3, 148 over fp16.
+// take 149 us over e4m3, 195 over fp16 (149 with one product of V per weight).
 //
 // Per tile of 32 tokens, on v_mfma_f32_32x32x16_f16:
 //   * S^T = K . Q^T: A = the tile's rows of K from LDS, B = the wave's Q columns (registers). Lane (h, r) receives column r,
 //     tokens 8 q + 4 h + v: a column's scores, sum and output live in the lane pair (r, r + 32).
 //   * the weights (attn_window.hpp), while the next tile's products run;
-//   * O^T += V^T . P^T: the score accumulator, rounded to fp16, is the B operand as it is; V^T comes out of the row-major V
-//     tile through the transposing LDS read.
+//   * O^T += V^T . P^T: the score accumulator, rounded to fp16, is the B operand as it is (over fp16 caches a second time, with
+//     what the rounding left); V^T comes out of the row-major V tile through the transposing LDS read.
 // Masks cost nothing where every column of the wave sees the whole block and every page of the split is mapped (asked once).
 // Elsewhere a lane compares its column's bounds to 32 token bits per tile. Scores of tokens that are not seen become -inf
 // whatever K holds; their p is an exact 0. Since 0 times NaN or infinity is NaN, V chunks of tokens that do not exist are
@@ -208,6 +208,7 @@ __global__ void __launch_bounds__(CW * KVS * kWave, 2) attn_window_kernel(const 
   // ---- a block, by tiles of 32 tokens
   f32x16 sc[2];        // scores of a tile and the next
   u32x4 pw[2];         // p in fp16: the B operand of the output's products
+  u32x4 pl[2];         // fp16 caches: what pw leaves of p
   constexpr int RA = 4;  // K fragments in flight from LDS
   u32x4 ka[RA + 1];
   h8 va[2][DT];        // V fragments: 16 tokens, in two sets
@@ -221,6 +222,12 @@ __global__ void __launch_bounds__(CW * KVS * kWave, 2) attn_window_kernel(const 
     uint32_t pair = __builtin_bit_cast(uint32_t, p);
     asm volatile("" : "+v"(pair), "+v"(psum[0]), "+v"(psum[1]));  // here, beside the products, not where they are used
     pw[e >> 3][(e & 7) >> 1] = pair;
+    if constexpr (F16) {
+      const h2 rest = __builtin_convertvector(f2{minus_lo(p0, pair), minus_hi(p1, pair)}, h2);
+      uint32_t word = __builtin_bit_cast(uint32_t, rest);
+      asm volatile("" : "+v"(word));
+      pl[e >> 3][(e & 7) >> 1] = word;
+    }
   };
   auto block = [&](int rnd, const uint8_t* kb, const uint8_t* vb, auto send) __attribute__((always_inline)) {
     const int v0 = (rnd * KVS + grp) * BT, t0 = v0 + gap;
@@ -320,6 +327,10 @@ __global__ void __launch_bounds__(CW * KVS * kWave, 2) attn_window_kernel(const 
       for (int ks = 0; ks < 2; ++ks) {
 #pragma unroll
         for (int t = 0; t < DT; ++t) acc[t] = mfma32x32(va[ks][t], __builtin_bit_cast(h8, pw[ks]), acc[t]);
+        if constexpr (F16) {
+#pragma unroll
+          for (int t = 0; t < DT; ++t) acc[t] = mfma32x32(va[ks][t], __builtin_bit_cast(h8, pl[ks]), acc[t]);
+        }
       }
     }
     if (!whole || partial(rnd)) {  // uniform in the workgroup

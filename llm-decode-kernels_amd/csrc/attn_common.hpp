@@ -67,6 +67,18 @@ __device__ __forceinline__ f32x16 mfma32x32(h8 a, h8 b, f32x16 c) {
 
 __device__ __forceinline__ f4 mfma16x32(h8 a, h8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
+// p - (float)(low / high half of an fp16 pair), one instruction each (the compiler converts and subtracts)
+__device__ __forceinline__ float minus_lo(float p, uint32_t pair) {
+  float r;
+  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(pair), "v"(p));
+  return r;
+}
+__device__ __forceinline__ float minus_hi(float p, uint32_t pair) {
+  float r;
+  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(pair), "v"(p));
+  return r;
+}
+
 // Keeps loads where they are written (no sinking to their first use).
 __device__ __forceinline__ void pf_fence() { asm volatile("" ::: "memory"); }
 

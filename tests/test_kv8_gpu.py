@@ -968,3 +968,21 @@ def test_attention_of_tokens_without_weight(K, M, pos, cap):
                 kv = [torch.stack([x[c[0], :, c[1]] for c in left], 1)[None] for x in vals]   # one page of the tokens left
                 want, bound = R.attention(q[m:m + 1], len(left) - 1, torch.zeros(1, dtype=torch.int32), *kv, len(left))
                 R.within(out[m:m + 1], want, bound)
+
+
+@pytest.mark.parametrize("dtype", CACHES, ids=name)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("M,pos,cap,window,hpg,n_kv", [(1, 17, 18, 0, 8, 2), (1, 40, 5000, 0, 4, 2), (1, 30, 1 << 20, 20, 4, 2),
+                                                       (3, 25, 28, 9, 4, 2), (40, 3, 43, 0, 4, 2), (40, 0, 20000, 12, 4, 2),
+                                                       (130, 0, 130, 30, 8, 8), (700, 0, 700, 25, 4, 8)])
+def test_attention_weights_keep_their_bits(K, dtype, D, M, pos, cap, window, hpg, n_kv):
+    """Small scores over few tokens, where a weight's rounding would be the largest error but the output's own. A weight p meets
+    V as two fp16 numbers, hi = fp16(p) and fp16(p - hi): |p - hi| <= 2^-11 p, half a step of that is 2^-22 p, or 2^-25 below
+    fp16's normal range, which the bound has already. (More than 16 columns over codes: one number, 11 bits.)"""
+    bits = 22 if dtype == torch.half or M * hpg <= 16 else 11
+    caches, scales, bt, vals = paged_kv(pos + M, n_kv, D, 16, dtype, gen(M + D))
+    q = (torch.randn(M, hpg * n_kv, D, generator=gen(5)) * 0.1).half()
+    want, bound = R.attention(q, pos, bt, *vals, cap, window, 0, weight=2.0 ** -bits)
+    a = dev(q, bt, *caches, *scales)
+    for ws in ("full", "none"):
+        R.within(run(K, a[0], i32(pos), a[1], a[2:4], a[4:6], cap, window, 0, ws), want, bound)
