@@ -36,6 +36,14 @@ __device__ __forceinline__ float over_rows(float v, F f) {
   return f(__uint_as_float(b0), __uint_as_float(b1));
 }
 
+// A value that the whole wave reads and that nothing writes ahead of that read, through the scalar cache. Elsewhere a load like
+// it is a vector load wherever the kernel may store or an asm block stands between, and those return in order: a page looked
+// up behind a tile's loads would come only after all of them.
+template <class T>
+__device__ __forceinline__ T load_scalar(const T* p) {
+  return *(const __attribute__((address_space(4))) T*)p;
+}
+
 template <int D, int CACHE>
 struct FewShape {
   static constexpr bool F16 = CACHE == kCacheF16;
@@ -75,7 +83,7 @@ attn_few_kernel(const WinArgs a, const WinDecode dec) {
     int p[2];
   };
   auto pages_at = [&](int t) __attribute__((always_inline)) {
-    return Pages{{a.bt[min(t >> a.log2P, a.n_bt - 1)], a.bt[min((t + 16) >> a.log2P, a.n_bt - 1)]}};
+    return Pages{{load_scalar(a.bt + min(t >> a.log2P, a.n_bt - 1)), load_scalar(a.bt + min((t + 16) >> a.log2P, a.n_bt - 1))}};
   };
   const int pos = *a.pos;
   Pages pg = pages_at(kFewTile * i0);
@@ -135,8 +143,8 @@ attn_few_kernel(const WinArgs a, const WinDecode dec) {
         x.v[s][v] = NT ? __builtin_nontemporal_load(p) : *p;
       }
       if constexpr (!F16) {
-        x.ks[s] = a.ks[row >> 4];
-        x.vs[s] = a.vs[row >> 4];
+        x.ks[s] = load_scalar(a.ks + (row >> 4));
+        x.vs[s] = load_scalar(a.vs + (row >> 4));
       }
     }
     return x;
@@ -224,7 +232,7 @@ attn_few_kernel(const WinArgs a, const WinDecode dec) {
   }
   auto append = [&](Tile& x) __attribute__((always_inline)) {
     if constexpr (DECODE) {
-      const int row = pos & 15, page = a.bt[min(pos >> a.log2P, a.n_bt - 1)];
+      const int row = pos & 15, page = load_scalar(a.bt + min(pos >> a.log2P, a.n_bt - 1));
       if (pos >> a.log2P >= a.n_bt || (unsigned)page >= (unsigned)a.n_pages) return;  // uniform
       const size_t at = (((size_t)page * a.n_kv + kvh) << a.log2P) + (pos & (P - 1) & ~15);  // the block's first row
       uint8_t* kb = const_cast<uint8_t*>(a.kc) + at * D + c * D + 16 * g;
