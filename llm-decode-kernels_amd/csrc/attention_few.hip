@@ -14,10 +14,10 @@
 // words hold anything that may be NaN or infinite such values are taken out of the products and added one by one for the
 // columns that see their token.
 //
-// What bounds it: one int8 token at 131072, 8 x 4 heads of 128, takes 47 us for 269 MB, 5.7 TB/s. Small ones are launch and a
+// What bounds it: one int8 token at 131072, 8 x 4 heads of 128, takes 48 us for 269 MB, 5.6 TB/s. Small ones are launch and a
 // chain of dependent loads (position and page, K / V), the waves' merge in LDS, and where they are split the join: captured,
-// 4.9 us at 300 tokens of 4 x 8 heads of 64 (one launch), 8.1 at 4096 of 8 x 4 heads of 128 (5.5 and 2.6). Of those, masks
-// as compares and the look for NaN on unpacked values cost 1 us (every decode step's last tile takes that path), reductions
+// 4.9 us at 300 tokens of 4 x 8 heads of 64 (one launch), 7.7 at 4096 of 8 x 4 heads of 128 (traced 5.3 and 3.4). Masks as
+// compares and the look for NaN on unpacked values cost 1 us (every decode step's last tile takes that path), reductions
 // through LDS and a second copy of the tile's code 0.2. No gain: 16 waves (the registers of a tile do not fit).
 #include "attn_window.hpp"
 
@@ -64,7 +64,7 @@ __device__ __forceinline__ float over_lanes16(float v) {
 // DECODE: one row, whose q is rotated here and whose K / V are appended by the wave that has their tile: it takes the new
 // row's codes into the tile that it has loaded, takes the block's others anew where its scale grows, and stores them. So the
 // append adds no launch and no round trip to the cache, only this wave's arithmetic: in a decode step of 8 layers of 8 x 4
-// heads of 128 at 512 tokens, e4m3, the step takes 342 us, with the append in a launch of its own 358 (at 65536 531 and 535).
+// heads of 128 at 512 tokens, e4m3, the step takes 341 us, with the append in a launch of its own 354 (at 65536 502 and 529).
 template <int D, int CACHE, int NW, bool NT, bool DECODE>
 __global__ void __launch_bounds__(NW * kWave, 2)
 attn_few_kernel(const WinArgs a, const WinDecode dec) {
@@ -593,11 +593,12 @@ attn_few_join_kernel(const f4* __restrict__ part_o, const float2* __restrict__ p
 // tokens in e4m3, 384 in int8 (more arithmetic per code) and 256 in fp16 (twice the bytes) at D 128, twice that at D 64. From
 // there to 4096 tiles over all kv heads workgroups of four waves, so that one tile per wave reaches twice the CUs; then of
 // eight. At most one workgroup per CU, none with less than a tile per wave. Captured, in us, one token, e4m3 if nothing else:
-//   8 x 4 heads of 128   384 tokens unsplit 7.0, split 7.8 | 512: 7.7, 7.8 | int8 384: 7.6, 8.0 | 448: 8.6, 8.0
-//                        fp16 256: 7.9, 8.3 | 320: 8.6, 8.4 | 4096: waves 4 8.2, 8 10.5 | 32768: 18.8, eight
-//                        in 512 workgroups 23.2, four in 256 18.4
-//   4 x 8 heads of 64    768 tokens unsplit 6.0, split 6.9 | 1024: 6.7, 6.8 | int8 768: 6.7, 7.0 | 1024: 7.8, 7.0
-//                        fp16 512: 7.1, 7.4 | 640: 7.8, 7.4 | 16384: waves 4 7.8, 8 8.4 | 32768: 9.4, 8.9
+//   8 x 4 heads of 128   384 tokens unsplit 6.4, split 7.3 | 512: 7.5, 7.2 | int8 384: 7.0, 7.6 | 448: 8.2, 7.6
+//                        fp16 256: 7.4, 7.8 | 320: 7.9, 7.9 | 4096: waves 4 7.8, 8 9.1 | 16384: 12.8, 12.2 | 32768: 21.7, 18.8
+//   4 x 8 heads of 64    768 tokens unsplit 5.8, split 6.8 | 1024: 6.6, 6.8 | int8 768: 6.8, 7.0 | 1024: 7.8, 7.0
+//                        fp16 512: 6.7, 7.1 | 640: 7.4, 7.1 | 16384: waves 4 and 8 7.9 | 32768: 9.4, 9.0
+// One or two kv heads of a long cache reach kWinMaxSplits and leave CUs idle: one e4m3 token at 131072 takes 21 us with one kv
+// head, 23 with two, 29 with four, 49 with eight.
 struct FewPlan {
   int waves, splits;
 };
@@ -615,8 +616,9 @@ template <int D, int CACHE, bool DECODE>
 void launch(const WindowAttn& w, WinArgs a, const WinDecode& dec, hipStream_t st) {
   a.part_ml = (float2*)(a.part_o + (size_t)w.splits * w.n_kv * kFewCols * (D / 4));
   const FewPlan p = few_plan(w.M, w.n_kv, D, w.max_ctx, w.window, w.sinks, w.cache);
-  // K and V that fill half of the last cache (256 MB) are not kept there for the next call. (8 x 4 heads of 128: one token at
-  // 131072, int8, cold 55.1 -> 51.2 us; at 16384, e4m3, from the cache 12.1, past it 14.0)
+  // K and V that may fill half of the last cache (256 MB) are not kept there for the next call. max_ctx decides, not the
+  // position, which the host does not know: 16 e4m3 caches of 8 heads of 128 in turn, max_ctx 131072, take 49.5 us a token at
+  // 131072 (from the cache 54.3), 13.6 at 16384 (14.8), and short contexts pay for it: 10.3 at 4096 (9.7), 8.9 at 512 (8.7)
   const long long bytes = win_tokens(w.M, w.max_ctx, w.window, w.sinks) * w.n_kv * 2 * D * (CACHE == kCacheF16 ? 2 : 1);
   const dim3 grid(w.n_kv, w.splits);
   if (p.waves == 4)

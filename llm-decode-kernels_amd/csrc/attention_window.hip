@@ -25,11 +25,12 @@
 // zeroed on the way, and those with such values in rounds that some column does not see whole; the latter are added behind the
 // block, value by value, for the columns that see their token.
 //
-// What bounds it: 4096 rows at 0, 8 x 4 heads of 128, take 148-155 us, 0.89-0.93 PFLOP/s of what they need, against 117 at the
-// rate of a large matrix product: the softmax and LDS reads beside the products at the clock that the card keeps up under
-// them, and blocks on the diagonal that are computed whole. Under a window of 1024 they take 93-95 (floor 51): two turns of 18
-// rounds of 64 tokens, 16 of them needed, and about 8 us each to start. 100 rows behind 8000 tokens take 31 (floor 11): 78% of
-// the columns are real, four rounds in 256 workgroups (17 us), 10 for launch and first loads, 28 MB of partials.
+// What bounds it: 4096 rows of e4m3 at 0, 8 x 4 heads of 128, take 148-155 us, 0.89-0.93 PFLOP/s of what they need, against
+// 117 at the rate of a large matrix product: the softmax and LDS reads beside the products at the clock that the card keeps up
+// under them, and blocks on the diagonal that are computed whole. Over fp16, whose weights meet V twice, they take 195. Under a
+// window of 1024 fp16 takes 115 (floor 51, with the second product 77), e4m3 96: two turns of 18 rounds of 64 tokens, 16 of
+// them needed, and about 8 us each to start. 100 rows behind 8000 tokens take 31 (floor 11): 78% of the columns are real, four
+// rounds in 256 workgroups (17 us), 10 for launch and first loads, 28 MB of partials.
 // No gain: tiles that no column of a wave sees left out (the accumulators meet at the branch: 10 to 250 registers spilled);
 // blocks of 64 tokens for eight waves (157 us instead of 150); the halves of V's codes in another order for every other row, so
 // that their writes to LDS conflict no more (17% of LDS's cycles; 152 us instead of 147).
@@ -616,8 +617,9 @@ constexpr WinShape kWinShapes[4] = {{2, 4, 32, 1}, {4, 1, 64, 1}, {4, 2, 64, 1},
 
 // The shape with the least estimated time: a fixed part, a round's time times the rounds of the longest workgroup, or of all
 // of them over the CUs with what it takes to start each. Fitted to the times of all four shapes in 75 cases (8 to 4096 rows
-// behind 0 to 30000 tokens, windows of 256 to 2048 and none, five head layouts); the choice is 0.8% above the best of the four
-// in the geometric mean, 15% at worst. In us, D 128 (e4m3, 8 x 4 heads):
+// behind 0 to 30000 tokens, windows of 256 to 2048 and none, five head layouts), before weights met fp16 caches' V twice; as it
+// stands the choice is 0.6% above the best of the four in the geometric mean for e4m3 and 0.9% for fp16, 7% at worst. In us,
+// D 128 (e4m3, 8 x 4 heads):
 //                              (2,4,32) (4,1,64) (4,2,64) (8,1,128)
 //   512 rows at 0                15.3     19.2     19.3     20.5
 //   64 behind 4000               18.4     19.3     19.7     23.7
