@@ -96,9 +96,9 @@ def cells_of(pos, M, bt, page, n_pages, max_ctx):
     return [token_row(bt, t, page, n_pages, max_ctx) for t in range(max(pos + M, 0))]
 
 
-def attention(q, pos, bt, kc, vc, max_ctx, window=0, sinks=0, weight=2.0 ** -11):
+def attention(q, pos, bt, kc, vc, max_ctx, window=0, sinks=0):
     """q [M, n_q, D]; kc, vc values [pages, n_kv, P, D] (fp16 or fp64) -> (out fp64 [M, n_q * D], bound). A token that a row
-    does not attend is left out altogether, whatever its K and V hold. weight: what a weight's rounding may cost, relative."""
+    does not attend is left out altogether, whatever its K and V hold."""
     M, n_q, D = q.shape
     n_kv, page, n_pages = kc.size(1), kc.size(2), kc.size(0)
     cells = cells_of(pos, M, bt.tolist(), page, n_pages, max_ctx)
@@ -124,7 +124,7 @@ def attention(q, pos, bt, kc, vc, max_ctx, window=0, sinks=0, weight=2.0 ** -11)
         # output half a step of its own
         ds = 2.0 ** -24 * ((D + 4) * (qh.abs() @ k.abs().transpose(1, 2).contiguous()) / math.sqrt(D)
                            + 4 * sc.abs()).amax(-1, keepdim=True)
-        rel = weight + 2 * (ds + 2.0 ** -21) + 2.0 ** -24 * (len(toks) / 16 + 64)
+        rel = 2.0 ** -11 + 2 * (ds + 2.0 ** -21) + 2.0 ** -24 * (len(toks) / 16 + 64)
         out[m] = o.view(n_q, D)
         bound[m] = (2.0 ** -11 * o.abs() + rel * (w @ v.abs()) + 2.0 ** -32 * v.abs().sum(1, keepdim=True)
                     + 2.0 ** -25).view(n_q, D)

@@ -982,7 +982,9 @@ def test_attention_weights_keep_their_bits(K, dtype, D, M, pos, cap, window, hpg
     bits = 22 if dtype == torch.half or M * hpg <= 16 else 11
     caches, scales, bt, vals = paged_kv(pos + M, n_kv, D, 16, dtype, gen(M + D))
     q = (torch.randn(M, hpg * n_kv, D, generator=gen(5)) * 0.1).half()
-    want, bound = R.attention(q, pos, bt, *vals, cap, window, 0, weight=2.0 ** -bits)
+    want, bound = R.attention(q, pos, bt, *vals, cap, window, 0)
+    size = R.attention(q, pos, bt, vals[0], vals[1].abs(), cap, window, 0)[0]      # sum of w |v|, of which the bound has 2^-11
+    bound = bound - (2.0 ** -11 - 2.0 ** -bits) * size
     a = dev(q, bt, *caches, *scales)
     for ws in ("full", "none"):
         R.within(run(K, a[0], i32(pos), a[1], a[2:4], a[4:6], cap, window, 0, ws), want, bound)
